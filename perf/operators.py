@@ -130,7 +130,8 @@ def draw(rng: random.Random):
         query = rng.choice([1, 1, 1, 3, 5, 8])
         hi = rng.randint(query, 400)
         n = _log(rng, 1, 4000)
-        seqs = _log(rng, 1, max(1, min(64, (500000 if n_layer == 1 else 220000) // (query * (n + hi)))))
+        most, pairs = (64, 500000) if n_layer == 1 else (32, 220000)
+        seqs = _log(rng, 1, max(1, min(most, pairs // (query * (n + hi)))))
         return _prefix(shape, n_layer, seqs, rng.randint(query, hi), hi, query, n,
                        groups=rng.randint(1, min(4, seqs)), bare=rng.random() < 0.3, q8=rng.random() < 0.3, ctx_seed=cs)
     if kind == "prefix-long":
