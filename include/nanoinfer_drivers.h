@@ -108,6 +108,10 @@ int ni_spec_plan(ni_spec* s, const ni_work** work, uint32_t* n_work, const uint3
 /* After the step ran: accept acc ~ U[0, draft_k] per sequence and
  * truncate(seq, tlen + 1 + acc) (metal_spec.rs:146-163). */
 int ni_spec_commit(ni_spec* s, const uint32_t** accepted);
+/* The same with the caller's numbers, one per sequence (0 .. draft_k), as
+ * ni_verify_drafts finds them, in place of the draws; nothing is truncated
+ * unless all of them are in range. */
+int ni_spec_commit_accepted(ni_spec* s, const uint32_t* accepted);
 /* Restart rule for long runs: a sequence that has grown more than `window`
  * rows past its length at ni_spec_create is truncated back to that length
  * after the round (a request ends; the next, with the same prompt length,

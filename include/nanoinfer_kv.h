@@ -115,7 +115,7 @@ typedef struct ni_work {
 int ni_kv_create(const ni_kv_opts* opts, ni_kv** out);
 void ni_kv_destroy(ni_kv* kv);
 /* Text of the last failure on this handle; with kv == NULL, of the last
- * failed ni_kv_create or ni_attention on this thread. */
+ * failed ni_kv_create, ni_attention, ni_rotary_* or ni_verify_* on this thread. */
 const char* ni_kv_last_error(const ni_kv* kv);
 /* Bytes of one page over all layers, K and V (BatchEngine::kv_block_bytes, batch.rs:107-109). */
 size_t ni_kv_page_bytes(const ni_kv* kv);
@@ -270,6 +270,131 @@ int ni_kv_decode_steps(ni_kv* kv, const uint32_t* seqs, uint32_t n, uint32_t ste
                        const float* v, int64_t row_stride, int64_t layer_stride, int64_t step_stride, float* out,
                        int64_t out_row_stride, int64_t out_layer_stride, int64_t out_step_stride,
                        uint32_t split_tokens, ni_stream stream);
+
+/* ---- rotary positions, shared prefixes, drafts (no counterpart in the
+ * reference, whose model has learned positions, equal head counts and greedy
+ * drafts) ---- */
+
+/* Types of rows and probabilities. */
+#define NI_F32 0u
+#define NI_F16 1u
+#define NI_BF16 2u
+
+/* Rotary positions: pair i of the first rot_dim dims of a head turns by
+ * pos * f_i, (x1, x2) -> m (x1 cos - x2 sin, x2 cos + x1 sin); the dims past
+ * rot_dim stay as they are.  A pair is (x[i], x[i + rot_dim/2]), or
+ * interleaved (x[2i], x[2i+1]).  f_i = base^(-2i/rot_dim), for contexts past
+ * the trained one scaled by `factor` s:
+ *   NI_ROTARY_LINEAR  f_i / s
+ *   NI_ROTARY_NTK     base * s^(rot_dim/(rot_dim-2)) in place of base
+ *   NI_ROTARY_YARN    (Peng et al., 2023) f_i where a pair makes beta_fast
+ *                     turns or more over orig_ctx positions, f_i / s where it
+ *                     makes beta_slow or fewer, a ramp between; m = 0.1 ln s + 1
+ * m is 1 otherwise; attn_scale > 0 sets it. */
+#define NI_ROTARY_PLAIN 0u
+#define NI_ROTARY_LINEAR 1u
+#define NI_ROTARY_NTK 2u
+#define NI_ROTARY_YARN 3u
+#define NI_ROTARY_MAX_PAIRS 128
+typedef struct ni_rotary_opts {
+    double base;          /* > 0 (10000 is usual) */
+    uint32_t rot_dim;     /* even, at most head_dim; 0 = head_dim */
+    uint32_t interleaved; /* 0 or 1 */
+    uint32_t scaling;     /* NI_ROTARY_* */
+    uint32_t orig_ctx;    /* YARN */
+    double factor;        /* s >= 1 */
+    double beta_fast, beta_slow; /* YARN; 0 = 32 and 1 */
+    double attn_scale;    /* m; 0 = the scaling's own */
+} ni_rotary_opts;
+/* A rotation ready for use: plain data, filled by ni_rotary_init, read during
+ * the calls it is passed to and not kept.  turns[i] is f_i / 2 pi in units of
+ * 2^-64 turns a position, so angles are exact to 2^-33 turns at any 32-bit
+ * position. */
+typedef struct ni_rotary {
+    uint32_t head_dim;
+    uint32_t rot_dim;
+    uint32_t interleaved;
+    float scale; /* m */
+    uint64_t turns[NI_ROTARY_MAX_PAIRS];
+} ni_rotary;
+/* head_dim even, at most 256. */
+int ni_rotary_init(ni_rotary* r, uint32_t head_dim, const ni_rotary_opts* opts);
+
+/* Rotate n rows of n_head heads (row i at x + i * x_row_stride, head_dim
+ * values a head) to out.  x and out are of `dtype` (rounded once, to nearest
+ * even; computed in f32) and aligned to it (16-byte aligned rows of heads whose
+ * head_dim and rot_dim are multiples of 8 are read 16 bytes at a time, others
+ * value by value).  Row i is at positions[i] (int32 on the device; negative ones
+ * turn backwards), or at pos0 + i where positions is NULL.  out may be x with
+ * the same stride; rows that overlap otherwise are undefined.  Enqueued on
+ * `stream`; failures are reported by ni_kv_last_error(NULL). */
+int ni_rotary_apply(const ni_rotary* r, uint32_t dtype, const void* x, int64_t x_row_stride, void* out,
+                    int64_t out_row_stride, uint32_t n, uint32_t n_head, const int32_t* positions, uint32_t pos0,
+                    ni_stream stream);
+
+/* ni_kv_append with the rotation on the way: row i's keys are rotated to
+ * positions[i] (host memory; NULL = rows[i].pos), in f32, and stored as
+ * ni_kv_append stores them (f16 or Q8); v is stored as it is.  n_q_head > 0:
+ * row i's n_q_head query heads are rotated alike from q to q_out (f32; q_out
+ * may be q with the same strides), for models whose query heads outnumber the
+ * cache's too.  One launch.  The rotation's head_dim must be the cache's and
+ * its rot_dim a multiple of 8.  A (seq, pos) may appear once in rows. */
+int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, const ni_rotary* rotary,
+                        const uint32_t* positions, const float* k, const float* v, int64_t row_stride,
+                        int64_t layer_stride, const float* q, int64_t q_row_stride, int64_t q_layer_stride,
+                        uint32_t n_q_head, float* q_out, int64_t q_out_row_stride, int64_t q_out_layer_stride,
+                        ni_stream stream);
+
+/* The next n_rows rows of a call attend to positions 0 .. len-1 of sequence
+ * `seq` before their own sequence's (len == 0: to no prefix; seq is then not
+ * looked at). */
+typedef struct ni_prefix {
+    uint32_t seq;
+    uint32_t len;
+    uint32_t n_rows;
+} ni_prefix;
+/* Paged attention behind shared prefixes: row i attends to the prefix that
+ * covers it and causally to keys 0 .. rows[i].pos of rows[i].seq, under one
+ * softmax of q.K^T / sqrt(head_dim).  The prefix is one sequence of the cache
+ * (reserved to len at least, and not freed before the call), read once for
+ * all its rows rather than once a row.  prefixes[0..n_prefix) cover the rows
+ * in order and in full.  A row of q and out holds n_q_head heads, a multiple
+ * of the cache's n_head: query head h reads cache head h / (n_q_head /
+ * n_head).  out may be q.  A row's own sequence may not be its prefix.
+ * split_tokens: keys per partition, a multiple of 16; 0 = automatic.
+ * Under stream capture the call allocates nothing: make the same call once
+ * before, so that the handle holds the partials it needs (graphs captured from
+ * one handle share them, so their replays must not overlap), and the plan
+ * must fit the launch arguments (32 KB). */
+int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_row_stride, int64_t q_layer_stride,
+                           uint32_t n_q_head, const ni_row* rows, uint32_t n, const ni_prefix* prefixes,
+                           uint32_t n_prefix, float* out, int64_t out_row_stride, int64_t out_layer_stride,
+                           uint32_t split_tokens, ni_stream stream);
+
+/* Verify drafted tokens against the target's probabilities (speculative
+ * sampling: the tokens that come out are distributed as the target's own).
+ * Sequence b drafted d_i = drafted[b][i] for i < n_b (n_drafts[b] held to
+ * 0..n_draft; NULL = n_draft each).  target holds p_i = target[b][i][vocab]
+ * for i in 0 .. n_draft (p_{n_b}: after the last draft), draft q_i =
+ * draft[b][i][vocab] (NULL: the drafter was certain, q_i(d_i) = 1).  Draft i
+ * is accepted while accept_u[b][i] * q_i(d_i) < p_i(d_i); a token outside
+ * 0..vocab-1 is not.  With a drafts accepted, accepted[b] = a and
+ * tokens[b][0..n_draft] = d_0 .. d_{a-1}, the drawn token, then -1.  The
+ * token is drawn from max(p_a - q_a, 0) if a < n_b (from p_a where that is 0
+ * everywhere), else from p_a: the first v at which the sum of the weights
+ * 0..v passes sample_u[b] times the whole.  Differences, products and sums
+ * are taken in 64 bits.  Uniform numbers are in [0, 1).  Probabilities should
+ * be finite; negative and NaN ones weigh nothing, and -1 is drawn where none
+ * is positive.  target and draft are of `dtype`; strides count elements, rows
+ * are dense.  workspace: ni_verify_workspace(n_seq, vocab) bytes of device
+ * memory that no other work on the GPU uses meanwhile.  Enqueued on
+ * `stream`; failures are reported by ni_kv_last_error(NULL). */
+size_t ni_verify_workspace(uint32_t n_seq, uint32_t vocab);
+int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stride, int64_t target_row_stride,
+                     const void* draft, int64_t draft_seq_stride, int64_t draft_row_stride, const int32_t* drafted,
+                     int64_t drafted_stride, const int32_t* n_drafts, const float* accept_u, int64_t accept_stride,
+                     const float* sample_u, uint32_t n_seq, uint32_t n_draft, uint32_t vocab, int32_t* accepted,
+                     int32_t* tokens, int64_t tokens_stride, void* workspace, size_t workspace_bytes, ni_stream stream);
 
 /* Wait for all work this handle enqueued on `stream`; afterwards no call of
  * the handle waits for that work, and `stream` may be destroyed. */

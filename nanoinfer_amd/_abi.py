@@ -37,6 +37,11 @@ NI_K_APPEND, NI_K_ATTN, NI_K_MERGE, NI_K_QKV, NI_K_COUNT = 0, 1, 2, 3, 4
 NI_W_F32, NI_W_F16, NI_W_Q8_0, NI_W_Q4_0 = 0, 1, 2, 3
 
 
+NI_F32, NI_F16, NI_BF16 = 0, 1, 2
+NI_ROTARY_PLAIN, NI_ROTARY_LINEAR, NI_ROTARY_NTK, NI_ROTARY_YARN = 0, 1, 2, 3
+NI_ROTARY_MAX_PAIRS = 128
+
+
 class ni_kv_opts(C.Structure):
     _fields_ = [
         ("n_layer", C.c_uint32),
@@ -57,6 +62,21 @@ class ni_row(C.Structure):
 
 class ni_work(C.Structure):
     _fields_ = [("seq", C.c_uint32), ("n_new", C.c_uint32), ("n_query", C.c_uint32)]
+
+
+class ni_rotary_opts(C.Structure):
+    _fields_ = [("base", C.c_double), ("rot_dim", C.c_uint32), ("interleaved", C.c_uint32), ("scaling", C.c_uint32),
+                ("orig_ctx", C.c_uint32), ("factor", C.c_double), ("beta_fast", C.c_double),
+                ("beta_slow", C.c_double), ("attn_scale", C.c_double)]
+
+
+class ni_rotary(C.Structure):
+    _fields_ = [("head_dim", C.c_uint32), ("rot_dim", C.c_uint32), ("interleaved", C.c_uint32),
+                ("scale", C.c_float), ("turns", C.c_uint64 * NI_ROTARY_MAX_PAIRS)]
+
+
+class ni_prefix(C.Structure):
+    _fields_ = [("seq", C.c_uint32), ("len", C.c_uint32), ("n_rows", C.c_uint32)]
 
 
 _lib = None
@@ -129,6 +149,21 @@ def _declare(L):
     L.ni_kv_decode_steps.restype = C.c_int
     L.ni_kv_decode_steps.argtypes = [_vp, C.POINTER(_u32), _u32, _u32, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64,
                                      _i64, _u32, _vp]
+    L.ni_rotary_init.restype = C.c_int
+    L.ni_rotary_init.argtypes = [C.POINTER(ni_rotary), _u32, C.POINTER(ni_rotary_opts)]
+    L.ni_rotary_apply.restype = C.c_int
+    L.ni_rotary_apply.argtypes = [C.POINTER(ni_rotary), _u32, _vp, _i64, _vp, _i64, _u32, _u32, _vp, _u32, _vp]
+    L.ni_kv_append_rotary.restype = C.c_int
+    L.ni_kv_append_rotary.argtypes = [_vp, C.c_int32, C.POINTER(ni_row), _u32, C.POINTER(ni_rotary), _vp, _vp, _vp, _i64,
+                                      _i64, _vp, _i64, _i64, _u32, _vp, _i64, _i64, _vp]
+    L.ni_kv_prefix_attention.restype = C.c_int
+    L.ni_kv_prefix_attention.argtypes = [_vp, C.c_int32, _vp, _i64, _i64, _u32, C.POINTER(ni_row), _u32,
+                                         C.POINTER(ni_prefix), _u32, _vp, _i64, _i64, _u32, _vp]
+    L.ni_verify_workspace.restype = C.c_size_t
+    L.ni_verify_workspace.argtypes = [_u32, _u32]
+    L.ni_verify_drafts.restype = C.c_int
+    L.ni_verify_drafts.argtypes = [_u32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _u32, _u32,
+                                   _u32, _vp, _vp, _i64, _vp, C.c_size_t, _vp]
     L.ni_kv_sync.restype = C.c_int
     L.ni_kv_sync.argtypes = [_vp, _vp]
     L.ni_kv_pools.restype = C.c_int

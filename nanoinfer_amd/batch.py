@@ -100,6 +100,33 @@ def _stream_ptr(stream) -> int:
     return int(torch.cuda.current_stream().cuda_stream)
 
 
+class _on:
+    """The device made current where it is not, and `stream` where one is
+    given, for what a call allocates and launches; gives the stream's handle."""
+
+    __slots__ = ("_scopes", "_ptr")
+
+    def __init__(self, device, stream):
+        torch = _torch()
+        scopes = []
+        if device is not None and torch.cuda.is_initialized() and \
+                (_get_device() if _get_device is not None else torch.cuda.current_device()) != device:
+            scopes.append(torch.cuda.device(device))
+        if stream is not None and hasattr(stream, "stream_id"):
+            scopes.append(torch.cuda.stream(stream))
+        self._scopes = scopes
+        self._ptr = stream
+
+    def __enter__(self):
+        for s in self._scopes:
+            s.__enter__()
+        return _stream_ptr(self._ptr)
+
+    def __exit__(self, *exc):
+        for s in reversed(self._scopes):
+            s.__exit__(*exc)
+
+
 def _fits(t, rows, c, device):
     """The row stride of a float32 tensor [>= rows, c] on the GPU `device` with
     unit stride in its last dimension, or None: the quick form of _f32_arg and
@@ -133,7 +160,7 @@ def _fits_wide(t, rows, c, device) -> bool:
     return False
 
 
-_no_rows, _no_work = _abi.ni_row * 0, _abi.ni_work * 0
+_no_rows, _no_work, _no_prefixes = _abi.ni_row * 0, _abi.ni_work * 0, _abi.ni_prefix * 0
 
 
 def _pointer(arr, empty, item):
@@ -281,6 +308,22 @@ class PagedKv:
 
     def _on_device(self, **tensors):
         _on_device(self.device, **tensors)
+
+    def _strides(self, t, name, layered, rows, c=None):
+        """(row stride, layer stride) of t: [n_layer, >= rows, c] or [>= rows, c]."""
+        c = self._c if c is None else c
+        if layered:
+            s = _fits_layers(t, rows, c, self._n_layer, self.device)
+        else:
+            s = _fits(t, rows, c, self.device)
+            s = None if s is None else (s, 0)
+        return self._f32(t, name, layered, rows, c) if s is None else s
+
+    def _query_heads(self, q) -> int:
+        torch = _torch()
+        if not isinstance(q, torch.Tensor) or q.dim() == 0 or q.shape[-1] == 0 or q.shape[-1] % self.opts.head_dim:
+            raise ValueError(f"q must hold whole heads of {self.opts.head_dim} in its last dimension")
+        return q.shape[-1] // self.opts.head_dim
 
     @property
     def max_blocks(self) -> int:
@@ -450,6 +493,77 @@ class PagedKv:
         (qrs, qls), (ors, ols) = qs, os_
         self._check(self._L.ni_paged_decode_attention(self._h, layer, q.data_ptr(), qrs, qls, rp, n, out.data_ptr(),
                                                       ors, ols, split_tokens, _stream_ptr(stream)))
+        return out
+
+    def append_rotary(self, rows, k, v, rotary, q=None, q_out=None, positions=None, layer: int = ALL_LAYERS,
+                      stream=None):
+        """:meth:`append` with k rotated on its way into the pages, and q (heads
+        of any number, ``[n_layer, n, heads * head_dim]`` or ``[n, ...]`` for one
+        layer) rotated alike to ``q_out``, which is returned (allocated if not
+        given; ``q_out=q`` rotates in place).  ``rotary`` is a
+        :class:`~nanoinfer_amd.Rotary`; ``positions`` (host integers, one a row)
+        default to the rows' own."""
+        torch = _torch()
+        arr, rp, n = _rows(rows)
+        layered = layer == ALL_LAYERS
+        ks, vs = self._strides(k, "k", layered, n), self._strides(v, "v", layered, n)
+        if ks != vs:
+            raise ValueError("k and v must share strides")
+        pos, pp = None, None
+        if positions is not None:
+            pos = np.asarray(positions)
+            if pos.size != n or (n and (pos.dtype.kind not in "iu" or pos.min() < 0 or pos.max() > 0xffffffff)):
+                raise ValueError(f"positions must be {n} integers in 0..2^32-1")
+            pos = np.ascontiguousarray(pos.reshape(-1), dtype=np.uint32)
+            pp = pos.ctypes.data
+        heads, qs, qos = 0, (0, 0), (0, 0)
+        if q is not None:
+            heads = self._query_heads(q)
+            cq = heads * self.opts.head_dim
+            qs = self._strides(q, "q", layered, n, cq)
+            if q_out is not None:
+                qos = self._strides(q_out, "q_out", layered, n, cq)
+        elif q_out is not None:
+            raise ValueError("q_out without q")
+        self._on_device(k=k, v=v, q=q, q_out=q_out)
+        with _on(self.device, stream) as s:
+            if q is not None and q_out is None:
+                q_out = torch.empty((self._n_layer, n, cq) if layered else (n, cq), dtype=torch.float32, device=q.device)
+                qos = (cq, n * cq if layered else 0)
+            self._check(self._L.ni_kv_append_rotary(
+                self._h, layer, rp, n, rotary.ref, pp, k.data_ptr(), v.data_ptr(), ks[0], ks[1],
+                None if q is None else q.data_ptr(), qs[0], qs[1], heads, None if q is None else q_out.data_ptr(),
+                qos[0], qos[1], s))
+        return q_out
+
+    def prefix_attention(self, q, rows, prefixes, out=None, layer: int = ALL_LAYERS, split_tokens: int = 0,
+                         stream=None):
+        """Paged attention behind shared prefixes: ``prefixes`` lists ``(seq,
+        length, n_rows)`` -- the next ``n_rows`` rows attend to the first
+        ``length`` positions of ``seq`` (0: to no prefix) and then causally to
+        their own sequences up to their positions, under one softmax.  A prefix
+        is read once for all its rows.  q and out hold any multiple of the
+        cache's heads a row; out is returned ([.., n, heads * head_dim],
+        allocated if not given; it may be q)."""
+        torch = _torch()
+        arr, rp, n = _rows(rows)
+        pre = np.asarray(prefixes, dtype=np.int64).reshape(-1, 3)
+        if pre.size and (pre.min() < 0 or pre.max() > 0xffffffff):
+            raise ValueError("prefixes must be (seq, length, n_rows) of numbers in 0..2^32-1")
+        pre = np.ascontiguousarray(pre, dtype=np.uint32)
+        layered = layer == ALL_LAYERS
+        heads = self._query_heads(q)
+        cq = heads * self.opts.head_dim
+        qs = self._strides(q, "q", layered, n, cq)
+        os_ = None if out is None else self._strides(out, "out", layered, n, cq)
+        self._on_device(q=q, out=out)
+        with _on(self.device, stream) as s:
+            if out is None:
+                out = torch.empty((self._n_layer, n, cq) if layered else (n, cq), dtype=torch.float32, device=q.device)
+                os_ = (cq, n * cq if layered else 0)
+            self._check(self._L.ni_kv_prefix_attention(
+                self._h, layer, q.data_ptr(), qs[0], qs[1], heads, rp, n, _pointer(pre, _no_prefixes, _abi.ni_prefix),
+                pre.shape[0], out.data_ptr(), os_[0], os_[1], split_tokens, s))
         return out
 
     def step(self, work, q, k, v, out=None, split_tokens: int = 0, stream=None):

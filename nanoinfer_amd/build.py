@@ -23,8 +23,10 @@ ARCH = "gfx950"
 DRIVERS_LIB = os.path.join(HERE, "libnanoinfer_drivers.so")
 DRIVE_EXE = os.path.join(HERE, "ni_drive")
 
-SOURCES = [os.path.join(CSRC, "kv_kernels.hip"), os.path.join(CSRC, "kv_host.cpp")]
-HEADERS = [os.path.join(CSRC, "kv_plan.h"), os.path.join(INCLUDE, "nanoinfer_kv.h")]
+SOURCES = [os.path.join(CSRC, f) for f in ("kv_kernels.hip", "rotary_kernels.hip", "prefix_kernels.hip",
+                                           "verify_kernels.hip", "kv_host.cpp", "ops_host.cpp")]
+HEADERS = [os.path.join(CSRC, f) for f in ("kv_plan.h", "kv_device.h", "ops_plan.h")] + \
+    [os.path.join(INCLUDE, "nanoinfer_kv.h")]
 DRIVER_SOURCES = [os.path.join(CSRC, "drivers.cpp")]
 DRIVER_HEADERS = [os.path.join(INCLUDE, "nanoinfer_drivers.h")]
 

@@ -336,22 +336,38 @@ int ni_spec_plan(ni_spec* s, const ni_work** work, uint32_t* n_work, const uint3
     return NI_OK;
 }
 
-// metal_spec.rs:146-163: accept a prefix of the drafts, truncate the rest.
-int ni_spec_commit(ni_spec* s, const uint32_t** accepted) {
-    if (!s) return NI_ERR_BAD_ARG;
-    if (!s->planned) return drive_fail(NI_ERR_BAD_ARG, "commit without a planned round");
+// metal_spec.rs:146-163: keep a prefix of the drafts (`accepted`, or drawn
+// where it is null), truncate the rest.
+static int spec_commit(ni_spec* s, const uint32_t* accepted) {
     s->planned = false;
     s->accepted.clear();
     for (size_t i = 0; i < s->seqs.size(); i++) {
-        const uint32_t acc = s->rng.range(0, s->k);
+        const uint32_t acc = accepted ? accepted[i] : s->rng.range(0, s->k);
         const uint32_t keep = s->tlen[i] + 1 + acc;
         if (int rc = ni_kv_truncate(s->kv, s->seqs[i], keep)) return rc;
         if (s->window && keep > s->base[i] + s->window)
             if (int rc = ni_kv_truncate(s->kv, s->seqs[i], s->base[i])) return rc;
         s->accepted.push_back(acc);
     }
+    return NI_OK;
+}
+
+int ni_spec_commit(ni_spec* s, const uint32_t** accepted) {
+    if (!s) return NI_ERR_BAD_ARG;
+    if (!s->planned) return drive_fail(NI_ERR_BAD_ARG, "commit without a planned round");
+    if (int rc = spec_commit(s, nullptr)) return rc;
     if (accepted) *accepted = s->accepted.data();
     return NI_OK;
+}
+
+int ni_spec_commit_accepted(ni_spec* s, const uint32_t* accepted) {
+    if (!s) return NI_ERR_BAD_ARG;
+    if (!s->planned) return drive_fail(NI_ERR_BAD_ARG, "commit without a planned round");
+    if (!accepted && !s->seqs.empty()) return drive_fail(NI_ERR_BAD_ARG, "accepted is NULL");
+    for (size_t i = 0; i < s->seqs.size(); i++)
+        if (accepted[i] > s->k)
+            return drive_fail(NI_ERR_BAD_ARG, "sequence %u: %u drafts accepted of %u", s->seqs[i], accepted[i], s->k);
+    return spec_commit(s, accepted);
 }
 
 }  // extern "C"

@@ -23,11 +23,13 @@
 #include <cstdio>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <vector>
 
 #include "kv_plan.h"
 #include "nanoinfer_kv.h"
+#include "ops_plan.h"
 
 using namespace ni;
 
@@ -132,6 +134,17 @@ struct Plan {
     }
 };
 
+// Work of one ni_kv_prefix_attention call, before serialisation.
+struct PrefixPlan {
+    std::vector<PrefixItem> items;
+    std::vector<PrefixMerge> merges;
+    std::vector<uint32_t> table;
+    uint64_t n_parts = 0;
+};
+// Query heads per cache head that call takes: a row's slots are numbered in 32
+// bits with room to spare.
+constexpr uint32_t kMaxQueryGroup = 1024;
+
 // Byte offsets of each part of a serialised plan.
 struct Offsets {
     size_t app, orphans, items, merges, pitems, pmerges, pseqs, table, order, porder, total;
@@ -184,6 +197,11 @@ struct ni_kv {
     // retired: launches enqueued before may still use it, so it is freed by
     // the next ni_kv_sync that finds its event complete (or ni_kv_destroy).
     std::vector<std::pair<float*, hipEvent_t>> partials_retired;
+    // A call captured into a graph took `partials`: replays use it whenever
+    // they run, so once outgrown it is kept until ni_kv_destroy.
+    bool partials_captured = false;
+    std::vector<float*> partials_kept;
+    bool capturing = false;  // the current call's stream is capturing (begin_call)
     // ni_kv_step_noalloc: this device's scratch array (null if its address
     // could not be found), and set for the duration of such a call.
     float* scratch = nullptr;
@@ -206,6 +224,9 @@ struct ni_kv {
 
     // scratch reused across calls
     Plan plan;
+    PrefixPlan prefix_plan;
+    std::vector<uint32_t> slot_mark;  // (page, slot) -> stamp of the last ni_kv_append_rotary that wrote it
+    uint32_t slot_stamp = 0;
     std::vector<uint8_t> blob;  // the serialised plan
     std::vector<QRow> qrows;
     std::vector<int64_t> seq_tab;     // seq -> offset in plan.table, -1 if absent
@@ -1022,7 +1043,10 @@ int ensure_partials(ni_kv* kv, size_t bytes, hipStream_t s, float** out) {
         return NI_OK;
     }
     *out = kv->partials;
-    if (bytes <= kv->partials_bytes) return NI_OK;
+    if (bytes <= kv->partials_bytes) {
+        kv->partials_captured |= kv->capturing;
+        return NI_OK;
+    }
     // Launches already enqueued may still use the old buffer: retire it
     // (no host wait here) rather than free it.  Every earlier call's work is
     // ordered before this point of `s` (begin_call), so an event recorded
@@ -1031,7 +1055,9 @@ int ensure_partials(ni_kv* kv, size_t bytes, hipStream_t s, float** out) {
     float* p = nullptr;
     hipError_t e = hipMalloc(reinterpret_cast<void**>(&p), cap);
     if (e != hipSuccess) return kv->hip_fail(e, "hipMalloc(partials)");
-    if (kv->partials) {
+    if (kv->partials && kv->partials_captured) {
+        kv->partials_kept.push_back(kv->partials);
+    } else if (kv->partials) {
         hipEvent_t ev = take_event(kv);
         if (!ev) {
             (void)hipFree(p);
@@ -1047,6 +1073,7 @@ int ensure_partials(ni_kv* kv, size_t bytes, hipStream_t s, float** out) {
     }
     kv->partials = p;
     kv->partials_bytes = cap;
+    kv->partials_captured = kv->capturing;
     *out = p;
     return NI_OK;
 }
@@ -1080,7 +1107,8 @@ int begin_call(ni_kv* kv, hipStream_t s) {
     hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
     hipError_t e = hipStreamIsCapturing(s, &cap);
     if (e != hipSuccess) return kv->hip_fail(e, "hipStreamIsCapturing");
-    if (cap != hipStreamCaptureStatusNone) return NI_OK;
+    kv->capturing = cap != hipStreamCaptureStatusNone;
+    if (kv->capturing) return NI_OK;
     if (kv->dirty && kv->dirty_stream != s) {
         e = hipEventRecord(kv->order, kv->dirty_stream);
         if (e != hipSuccess) return kv->hip_fail(e, "hipEventRecord(call order)");
@@ -1096,9 +1124,32 @@ int begin_call(ni_kv* kv, hipStream_t s) {
     return NI_OK;
 }
 
-// Serialise plan P into `blob` and make it reachable from `s`: inside the
-// launch arguments when it fits, else through a staging slot uploaded on the
-// handle's copy stream (`s` waits for the upload).
+// Make a serialised plan reachable from `s`: inside the launch arguments when
+// it fits, else through a staging slot uploaded on the handle's copy stream
+// (`s` waits for the upload).
+int place_blob(ni_kv* kv, const std::vector<uint8_t>& blob, hipStream_t s, PlanRef* ref) {
+    *ref = PlanRef{};
+    if (blob.size() <= kInlinePlanBytes) {
+        ref->inl = blob.data();
+        ref->inl_bytes = (uint32_t)blob.size();
+        return NI_OK;
+    }
+    StagingSlot* sl = nullptr;
+    int rc = acquire_slot(kv, blob.size(), &sl);
+    if (rc) return rc;
+    memcpy(sl->host, blob.data(), blob.size());
+    hipError_t e = hipMemcpyAsync(sl->dev, sl->host, blob.size(), hipMemcpyHostToDevice, kv->copy_stream);
+    if (e != hipSuccess) return kv->hip_fail(e, "hipMemcpyAsync(plan)");
+    e = hipEventRecord(sl->uploaded, kv->copy_stream);
+    if (e != hipSuccess) return kv->hip_fail(e, "hipEventRecord(upload)");
+    e = hipStreamWaitEvent(s, sl->uploaded, 0);
+    if (e != hipSuccess) return kv->hip_fail(e, "hipStreamWaitEvent(upload)");
+    ref->dev = sl->dev;
+    ref->slot = sl;
+    return NI_OK;
+}
+
+// Serialise plan P into `blob` and make it reachable from `s` (place_blob).
 int place_plan(ni_kv* kv, const Plan& P, std::vector<uint8_t>& blob, hipStream_t s, Offsets* off, PlanRef* ref) {
     if (int rc = begin_call(kv, s)) return rc;
     *off = layout(P);
@@ -1129,24 +1180,7 @@ int place_plan(ni_kv* kv, const Plan& P, std::vector<uint8_t>& blob, hipStream_t
         ref->inl_bytes = (uint32_t)off->total;
         return NI_OK;
     }
-    if (off->total <= kInlinePlanBytes) {
-        ref->inl = blob.data();
-        ref->inl_bytes = (uint32_t)off->total;
-        return NI_OK;
-    }
-    StagingSlot* sl = nullptr;
-    int rc = acquire_slot(kv, off->total, &sl);
-    if (rc) return rc;
-    memcpy(sl->host, blob.data(), off->total);
-    hipError_t e = hipMemcpyAsync(sl->dev, sl->host, off->total, hipMemcpyHostToDevice, kv->copy_stream);
-    if (e != hipSuccess) return kv->hip_fail(e, "hipMemcpyAsync(plan)");
-    e = hipEventRecord(sl->uploaded, kv->copy_stream);
-    if (e != hipSuccess) return kv->hip_fail(e, "hipEventRecord(upload)");
-    e = hipStreamWaitEvent(s, sl->uploaded, 0);
-    if (e != hipSuccess) return kv->hip_fail(e, "hipStreamWaitEvent(upload)");
-    ref->dev = sl->dev;
-    ref->slot = sl;
-    return NI_OK;
+    return place_blob(kv, blob, s, ref);
 }
 
 // After the launches that read a staged plan: mark its slot busy until they end.
@@ -1299,12 +1333,162 @@ int run_plan(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const float* k, const f
     return rc ? rc : rc2;
 }
 
+// The handle's device current for the scope of a call.
+struct DeviceScope {
+    int before = -1, now;
+    explicit DeviceScope(int device) : now(device) {
+        if (hipGetDevice(&before) != hipSuccess) before = -1;
+        if (before != now) (void)hipSetDevice(now);
+    }
+    ~DeviceScope() {
+        if (before >= 0 && before != now) (void)hipSetDevice(before);
+    }
+};
+
+// Cut a ni_kv_prefix_attention call into items.  Queries travel as slots (the
+// `group` query heads of a row that read one cache head), kSlotTile to an
+// item.  A prefix is read by its rows' slots together, each sequence's own
+// keys by its rows' (consecutive rows of one sequence at consecutive
+// positions form a run); both in partitions of the same number of keys.
+int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32_t n_prefix, uint32_t group,
+                uint32_t n_lay, uint32_t split_tokens, PrefixPlan& P) {
+    P.items.clear();
+    P.merges.clear();
+    P.table.clear();
+    P.n_parts = 0;
+    struct Run {
+        uint32_t seq, row0, pos0, n;
+        uint32_t prefix;  // index into prefixes
+    };
+    std::vector<Run> runs;
+    for (uint32_t i = 0, r = 0; i < n_prefix; i++)
+        for (uint32_t e = r + prefixes[i].n_rows; r < e; r++) {
+            if (!runs.empty()) {
+                Run& u = runs.back();
+                if (u.prefix == i && u.seq == rows[r].seq && u.pos0 + u.n == rows[r].pos) {
+                    u.n++;
+                    continue;
+                }
+            }
+            runs.push_back({rows[r].seq, r, rows[r].pos, 1, i});
+        }
+    // Page lists, one per sequence: as many pages as any of its runs reads.
+    struct Scratch {  // seq_need and seq_tab as they were, whatever happens
+        ni_kv* kv;
+        const ni_prefix* prefixes;
+        uint32_t n_prefix;
+        const std::vector<Run>& runs;
+        void clear(uint32_t seq) {
+            kv->seq_need[seq] = 0;
+            kv->seq_tab[seq] = -1;
+        }
+        ~Scratch() {
+            for (uint32_t i = 0; i < n_prefix; i++)
+                if (prefixes[i].n_rows && prefixes[i].len) clear(prefixes[i].seq);
+            for (const Run& u : runs) clear(u.seq);
+        }
+    } scratch{kv, prefixes, n_prefix, runs};
+    auto need = [&](uint32_t seq, uint32_t keys) {
+        kv->seq_need[seq] = std::max(kv->seq_need[seq], (keys + kPage - 1) / kPage);
+    };
+    for (uint32_t i = 0; i < n_prefix; i++)
+        if (prefixes[i].n_rows && prefixes[i].len) need(prefixes[i].seq, prefixes[i].len);
+    for (const Run& u : runs) need(u.seq, u.pos0 + u.n);
+    auto tab_of = [&](uint32_t seq) {
+        if (kv->seq_tab[seq] < 0) {
+            kv->seq_tab[seq] = (int64_t)P.table.size();
+            const auto& pg = kv->pages[seq];
+            P.table.insert(P.table.end(), pg.begin(), pg.begin() + kv->seq_need[seq]);
+        }
+        return (uint32_t)kv->seq_tab[seq];
+    };
+    auto tiles = [](uint64_t slots) { return (slots + kSlotTile - 1) / kSlotTile; };
+    // Keys per partition: enough workgroups to give every CU four, so that no
+    // CU idles at the end, but 128 keys (two pages a wave) at least, below
+    // which a workgroup is mostly its own start and end.
+    uint64_t keys = 0;
+    for (uint32_t i = 0; i < n_prefix; i++)
+        if (prefixes[i].n_rows) keys += tiles((uint64_t)prefixes[i].n_rows * group) * prefixes[i].len;
+    for (const Run& u : runs) keys += tiles((uint64_t)u.n * group) * (u.pos0 + u.n);
+    uint64_t part = split_tokens;
+    if (!part) {
+        part = keys * n_lay * kv->o.n_head / (4ull * device_cus());
+        part = std::min<uint64_t>(std::max<uint64_t>(align_up(part, 4 * kPage), 128), 16384);
+    }
+    std::vector<uint64_t> pre0(n_prefix, 0);
+    for (uint32_t i = 0, r = 0; i < n_prefix; r += prefixes[i].n_rows, i++) {
+        const ni_prefix& p = prefixes[i];
+        if (!p.n_rows || !p.len) continue;
+        const uint64_t slots = (uint64_t)p.n_rows * group;
+        const uint32_t tab = tab_of(p.seq);
+        pre0[i] = P.n_parts;
+        for (uint64_t k0 = 0; k0 < p.len; k0 += part) {
+            for (uint64_t s0 = 0; s0 < slots; s0 += kSlotTile)
+                P.items.push_back({tab, r, (uint32_t)s0, (uint32_t)std::min<uint64_t>(kSlotTile, slots - s0), kWholePos,
+                                   (uint32_t)k0, (uint32_t)std::min<uint64_t>(p.len, k0 + part),
+                                   (uint32_t)(P.n_parts + s0)});
+            P.n_parts += slots;
+        }
+    }
+    for (uint32_t i = 0, r = 0, u0 = 0; i < n_prefix; r += prefixes[i].n_rows, i++) {
+        const ni_prefix& p = prefixes[i];
+        const uint64_t p_slots = (uint64_t)p.n_rows * group;
+        const uint32_t n_pre = (uint32_t)((p.len + part - 1) / part);
+        for (; u0 < runs.size() && runs[u0].prefix == i; u0++) {
+            const Run& u = runs[u0];
+            const uint64_t slots = (uint64_t)u.n * group, n_own = (u.pos0 + u.n + part - 1) / part;
+            const bool whole = n_pre == 0 && n_own == 1;
+            const uint32_t tab = tab_of(u.seq);
+            for (uint64_t j = 0; j < n_own; j++)
+                for (uint64_t s0 = 0; s0 < slots; s0 += kSlotTile) {
+                    const uint32_t ns = (uint32_t)std::min<uint64_t>(kSlotTile, slots - s0);
+                    const uint64_t end = u.pos0 + (s0 + ns - 1) / group + 1;  // of the tile's last row
+                    if (j * part >= end) continue;
+                    P.items.push_back({tab, u.row0, (uint32_t)s0, ns, u.pos0, (uint32_t)(j * part),
+                                       (uint32_t)std::min<uint64_t>(end, (j + 1) * part),
+                                       whole ? kNoSlot : (uint32_t)(P.n_parts + j * slots + s0)});
+                }
+            if (whole) continue;
+            for (uint32_t t = 0; t < u.n; t++)
+                P.merges.push_back({u.row0 + t, (uint32_t)(P.n_parts + (uint64_t)t * group), (uint32_t)slots,
+                                    (uint32_t)((u.pos0 + t) / part + 1),
+                                    (uint32_t)(pre0[i] + (uint64_t)(u.row0 + t - r) * group), (uint32_t)p_slots, n_pre,
+                                    0});
+            P.n_parts += n_own * slots;
+        }
+    }
+    // Longest first, so that the launch does not end on a long item.
+    std::stable_sort(P.items.begin(), P.items.end(), [](const PrefixItem& x, const PrefixItem& y) {
+        return x.kv_end - x.kv_begin > y.kv_end - y.kv_begin;
+    });
+    if (P.n_parts >= (1ull << 31) || (uint64_t)P.items.size() * n_lay * kv->o.n_head >= (1ull << 31) ||
+        (uint64_t)P.merges.size() * n_lay * kv->o.n_head * group >= (1ull << 31))
+        return kv->fail(NI_ERR_BAD_ARG, "rows * layers * heads too large for one call");
+    return NI_OK;
+}
+
+// Heads one thread rotates with the cosines it computes: four once that still
+// gives every CU 2048 threads.
+uint32_t rotary_heads_per(uint64_t threads_per_head, uint32_t heads) {
+    return threads_per_head * heads >= 4ull * 2048 * device_cus() ? 4u : 1u;
+}
+
 void reset_plan(ni_kv* kv) {
     kv->plan.clear();
     kv->qrows.clear();
 }
 
 }  // namespace
+
+int ni::call_error(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_create_error = buf;
+    return code;
+}
 
 static int enqueue_step(ni_kv* kv, const ni_work* work, uint32_t n_work, const float* q, const float* k,
                         const float* v, int64_t row_stride, int64_t layer_stride, float* out, int64_t out_row_stride,
@@ -1437,6 +1621,7 @@ void ni_kv_destroy(ni_kv* kv) {
         for (hipEvent_t e : kv->ev_pool) (void)hipEventDestroy(e);
         if (kv->order) (void)hipEventDestroy(kv->order);
         if (kv->partials) (void)hipFree(kv->partials);
+        for (float* p : kv->partials_kept) (void)hipFree(p);
         for (auto& pr : kv->partials_retired) {
             (void)hipFree(pr.first);
             (void)hipEventDestroy(pr.second);
@@ -1746,6 +1931,212 @@ int ni_paged_decode_attention(ni_kv* kv, int32_t layer, const float* q, int64_t 
     if (int rc = plan_attention(kv, split_tokens, n_lay)) return rc;
     return run_plan(kv, layer0, n_lay, nullptr, nullptr, 0, 0, q, q_row_stride, all ? q_layer_stride : 0, out,
                     out_row_stride, all ? out_layer_stride : 0, (hipStream_t)stream);
+}
+
+// The head checks ni_kv_append_rotary and ni_kv_prefix_attention share.
+static int check_call(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, uint32_t* layer0, uint32_t* n_lay) {
+    if (kv->host_only) return kv->fail(NI_ERR_NO_DEVICE, "host-only handle has no device pools");
+    if (int rc = layer_range(kv, layer, layer0, n_lay)) return rc;
+    if (n == 0) return NI_OK;
+    if (!rows) return kv->fail(NI_ERR_BAD_ARG, "rows is NULL");
+    if (n > kv->o.max_rows) return kv->fail(NI_ERR_TOO_MANY_ROWS, "%u rows > max_rows %u", n, kv->o.max_rows);
+    return NI_OK;
+}
+
+// A plan too long for the launch arguments is uploaded on another stream,
+// which a capture cannot record.
+static int check_capture(ni_kv* kv, size_t plan_bytes) {
+    if (kv->capturing && plan_bytes > kInlinePlanBytes)
+        return kv->fail(NI_ERR_BAD_ARG,
+                        "the call's plan is %zu bytes; under stream capture it travels with the launch, at most %u "
+                        "(fewer rows or shorter contexts per call)",
+                        plan_bytes, kInlinePlanBytes);
+    return NI_OK;
+}
+
+int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, const ni_rotary* rotary,
+                        const uint32_t* positions, const float* k, const float* v, int64_t row_stride,
+                        int64_t layer_stride, const float* q, int64_t q_row_stride, int64_t q_layer_stride,
+                        uint32_t n_q_head, float* q_out, int64_t q_out_row_stride, int64_t q_out_layer_stride,
+                        ni_stream stream) try {
+    if (!kv) return NI_ERR_BAD_ARG;
+    uint32_t layer0, n_lay;
+    if (int rc = check_call(kv, layer, rows, n, &layer0, &n_lay)) return rc;
+    if (n == 0) return NI_OK;
+    const bool all = layer == NI_ALL_LAYERS;
+    const uint32_t D = kv->o.head_dim;
+    if (int rc = check_f32_operand(kv, "k", k, row_stride, layer_stride, all)) return rc;
+    if (int rc = check_f32_operand(kv, "v", v, row_stride, layer_stride, all)) return rc;
+    if (n_q_head) {
+        if (int rc = check_f32_operand(kv, "q", q, q_row_stride, q_layer_stride, all)) return rc;
+        if (int rc = check_f32_operand(kv, "q_out", q_out, q_out_row_stride, q_out_layer_stride, all)) return rc;
+        if ((n > 1 && (uint64_t)q_out_row_stride < (uint64_t)n_q_head * D) ||
+            (all && n_lay > 1 && (uint64_t)q_out_layer_stride < (uint64_t)n_q_head * D))
+            return kv->fail(NI_ERR_BAD_ARG, "q_out's rows overlap: strides must be at least %llu",
+                            (unsigned long long)n_q_head * D);
+    }
+    if (!rotary) return kv->fail(NI_ERR_BAD_ARG, "rotary is NULL");
+    if (rotary->head_dim != D)
+        return kv->fail(NI_ERR_BAD_ARG, "the rotation is for heads of %u, the cache holds heads of %u",
+                        rotary->head_dim, D);
+    if (rotary->rot_dim == 0 || rotary->rot_dim > D || rotary->rot_dim % 8 != 0)
+        return kv->fail(NI_ERR_BAD_ARG, "rot_dim %u: the cache rotates a multiple of 8, at most %u", rotary->rot_dim, D);
+    if ((uint64_t)n_lay * n * (n_q_head + 2ull * kv->o.n_head) * (D / 8) >= (1ull << 37))
+        return kv->fail(NI_ERR_BAD_ARG, "n_layer * rows * heads too large");
+    // Two rows at one position would race on its slot.
+    kv->slot_mark.resize((size_t)kv->o.kv_pages * kPage, 0);
+    if (++kv->slot_stamp == 0) {
+        std::fill(kv->slot_mark.begin(), kv->slot_mark.end(), 0);
+        kv->slot_stamp = 1;
+    }
+    std::vector<uint8_t>& blob = kv->blob;
+    blob.resize(align_up((size_t)n * sizeof(AppendEntry), kAlign));
+    AppendEntry* entries = reinterpret_cast<AppendEntry*>(blob.data());
+    for (uint32_t i = 0; i < n; i++) {
+        if (int rc = check_row(kv, rows[i])) return rc;
+        const ni_row& r = rows[i];
+        const uint32_t page = kv->pages[r.seq][r.pos / kPage], slot = r.pos % kPage;
+        uint32_t& mark = kv->slot_mark[(size_t)page * kPage + slot];
+        if (mark == kv->slot_stamp)
+            return kv->fail(NI_ERR_BAD_ARG, "sequence %u: position %u appears twice", r.seq, r.pos);
+        mark = kv->slot_stamp;
+        entries[i] = {i, page, slot, positions ? positions[i] : r.pos};
+    }
+    DeviceScope device(kv->device);
+    const hipStream_t s = (hipStream_t)stream;
+    if (int rc = begin_call(kv, s)) return rc;
+    if (int rc = check_capture(kv, blob.size())) return rc;
+    PlanRef ref;
+    if (int rc = place_blob(kv, blob, s, &ref)) return rc;
+    AppendRotaryLaunch a{};
+    a.pool = kv->geom();
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_out = q_out;
+    a.q_row_stride = q_row_stride;
+    a.q_layer_stride = all ? q_layer_stride : 0;
+    a.q_out_row_stride = q_out_row_stride;
+    a.q_out_layer_stride = all ? q_out_layer_stride : 0;
+    a.row_stride = row_stride;
+    a.layer_stride = all ? layer_stride : 0;
+    a.plan = ref.dev;
+    a.n_rows = n;
+    a.layer0 = layer0;
+    a.n_lay = n_lay;
+    a.n_q_head = n_q_head;
+    a.heads_per = rotary_heads_per((uint64_t)n_lay * n * (D / 8), n_q_head + 2 * kv->o.n_head);
+    CacheRotary r{};
+    r.rot_dim = rotary->rot_dim;
+    r.interleaved = rotary->interleaved;
+    r.scale = rotary->scale;
+    std::copy(rotary->turns, rotary->turns + r.rot_dim / 2, r.turns);
+    hipError_t e;
+    {
+        ProfileScope ps(kv, NI_K_APPEND);
+        e = launch_append_rotary(a, r, ref.inl, ref.inl_bytes, s, ps.t);
+    }
+    const int rc2 = release_plan(kv, ref, s);
+    return e != hipSuccess ? kv->hip_fail(e, "rotary append kernel") : rc2;
+} catch (const std::bad_alloc&) {
+    return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
+}
+
+int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_row_stride, int64_t q_layer_stride,
+                           uint32_t n_q_head, const ni_row* rows, uint32_t n, const ni_prefix* prefixes,
+                           uint32_t n_prefix, float* out, int64_t out_row_stride, int64_t out_layer_stride,
+                           uint32_t split_tokens, ni_stream stream) try {
+    if (!kv) return NI_ERR_BAD_ARG;
+    uint32_t layer0, n_lay;
+    if (int rc = check_call(kv, layer, rows, n, &layer0, &n_lay)) return rc;
+    const uint32_t D = kv->o.head_dim, H = kv->o.n_head;
+    if (n_q_head == 0 || n_q_head % H != 0 || n_q_head / H > kMaxQueryGroup)
+        return kv->fail(NI_ERR_BAD_ARG, "n_q_head %u must be a multiple (1..%u) of the cache's %u heads", n_q_head,
+                        kMaxQueryGroup, H);
+    if (split_tokens % kPage != 0)
+        return kv->fail(NI_ERR_BAD_ARG, "split_tokens %u must be a multiple of %u", split_tokens, kPage);
+    if (n_prefix && !prefixes) return kv->fail(NI_ERR_BAD_ARG, "prefixes is NULL");
+    uint64_t covered = 0;
+    for (uint32_t i = 0; i < n_prefix; i++) covered += prefixes[i].n_rows;
+    if (covered != n)
+        return kv->fail(NI_ERR_BAD_ARG, "the prefixes cover %llu rows, the call has %u", (unsigned long long)covered, n);
+    if (n == 0) return NI_OK;
+    const bool all = layer == NI_ALL_LAYERS;
+    if (int rc = check_f32_operand(kv, "q", q, q_row_stride, q_layer_stride, all)) return rc;
+    if (int rc = check_f32_operand(kv, "out", out, out_row_stride, out_layer_stride, all)) return rc;
+    if ((n > 1 && (uint64_t)out_row_stride < (uint64_t)n_q_head * D) ||
+        (all && n_lay > 1 && (uint64_t)out_layer_stride < (uint64_t)n_q_head * D))
+        return kv->fail(NI_ERR_BAD_ARG, "out's rows overlap: strides must be at least %llu",
+                        (unsigned long long)n_q_head * D);
+    for (uint32_t i = 0, r = 0; i < n_prefix; i++) {
+        const ni_prefix& p = prefixes[i];
+        if (p.len && p.n_rows)
+            if (int rc = check_row(kv, {p.seq, p.len - 1})) return rc;
+        for (uint32_t e = r + p.n_rows; r < e; r++) {
+            if (int rc = check_row(kv, rows[r])) return rc;
+            if (p.len && rows[r].seq == p.seq)
+                return kv->fail(NI_ERR_BAD_ARG, "row %u: sequence %u is its own prefix", r, p.seq);
+        }
+    }
+    PrefixPlan& P = kv->prefix_plan;
+    if (int rc = plan_prefix(kv, rows, prefixes, n_prefix, n_q_head / H, n_lay, split_tokens, P)) return rc;
+    std::vector<uint8_t>& blob = kv->blob;
+    const size_t off_merges = align_up(P.items.size() * sizeof(PrefixItem), kAlign);
+    const size_t off_table = align_up(off_merges + P.merges.size() * sizeof(PrefixMerge), kAlign);
+    blob.resize(align_up(off_table + P.table.size() * sizeof(uint32_t), kAlign));
+    memcpy(blob.data(), P.items.data(), P.items.size() * sizeof(PrefixItem));
+    if (!P.merges.empty()) memcpy(blob.data() + off_merges, P.merges.data(), P.merges.size() * sizeof(PrefixMerge));
+    memcpy(blob.data() + off_table, P.table.data(), P.table.size() * sizeof(uint32_t));
+
+    DeviceScope device(kv->device);
+    const hipStream_t s = (hipStream_t)stream;
+    if (int rc = begin_call(kv, s)) return rc;
+    if (int rc = check_capture(kv, blob.size())) return rc;
+    const size_t parts = (size_t)P.n_parts * n_lay * H;
+    const size_t o_bytes = align_up(parts * D * sizeof(float), kAlign), bytes = o_bytes + parts * 2 * sizeof(float);
+    float* partials = nullptr;
+    if (parts) {
+        if (kv->capturing && bytes > kv->partials_bytes)
+            return kv->fail(NI_ERR_BAD_ARG,
+                            "the call needs %zu bytes of partials, the handle holds %zu: make it once outside the "
+                            "capture",
+                            bytes, kv->partials_bytes);
+        if (int rc = ensure_partials(kv, bytes, s, &partials)) return rc;
+    }
+    PlanRef ref;
+    if (int rc = place_blob(kv, blob, s, &ref)) return rc;
+    PrefixLaunch a{};
+    a.pool = kv->geom();
+    a.q = q;
+    a.out = out;
+    a.q_row_stride = q_row_stride;
+    a.q_layer_stride = all ? q_layer_stride : 0;
+    a.out_row_stride = out_row_stride;
+    a.out_layer_stride = all ? out_layer_stride : 0;
+    a.plan = ref.dev;
+    a.off_merges = (uint32_t)off_merges;
+    a.off_table = (uint32_t)off_table;
+    a.part_o = partials;
+    a.part_ml = partials ? partials + o_bytes / sizeof(float) : nullptr;
+    a.n_items = (uint32_t)P.items.size();
+    a.n_merges = (uint32_t)P.merges.size();
+    a.layer0 = layer0;
+    a.n_lay = n_lay;
+    a.group = n_q_head / H;
+    a.qscale = (float)(1.4426950408889634 / std::sqrt((double)D));
+    hipError_t e;
+    {
+        ProfileScope ps(kv, NI_K_ATTN);
+        e = launch_prefix_attention(a, ref.inl, ref.inl_bytes, s, ps.t);
+    }
+    if (e == hipSuccess && a.n_merges) {
+        ProfileScope ps(kv, NI_K_MERGE);
+        e = launch_prefix_merge(a, ref.inl, ref.inl_bytes, s, ps.t);
+    }
+    const int rc2 = release_plan(kv, ref, s);
+    return e != hipSuccess ? kv->hip_fail(e, "shared-prefix attention kernel") : rc2;
+} catch (const std::bad_alloc&) {
+    return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
 }
 
 int ni_kv_step(ni_kv* kv, const ni_work* work, uint32_t n_work, const float* q, const float* k, const float* v,

@@ -41,33 +41,11 @@
 #include <type_traits>
 #include <vector>
 
+#include "kv_device.h"
 #include "kv_plan.h"
 
 namespace ni {
 namespace {
-
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-
-// f32 -> f16 bits with round to nearest even (the hardware conversion under
-// the default rounding mode keeps f16 subnormals and overflows to inf), NaN
-// made canonical sign|0x7e00 -- the rules of crates/core/src/quant.rs:25-54.
-__device__ __forceinline__ uint32_t f16_bits(float x) {
-    uint32_t h = __builtin_bit_cast(uint16_t, static_cast<_Float16>(x));
-    const uint32_t b = __float_as_uint(x);
-    if ((b & 0x7fffffffu) > 0x7f800000u) h = ((b >> 16) & 0x8000u) | 0x7e00u;
-    return h;
-}
-
-__device__ __forceinline__ uint4 pack8(const float4 a, const float4 b) {
-    uint4 r;
-    r.x = f16_bits(a.x) | (f16_bits(a.y) << 16);
-    r.y = f16_bits(a.z) | (f16_bits(a.w) << 16);
-    r.z = f16_bits(b.x) | (f16_bits(b.y) << 16);
-    r.w = f16_bits(b.z) | (f16_bits(b.w) << 16);
-    return r;
-}
-
-__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Cross-lane move inside a row of 16 lanes (DPP; no LDS traffic).
 template <int CTRL>
@@ -98,10 +76,6 @@ __device__ __forceinline__ void merge_state(float& m, float& l, float (&o)[N], f
     m = mn;
 }
 
-// Running max starts at a finite sentinel so that exp2(m - m_new) of two
-// empty states is 1 (not NaN); masked scores are -inf and weigh 0.
-constexpr float kMinScore = -1e30f;
-
 // The states (m, l, o) of W waves for one output of a row, wave w's at red +
 // w * stride: weighed by exp2(m - M) and added pairwise, as a tree (a chain
 // over 16 waves rounds each sum 15 times, the tree 4).
@@ -127,22 +101,6 @@ __device__ __forceinline__ void merge_waves(const float* red, uint32_t stride, u
         }
     L = l[0];
     O = o[0];
-}
-
-// A plan passed with the kernel arguments (N > 0) or left in device memory
-// (N == 0: the launch struct's `plan` pointer).  Arguments live in the
-// read-only kernarg segment; the kernels index it in place.
-template <int N>
-struct PlanArg {
-    uint8_t b[N > 0 ? N : 4];
-};
-
-template <int N>
-__device__ __forceinline__ const uint8_t* plan_base(const PlanArg<N>& pa, const uint8_t* dev) {
-    if constexpr (N > 0)
-        return pa.b;
-    else
-        return dev;
 }
 
 // ------------------------------------------------------------------ append
@@ -185,15 +143,6 @@ __device__ __forceinline__ void append_chunk(const PoolGeom& pool, const float* 
 // q = clamp(rint(x * (1 / scale)), -127, 127) (inverse 0 when amax is 0);
 // both divisions correctly rounded, rint to nearest even.  Inputs must be
 // finite.
-
-// A (page, head) block of a Q8 pool as bytes: [16][D] int8, then 16 scales.
-__device__ __forceinline__ uint8_t* q8_block(const PoolGeom& pool, bool is_v, uint64_t off_halves) {
-    return reinterpret_cast<uint8_t*>((is_v ? pool.v : pool.k) + off_halves);
-}
-
-__device__ __forceinline__ uint32_t q8_byte(float x, float inv) {
-    return (uint32_t)(int32_t)fminf(fmaxf(rintf(x * inv), -127.f), 127.f) & 0xffu;
-}
 
 // Quantise 8 values of one (position, head) held by a lane whose aligned
 // group of g = D/8 neighbouring lanes holds the rest; stores the 8 bytes at
@@ -306,8 +255,6 @@ __global__ __launch_bounds__(256) void f32_to_f16_kernel(const float* __restrict
     if (i < n) out[i] = static_cast<uint16_t>(f16_bits(in[i]));
 }
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 // ------------------------------------------------------- bandwidth probe
 
 // The memory system's streaming rate, beside which the hot path's roofline
@@ -366,10 +313,6 @@ __global__ __launch_bounds__(256) void stream_kernel(const u32x4* __restrict__ s
 constexpr int kWaves = 4;         // waves per workgroup sharing one item's pages
 constexpr int kPagesPerIter = 2;  // pages per wave per loop iteration (head_dim 64)
 constexpr int kPagesD128 = 2;     // the same at head_dim 128
-
-// K/V loads are non-temporal: each byte is streamed once per step (156 -> 140
-// us per config-3 launch against ordinary loads).
-__device__ __forceinline__ u32x4 load16(const u32x4* p) { return __builtin_nontemporal_load(p); }
 
 // The (item, layer, head) unit workgroup b of an attention launch runs:
 // unit b itself (item-major, b = (item * n_lay + layer) * n_head + head), or
@@ -1481,27 +1424,6 @@ __global__ __launch_bounds__(64 * kQkvParts) void qkv_small_kernel(const QkvLaun
 
 // ------------------------------------------------ attention, several queries
 
-typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
-typedef float float4_t __attribute__((ext_vector_type(4)));
-
-typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-
-// Four signed int8 values (bytes 0..3 of w) as f16, exactly and bit for bit
-// as static_cast<_Float16>: the f16 bit pattern 0x6400 | (b ^ 0x80) is 1024 +
-// (b + 128), and subtracting 1152 leaves b (operands and result exactly
-// representable, so the subtraction does not round).  Two values per byte
-// permute (a byte to the low byte of each 16-bit half, zeros above), XOR and
-// packed f16 subtract, against a bit extract and two conversions per value.
-__device__ __forceinline__ half4_t i8x4_f16(uint32_t w) {
-    const uint32_t lo = __builtin_amdgcn_perm(w, w, 0x0c010c00u) ^ 0x64806480u;  // bytes 0, 1
-    const uint32_t hi = __builtin_amdgcn_perm(w, w, 0x0c030c02u) ^ 0x64806480u;  // bytes 2, 3
-    const half2_t k1152 = {static_cast<_Float16>(1152.f), static_cast<_Float16>(1152.f)};
-    const half2_t a = __builtin_bit_cast(half2_t, lo) - k1152;
-    const half2_t b = __builtin_bit_cast(half2_t, hi) - k1152;
-    return half4_t{a[0], a[1], b[0], b[1]};
-}
-
 // f32 -> f16 hi plus the residual scaled by 2^11 (kept in the normal range
 // of f16, where the residual itself would often be subnormal): x ~= hi +
 // lo * 2^-11 to ~2^-22 relative.  Products of hi and of lo are accumulated
@@ -1518,49 +1440,6 @@ __device__ __forceinline__ void split_f16(float x, _Float16& hi, _Float16& lo) {
     hi = static_cast<_Float16>(x);
     lo = static_cast<_Float16>((x - static_cast<float>(hi)) * kLoScale);
 }
-// The same split for two softmax weights already scaled up (x in [0,
-// 2^15]), packed: hi = f16(x), lo = f16(x - hi) unscaled, ~2^-22 relative
-// where lo is normal and within 2^-25 absolute where it is subnormal.  One
-// packed convert and one mixed-precision FMA per weight (x * 1 - hi, hi
-// read as the f16 half of the packed register) instead of convert, convert
-// back, subtract and convert; the same bits (checked on gfx950 against the
-// plain formula over 2^21 pairs from 2^-40 to 2^16, zeros included).
-__device__ __forceinline__ void split_w16x2(float x0, float x1, uint32_t& hi, uint32_t& lo) {
-    const half2_t h = {static_cast<_Float16>(x0), static_cast<_Float16>(x1)};
-    hi = __builtin_bit_cast(uint32_t, h);
-    asm("v_fma_mixlo_f16 %0, %1, 1.0, -%2 op_sel_hi:[0,0,1]" : "=v"(lo) : "v"(x0), "v"(hi));
-    asm("v_fma_mixhi_f16 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(lo) : "v"(x1), "v"(hi));
-}
-// Max and sum over lanes l, l ^ 16, l ^ 32, l ^ 48 (the four lanes holding
-// one query column of an MFMA 16x16 output): v_permlane16_swap and
-// v_permlane32_swap of a value with itself leave the two halves of each
-// lane pair in the two results, so combining them is the pair's max or sum
-// in both lanes.  No LDS round trip; the same bits as __shfl_xor.
-__device__ __forceinline__ float rows4_max(float v) {
-    u32x2_t s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
-}
-__device__ __forceinline__ float rows4_sum(float v) {
-    u32x2_t s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(s[0]) + __uint_as_float(s[1]);
-}
-// Position, in 16-byte chunks, of chunk q of row `key` in an LDS tile of
-// CH-chunk rows: row major, the chunk index XORed with a permutation of the
-// row's 256-byte window index, so that the 16 lanes reading one chunk of 16
-// consecutive rows (the K operand) and the 32 lanes reading 4 dims of 8 rows
-// for the transposed V operand each hit distinct banks.
-template <int CH>
-__device__ __forceinline__ uint32_t tile_chunk(uint32_t key, uint32_t q) {
-    const uint32_t i = (key * CH / 16) % CH;
-    const uint32_t sw = ((i & (CH / 2 - 1)) << 1) | (i / (CH / 2));
-    return key * CH + (q ^ sw);
-}
-typedef __fp16 v4fp16_t __attribute__((__vector_size__(4 * sizeof(__fp16))));
-#define NI_LDS(p) ((__attribute__((address_space(3))) void*)(p))
 // p in [0, 1] enters PV scaled by 2^14, so that p down to ~4e-9 is a normal
 // f16.
 constexpr float kPScale = 16384.f, kPUnscale = 1.f / kPScale;
@@ -1973,25 +1852,6 @@ constexpr int kPrefillPages = 2;
 constexpr int kPrefillStages = 3;
 static_assert(kPrefillStages == 3 || kPrefillStages == 4, "ring of 3 or 4 tiles");
 
-// 16 bytes per lane from g to LDS at the wave-uniform dst + 16 * lane
-// (global_load_lds_dwordx4, M0 = dst's LDS address).  Written as assembly
-// so that the compiler does not add a wait for every DMA in flight before
-// each LDS read it cannot prove disjoint from them: the caller waits
-// (vmcnt) and synchronises itself.  The "memory" clobber and dst as an
-// operand tell the compiler that LDS may change here.  The s_nop is the one
-// wait state CDNA requires between a scalar write of M0 and an LDS-DMA load
-// reading it; the compiler inserts it for its own code but cannot see into
-// the asm.
-__device__ __forceinline__ void lds_dma16(const void* g, void* dst) {
-    const uint32_t m0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)NI_LDS(dst));
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(g), "s"(m0) : "memory", "m0");
-}
-// The same from a wave-uniform base plus a per-lane 32-bit byte offset (the
-// SADDR form: no 64-bit address per lane), to the LDS byte address lds.
-__device__ __forceinline__ void lds_dma16_sbase(const void* base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(lds)
-                 : "memory", "m0");
-}
 // The prefill kernel keeps its exponent reference m until some query's max
 // exceeds it by more than kRefSlack (log2 units): weights are then up to
 // 2^kRefSlack, so p enters PV scaled by 2^(15 - kRefSlack) (at most 2^15 in
@@ -2855,7 +2715,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 6
     const uint32_t kend_w = min(it.kv_end, it.pos0 + r0 + nqw);  // keys this wave needs end here
     const uint32_t kfull_w = min(it.kv_end, it.pos0 + r0 + 1);   // keys below this: visible to all its queries
 
-
     // Tile DMA: thread t copies LDS chunk t of the tile's K and of its V (row
     // t / CH, logical chunk (t % CH) ^ sw, tile_chunk's inverse); a row past
     // the item's end copies row 0 of its page (a key of this item).
@@ -3189,39 +3048,6 @@ __global__ __launch_bounds__(kMergeThreads) void attn_merge_kernel(const AttnLau
 // PV through the 32-key product, 154 registers and 3 waves per SIMD: config 5
 // -0.9%, Q8 -3.3%).
 constexpr int kMfmaPages = 1;
-
-// One kernel launch; with timing events the dispatch packet itself records
-// the kernel's start and end (no separate event commands in the stream).
-template <typename K, typename... Args>
-hipError_t go(K kern, uint64_t blocks, uint32_t threads, hipStream_t s, const LaunchTiming& t, const Args&... args) {
-    hipExtLaunchKernelGGL(kern, dim3((uint32_t)blocks), dim3(threads), 0, s, t.start, t.stop, 0, args...);
-    return hipGetLastError();
-}
-
-// Launch `kern<INL>` with the plan inline (kInlinePlanTiny, kInlinePlanSmall
-// or kInlinePlanBytes of arguments, the smallest that holds it) or through the
-// device pointer in the launch struct.
-template <typename L, typename Fn>
-hipError_t with_plan(const L& a, const void* inline_plan, uint32_t inline_bytes, Fn&& launch) {
-    if (inline_plan) {
-        if (inline_bytes > kInlinePlanBytes) return hipErrorInvalidValue;
-        if (inline_bytes <= kInlinePlanTiny) {
-            PlanArg<kInlinePlanTiny> pa;
-            memcpy(pa.b, inline_plan, inline_bytes);
-            return launch(pa);
-        }
-        if (inline_bytes <= kInlinePlanSmall) {
-            PlanArg<kInlinePlanSmall> pa;
-            memcpy(pa.b, inline_plan, inline_bytes);
-            return launch(pa);
-        }
-        PlanArg<kInlinePlanBytes> pa;
-        memcpy(pa.b, inline_plan, inline_bytes);
-        return launch(pa);
-    }
-    return launch(PlanArg<0>{});
-}
-
 
 template <int D, int NQ>
 hipError_t attn_launch_t(const AttnLaunch& a, const void* ip, uint32_t ib, hipStream_t s, const LaunchTiming& t) {

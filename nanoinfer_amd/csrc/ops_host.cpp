@@ -1,0 +1,177 @@
+// ops_host.cpp -- C ABI of the operators that need no cache handle: rotary
+// positions over contiguous rows (ni_rotary_*) and the verification of drafted
+// tokens (ni_verify_*).  Checks come before anything touches the device.
+#include <hip/hip_runtime_api.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "nanoinfer_kv.h"
+#include "ops_plan.h"
+
+using namespace ni;
+
+namespace {
+
+bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+uint32_t type_bytes(uint32_t dtype) { return dtype == NI_F32 ? 4u : 2u; }
+
+}  // namespace
+
+extern "C" {
+
+int ni_rotary_init(ni_rotary* r, uint32_t head_dim, const ni_rotary_opts* o) {
+    if (!r || !o) return call_error(NI_ERR_BAD_ARG, "rotary and opts must not be NULL");
+    const uint32_t rot = o->rot_dim ? o->rot_dim : head_dim;
+    if (head_dim == 0 || head_dim % 2 != 0 || head_dim > 2 * NI_ROTARY_MAX_PAIRS)
+        return call_error(NI_ERR_BAD_ARG, "head_dim %u must be even, 2..%u", head_dim, 2 * NI_ROTARY_MAX_PAIRS);
+    if (rot % 2 != 0 || rot > head_dim)
+        return call_error(NI_ERR_BAD_ARG, "rot_dim %u must be even and at most head_dim %u", rot, head_dim);
+    if (o->interleaved > 1) return call_error(NI_ERR_BAD_ARG, "interleaved must be 0 or 1");
+    if (!(o->base > 0) || !std::isfinite(o->base)) return call_error(NI_ERR_BAD_ARG, "base must be positive and finite");
+    if (o->scaling > NI_ROTARY_YARN) return call_error(NI_ERR_BAD_ARG, "unknown scaling %u", o->scaling);
+    if (o->scaling != NI_ROTARY_PLAIN && (!(o->factor >= 1) || !std::isfinite(o->factor)))
+        return call_error(NI_ERR_BAD_ARG, "factor must be finite and at least 1");
+    if (o->attn_scale < 0 || !std::isfinite(o->attn_scale))
+        return call_error(NI_ERR_BAD_ARG, "attn_scale must be finite and not negative");
+    const double s = o->scaling == NI_ROTARY_PLAIN ? 1. : o->factor;
+    double base = o->base, lo = 0., hi = 0., scale = 1.;
+    if (o->scaling == NI_ROTARY_NTK) {
+        if (rot <= 2) return call_error(NI_ERR_BAD_ARG, "ntk scaling needs a rot_dim above 2");
+        base *= std::pow(s, (double)rot / (rot - 2));
+    } else if (o->scaling == NI_ROTARY_YARN) {
+        const double fast = o->beta_fast > 0 ? o->beta_fast : 32., slow = o->beta_slow > 0 ? o->beta_slow : 1.;
+        if (!(base > 1)) return call_error(NI_ERR_BAD_ARG, "yarn scaling needs a base above 1");
+        if (o->orig_ctx == 0) return call_error(NI_ERR_BAD_ARG, "yarn scaling needs orig_ctx");
+        if (!(fast >= slow)) return call_error(NI_ERR_BAD_ARG, "beta_fast must be at least beta_slow");
+        // The pair that makes `turns` turns over the original context.
+        auto pair = [&](double turns) {
+            return rot * std::log(o->orig_ctx / (turns * 2 * M_PI)) / (2 * std::log(base));
+        };
+        lo = std::max(std::floor(pair(fast)), 0.);
+        hi = std::min(std::ceil(pair(slow)), (double)rot - 1);
+        if (s > 1) scale = 0.1 * std::log(s) + 1;
+    }
+    *r = ni_rotary{};
+    r->head_dim = head_dim;
+    r->rot_dim = rot;
+    r->interleaved = o->interleaved;
+    r->scale = (float)(o->attn_scale > 0 ? o->attn_scale : scale);
+    for (uint32_t i = 0; i < rot / 2; i++) {
+        double f = std::pow(base, -2. * i / rot);
+        if (o->scaling == NI_ROTARY_LINEAR) f /= s;
+        if (o->scaling == NI_ROTARY_YARN) {
+            // Pairs that turn often keep their frequency, slow ones take the
+            // stretched one, those between a mixture.
+            const double ramp = std::min(std::max((i - lo) / std::max(hi - lo, 0.001), 0.), 1.);
+            f = f / s * ramp + f * (1 - ramp);
+        }
+        const long double turns = (long double)f / (2 * M_PIl);
+        r->turns[i] = (uint64_t)std::ldexp(turns - std::floor(turns), 64);  // 2^-64 of a turn: below 2^64
+    }
+    return NI_OK;
+}
+
+int ni_rotary_apply(const ni_rotary* r, uint32_t dtype, const void* x, int64_t x_row_stride, void* out,
+                    int64_t out_row_stride, uint32_t n, uint32_t n_head, const int32_t* positions, uint32_t pos0,
+                    ni_stream stream) {
+    if (!r) return call_error(NI_ERR_BAD_ARG, "rotary is NULL");
+    if (r->head_dim == 0 || r->head_dim % 2 != 0 || r->head_dim > 2 * NI_ROTARY_MAX_PAIRS || r->rot_dim == 0 ||
+        r->rot_dim % 2 != 0 || r->rot_dim > r->head_dim || r->interleaved > 1)
+        return call_error(NI_ERR_BAD_ARG, "rotary was not filled by ni_rotary_init");
+    if (dtype > NI_BF16) return call_error(NI_ERR_BAD_ARG, "unknown type %u", dtype);
+    if (n == 0 || n_head == 0) return NI_OK;
+    const int64_t unit = 16 / type_bytes(dtype);
+    const int64_t width = (int64_t)n_head * r->head_dim;
+    if (!x || !out) return call_error(NI_ERR_BAD_ARG, "%s is NULL", x ? "out" : "x");
+    if (!aligned(x, type_bytes(dtype)) || !aligned(out, type_bytes(dtype)) || x_row_stride < 0 || out_row_stride < 0)
+        return call_error(NI_ERR_BAD_ARG, "x and out must be aligned to their type with non-negative row strides");
+    if (n > 1 && out_row_stride < width)
+        return call_error(NI_ERR_BAD_ARG, "out's rows overlap: the row stride must be at least %lld", (long long)width);
+    if (!aligned(positions, 4)) return call_error(NI_ERR_BAD_ARG, "positions must be 4-byte aligned");
+    if ((uint64_t)n * width >= (1ull << 38)) return call_error(NI_ERR_BAD_ARG, "n * n_head * head_dim too large");
+    RotaryLaunch a{};
+    a.x = x;
+    a.out = out;
+    a.positions = positions;
+    a.x_stride = x_row_stride;
+    a.out_stride = out_row_stride;
+    a.pos0 = pos0;
+    a.n_rows = n;
+    a.n_head = n_head;
+    a.dtype = dtype;
+    a.wide = r->head_dim % 8 == 0 && r->rot_dim % 8 == 0 && aligned(x, 16) && aligned(out, 16) &&
+             x_row_stride % unit == 0 && out_row_stride % unit == 0;
+    // Four heads to a thread once that still gives every CU 2048 threads.
+    a.heads_per = (uint64_t)n * width / 8 >= 4ull * 2048 * device_cus() ? 4u : 1u;
+    const hipError_t e = launch_rotary(a, *r, (hipStream_t)stream);
+    if (e != hipSuccess) return call_error(NI_ERR_HIP, "rotary launch failed: %s", hipGetErrorString(e));
+    return NI_OK;
+}
+
+size_t ni_verify_workspace(uint32_t n_seq, uint32_t vocab) {
+    return (size_t)n_seq * ((vocab + (uint64_t)kVerifyChunk - 1) / kVerifyChunk) * 2 * sizeof(double);
+}
+
+int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stride, int64_t target_row_stride,
+                     const void* draft, int64_t draft_seq_stride, int64_t draft_row_stride, const int32_t* drafted,
+                     int64_t drafted_stride, const int32_t* n_drafts, const float* accept_u, int64_t accept_stride,
+                     const float* sample_u, uint32_t n_seq, uint32_t n_draft, uint32_t vocab, int32_t* accepted,
+                     int32_t* tokens, int64_t tokens_stride, void* workspace, size_t workspace_bytes, ni_stream stream) {
+    if (dtype > NI_BF16) return call_error(NI_ERR_BAD_ARG, "unknown type %u", dtype);
+    if (n_seq == 0) return NI_OK;
+    if (vocab == 0 || vocab > (1u << 30)) return call_error(NI_ERR_BAD_ARG, "vocab %u must be 1..2^30", vocab);
+    if (n_seq > 65535) return call_error(NI_ERR_BAD_ARG, "%u sequences: at most 65535 a call", n_seq);
+    if (n_draft > (1u << 20)) return call_error(NI_ERR_BAD_ARG, "n_draft %u too large", n_draft);
+    const struct {
+        const char* name;
+        const void* p;
+        bool needed;
+        uintptr_t align;
+        int64_t stride;
+    } args[] = {{"target", target, true, type_bytes(dtype), std::min(target_seq_stride, target_row_stride)},
+                {"draft", draft, false, type_bytes(dtype), draft ? std::min(draft_seq_stride, draft_row_stride) : 0},
+                {"drafted", drafted, n_draft > 0, 4, n_draft ? drafted_stride : 0},
+                {"n_drafts", n_drafts, false, 4, 0},
+                {"accept_u", accept_u, n_draft > 0, 4, n_draft ? accept_stride : 0},
+                {"sample_u", sample_u, true, 4, 0},
+                {"accepted", accepted, true, 4, 0},
+                {"tokens", tokens, true, 4, tokens_stride}};
+    for (const auto& x : args) {
+        if (x.needed && !x.p) return call_error(NI_ERR_BAD_ARG, "%s is NULL", x.name);
+        if (!aligned(x.p, x.align)) return call_error(NI_ERR_BAD_ARG, "%s is not aligned to its type", x.name);
+        if (x.stride < 0) return call_error(NI_ERR_BAD_ARG, "%s must have non-negative strides", x.name);
+    }
+    if (n_seq > 1 && tokens_stride < (int64_t)n_draft + 1)
+        return call_error(NI_ERR_BAD_ARG, "tokens' rows overlap: the stride must be at least %u", n_draft + 1);
+    const size_t need = ni_verify_workspace(n_seq, vocab);
+    if (!workspace || !aligned(workspace, 8) || workspace_bytes < need)
+        return call_error(NI_ERR_BAD_ARG, "workspace must be %zu bytes, 8-byte aligned", need);
+    VerifyLaunch a{};
+    a.target = target;
+    a.target_seq_stride = target_seq_stride;
+    a.target_row_stride = target_row_stride;
+    a.draft = draft;
+    a.draft_seq_stride = draft_seq_stride;
+    a.draft_row_stride = draft_row_stride;
+    a.drafted = drafted;
+    a.drafted_stride = drafted_stride;
+    a.n_drafts = n_drafts;
+    a.accept_u = accept_u;
+    a.accept_stride = accept_stride;
+    a.sample_u = sample_u;
+    a.accepted = accepted;
+    a.tokens = tokens;
+    a.tokens_stride = tokens_stride;
+    a.sums = static_cast<double*>(workspace);
+    a.n_seq = n_seq;
+    a.n_draft = n_draft;
+    a.vocab = vocab;
+    a.dtype = dtype;
+    const hipError_t e = launch_verify(a, (hipStream_t)stream);
+    if (e != hipSuccess) return call_error(NI_ERR_HIP, "verification launch failed: %s", hipGetErrorString(e));
+    return NI_OK;
+}
+
+}  // extern "C"

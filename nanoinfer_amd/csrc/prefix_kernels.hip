@@ -1,0 +1,384 @@
+// prefix_kernels.hip -- gfx950 kernels of attention behind shared prefixes
+// (ni_kv_prefix_attention): every row attends to the keys of its group's
+// prefix, held once in the cache, and to its own sequence's.
+//
+//   prefix_attn_kernel   16 slots (query heads of rows that read the same
+//                        cache head) over a run of keys
+//   prefix_merge_kernel  each slot's partial softmax states joined
+//
+// A prefix's keys leave memory once per 16 slots instead of once per row, and
+// each product of the matrix cores serves all of them.
+#include "kv_device.h"
+#include "ops_plan.h"
+
+namespace ni {
+namespace {
+
+constexpr int kPW = 4;               // waves of a workgroup: each takes every fourth page of the item
+constexpr int kMergeWaves = 4;       // slots a merge workgroup joins
+constexpr float kPScale = 16384.f;   // weights enter PV times 2^14: down to 4e-9 they are normal f16
+constexpr float kPUnscale = 1.f / kPScale;
+
+// One (item, layer, head): S^T = K Q^T (16 keys x 16 slots; q in f16 hi + lo
+// parts), the online softmax down its columns, O^T += V^T P^T (p in hi + lo
+// parts).  Lane l holds slot l % 16 and keys, then dims, 4 (l / 16) .. + 3.
+// Pages go to LDS row major and come back as operands, V through the
+// transposing read.  The four waves' states are joined through LDS.
+template <int D, int INL, bool Q8>
+__global__ __launch_bounds__(64 * kPW) void prefix_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
+    constexpr int QC = D / 32;       // 32-dim chunks of QK
+    constexpr int VC = D / 16;       // 16-dim chunks of PV
+    constexpr int CH = D / 8;        // 16-byte chunks of an f16 row
+    constexpr int LD = Q8 ? D / 64 : D / 32;  // 16-byte loads a lane makes of a page's K, and of its V
+    constexpr size_t kTile = (size_t)kPage * D * 2;
+    constexpr size_t kRed = (size_t)kPW * kSlotTile * (D + 2) * 4;
+    constexpr size_t kLds = 2 * kPW * kTile > kRed ? 2 * kPW * kTile : kRed;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
+    auto& red = *reinterpret_cast<float(*)[kPW][kSlotTile][D + 2]>(lds);
+
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t H = a.pool.n_head, lh = a.n_lay * H;
+    const uint8_t* plan = plan_base(pa, a.plan);
+    const uint32_t item_i = blockIdx.x / lh;
+    const uint32_t rem = blockIdx.x - item_i * lh;
+    const uint32_t lay = rem / H, head = rem - lay * H;
+    const PrefixItem it = reinterpret_cast<const PrefixItem*>(plan + a.off_items)[item_i];
+    const int col = lane & 15, rg = lane >> 4;
+    _Float16* const kt = reinterpret_cast<_Float16*>(lds + wave * 2 * kTile);
+    _Float16* const vt = kt + kPage * D;
+
+    const uint64_t off = (uint64_t)(a.layer0 + lay) * a.pool.layer_halves + (uint64_t)head * a.pool.head_halves;
+    const uint32_t* __restrict__ tab = reinterpret_cast<const uint32_t*>(plan + a.off_table) + it.tab;
+    const uint32_t pg_end = (it.kv_end + kPage - 1) / kPage;
+
+    struct Regs {
+        u32x4 k[LD], v[LD];
+        float4 ks, vs;  // Q8: the scales of keys 4 rg .. + 3
+    };
+    auto load = [&](uint32_t pg, Regs& r) {
+        const uint64_t at = off + (uint64_t)tab[pg] * a.pool.page_halves;
+        const u32x4* kp = reinterpret_cast<const u32x4*>(a.pool.k + at) + lane;
+        const u32x4* vp = reinterpret_cast<const u32x4*>(a.pool.v + at) + lane;
+#pragma unroll
+        for (int i = 0; i < LD; i++) r.k[i] = load16(kp + 64 * i);
+#pragma unroll
+        for (int i = 0; i < LD; i++) r.v[i] = load16(vp + 64 * i);
+        if constexpr (Q8) {
+            r.ks = *reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(a.pool.k + at) + kPage * D + 16 * rg);
+            r.vs = *reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(a.pool.v + at) + kPage * D + 16 * rg);
+        }
+    };
+    Regs cur;
+    uint32_t pg = it.kv_begin / kPage + wave;
+    if (pg < pg_end) load(pg, cur);
+
+    const bool has = col < (int)it.ns;
+    const uint32_t slot = it.slot0 + (has ? (uint32_t)col : 0u);
+    const uint32_t row = slot / a.group, g = slot - row * a.group;
+    const uint32_t qpos = min(it.pos0 + row, kWholePos);
+    const uint32_t first_pos = min(it.pos0 + it.slot0 / a.group, kWholePos);  // of the item's first slot
+    half8_t qh[QC], ql[QC];
+    {
+        const float* qb = a.q + (int64_t)lay * a.q_layer_stride + (int64_t)(it.row0 + row) * a.q_row_stride +
+                          (head * a.group + g) * D + 8 * rg;
+#pragma unroll
+        for (int c = 0; c < QC; c++) {
+            const float4 x0 = reinterpret_cast<const float4*>(qb + c * 32)[0];
+            const float4 x1 = reinterpret_cast<const float4*>(qb + c * 32)[1];
+            const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                float y0 = has ? x[e] * a.qscale : 0.f, y1 = has ? x[e + 1] * a.qscale : 0.f;
+                asm("" : "+v"(y0), "+v"(y1));  // the f32 products, as the split's residual sees them
+                uint32_t h, l;
+                split_w16x2(y0, y1, h, l);
+                const half2_t hh = __builtin_bit_cast(half2_t, h), ll = __builtin_bit_cast(half2_t, l);
+                qh[c][e] = hh[0];
+                qh[c][e + 1] = hh[1];
+                ql[c][e] = ll[0];
+                ql[c][e + 1] = ll[1];
+            }
+        }
+    }
+    float m = kMinScore, lsum = 0.f;
+    float4_t o[VC];
+#pragma unroll
+    for (int c = 0; c < VC; c++) o[c] = float4_t{0.f, 0.f, 0.f, 0.f};
+    // Q8: weights enter PV times scale / vref, so that no f16 overflows: vref
+    // starts at 1 and follows the largest value scale past it.
+    float vref = 1.f, vinv = 1.f;
+
+    for (; pg < pg_end; pg += kPW) {
+        Regs nxt;
+        if (pg + kPW < pg_end) load(pg + kPW, nxt);
+        // Rows past kv_end enter as zeros: whatever the page holds there may
+        // not reach a product, not even with weight 0.
+#pragma unroll
+        for (int i = 0; i < LD; i++) {
+            if constexpr (Q8) {  // 16 values: chunks 2q, 2q + 1 of the row
+                const uint32_t key = i * (1024 / D) + lane / (D / 16), q = 2 * (lane % (D / 16));
+                const bool in = pg * kPage + key < it.kv_end;
+                const u32x4 kq = in ? cur.k[i] : u32x4{0, 0, 0, 0}, vq = in ? cur.v[i] : u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    *reinterpret_cast<half8_t*>(kt + tile_chunk<CH>(key, q + x) * 8) =
+                        __builtin_shufflevector(i8x4_f16(kq[2 * x]), i8x4_f16(kq[2 * x + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+                    *reinterpret_cast<half8_t*>(vt + tile_chunk<CH>(key, q + x) * 8) =
+                        __builtin_shufflevector(i8x4_f16(vq[2 * x]), i8x4_f16(vq[2 * x + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+                }
+            } else {
+                const uint32_t key = i * (512 / D) + lane / CH, q = lane % CH;
+                const bool in = pg * kPage + key < it.kv_end;
+                *reinterpret_cast<u32x4*>(kt + tile_chunk<CH>(key, q) * 8) = in ? cur.k[i] : u32x4{0, 0, 0, 0};
+                *reinterpret_cast<u32x4*>(vt + tile_chunk<CH>(key, q) * 8) = in ? cur.v[i] : u32x4{0, 0, 0, 0};
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        // An infinity or NaN among the values that only the later of the item's
+        // rows see: 0 times it would reach the earlier rows.
+        bool stray = false;
+        if constexpr (!Q8) {
+            if (pg * kPage + kPage - 1 > first_pos) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int i = 0; i < LD; i++) {
+                    const uint32_t key = pg * kPage + i * (512 / D) + lane / CH;
+                    if (key > first_pos && key < it.kv_end) {
+#pragma unroll
+                        for (int w = 0; w < 4; w++)
+                            top |= (uint32_t)((cur.v[i][w] & 0x7c00u) == 0x7c00u) |
+                                   (uint32_t)((cur.v[i][w] & 0x7c000000u) == 0x7c000000u);
+                    }
+                }
+                stray = __any(top != 0);
+            }
+        }
+        float4_t st = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < QC; c++) {
+            const half8_t kh = *reinterpret_cast<const half8_t*>(kt + tile_chunk<CH>(col, 4 * c + rg) * 8);
+            st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[c], st, 0, 0, 0);
+            st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[c], st, 0, 0, 0);
+        }
+        float s[4], mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t key = pg * kPage + 4 * rg + j;
+            float x = st[j];
+            if constexpr (Q8) x *= cur.ks[j];
+            s[j] = key < it.kv_end && key <= qpos ? x : -INFINITY;
+            mx = fmaxf(mx, s[j]);
+        }
+        mx = rows4_max(mx);
+        const float mn = fmaxf(m, mx);
+        const float alpha = fast_exp2(m - mn);
+        float oalpha = alpha;
+        m = mn;
+        float vs[4];
+        if constexpr (Q8) {
+            float vm = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                vs[j] = pg * kPage + 4 * rg + j < it.kv_end ? cur.vs[j] : 0.f;
+                vm = fmaxf(vm, vs[j]);
+            }
+            if (__any(vm > vref)) {
+                vm = fmaxf(rows4_max(vm), vref);
+                oalpha *= vref / vm;
+                vref = vm;
+                vinv = 1.f / vm;
+            }
+        }
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) p[j] = fast_exp2(s[j] - mn) * kPScale;
+        lsum = lsum * alpha + ((p[0] + p[1]) + (p[2] + p[3]));
+        if constexpr (Q8) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) p[j] *= vs[j] * vinv;
+        }
+        uint32_t h0, l0, h1, l1;
+        split_w16x2(p[0], p[1], h0, l0);
+        split_w16x2(p[2], p[3], h1, l1);
+        const half4_t ph = __builtin_bit_cast(half4_t, u32x2_t{h0, h1});
+        const half4_t pl = __builtin_bit_cast(half4_t, u32x2_t{l0, l1});
+        if (__any(oalpha != 1.f)) {
+#pragma unroll
+            for (int c = 0; c < VC; c++) o[c] *= oalpha;
+        }
+        auto pv = [&](int c, float4_t acc) {
+            const int t = (lane >> 2) & 3, av = lane & 3;
+            const _Float16* vp = vt + tile_chunk<CH>(4 * rg + t, 2 * c + (av >> 1)) * 8 + (av & 1) * 4;
+            const half4_t v4 = __builtin_bit_cast(
+                half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) v4fp16_t*)(vp)));
+            acc = __builtin_amdgcn_mfma_f32_16x16x16f16(v4, pl, acc, 0, 0, 0);
+            return __builtin_amdgcn_mfma_f32_16x16x16f16(v4, ph, acc, 0, 0, 0);
+        };
+        if (!stray) {
+#pragma unroll
+            for (int c = 0; c < VC; c++) o[c] = pv(c, o[c]);
+        } else {
+            // Row by row, each with the values past its position as zeros, the
+            // sums kept by the row's own slots alone.
+            for (uint32_t r = it.slot0 / a.group; r <= (it.slot0 + it.ns - 1) / a.group; r++) {
+#pragma unroll
+                for (int i = 0; i < LD; i++) {
+                    const uint32_t key = i * (512 / D) + lane / CH, q = lane % CH;
+                    const bool in = pg * kPage + key < it.kv_end && pg * kPage + key <= it.pos0 + r;
+                    *reinterpret_cast<u32x4*>(vt + tile_chunk<CH>(key, q) * 8) = in ? cur.v[i] : u32x4{0, 0, 0, 0};
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+                for (int c = 0; c < VC; c++) {
+                    const float4_t sum = pv(c, float4_t{0.f, 0.f, 0.f, 0.f});
+                    if (row == r) o[c] += sum;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if (pg + kPW < pg_end) cur = nxt;
+    }
+    lsum = rows4_sum(lsum);
+    __syncthreads();  // the tiles' LDS becomes `red`
+    if (has) {
+        if (rg == 0) {
+            red[wave][col][0] = m;
+            red[wave][col][1] = lsum * kPUnscale;
+        }
+#pragma unroll
+        for (int c = 0; c < VC; c++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) red[wave][col][2 + c * 16 + 4 * rg + j] = o[c][j] * (kPUnscale * vref);
+    }
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < it.ns * D; t += 64 * kPW) {
+        const uint32_t sl = t / D, d = t - sl * D;
+        float M = red[0][sl][0];
+#pragma unroll
+        for (int w = 1; w < kPW; w++) M = fmaxf(M, red[w][sl][0]);
+        float L = 0.f, O = 0.f;
+#pragma unroll
+        for (int w = 0; w < kPW; w++) {
+            const float wt = fast_exp2(red[w][sl][0] - M);
+            L += red[w][sl][1] * wt;
+            O += red[w][sl][2 + d] * wt;
+        }
+        if (it.part0 == kNoSlot) {
+            const uint32_t r = (it.slot0 + sl) / a.group, gg = it.slot0 + sl - r * a.group;
+            a.out[(int64_t)lay * a.out_layer_stride + (int64_t)(it.row0 + r) * a.out_row_stride +
+                  (head * a.group + gg) * D + d] = O / L;
+        } else {
+            const uint64_t part = ((uint64_t)(it.part0 + sl) * a.n_lay + lay) * H + head;
+            a.part_o[part * D + d] = O;
+            if (d == 0) {
+                a.part_ml[2 * part] = M;
+                a.part_ml[2 * part + 1] = L;
+            }
+        }
+    }
+}
+
+// One wave per (row, layer, query head): its partials' states weighed by
+// exp2(m - M) and added; lane l holds dims l, l + 64.
+template <int D, int INL>
+__global__ __launch_bounds__(64 * kMergeWaves) void prefix_merge_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
+    constexpr int N = D / 64;
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t H = a.pool.n_head, hq = H * a.group;
+    const uint64_t unit = (uint64_t)blockIdx.x * kMergeWaves + (threadIdx.x >> 6);
+    const uint64_t per = (uint64_t)a.n_lay * hq;
+    if (unit >= per * a.n_merges) return;
+    const uint32_t mi = (uint32_t)(unit / per);
+    const uint32_t rem = (uint32_t)(unit - (uint64_t)mi * per);
+    const uint32_t lay = rem / hq, qhead = rem - lay * hq;
+    const uint32_t head = qhead / a.group, g = qhead - head * a.group;
+    const PrefixMerge me = reinterpret_cast<const PrefixMerge*>(plan_base(pa, a.plan) + a.off_merges)[mi];
+    auto part_of = [&](uint32_t i) {
+        const uint32_t idx = i < me.n_own ? me.own0 + i * me.own_stride : me.pre0 + (i - me.n_own) * me.pre_stride;
+        return ((uint64_t)(idx + g) * a.n_lay + lay) * H + head;
+    };
+    const uint32_t n = me.n_own + me.n_pre;
+    float M = kMinScore, L = 0.f, O[N] = {};
+    for (uint32_t i0 = 0; i0 < n; i0 += 64) {  // 64 partials' (m, l) at a time, one a lane
+        const uint32_t cnt = min(64u, n - i0);
+        float m = kMinScore, l = 0.f;
+        if (lane < cnt) {
+            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * part_of(i0 + lane));
+            m = ml.x;
+            l = ml.y;
+        }
+        float mx = m;
+        for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+        const float mn = fmaxf(M, mx);
+        const float alpha = fast_exp2(M - mn);
+        M = mn;
+        const float w = fast_exp2(m - mn);
+        float ls = l * w;
+        for (int off = 32; off > 0; off >>= 1) ls += __shfl_xor(ls, off);
+        L = L * alpha + ls;
+#pragma unroll
+        for (int e = 0; e < N; e++) O[e] *= alpha;
+        constexpr int B = 8;  // partials in flight; past the last it is read again and weighs nothing
+        for (uint32_t i = 0; i < cnt; i += B) {
+            float x[B][N];
+#pragma unroll
+            for (int j = 0; j < B; j++) {
+                const float* p = a.part_o + part_of(i0 + min(i + j, cnt - 1)) * D + lane;
+#pragma unroll
+                for (int e = 0; e < N; e++) x[j][e] = p[64 * e];
+            }
+#pragma unroll
+            for (int j = 0; j < B; j++) {
+                const float wi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), (int)min(i + j, 63u)));
+#pragma unroll
+                for (int e = 0; e < N; e++)
+                    if (i + j < cnt) O[e] += x[j][e] * wi;
+            }
+        }
+    }
+    float* dst = a.out + (int64_t)lay * a.out_layer_stride + (int64_t)me.row * a.out_row_stride + qhead * D + lane;
+#pragma unroll
+    for (int e = 0; e < N; e++) dst[64 * e] = O[e] / L;
+}
+
+template <int D, bool Q8>
+hipError_t attn_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s, const LaunchTiming& t) {
+    return with_plan(a, ip, ib, [&](auto pa) {
+        constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
+        return go(prefix_attn_kernel<D, INL, Q8>, (uint64_t)a.n_items * a.n_lay * a.pool.n_head, 64 * kPW, s, t, a, pa);
+    });
+}
+
+}  // namespace
+
+hipError_t launch_prefix_attention(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s,
+                                   const LaunchTiming& t) {
+    if (a.pool.head_dim == 64) return a.pool.q8 ? attn_t<64, true>(a, ip, ib, s, t) : attn_t<64, false>(a, ip, ib, s, t);
+    if (a.pool.head_dim == 128)
+        return a.pool.q8 ? attn_t<128, true>(a, ip, ib, s, t) : attn_t<128, false>(a, ip, ib, s, t);
+    return hipErrorInvalidValue;
+}
+
+hipError_t launch_prefix_merge(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s,
+                               const LaunchTiming& t) {
+    const uint64_t units = (uint64_t)a.n_merges * a.n_lay * a.pool.n_head * a.group;
+    if (units == 0) return hipSuccess;
+    return with_plan(a, ip, ib, [&](auto pa) {
+        constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
+        const uint64_t blocks = (units + kMergeWaves - 1) / kMergeWaves;
+        if (a.pool.head_dim == 64) return go(prefix_merge_kernel<64, INL>, blocks, 64 * kMergeWaves, s, t, a, pa);
+        return go(prefix_merge_kernel<128, INL>, blocks, 64 * kMergeWaves, s, t, a, pa);
+    });
+}
+
+}  // namespace ni

@@ -87,6 +87,7 @@ def lib():
     L.ni_spec_destroy.restype = None
     L.ni_spec_plan.argtypes = [_vp, C.POINTER(C.POINTER(_abi.ni_work)), C.POINTER(_u32), C.POINTER(C.POINTER(_u32))]
     L.ni_spec_commit.argtypes = [_vp, C.POINTER(C.POINTER(_u32))]
+    L.ni_spec_commit_accepted.argtypes = [_vp, C.POINTER(_u32)]
     L.ni_spec_set_window.argtypes = [_vp, _u32]
     L.ni_drive_run.argtypes = [C.POINTER(ni_drive_opts), C.POINTER(ni_drive_result)]
     L.ni_drive_last_error.restype = C.c_char_p
@@ -176,7 +177,20 @@ class Spec:
         _check(self._L.ni_spec_plan(self._h, C.byref(w), C.byref(n), C.byref(ctx)), "ni_spec_plan")
         return _work(w, n.value), np.asarray([ctx[i] for i in range(n.value)], np.int64)
 
-    def commit(self):
+    def commit(self, accepted=None):
+        """Truncate the rejected drafts and return the accepted numbers: drawn
+        from the driver's seed, or ``accepted`` (one per sequence, as
+        ``verify_drafts`` returns them; a CUDA tensor is copied to the host)."""
+        if accepted is not None:
+            if hasattr(accepted, "cpu"):
+                accepted = accepted.cpu()
+            arr = np.asarray(accepted, np.int64).reshape(-1)
+            if arr.size != self.n or (arr < 0).any():
+                raise ValueError(f"accepted must be {self.n} numbers, none negative")
+            arr = np.ascontiguousarray(arr, dtype=np.uint32)
+            _check(self._L.ni_spec_commit_accepted(self._h, arr.ctypes.data_as(C.POINTER(_u32))),
+                   "ni_spec_commit_accepted")
+            return [int(a) for a in arr]
         acc = C.POINTER(_u32)()
         _check(self._L.ni_spec_commit(self._h, C.byref(acc)), "ni_spec_commit")
         return [int(acc[i]) for i in range(self.n)]
