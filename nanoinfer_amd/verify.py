@@ -12,7 +12,7 @@ def _need(t, name, dtype, shape, strided=False):
     torch = _torch()
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise TypeError(f"{name} must be a {dtype} tensor")
-    if tuple(t.shape) != shape or (t.numel() and t.stride(-1) != 1) or not (strided or t.is_contiguous()):
+    if tuple(t.shape) != shape or (t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1) or not (strided or t.is_contiguous()):
         raise ValueError(f"{name} must be a {'' if strided else 'contiguous '}{list(shape)} tensor with unit stride, "
                          f"not {list(t.shape)}")
 

@@ -159,6 +159,16 @@ def test_strided_inputs_and_given_outputs(gpu):
     assert (tokb[:, 0] == 77).all() and (tokb[:, k + 2:] == 77).all() and (tokb[b] == 77).all()
 
 
+def test_one_sequence_of_a_column(gpu):
+    """A dimension of one entry has no stride to hold to."""
+    t, d, _, _, q = inputs(1, 4, 500, seed=10)
+    u = torch.rand((1, 5), device=gpu)
+    check((t, d, u[:, :4], u[:, 4]), draft=q)
+    u = torch.rand((3, 2), device=gpu)
+    t, d, _, _, q = inputs(3, 1, 500, seed=11)
+    check((t, d, u[:, :1], u[:, 1].contiguous()), draft=q)
+
+
 def test_the_tokens_follow_the_target(gpu):
     """Over many sequences alike the first token's frequencies are the target's
     (within 5 standard deviations of each count), whatever the drafter."""
