@@ -387,7 +387,7 @@ int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_r
  * be finite; negative and NaN ones weigh nothing, and -1 is drawn where none
  * is positive.  target and draft are of `dtype`; strides count elements, rows
  * are dense.  workspace: ni_verify_workspace(n_seq, vocab) bytes of device
- * memory that no other work on the GPU uses meanwhile.  Enqueued on
+ * memory, 16-byte aligned, that no other work on the GPU uses meanwhile.  Enqueued on
  * `stream`; failures are reported by ni_kv_last_error(NULL). */
 size_t ni_verify_workspace(uint32_t n_seq, uint32_t vocab);
 int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stride, int64_t target_row_stride,

@@ -154,8 +154,8 @@ def _declare(L):
     L.ni_rotary_apply.restype = C.c_int
     L.ni_rotary_apply.argtypes = [C.POINTER(ni_rotary), _u32, _vp, _i64, _vp, _i64, _u32, _u32, _vp, _u32, _vp]
     L.ni_kv_append_rotary.restype = C.c_int
-    L.ni_kv_append_rotary.argtypes = [_vp, C.c_int32, C.POINTER(ni_row), _u32, C.POINTER(ni_rotary), _vp, _vp, _vp, _i64,
-                                      _i64, _vp, _i64, _i64, _u32, _vp, _i64, _i64, _vp]
+    L.ni_kv_append_rotary.argtypes = [_vp, C.c_int32, C.POINTER(ni_row), _u32, C.POINTER(ni_rotary), C.POINTER(_u32),
+                                      _vp, _vp, _i64, _i64, _vp, _i64, _i64, _u32, _vp, _i64, _i64, _vp]
     L.ni_kv_prefix_attention.restype = C.c_int
     L.ni_kv_prefix_attention.argtypes = [_vp, C.c_int32, _vp, _i64, _i64, _u32, C.POINTER(ni_row), _u32,
                                          C.POINTER(ni_prefix), _u32, _vp, _i64, _i64, _u32, _vp]

@@ -100,6 +100,15 @@ def _stream_ptr(stream) -> int:
     return int(torch.cuda.current_stream().cuda_stream)
 
 
+def _stream_now(device, stream):
+    """The current stream's handle where no stream is given and `device` is the
+    current one: the quick form of _on.  None otherwise."""
+    if stream is None and _raw_stream is not None and _get_device is not None and _tc.cuda.is_initialized() \
+            and _get_device() == device:
+        return _raw_stream(device)
+    return None
+
+
 class _on:
     """The device made current where it is not, and `stream` where one is
     given, for what a call allocates and launches; gives the stream's handle."""
@@ -151,6 +160,12 @@ def _fits_layers(t, rows, c, n_layer, device):
     return None
 
 
+def _fits_row(t, rows, c, n_layer, device):
+    """_fits as (row stride, layer stride) or None."""
+    s = _fits(t, rows, c, device)
+    return None if s is None else (s, 0)
+
+
 def _fits_wide(t, rows, c, device) -> bool:
     """Whether t is a float32 tensor [>= rows, >= c] on the GPU `device` with
     unit stride in its last dimension."""
@@ -160,7 +175,8 @@ def _fits_wide(t, rows, c, device) -> bool:
     return False
 
 
-_no_rows, _no_work, _no_prefixes = _abi.ni_row * 0, _abi.ni_work * 0, _abi.ni_prefix * 0
+_no_rows, _no_work, _no_u32 = _abi.ni_row * 0, _abi.ni_work * 0, C.c_uint32 * 0
+_uint32 = np.dtype(np.uint32)
 
 
 def _pointer(arr, empty, item):
@@ -312,18 +328,14 @@ class PagedKv:
     def _strides(self, t, name, layered, rows, c=None):
         """(row stride, layer stride) of t: [n_layer, >= rows, c] or [>= rows, c]."""
         c = self._c if c is None else c
-        if layered:
-            s = _fits_layers(t, rows, c, self._n_layer, self.device)
-        else:
-            s = _fits(t, rows, c, self.device)
-            s = None if s is None else (s, 0)
+        s = (_fits_layers if layered else _fits_row)(t, rows, c, self._n_layer, self.device)
         return self._f32(t, name, layered, rows, c) if s is None else s
 
     def _query_heads(self, q) -> int:
-        torch = _torch()
-        if not isinstance(q, torch.Tensor) or q.dim() == 0 or q.shape[-1] == 0 or q.shape[-1] % self.opts.head_dim:
-            raise ValueError(f"q must hold whole heads of {self.opts.head_dim} in its last dimension")
-        return q.shape[-1] // self.opts.head_dim
+        d = self.opts.head_dim
+        if not isinstance(q, _torch().Tensor) or q.dim() == 0 or q.shape[-1] == 0 or q.shape[-1] % d:
+            raise ValueError(f"q must hold whole heads of {d} in its last dimension")
+        return q.shape[-1] // d
 
     @property
     def max_blocks(self) -> int:
@@ -506,20 +518,33 @@ class PagedKv:
         torch = _torch()
         arr, rp, n = _rows(rows)
         layered = layer == ALL_LAYERS
+        heads = 0 if q is None else self._query_heads(q)
+        cq, pos, pp = heads * self.opts.head_dim, None, None
+        if positions is not None:
+            pos = np.asarray(positions)
+            if pos.size != n or (n and pos.dtype is not _uint32 and
+                                 (pos.dtype.kind not in "iu" or pos.min() < 0 or pos.max() > 0xffffffff)):
+                raise ValueError(f"positions must be {n} integers in 0..2^32-1")
+            pos = np.ascontiguousarray(pos.reshape(-1), dtype=np.uint32)
+            pp = _pointer(pos, _no_u32, C.c_uint32)
+        fits = _fits_layers if layered else _fits_row
+        nl, dev = self._n_layer, self.device
+        ks, s = fits(k, n, self._c, nl, dev), _stream_now(dev, stream)
+        if ks is not None and s is not None and fits(v, n, self._c, nl, dev) == ks:
+            qs = qos = (0, 0)
+            if q is not None:
+                qs, qos = fits(q, n, cq, nl, dev), fits(q_out, n, cq, nl, dev)
+            if qs is not None and qos is not None and (q is None) == (q_out is None):
+                self._check(self._L.ni_kv_append_rotary(
+                    self._h, layer, rp, n, rotary.ref, pp, k.data_ptr(), v.data_ptr(), ks[0], ks[1],
+                    None if q is None else q.data_ptr(), qs[0], qs[1], heads, None if q is None else q_out.data_ptr(),
+                    qos[0], qos[1], s))
+                return q_out
         ks, vs = self._strides(k, "k", layered, n), self._strides(v, "v", layered, n)
         if ks != vs:
             raise ValueError("k and v must share strides")
-        pos, pp = None, None
-        if positions is not None:
-            pos = np.asarray(positions)
-            if pos.size != n or (n and (pos.dtype.kind not in "iu" or pos.min() < 0 or pos.max() > 0xffffffff)):
-                raise ValueError(f"positions must be {n} integers in 0..2^32-1")
-            pos = np.ascontiguousarray(pos.reshape(-1), dtype=np.uint32)
-            pp = pos.ctypes.data
-        heads, qs, qos = 0, (0, 0), (0, 0)
+        qs = qos = (0, 0)
         if q is not None:
-            heads = self._query_heads(q)
-            cq = heads * self.opts.head_dim
             qs = self._strides(q, "q", layered, n, cq)
             if q_out is not None:
                 qos = self._strides(q_out, "q_out", layered, n, cq)
@@ -547,13 +572,23 @@ class PagedKv:
         allocated if not given; it may be q)."""
         torch = _torch()
         arr, rp, n = _rows(rows)
-        pre = np.asarray(prefixes, dtype=np.int64).reshape(-1, 3)
-        if pre.size and (pre.min() < 0 or pre.max() > 0xffffffff):
-            raise ValueError("prefixes must be (seq, length, n_rows) of numbers in 0..2^32-1")
-        pre = np.ascontiguousarray(pre, dtype=np.uint32)
+        pre = (_abi.ni_prefix * len(prefixes))()
+        for p, x in zip(pre, prefixes):
+            seq, length, count = map(int, x)
+            if not (0 <= seq <= 0xffffffff and 0 <= length <= 0xffffffff and 0 <= count <= 0xffffffff):
+                raise ValueError("prefixes must be (seq, length, n_rows) of numbers in 0..2^32-1")
+            p.seq, p.len, p.n_rows = seq, length, count
         layered = layer == ALL_LAYERS
         heads = self._query_heads(q)
         cq = heads * self.opts.head_dim
+        fits = _fits_layers if layered else _fits_row
+        qs, os_ = fits(q, n, cq, self._n_layer, self.device), fits(out, n, cq, self._n_layer, self.device)
+        s = _stream_now(self.device, stream)
+        if qs is not None and os_ is not None and s is not None:
+            self._check(self._L.ni_kv_prefix_attention(
+                self._h, layer, q.data_ptr(), qs[0], qs[1], heads, rp, n, pre, len(pre), out.data_ptr(), os_[0], os_[1],
+                split_tokens, s))
+            return out
         qs = self._strides(q, "q", layered, n, cq)
         os_ = None if out is None else self._strides(out, "out", layered, n, cq)
         self._on_device(q=q, out=out)
@@ -562,8 +597,8 @@ class PagedKv:
                 out = torch.empty((self._n_layer, n, cq) if layered else (n, cq), dtype=torch.float32, device=q.device)
                 os_ = (cq, n * cq if layered else 0)
             self._check(self._L.ni_kv_prefix_attention(
-                self._h, layer, q.data_ptr(), qs[0], qs[1], heads, rp, n, _pointer(pre, _no_prefixes, _abi.ni_prefix),
-                pre.shape[0], out.data_ptr(), os_[0], os_[1], split_tokens, s))
+                self._h, layer, q.data_ptr(), qs[0], qs[1], heads, rp, n, pre, len(pre), out.data_ptr(), os_[0], os_[1],
+                split_tokens, s))
         return out
 
     def step(self, work, q, k, v, out=None, split_tokens: int = 0, stream=None):

@@ -146,8 +146,8 @@ int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stri
     if (n_seq > 1 && tokens_stride < (int64_t)n_draft + 1)
         return call_error(NI_ERR_BAD_ARG, "tokens' rows overlap: the stride must be at least %u", n_draft + 1);
     const size_t need = ni_verify_workspace(n_seq, vocab);
-    if (!workspace || !aligned(workspace, 8) || workspace_bytes < need)
-        return call_error(NI_ERR_BAD_ARG, "workspace must be %zu bytes, 8-byte aligned", need);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+        return call_error(NI_ERR_BAD_ARG, "workspace must be %zu bytes, 16-byte aligned", need);
     VerifyLaunch a{};
     a.target = target;
     a.target_seq_stride = target_seq_stride;
@@ -169,6 +169,9 @@ int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stri
     a.n_draft = n_draft;
     a.vocab = vocab;
     a.dtype = dtype;
+    // As many chunks to a workgroup as leave every CU eight of them.
+    const uint64_t chunks = (uint64_t)n_seq * ((vocab + (uint64_t)kVerifyChunk - 1) / kVerifyChunk);
+    a.per = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(chunks / (8ull * device_cus()), 1), 16);
     const hipError_t e = launch_verify(a, (hipStream_t)stream);
     if (e != hipSuccess) return call_error(NI_ERR_HIP, "verification launch failed: %s", hipGetErrorString(e));
     return NI_OK;

@@ -128,6 +128,7 @@ struct VerifyLaunch {
     int64_t tokens_stride;
     double* sums;  // [n_seq][chunks][2]: what is left of the target's row, and the row itself
     uint32_t n_seq, n_draft, vocab, dtype;
+    uint32_t per;  // chunks one workgroup of the sums adds up
 };
 hipError_t launch_verify(const VerifyLaunch& a, hipStream_t s);
 

@@ -4,15 +4,21 @@
 from __future__ import annotations
 
 from . import _abi
-from .batch import KvError, _on, _torch
+from .batch import KvError, _on, _stream_now, _torch
 from .rotation import dtype_code
+
+
+def _fits(t, dtype, shape, device) -> bool:
+    """The quick form of the checks below for a contiguous tensor."""
+    return t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == device
 
 
 def _need(t, name, dtype, shape, strided=False):
     torch = _torch()
     if not isinstance(t, torch.Tensor) or t.dtype != dtype:
         raise TypeError(f"{name} must be a {dtype} tensor")
-    if tuple(t.shape) != shape or (t.numel() and t.shape[-1] > 1 and t.stride(-1) != 1) or not (strided or t.is_contiguous()):
+    dense = t.numel() == 0 or t.shape[-1] == 1 or t.stride(-1) == 1
+    if tuple(t.shape) != shape or not dense or not (strided or t.is_contiguous()):
         raise ValueError(f"{name} must be a {'' if strided else 'contiguous '}{list(shape)} tensor with unit stride, "
                          f"not {list(t.shape)}")
 
@@ -39,6 +45,19 @@ def verify_drafts(target, drafted, accept_u, sample_u, draft=None, n_drafts=None
     if not isinstance(target, torch.Tensor) or target.dim() != 3 or dtype_code(target.dtype) is None:
         raise TypeError("target must be a float32, float16 or bfloat16 tensor [sequences, drafts + 1, vocabulary]")
     b, k, v = target.shape[0], target.shape[1] - 1, target.shape[2]
+    dtype, device = target.dtype, target.get_device()
+    s = _stream_now(device, stream) if target.is_cuda else None
+    Tensor, i32 = torch.Tensor, torch.int32
+    if (s is not None and k > 0 and v > 0 and target.is_contiguous() and type(drafted) is Tensor
+            and type(accept_u) is Tensor and type(sample_u) is Tensor and type(accepted) is Tensor
+            and type(tokens) is Tensor
+            and (draft is None or type(draft) is Tensor and _fits(draft, dtype, (b, k, v), device))
+            and (n_drafts is None or type(n_drafts) is Tensor and _fits(n_drafts, i32, (b,), device))
+            and _fits(drafted, i32, (b, k), device) and _fits(accept_u, torch.float32, (b, k), device)
+            and _fits(sample_u, torch.float32, (b,), device) and _fits(accepted, i32, (b,), device)
+            and _fits(tokens, i32, (b, k + 1), device)):
+        _call(torch, target, drafted, accept_u, sample_u, draft, n_drafts, accepted, tokens, b, k, v, s)
+        return accepted, tokens
     if k < 0 or v == 0:
         raise ValueError(f"target is {list(target.shape)}: needs [sequences, drafts + 1, vocabulary]")
     _need(target, "target", target.dtype, (b, k + 1, v), strided=True)
@@ -59,22 +78,29 @@ def verify_drafts(target, drafted, accept_u, sample_u, draft=None, n_drafts=None
                     ("n_drafts", n_drafts), ("accepted", accepted), ("tokens", tokens)):
         if t is not None and t.device != target.device:
             raise ValueError(f"{name} is on {t.device}, target on {target.device}")
-    L = _abi.lib()
     with _on(target.get_device(), stream) as s:
         if accepted is None:
             accepted = torch.empty((b,), dtype=torch.int32, device=target.device)
         if tokens is None:
             tokens = torch.empty((b, k + 1), dtype=torch.int32, device=target.device)
-        # From torch's allocator: of this stream, and of the graph where one is captured.
-        need = L.ni_verify_workspace(b, v)
-        work = torch.empty((need // 8,), dtype=torch.float64, device=target.device)
-        rc = L.ni_verify_drafts(dtype_code(target.dtype), target.data_ptr(), target.stride(0), target.stride(1),
-                                None if draft is None or k == 0 else draft.data_ptr(),
-                                0 if draft is None else draft.stride(0), 0 if draft is None else draft.stride(1),
-                                drafted.data_ptr() if k else None, drafted.stride(0),
-                                None if n_drafts is None else n_drafts.data_ptr(), accept_u.data_ptr() if k else None,
-                                accept_u.stride(0), sample_u.data_ptr(), b, k, v, accepted.data_ptr(),
-                                tokens.data_ptr(), tokens.stride(0), work.data_ptr(), need, s)
+        _call(torch, target, drafted, accept_u, sample_u, draft, n_drafts, accepted, tokens, b, k, v, s)
+    return accepted, tokens
+
+
+def _call(torch, target, drafted, accept_u, sample_u, draft, n_drafts, accepted, tokens, b, k, v, s):
+    L = _abi.lib()
+    need = L.ni_verify_workspace(b, v)
+    # From torch's allocator: of this stream, and of the graph where one is captured.
+    work = torch.empty((need,), dtype=torch.uint8, device=target.device)
+    if draft is None or k == 0:
+        dp, ds = None, (0, 0)
+    else:
+        dp, ds = draft.data_ptr(), draft.stride()
+    ts = target.stride()
+    rc = L.ni_verify_drafts(dtype_code(target.dtype), target.data_ptr(), ts[0], ts[1], dp, ds[0], ds[1],
+                            drafted.data_ptr() if k else None, drafted.stride(0),
+                            None if n_drafts is None else n_drafts.data_ptr(), accept_u.data_ptr() if k else None,
+                            accept_u.stride(0), sample_u.data_ptr(), b, k, v, accepted.data_ptr(), tokens.data_ptr(),
+                            tokens.stride(0), work.data_ptr(), need, s)
     if rc != 0:
         raise KvError(rc, (L.ni_kv_last_error(None) or b"").decode())
-    return accepted, tokens

@@ -223,7 +223,7 @@ def test_verify_refuses_misaligned_pointers():
     _, _, p = _verify_call(vocab=0)
     for name in ("target", "draft", "drafted", "n_drafts", "au", "su", "accepted", "tokens", "work"):
         buf = (C.c_float * 16)()
-        q = C.addressof(buf) + 2 if name != "work" else C.addressof(buf) // 8 * 8 + 4
+        q = C.addressof(buf) + 2 if name != "work" else C.addressof(buf) // 16 * 16 + 8
         rc, msg, _ = _verify_call(**{name: q})
         assert rc == _abi.NI_ERR_BAD_ARG and "align" in msg, name
 
