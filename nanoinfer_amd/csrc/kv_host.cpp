@@ -136,7 +136,9 @@ struct Plan {
 
 // Work of one ni_kv_prefix_attention call, before serialisation.
 struct PrefixPlan {
-    std::vector<PrefixItem> items;
+    std::vector<PrefixItem> pitems;  // over the prefixes' keys
+    std::vector<PrefixItem> items;   // over the sequences' own
+    uint32_t waves = 0;              // of pitems: PrefixLaunch::waves
     std::vector<PrefixMerge> merges;
     std::vector<uint32_t> table;
     uint64_t n_parts = 0;
@@ -1346,12 +1348,12 @@ struct DeviceScope {
 };
 
 // Cut a ni_kv_prefix_attention call into items.  Queries travel as slots (the
-// `group` query heads of a row that read one cache head), kSlotTile to an
-// item.  A prefix is read by its rows' slots together, each sequence's own
-// keys by its rows' (consecutive rows of one sequence at consecutive
-// positions form a run); both in partitions of the same number of keys.
+// `group` query heads of a row that read one cache head).  A prefix is read by
+// its rows' slots together, each sequence's own keys by its rows' (consecutive
+// rows of one sequence at consecutive positions form a run).
 int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32_t n_prefix, uint32_t group,
                 uint32_t n_lay, uint32_t split_tokens, PrefixPlan& P) {
+    P.pitems.clear();
     P.items.clear();
     P.merges.clear();
     P.table.clear();
@@ -1402,18 +1404,30 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
         }
         return (uint32_t)kv->seq_tab[seq];
     };
-    auto tiles = [](uint64_t slots) { return (slots + kSlotTile - 1) / kSlotTile; };
-    // Keys per partition: enough workgroups to give every CU four, so that no
-    // CU idles at the end, but 128 keys (two pages a wave) at least, below
-    // which a workgroup is mostly its own start and end.
-    uint64_t keys = 0;
+    auto tiles = [](uint64_t slots, uint64_t tile) { return (slots + tile - 1) / tile; };
+    const uint64_t lh = (uint64_t)n_lay * kv->o.n_head, cus = device_cus();
+    auto between = [](uint64_t x, uint64_t lo, uint64_t hi) { return std::min(std::max(x, lo), hi); };
+
+    // The prefixes.  More than kSlotTile slots behind one go through wide items
+    // (f16): the fewest that hold them, of equal waves.
+    uint64_t most = 0;
     for (uint32_t i = 0; i < n_prefix; i++)
-        if (prefixes[i].n_rows) keys += tiles((uint64_t)prefixes[i].n_rows * group) * prefixes[i].len;
-    for (const Run& u : runs) keys += tiles((uint64_t)u.n * group) * (u.pos0 + u.n);
-    uint64_t part = split_tokens;
-    if (!part) {
-        part = keys * n_lay * kv->o.n_head / (4ull * device_cus());
-        part = std::min<uint64_t>(std::max<uint64_t>(align_up(part, 4 * kPage), 128), 16384);
+        if (prefixes[i].len) most = std::max<uint64_t>(most, (uint64_t)prefixes[i].n_rows * group);
+    P.waves = 0;
+    uint64_t p_tile = kSlotTile;
+    if (most > kSlotTile && !is_q8(kv->o)) {
+        const uint64_t n = tiles(most, (uint64_t)kWideSlots * kWideWavesMax);
+        P.waves = (uint32_t)tiles(most, kWideSlots * n);
+        p_tile = (uint64_t)kWideSlots * P.waves;
+    }
+    // Keys per partition: as many workgroups as the CUs hold at once.
+    uint64_t p_keys = 0;
+    for (uint32_t i = 0; i < n_prefix; i++)
+        if (prefixes[i].n_rows) p_keys += tiles((uint64_t)prefixes[i].n_rows * group, p_tile) * prefixes[i].len;
+    uint64_t p_part = split_tokens;
+    if (!p_part) {
+        const uint64_t held = P.waves ? std::max<uint64_t>((kv->o.head_dim == 64 ? 12 : 8) / P.waves, 1) : 4;
+        p_part = between(align_up(p_keys * lh / (held * cus), 2 * kPage), 128, 16384);
     }
     std::vector<uint64_t> pre0(n_prefix, 0);
     for (uint32_t i = 0, r = 0; i < n_prefix; r += prefixes[i].n_rows, i++) {
@@ -1422,22 +1436,29 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
         const uint64_t slots = (uint64_t)p.n_rows * group;
         const uint32_t tab = tab_of(p.seq);
         pre0[i] = P.n_parts;
-        for (uint64_t k0 = 0; k0 < p.len; k0 += part) {
-            for (uint64_t s0 = 0; s0 < slots; s0 += kSlotTile)
-                P.items.push_back({tab, r, (uint32_t)s0, (uint32_t)std::min<uint64_t>(kSlotTile, slots - s0), kWholePos,
-                                   (uint32_t)k0, (uint32_t)std::min<uint64_t>(p.len, k0 + part),
-                                   (uint32_t)(P.n_parts + s0)});
+        for (uint64_t k0 = 0; k0 < p.len; k0 += p_part) {
+            for (uint64_t s0 = 0; s0 < slots; s0 += p_tile)
+                P.pitems.push_back({tab, r, (uint32_t)s0, (uint32_t)std::min(p_tile, slots - s0), kWholePos,
+                                    (uint32_t)k0, (uint32_t)std::min<uint64_t>(p.len, k0 + p_part),
+                                    (uint32_t)(P.n_parts + s0), 0, 0, 0, 0});
             P.n_parts += slots;
         }
     }
+
+    // The sequences' own keys: whole where that leaves no long item, joining
+    // the prefix's partials at once; else in partitions that a merge joins.
+    uint64_t o_keys = 0;
+    for (const Run& u : runs) o_keys += tiles((uint64_t)u.n * group, kSlotTile) * (u.pos0 + u.n);
+    uint64_t part = split_tokens;
+    if (!part) part = between(align_up(o_keys * lh / (4 * cus), 4 * kPage), 512, 16384);
     for (uint32_t i = 0, r = 0, u0 = 0; i < n_prefix; r += prefixes[i].n_rows, i++) {
         const ni_prefix& p = prefixes[i];
-        const uint64_t p_slots = (uint64_t)p.n_rows * group;
-        const uint32_t n_pre = (uint32_t)((p.len + part - 1) / part);
+        const uint32_t p_slots = (uint32_t)((uint64_t)p.n_rows * group);
+        const uint32_t n_pre = (uint32_t)((p.len + p_part - 1) / p_part);
         for (; u0 < runs.size() && runs[u0].prefix == i; u0++) {
             const Run& u = runs[u0];
             const uint64_t slots = (uint64_t)u.n * group, n_own = (u.pos0 + u.n + part - 1) / part;
-            const bool whole = n_pre == 0 && n_own == 1;
+            const uint64_t pre = pre0[i] + (uint64_t)(u.row0 - r) * group;  // the run's first slot in the prefix's partials
             const uint32_t tab = tab_of(u.seq);
             for (uint64_t j = 0; j < n_own; j++)
                 for (uint64_t s0 = 0; s0 < slots; s0 += kSlotTile) {
@@ -1446,23 +1467,24 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
                     if (j * part >= end) continue;
                     P.items.push_back({tab, u.row0, (uint32_t)s0, ns, u.pos0, (uint32_t)(j * part),
                                        (uint32_t)std::min<uint64_t>(end, (j + 1) * part),
-                                       whole ? kNoSlot : (uint32_t)(P.n_parts + j * slots + s0)});
+                                       n_own == 1 ? kNoSlot : (uint32_t)(P.n_parts + j * slots + s0), (uint32_t)(pre + s0),
+                                       p_slots, n_pre, 0});
                 }
-            if (whole) continue;
+            if (n_own == 1) continue;
             for (uint32_t t = 0; t < u.n; t++)
                 P.merges.push_back({u.row0 + t, (uint32_t)(P.n_parts + (uint64_t)t * group), (uint32_t)slots,
-                                    (uint32_t)((u.pos0 + t) / part + 1),
-                                    (uint32_t)(pre0[i] + (uint64_t)(u.row0 + t - r) * group), (uint32_t)p_slots, n_pre,
-                                    0});
+                                    (uint32_t)((u.pos0 + t) / part + 1), (uint32_t)(pre + (uint64_t)t * group), p_slots,
+                                    n_pre, 0});
             P.n_parts += n_own * slots;
         }
     }
-    // Longest first, so that the launch does not end on a long item.
-    std::stable_sort(P.items.begin(), P.items.end(), [](const PrefixItem& x, const PrefixItem& y) {
-        return x.kv_end - x.kv_begin > y.kv_end - y.kv_begin;
-    });
-    if (P.n_parts >= (1ull << 31) || (uint64_t)P.items.size() * n_lay * kv->o.n_head >= (1ull << 31) ||
-        (uint64_t)P.merges.size() * n_lay * kv->o.n_head * group >= (1ull << 31))
+    // Longest first, so that no launch ends on a long item.
+    for (auto* items : {&P.items, &P.pitems})
+        std::stable_sort(items->begin(), items->end(), [](const PrefixItem& x, const PrefixItem& y) {
+            return x.kv_end - x.kv_begin > y.kv_end - y.kv_begin;
+        });
+    if (P.n_parts >= (1ull << 31) || std::max(P.items.size(), P.pitems.size()) * lh >= (1ull << 31) ||
+        P.merges.size() * lh * group >= (1ull << 31))
         return kv->fail(NI_ERR_BAD_ARG, "rows * layers * heads too large for one call");
     return NI_OK;
 }
@@ -2081,10 +2103,12 @@ int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_r
     PrefixPlan& P = kv->prefix_plan;
     if (int rc = plan_prefix(kv, rows, prefixes, n_prefix, n_q_head / H, n_lay, split_tokens, P)) return rc;
     std::vector<uint8_t>& blob = kv->blob;
-    const size_t off_merges = align_up(P.items.size() * sizeof(PrefixItem), kAlign);
+    const size_t off_pitems = align_up(P.items.size() * sizeof(PrefixItem), kAlign);
+    const size_t off_merges = align_up(off_pitems + P.pitems.size() * sizeof(PrefixItem), kAlign);
     const size_t off_table = align_up(off_merges + P.merges.size() * sizeof(PrefixMerge), kAlign);
     blob.resize(align_up(off_table + P.table.size() * sizeof(uint32_t), kAlign));
     memcpy(blob.data(), P.items.data(), P.items.size() * sizeof(PrefixItem));
+    if (!P.pitems.empty()) memcpy(blob.data() + off_pitems, P.pitems.data(), P.pitems.size() * sizeof(PrefixItem));
     if (!P.merges.empty()) memcpy(blob.data() + off_merges, P.merges.data(), P.merges.size() * sizeof(PrefixMerge));
     memcpy(blob.data() + off_table, P.table.data(), P.table.size() * sizeof(uint32_t));
 
@@ -2118,14 +2142,23 @@ int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_r
     a.off_table = (uint32_t)off_table;
     a.part_o = partials;
     a.part_ml = partials ? partials + o_bytes / sizeof(float) : nullptr;
-    a.n_items = (uint32_t)P.items.size();
     a.n_merges = (uint32_t)P.merges.size();
     a.layer0 = layer0;
     a.n_lay = n_lay;
     a.group = n_q_head / H;
     a.qscale = (float)(1.4426950408889634 / std::sqrt((double)D));
-    hipError_t e;
-    {
+    hipError_t e = hipSuccess;
+    if (!P.pitems.empty()) {
+        a.off_items = (uint32_t)off_pitems;
+        a.n_items = (uint32_t)P.pitems.size();
+        a.waves = P.waves;
+        ProfileScope ps(kv, NI_K_ATTN);
+        e = launch_prefix_attention(a, ref.inl, ref.inl_bytes, s, ps.t);
+    }
+    if (e == hipSuccess) {
+        a.off_items = 0;
+        a.n_items = (uint32_t)P.items.size();
+        a.waves = 0;
         ProfileScope ps(kv, NI_K_ATTN);
         e = launch_prefix_attention(a, ref.inl, ref.inl_bytes, s, ps.t);
     }

@@ -63,11 +63,16 @@ hipError_t launch_append_rotary(const AppendRotaryLaunch& a, const CacheRotary& 
 
 // Queries travel as slots: the G = n_q_head / n_head query heads that read one
 // cache head, row by row: slot s of a run of rows is head s % G of row s / G.
-constexpr uint32_t kSlotTile = 16;            // slots of one item
+constexpr uint32_t kSlotTile = 16;            // slots of an item
+constexpr uint32_t kWideSlots = 32;           // slots of one wave of a wide item ...
+constexpr uint32_t kWideWavesMax = 4;         // ... of this many waves at most
 constexpr uint32_t kWholePos = 0x7fffffffu;   // PrefixItem::pos0 of a prefix: every slot sees every key
 
 // One work item: slots slot0 .. slot0 + ns - 1 of the run of rows at row0 over
 // keys [kv_begin, kv_end) of one page list.  Slot s sees keys <= pos0 + s / G.
+// An item whose part0 is kNoSlot holds all its slots' own keys: it joins the
+// n_pre partials of their prefix (those of slot s at pre0 + s + j * pre_stride,
+// written by an earlier launch) and writes their outputs.
 struct PrefixItem {
     uint32_t tab;       // the page list, in the plan's table
     uint32_t row0;
@@ -76,7 +81,9 @@ struct PrefixItem {
     uint32_t pos0;
     uint32_t kv_begin;  // a multiple of kPage
     uint32_t kv_end;
-    uint32_t part0;     // partial of the first slot, or kNoSlot: the item is all its slots have
+    uint32_t part0;     // partial of the first slot, or kNoSlot
+    uint32_t pre0, pre_stride, n_pre;
+    uint32_t pad;
 };
 
 // The partials of one row's slots: n_own of its own keys' partitions, n_pre
@@ -101,6 +108,7 @@ struct PrefixLaunch {
     uint32_t n_items, n_merges;
     uint32_t layer0, n_lay;
     uint32_t group;  // G
+    uint32_t waves;  // 0: items of up to kSlotTile slots; else of kWideSlots * waves slots of a prefix (f16)
     float qscale;    // log2(e) / sqrt(head_dim)
 };
 hipError_t launch_prefix_attention(const PrefixLaunch& a, const void* inline_plan, uint32_t inline_bytes,

@@ -3,11 +3,14 @@
 // prefix, held once in the cache, and to its own sequence's.
 //
 //   prefix_attn_kernel   16 slots (query heads of rows that read the same
-//                        cache head) over a run of keys
-//   prefix_merge_kernel  each slot's partial softmax states joined
+//                        cache head) over a run of keys; of a sequence's own
+//                        keys it joins the prefix's partials and writes out
+//   prefix_wide_kernel   up to 128 slots over a run of a prefix's keys
+//   prefix_merge_kernel  each slot's partial softmax states joined, where a
+//                        sequence's own keys are partitioned too
 //
-// A prefix's keys leave memory once per 16 slots instead of once per row, and
-// each product of the matrix cores serves all of them.
+// A prefix's keys leave memory once per 16 to 128 slots instead of once per
+// row, and each product of the matrix cores serves all of them.
 #include "kv_device.h"
 #include "ops_plan.h"
 
@@ -274,6 +277,31 @@ __global__ __launch_bounds__(64 * kPW) void prefix_attn_kernel(const PrefixLaunc
             O += red[w][sl][2 + d] * wt;
         }
         if (it.part0 == kNoSlot) {
+            constexpr int B = 4;  // partials in flight; past the last it is read again and weighs nothing
+            for (uint32_t j = 0; j < it.n_pre; j += B) {
+                float pm[B], pl[B], po[B], mn = M;
+#pragma unroll
+                for (int i = 0; i < B; i++) {
+                    const uint32_t idx = it.pre0 + sl + min(j + i, it.n_pre - 1) * it.pre_stride;
+                    const uint64_t part = ((uint64_t)idx * a.n_lay + lay) * H + head;
+                    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * part);
+                    pm[i] = ml.x;
+                    pl[i] = ml.y;
+                    po[i] = a.part_o[part * D + d];
+                }
+#pragma unroll
+                for (int i = 0; i < B; i++) mn = fmaxf(mn, pm[i]);
+                const float wt = fast_exp2(M - mn);
+                L *= wt;
+                O *= wt;
+                M = mn;
+#pragma unroll
+                for (int i = 0; i < B; i++) {
+                    const float w = fast_exp2(pm[i] - mn);
+                    L += j + i < it.n_pre ? pl[i] * w : 0.f;
+                    O += j + i < it.n_pre ? po[i] * w : 0.f;
+                }
+            }
             const uint32_t r = (it.slot0 + sl) / a.group, gg = it.slot0 + sl - r * a.group;
             a.out[(int64_t)lay * a.out_layer_stride + (int64_t)(it.row0 + r) * a.out_row_stride +
                   (head * a.group + gg) * D + d] = O / L;
@@ -286,6 +314,237 @@ __global__ __launch_bounds__(64 * kPW) void prefix_attn_kernel(const PrefixLaunc
             }
         }
     }
+}
+
+// Wide items: W waves of 32 slots each over tiles of 32 keys of a prefix, which
+// the waves copy to LDS by DMA (a ring of three tiles, one barrier per tile) and
+// all read.  Of the 32 x 32 x 16 products S^T = K Q^T and O^T += V^T P^T lane l
+// holds slot l % 32: a slot's softmax state lives in two lanes, and S^T's
+// registers are PV's operand as they are (keys 8 (i / 4) + 4 (l / 32) + i % 4 of
+// register i, in V's transposing reads alike).  Every slot sees every key, so
+// only the last tile masks.  The exponent reference follows the running maximum
+// only past kWideSlack (weights up to 2^15 in f16, as hi + lo).
+constexpr float kWideSlack = 8.f, kWideLog2 = 7.f, kWideUnscale = 1.f / 128.f;
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+template <int N>
+__device__ __forceinline__ void wait_dma(uint32_t ahead) {  // at most `ahead` tiles of N copies of this wave in flight
+    static_assert(N < 64, "vmcnt");
+    if (ahead >= 1)
+        __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | ((N >> 4) << 14));
+    else
+        __builtin_amdgcn_s_waitcnt(0x0f70);
+}
+
+template <int D, int W, int INL>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : W >= 3 ? 4 : 3, 8))) void prefix_wide_kernel(
+    const PrefixLaunch a, const PlanArg<INL> pa) {
+    constexpr int KS = D / 16;                // 16-dim steps of QK
+    constexpr int DB = D / 32;                // 32-dim blocks of PV
+    constexpr int CH = D / 8;                 // 16-byte chunks of a row
+    constexpr int TP = 2, TK = TP * kPage;    // pages and keys of a tile
+    constexpr int TB = TK * D * 2;            // bytes of a K (or V) tile
+    constexpr int NI = 2 * TB / 1024;         // 1 KB copies of a tile
+    constexpr int ND = (NI + W - 1) / W;      // of one wave (the last again, where they do not divide)
+    constexpr int WR = 64 / CH;               // rows of one copy
+    constexpr int NS = 3;                     // tiles of the ring
+    constexpr float kHi = kWideSlack + kWideLog2;
+    __shared__ __attribute__((aligned(16))) uint8_t ring[NS][2 * TB];
+
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t H = a.pool.n_head, lh = a.n_lay * H;
+    const uint8_t* plan = plan_base(pa, a.plan);
+    const uint32_t item_i = blockIdx.x / lh;
+    const uint32_t rem = blockIdx.x - item_i * lh;
+    const uint32_t lay = rem / H, head = rem - lay * H;
+    const PrefixItem it = reinterpret_cast<const PrefixItem*>(plan + a.off_items)[item_i];
+    const int col = lane & 31, g2 = lane >> 5;
+    const uint64_t off = (uint64_t)(a.layer0 + lay) * a.pool.layer_halves + (uint64_t)head * a.pool.head_halves;
+    const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.pool.k + off);
+    const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.pool.v + off);
+    const uint64_t page_bytes = 2 * a.pool.page_halves;
+    const __attribute__((address_space(4))) uint32_t* tab =
+        (const __attribute__((address_space(4))) uint32_t*)(plan + a.off_table) + it.tab;
+    const uint32_t pg0 = it.kv_begin / kPage, pg_end = (it.kv_end + kPage - 1) / kPage;
+    const uint32_t n_tiles = (pg_end - pg0 + TP - 1) / TP;
+
+    // Copy i of a tile: rows (i % (NI/2)) * WR .. of K (i < NI/2) or V.  Lane
+    // l's 16 bytes land at 16 l of the copy's 1 KB: logical chunk (l % CH) ^ sw
+    // of row l / CH.  A row past the item's end copies row 0 of its page, a
+    // page past it the item's last page: keys of the item, whose weights the
+    // last tile makes 0.
+    const uint32_t lds_ring = (uint32_t)(uintptr_t)NI_LDS(&ring[0][0]);
+    auto issue = [&](uint32_t stage, uint32_t ti) {
+        const uint32_t pg = pg0 + ti * TP;
+        const uint32_t pid0 = tab[pg], pid1 = tab[min(pg + 1, pg_end - 1)];
+        const bool cut = (pg + TP) * kPage > it.kv_end;
+#pragma unroll
+        for (int j = 0; j < ND; j++) {
+            const uint32_t i = min(wave + j * W, (uint32_t)NI - 1);  // wave-uniform
+            const uint32_t r0 = (i % (NI / 2)) * WR, row = r0 + lane / CH;
+            const uint32_t chunk = (lane % CH) ^ (tile_chunk<CH>(row, 0) - row * CH);
+            uint32_t o = (row % kPage) * D * 2 + chunk * 16;
+            if (cut && pg * kPage + row >= it.kv_end) o = chunk * 16;
+            const uint64_t pb = (uint64_t)(r0 >= kPage ? pid1 : pid0) * page_bytes;
+            lds_dma16_sbase((i >= NI / 2 ? vbase : kbase) + pb, o, lds_ring + stage * 2 * TB + 1024 * i);
+        }
+    };
+    issue(0u, 0);
+    if (n_tiles > 1) issue(1u, 1);
+
+    const uint32_t s0 = wave * kWideSlots;
+    const bool mine = s0 < it.ns;  // the wave has slots
+    const bool has = s0 + col < it.ns;
+    const uint32_t slot = it.slot0 + (has ? s0 + col : 0u);
+    const uint32_t row = slot / a.group, gq = slot - row * a.group;
+    float4 xq[2 * KS];
+    {
+        const float* qb = a.q + (int64_t)lay * a.q_layer_stride + (int64_t)(it.row0 + row) * a.q_row_stride +
+                          (head * a.group + gq) * D + 8 * g2;
+#pragma unroll
+        for (int c = 0; c < KS; c++) {
+            xq[2 * c] = reinterpret_cast<const float4*>(qb + c * 16)[0];
+            xq[2 * c + 1] = reinterpret_cast<const float4*>(qb + c * 16)[1];
+        }
+    }
+    // The loads have landed (and the first tiles, issued before them) before
+    // any further copy: the loop's waits count copies alone.
+#pragma unroll
+    for (int c = 0; c < 2 * KS; c++) asm volatile("" : : "v"(xq[c].x), "v"(xq[c].y), "v"(xq[c].z), "v"(xq[c].w));
+    half8_t qh[KS], ql[KS];
+#pragma unroll
+    for (int c = 0; c < KS; c++) {
+        const float x[8] = {xq[2 * c].x, xq[2 * c].y, xq[2 * c].z, xq[2 * c].w,
+                            xq[2 * c + 1].x, xq[2 * c + 1].y, xq[2 * c + 1].z, xq[2 * c + 1].w};
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            float x0 = has ? x[e] * a.qscale : 0.f, x1 = has ? x[e + 1] * a.qscale : 0.f;
+            asm("" : "+v"(x0), "+v"(x1));  // the f32 products, as the split's residual sees them
+            uint32_t h, l;
+            split_w16x2(x0, x1, h, l);
+            const half2_t hh = __builtin_bit_cast(half2_t, h), ll = __builtin_bit_cast(half2_t, l);
+            qh[c][e] = hh[0];
+            qh[c][e + 1] = hh[1];
+            ql[c][e] = ll[0];
+            ql[c][e + 1] = ll[1];
+        }
+    }
+    float mref = 0.f, lsum = 0.f;
+    bool set = false;  // the reference is a score's (alike in both lanes of a slot)
+    float16_t o[DB];
+#pragma unroll
+    for (int b = 0; b < DB; b++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[b][i] = 0.f;
+    // Byte offsets in a stage: K chunk 2c + g2 of row col; V keys 8j + 4 g2 +
+    // (0..3), dims 32 b + 16 (l / 16 % 2) + (0..15) of a page.
+    uint32_t koff[KS], voff[2][DB];
+    const int vt = (lane >> 2) & 3, va = lane & 3, vh = (lane >> 4) & 1;
+#pragma unroll
+    for (int c = 0; c < KS; c++) koff[c] = tile_chunk<CH>(col, 2 * c + g2) * 16;
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int b = 0; b < DB; b++)
+            voff[j][b] = TB + tile_chunk<CH>(8 * j + 4 * g2 + vt, 4 * b + 2 * vh + (va >> 1)) * 16 + (va & 1) * 8;
+
+    // (the stage is a variable: the body instantiated per stage spills 70
+    // registers of 256 at head_dim 128)
+    auto tile = [&](uint32_t stage, uint32_t ti) {
+        wait_dma<ND>(min(n_tiles - 1 - ti, 1u));
+        __syncthreads();  // every wave's part of tile ti is there, and every wave is done with tile ti - 1
+        if (ti + NS - 1 < n_tiles) issue(stage == 0 ? NS - 1 : stage - 1, ti + NS - 1);
+        if (!mine) return;
+        const uint8_t* const st = &ring[stage][0];
+        float16_t sc;
+#pragma unroll
+        for (int i = 0; i < 16; i++) sc[i] = -mref;
+#pragma unroll
+        for (int c = 0; c < KS; c++) {
+            const half8_t kh = *reinterpret_cast<const half8_t*>(st + koff[c]);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[c], sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[c], sc, 0, 0, 0);
+        }
+        const uint32_t key0 = (pg0 + ti * TP) * kPage;
+        if (key0 + TK > it.kv_end) {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (key0 + 8 * (i / 4) + 4 * g2 + i % 4 >= it.kv_end) sc[i] = -INFINITY;
+        }
+        float lm = sc[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) lm = fmaxf(lm, sc[i]);
+        if (__any(lm > kHi || !set)) {
+            const u32x2_t sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(lm), __float_as_uint(lm), false, false);
+            const float mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - kWideLog2;
+            // The first finite maximum sets the reference, later ones only raise it.
+            const bool none = mx == -INFINITY;
+            const float d = set ? fmaxf(mx, 0.f) : none ? 0.f : mx;
+            const float alpha = set ? fast_exp2(-d) : 1.f;  // (nothing is summed yet)
+            set = set || !none;
+            lsum *= alpha;
+#pragma unroll
+            for (int b = 0; b < DB; b++) o[b] *= alpha;
+            mref += d;
+#pragma unroll
+            for (int i = 0; i < 16; i++) sc[i] -= d;
+        }
+        float p[16];
+#pragma unroll
+        for (int i = 0; i < 16; i++) p[i] = fast_exp2(sc[i]);
+        float ps[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) ps[i] = (p[4 * i] + p[4 * i + 1]) + (p[4 * i + 2] + p[4 * i + 3]);
+        lsum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+#pragma unroll
+        for (int t = 0; t < TP; t++) {
+            u32x4 h, l;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                uint32_t hh, ll;
+                split_w16x2(p[8 * t + 2 * e], p[8 * t + 2 * e + 1], hh, ll);
+                h[e] = hh;
+                l[e] = ll;
+            }
+            const half8_t ph = __builtin_bit_cast(half8_t, h), pl = __builtin_bit_cast(half8_t, l);
+#pragma unroll
+            for (int b = 0; b < DB; b++) {
+                half4_t v[2];
+#pragma unroll
+                for (int j = 0; j < 2; j++)
+                    v[j] = __builtin_bit_cast(
+                        half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) v4fp16_t*)(
+                                     st + voff[j][b] + t * (int)kPage * D * 2)));
+                const half8_t v8 = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl, o[b], 0, 0, 0);
+                o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph, o[b], 0, 0, 0);
+            }
+        }
+    };
+    for (uint32_t ti = 0, stage = 0; ti < n_tiles; ti++) {
+        tile(stage, ti);
+        stage = stage == NS - 1 ? 0 : stage + 1;
+    }
+    const u32x2_t sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(lsum), __float_as_uint(lsum), false, false);
+    lsum = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    if (!has) return;
+    const uint64_t part = ((uint64_t)(it.part0 + s0 + col) * a.n_lay + lay) * H + head;
+    if (g2 == 0) {
+        a.part_ml[2 * part] = set ? mref + kWideLog2 : kMinScore;
+        a.part_ml[2 * part + 1] = lsum * kWideUnscale;
+    }
+#pragma unroll
+    for (int b = 0; b < DB; b++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float4 y;
+            y.x = o[b][4 * i] * kWideUnscale;
+            y.y = o[b][4 * i + 1] * kWideUnscale;
+            y.z = o[b][4 * i + 2] * kWideUnscale;
+            y.w = o[b][4 * i + 3] * kWideUnscale;
+            *reinterpret_cast<float4*>(a.part_o + part * D + 32 * b + 8 * i + 4 * g2) = y;
+        }
 }
 
 // One wave per (row, layer, query head): its partials' states weighed by
@@ -359,10 +618,32 @@ hipError_t attn_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_
     });
 }
 
+template <int D>
+hipError_t wide_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s, const LaunchTiming& t) {
+    const uint64_t blocks = (uint64_t)a.n_items * a.n_lay * a.pool.n_head;
+    return with_plan(a, ip, ib, [&](auto pa) {
+        constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
+        switch (a.waves) {
+            case 1: return go(prefix_wide_kernel<D, 1, INL>, blocks, 64, s, t, a, pa);
+            case 2: return go(prefix_wide_kernel<D, 2, INL>, blocks, 128, s, t, a, pa);
+            case 3: return go(prefix_wide_kernel<D, 3, INL>, blocks, 192, s, t, a, pa);
+            case 4: return go(prefix_wide_kernel<D, 4, INL>, blocks, 256, s, t, a, pa);
+            default: return hipErrorInvalidValue;
+        }
+    });
+}
+
 }  // namespace
 
 hipError_t launch_prefix_attention(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s,
                                    const LaunchTiming& t) {
+    if (a.n_items == 0) return hipSuccess;
+    if (a.waves) {
+        if (a.pool.q8) return hipErrorInvalidValue;
+        if (a.pool.head_dim == 64) return wide_t<64>(a, ip, ib, s, t);
+        if (a.pool.head_dim == 128) return wide_t<128>(a, ip, ib, s, t);
+        return hipErrorInvalidValue;
+    }
     if (a.pool.head_dim == 64) return a.pool.q8 ? attn_t<64, true>(a, ip, ib, s, t) : attn_t<64, false>(a, ip, ib, s, t);
     if (a.pool.head_dim == 128)
         return a.pool.q8 ? attn_t<128, true>(a, ip, ib, s, t) : attn_t<128, false>(a, ip, ib, s, t);
