@@ -138,7 +138,8 @@ struct Plan {
 struct PrefixPlan {
     std::vector<PrefixItem> pitems;  // over the prefixes' keys
     std::vector<PrefixItem> items;   // over the sequences' own
-    uint32_t waves = 0;              // of pitems: PrefixLaunch::waves
+    uint32_t wide = 0, waves = 0;  // PrefixLaunch::wide and waves of pitems
+    uint32_t row_slots = 0;        // PrefixLaunch::row_slots of items
     std::vector<PrefixMerge> merges;
     std::vector<uint32_t> table;
     uint64_t n_parts = 0;
@@ -1413,21 +1414,33 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
     uint64_t most = 0;
     for (uint32_t i = 0; i < n_prefix; i++)
         if (prefixes[i].len) most = std::max<uint64_t>(most, (uint64_t)prefixes[i].n_rows * group);
+    P.wide = most > kSlotTile && !is_q8(kv->o);
     P.waves = 0;
     uint64_t p_tile = kSlotTile;
-    if (most > kSlotTile && !is_q8(kv->o)) {
+    if (P.wide) {
         const uint64_t n = tiles(most, (uint64_t)kWideSlots * kWideWavesMax);
         P.waves = (uint32_t)tiles(most, kWideSlots * n);
         p_tile = (uint64_t)kWideSlots * P.waves;
     }
-    // Keys per partition: as many workgroups as the CUs hold at once.
-    uint64_t p_keys = 0;
-    for (uint32_t i = 0; i < n_prefix; i++)
-        if (prefixes[i].n_rows) p_keys += tiles((uint64_t)prefixes[i].n_rows * group, p_tile) * prefixes[i].len;
+    // Keys per partition: wide workgroups fill a CU each, so as many as there are
+    // CUs and no second round; others four to a CU.
     uint64_t p_part = split_tokens;
     if (!p_part) {
-        const uint64_t held = P.waves ? std::max<uint64_t>((kv->o.head_dim == 64 ? 12 : 8) / P.waves, 1) : 4;
-        p_part = between(align_up(p_keys * lh / (held * cus), 2 * kPage), 128, 16384);
+        const uint64_t most_units = (P.wide ? 1 : 4) * cus;
+        auto units = [&](uint64_t part) {
+            uint64_t n = 0;
+            for (uint32_t i = 0; i < n_prefix; i++)
+                if (prefixes[i].n_rows)
+                    n += tiles((uint64_t)prefixes[i].n_rows * group, p_tile) * tiles(prefixes[i].len, part);
+            return n * lh;
+        };
+        uint64_t longest = 128;
+        for (uint32_t i = 0; i < n_prefix; i++)
+            if (prefixes[i].n_rows) longest = std::max<uint64_t>(longest, prefixes[i].len);
+        longest = align_up(longest, 2 * kPage);
+        p_part = 128;
+        while (p_part < longest && units(p_part) > most_units)
+            p_part = std::min<uint64_t>(longest, align_up(p_part + p_part / 16, 2 * kPage));
     }
     std::vector<uint64_t> pre0(n_prefix, 0);
     for (uint32_t i = 0, r = 0; i < n_prefix; r += prefixes[i].n_rows, i++) {
@@ -1445,8 +1458,11 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
         }
     }
 
-    // The sequences' own keys: whole where that leaves no long item, joining
-    // the prefix's partials at once; else in partitions that a merge joins.
+    // The sequences' own keys: whole where that leaves no long item.  Behind wide
+    // items they have a launch of their own and join the prefix's partials at once;
+    // else both kinds share a launch and a merge joins them (2 rows x 12 heads
+    // behind 515 keys: 7.2 us, joined at once 8.3; 32 x 5 rows of the Q8 cache behind
+    // 2001 17.5, 20.2).
     uint64_t o_keys = 0;
     for (const Run& u : runs) o_keys += tiles((uint64_t)u.n * group, kSlotTile) * (u.pos0 + u.n);
     uint64_t part = split_tokens;
@@ -1458,8 +1474,9 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
         for (; u0 < runs.size() && runs[u0].prefix == i; u0++) {
             const Run& u = runs[u0];
             const uint64_t slots = (uint64_t)u.n * group, n_own = (u.pos0 + u.n + part - 1) / part;
-            const uint64_t pre = pre0[i] + (uint64_t)(u.row0 - r) * group;  // the run's first slot in the prefix's partials
+            const uint64_t pre = pre0[i] + (uint64_t)(u.row0 - r) * group;  // the run's first partial of the prefix
             const uint32_t tab = tab_of(u.seq);
+            const bool whole = n_own == 1 && (P.wide || n_pre == 0);
             for (uint64_t j = 0; j < n_own; j++)
                 for (uint64_t s0 = 0; s0 < slots; s0 += kSlotTile) {
                     const uint32_t ns = (uint32_t)std::min<uint64_t>(kSlotTile, slots - s0);
@@ -1467,10 +1484,10 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
                     if (j * part >= end) continue;
                     P.items.push_back({tab, u.row0, (uint32_t)s0, ns, u.pos0, (uint32_t)(j * part),
                                        (uint32_t)std::min<uint64_t>(end, (j + 1) * part),
-                                       n_own == 1 ? kNoSlot : (uint32_t)(P.n_parts + j * slots + s0), (uint32_t)(pre + s0),
-                                       p_slots, n_pre, 0});
+                                       whole ? kNoSlot : (uint32_t)(P.n_parts + j * slots + s0),
+                                       (uint32_t)(pre + s0), p_slots, n_pre, 0});
                 }
-            if (n_own == 1) continue;
+            if (whole) continue;
             for (uint32_t t = 0; t < u.n; t++)
                 P.merges.push_back({u.row0 + t, (uint32_t)(P.n_parts + (uint64_t)t * group), (uint32_t)slots,
                                     (uint32_t)((u.pos0 + t) / part + 1), (uint32_t)(pre + (uint64_t)t * group), p_slots,
@@ -1478,11 +1495,28 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
             P.n_parts += n_own * slots;
         }
     }
-    // Longest first, so that no launch ends on a long item.
-    for (auto* items : {&P.items, &P.pitems})
+    // Rows of one or two slots leave tiles of 16 nearly empty: vector units (12
+    // layers x 64 rows of 1..255 keys, one slot: 64 against 71 us; four slots, 48
+    // rows x 8 heads x 128 of 1..511 keys: 17.1 against 16.0).
+    const bool shared = !P.wide && !P.pitems.empty();  // with the prefixes' items
+    if (shared) {
+        P.items.insert(P.items.end(), P.pitems.begin(), P.pitems.end());
+        P.pitems.clear();
+    }
+    const bool rows_alone = std::all_of(runs.begin(), runs.end(), [](const Run& u) { return u.n == 1; });
+    P.row_slots = !is_q8(kv->o) && !shared && group <= 2 && rows_alone ? group : 0;
+    // Longest first, so that no launch ends on a long item.  Of a launch whose
+    // workgroups are all on the CUs at once, block b shares a CU with blocks b +-
+    // CUs, b +- 2 CUs: every second round of CUs runs shortest first.
+    for (auto* items : {&P.items, &P.pitems}) {
         std::stable_sort(items->begin(), items->end(), [](const PrefixItem& x, const PrefixItem& y) {
             return x.kv_end - x.kv_begin > y.kv_end - y.kv_begin;
         });
+        const size_t round = (size_t)(cus / lh), n = items->size();
+        if (round > 0 && n * lh <= 4 * cus)
+            for (size_t i = round; i < n; i += 2 * round)
+                std::reverse(items->begin() + i, items->begin() + std::min(i + round, n));
+    }
     if (P.n_parts >= (1ull << 31) || std::max(P.items.size(), P.pitems.size()) * lh >= (1ull << 31) ||
         P.merges.size() * lh * group >= (1ull << 31))
         return kv->fail(NI_ERR_BAD_ARG, "rows * layers * heads too large for one call");
@@ -2151,6 +2185,7 @@ int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_r
     if (!P.pitems.empty()) {
         a.off_items = (uint32_t)off_pitems;
         a.n_items = (uint32_t)P.pitems.size();
+        a.wide = P.wide;
         a.waves = P.waves;
         ProfileScope ps(kv, NI_K_ATTN);
         e = launch_prefix_attention(a, ref.inl, ref.inl_bytes, s, ps.t);
@@ -2158,7 +2193,8 @@ int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_r
     if (e == hipSuccess) {
         a.off_items = 0;
         a.n_items = (uint32_t)P.items.size();
-        a.waves = 0;
+        a.wide = a.waves = 0;
+        a.row_slots = P.row_slots;
         ProfileScope ps(kv, NI_K_ATTN);
         e = launch_prefix_attention(a, ref.inl, ref.inl_bytes, s, ps.t);
     }

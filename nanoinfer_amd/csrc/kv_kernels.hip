@@ -47,22 +47,6 @@
 namespace ni {
 namespace {
 
-// Cross-lane move inside a row of 16 lanes (DPP; no LDS traffic).
-template <int CTRL>
-__device__ __forceinline__ float dpp_move(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
-}
-
-// Sum over the LPK consecutive lanes that hold one key row (LPK = 8 or 16).
-template <int LPK>
-__device__ __forceinline__ float key_sum(float x) {
-    x += dpp_move<0xb1>(x);                            // quad_perm(1,0,3,2): lane ^ 1
-    x += dpp_move<0x4e>(x);                            // quad_perm(2,3,0,1): lane ^ 2
-    if constexpr (LPK >= 8) x += dpp_move<0x141>(x);   // row_half_mirror: the other quad of 8
-    if constexpr (LPK >= 16) x += dpp_move<0x140>(x);  // row_mirror: the other 8 of 16
-    return x;
-}
-
 // (m, l, o) <- (m, l, o) (+) (m2, l2, o2): the log-sum-exp merge of two
 // partial softmax states (batch.metal:415-423), base 2.
 template <int N>

@@ -66,6 +66,8 @@ hipError_t launch_append_rotary(const AppendRotaryLaunch& a, const CacheRotary& 
 constexpr uint32_t kSlotTile = 16;            // slots of an item
 constexpr uint32_t kWideSlots = 32;           // slots of one wave of a wide item ...
 constexpr uint32_t kWideWavesMax = 4;         // ... of this many waves at most
+// Groups of waves that share a wide workgroup's keys.
+constexpr int wide_groups(int head_dim, int waves) { return head_dim == 64 ? (waves <= 2 ? 4 : 2) : 2; }
 constexpr uint32_t kWholePos = 0x7fffffffu;   // PrefixItem::pos0 of a prefix: every slot sees every key
 
 // One work item: slots slot0 .. slot0 + ns - 1 of the run of rows at row0 over
@@ -108,7 +110,9 @@ struct PrefixLaunch {
     uint32_t n_items, n_merges;
     uint32_t layer0, n_lay;
     uint32_t group;  // G
-    uint32_t waves;  // 0: items of up to kSlotTile slots; else of kWideSlots * waves slots of a prefix (f16)
+    uint32_t wide;       // items of up to kWideSlots * waves slots of a prefix (f16), else of up to kSlotTile
+    uint32_t waves;      // wide: waves of slots
+    uint32_t row_slots;  // 1, 2: every item is one row of at most this many slots (f16); 0: not so
     float qscale;    // log2(e) / sqrt(head_dim)
 };
 hipError_t launch_prefix_attention(const PrefixLaunch& a, const void* inline_plan, uint32_t inline_bytes,

@@ -5,19 +5,22 @@
 //   prefix_attn_kernel   16 slots (query heads of rows that read the same
 //                        cache head) over a run of keys; of a sequence's own
 //                        keys it joins the prefix's partials and writes out
+//   prefix_rows_kernel   the same for one or two slots of one row
 //   prefix_wide_kernel   up to 128 slots over a run of a prefix's keys
 //   prefix_merge_kernel  each slot's partial softmax states joined, where a
 //                        sequence's own keys are partitioned too
 //
 // A prefix's keys leave memory once per 16 to 128 slots instead of once per
 // row, and each product of the matrix cores serves all of them.
+#include <type_traits>
+
 #include "kv_device.h"
 #include "ops_plan.h"
 
 namespace ni {
 namespace {
 
-constexpr int kPW = 4;               // waves of a workgroup: each takes every fourth page of the item
+constexpr int kItemWaves = 4;        // waves of an item's workgroup
 constexpr int kMergeWaves = 4;       // slots a merge workgroup joins
 constexpr float kPScale = 16384.f;   // weights enter PV times 2^14: down to 4e-9 they are normal f16
 constexpr float kPUnscale = 1.f / kPScale;
@@ -26,18 +29,21 @@ constexpr float kPUnscale = 1.f / kPScale;
 // parts), the online softmax down its columns, O^T += V^T P^T (p in hi + lo
 // parts).  Lane l holds slot l % 16 and keys, then dims, 4 (l / 16) .. + 3.
 // Pages go to LDS row major and come back as operands, V through the
-// transposing read.  The four waves' states are joined through LDS.
+// transposing read.  The W waves take every W-th page each; their states are joined
+// through LDS.  An item that writes out starts from its prefix's partials, every
+// W-th of them a wave, which arrive while the first pages do.
 template <int D, int INL, bool Q8>
-__global__ __launch_bounds__(64 * kPW) void prefix_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
+__global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
+    constexpr int W = kItemWaves;
     constexpr int QC = D / 32;       // 32-dim chunks of QK
     constexpr int VC = D / 16;       // 16-dim chunks of PV
     constexpr int CH = D / 8;        // 16-byte chunks of an f16 row
     constexpr int LD = Q8 ? D / 64 : D / 32;  // 16-byte loads a lane makes of a page's K, and of its V
     constexpr size_t kTile = (size_t)kPage * D * 2;
-    constexpr size_t kRed = (size_t)kPW * kSlotTile * (D + 2) * 4;
-    constexpr size_t kLds = 2 * kPW * kTile > kRed ? 2 * kPW * kTile : kRed;
+    constexpr size_t kRed = (size_t)W * kSlotTile * (D + 2) * 4;
+    constexpr size_t kLds = 2 * W * kTile > kRed ? 2 * W * kTile : kRed;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
-    auto& red = *reinterpret_cast<float(*)[kPW][kSlotTile][D + 2]>(lds);
+    auto& red = *reinterpret_cast<float(*)[W][kSlotTile][D + 2]>(lds);
 
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -108,13 +114,29 @@ __global__ __launch_bounds__(64 * kPW) void prefix_attn_kernel(const PrefixLaunc
     float4_t o[VC];
 #pragma unroll
     for (int c = 0; c < VC; c++) o[c] = float4_t{0.f, 0.f, 0.f, 0.f};
+    if (it.part0 == kNoSlot && has) {
+        for (uint32_t j = wave; j < it.n_pre; j += W) {
+            const uint64_t part = ((uint64_t)(it.pre0 + col + j * it.pre_stride) * a.n_lay + lay) * H + head;
+            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * part);
+            float4_t x[VC];
+#pragma unroll
+            for (int c = 0; c < VC; c++)
+                x[c] = *reinterpret_cast<const float4_t*>(a.part_o + part * D + c * 16 + 4 * rg);
+            const float mn = fmaxf(m, ml.x);
+            const float keep = fast_exp2(m - mn), take = fast_exp2(ml.x - mn) * kPScale;
+            m = mn;
+            lsum = lsum * keep + (rg == 0 ? ml.y * take : 0.f);  // (summed over the slot's four lanes at the end)
+#pragma unroll
+            for (int c = 0; c < VC; c++) o[c] = o[c] * keep + x[c] * take;
+        }
+    }
     // Q8: weights enter PV times scale / vref, so that no f16 overflows: vref
     // starts at 1 and follows the largest value scale past it.
     float vref = 1.f, vinv = 1.f;
 
-    for (; pg < pg_end; pg += kPW) {
+    for (; pg < pg_end; pg += W) {
         Regs nxt;
-        if (pg + kPW < pg_end) load(pg + kPW, nxt);
+        if (pg + W < pg_end) load(pg + W, nxt);
         // Rows past kv_end enter as zeros: whatever the page holds there may
         // not reach a product, not even with weight 0.
 #pragma unroll
@@ -249,7 +271,7 @@ __global__ __launch_bounds__(64 * kPW) void prefix_attn_kernel(const PrefixLaunc
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        if (pg + kPW < pg_end) cur = nxt;
+        if (pg + W < pg_end) cur = nxt;
     }
     lsum = rows4_sum(lsum);
     __syncthreads();  // the tiles' LDS becomes `red`
@@ -264,44 +286,19 @@ __global__ __launch_bounds__(64 * kPW) void prefix_attn_kernel(const PrefixLaunc
             for (int j = 0; j < 4; j++) red[wave][col][2 + c * 16 + 4 * rg + j] = o[c][j] * (kPUnscale * vref);
     }
     __syncthreads();
-    for (uint32_t t = threadIdx.x; t < it.ns * D; t += 64 * kPW) {
+    for (uint32_t t = threadIdx.x; t < it.ns * D; t += 64 * W) {
         const uint32_t sl = t / D, d = t - sl * D;
         float M = red[0][sl][0];
 #pragma unroll
-        for (int w = 1; w < kPW; w++) M = fmaxf(M, red[w][sl][0]);
+        for (int w = 1; w < W; w++) M = fmaxf(M, red[w][sl][0]);
         float L = 0.f, O = 0.f;
 #pragma unroll
-        for (int w = 0; w < kPW; w++) {
+        for (int w = 0; w < W; w++) {
             const float wt = fast_exp2(red[w][sl][0] - M);
             L += red[w][sl][1] * wt;
             O += red[w][sl][2 + d] * wt;
         }
         if (it.part0 == kNoSlot) {
-            constexpr int B = 4;  // partials in flight; past the last it is read again and weighs nothing
-            for (uint32_t j = 0; j < it.n_pre; j += B) {
-                float pm[B], pl[B], po[B], mn = M;
-#pragma unroll
-                for (int i = 0; i < B; i++) {
-                    const uint32_t idx = it.pre0 + sl + min(j + i, it.n_pre - 1) * it.pre_stride;
-                    const uint64_t part = ((uint64_t)idx * a.n_lay + lay) * H + head;
-                    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * part);
-                    pm[i] = ml.x;
-                    pl[i] = ml.y;
-                    po[i] = a.part_o[part * D + d];
-                }
-#pragma unroll
-                for (int i = 0; i < B; i++) mn = fmaxf(mn, pm[i]);
-                const float wt = fast_exp2(M - mn);
-                L *= wt;
-                O *= wt;
-                M = mn;
-#pragma unroll
-                for (int i = 0; i < B; i++) {
-                    const float w = fast_exp2(pm[i] - mn);
-                    L += j + i < it.n_pre ? pl[i] * w : 0.f;
-                    O += j + i < it.n_pre ? po[i] * w : 0.f;
-                }
-            }
             const uint32_t r = (it.slot0 + sl) / a.group, gg = it.slot0 + sl - r * a.group;
             a.out[(int64_t)lay * a.out_layer_stride + (int64_t)(it.row0 + r) * a.out_row_stride +
                   (head * a.group + gg) * D + d] = O / L;
@@ -316,9 +313,188 @@ __global__ __launch_bounds__(64 * kPW) void prefix_attn_kernel(const PrefixLaunc
     }
 }
 
-// Wide items: W waves of 32 slots each over tiles of 32 keys of a prefix, which
-// the waves copy to LDS by DMA (a ring of three tiles, one barrier per tile) and
-// all read.  Of the 32 x 32 x 16 products S^T = K Q^T and O^T += V^T P^T lane l
+// Items of one row's own keys and up to NS slots (a row's query heads of one
+// cache head), on the vector units: fewer instructions a page than tiles of 16
+// slots that stay nearly empty.  A lane holds 8 dims of a key row (D / 8 lanes a
+// row, KPL rows a load), a group of lanes its own softmax state over the rows it
+// sees; q.k and p.v mix f32 with the f16 of the cache.  Groups and waves start
+// from the prefix's partials, every (W KPL)-th a group, and are joined at the end.
+template <int D, int NS, int INL>
+__global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
+    constexpr int W = kItemWaves;
+    constexpr int LPK = D / 8;               // lanes of a key row
+    constexpr int KPL = 64 / LPK;            // rows of a load
+    constexpr int LPP = (int)kPage / KPL;    // loads of a page
+    constexpr int PB = D == 64 ? 2 : 1;      // pages of an iteration
+    __shared__ float red[W][NS][D + 2];
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t H = a.pool.n_head, lh = a.n_lay * H;
+    const uint8_t* plan = plan_base(pa, a.plan);
+    const uint32_t item_i = blockIdx.x / lh;
+    const uint32_t rem = blockIdx.x - item_i * lh;
+    const uint32_t lay = rem / H, head = rem - lay * H;
+    const PrefixItem it = reinterpret_cast<const PrefixItem*>(plan + a.off_items)[item_i];
+    const int kl = lane / LPK, ds = lane % LPK;
+    const uint64_t off = (uint64_t)(a.layer0 + lay) * a.pool.layer_halves + (uint64_t)head * a.pool.head_halves;
+    const uint32_t* __restrict__ tab = reinterpret_cast<const uint32_t*>(plan + a.off_table) + it.tab;
+    const uint32_t pg_end = (it.kv_end + kPage - 1) / kPage;
+    struct Regs {
+        u32x4 k[PB][LPP], v[PB][LPP];
+    };
+    auto load = [&](uint32_t pg, Regs& r) {
+#pragma unroll
+        for (int b = 0; b < PB; b++) {
+            const uint64_t at = off + (uint64_t)tab[min(pg + b, pg_end - 1)] * a.pool.page_halves;  // (past the end: masked)
+            const u32x4* kp = reinterpret_cast<const u32x4*>(a.pool.k + at) + lane;
+            const u32x4* vp = reinterpret_cast<const u32x4*>(a.pool.v + at) + lane;
+#pragma unroll
+            for (int i = 0; i < LPP; i++) r.k[b][i] = load16(kp + 64 * i);
+#pragma unroll
+            for (int i = 0; i < LPP; i++) r.v[b][i] = load16(vp + 64 * i);
+        }
+    };
+    Regs cur;
+    uint32_t pg = it.kv_begin / kPage + wave * PB;
+    if (pg < pg_end) load(pg, cur);
+    float q[NS][8], m[NS], l[NS], o[NS][8];
+    {
+        // slot s of a row is query head s of the cache head (past ns: the first again, its result unused)
+        const float* qb = a.q + (int64_t)lay * a.q_layer_stride + (int64_t)it.row0 * a.q_row_stride +
+                          (head * a.group + it.slot0) * D + ds * 8;
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const float* p = qb + (s < (int)it.ns ? s : 0) * D;
+            const float4 x0 = reinterpret_cast<const float4*>(p)[0], x1 = reinterpret_cast<const float4*>(p)[1];
+            const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+            for (int e = 0; e < 8; e++) q[s][e] = x[e] * a.qscale;
+            m[s] = kMinScore;
+            l[s] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[s][e] = 0.f;
+        }
+    }
+    if (it.part0 == kNoSlot) {
+        for (uint32_t j = wave * KPL + kl; j < it.n_pre; j += W * KPL) {
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                const uint32_t idx = it.pre0 + (s < (int)it.ns ? s : 0) + j * it.pre_stride;
+                const uint64_t part = ((uint64_t)idx * a.n_lay + lay) * H + head;
+                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * part);
+                const float4* po = reinterpret_cast<const float4*>(a.part_o + part * D + ds * 8);
+                const float4 x0 = po[0], x1 = po[1];
+                const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+                const float mn = fmaxf(m[s], ml.x);
+                const float keep = fast_exp2(m[s] - mn), take = fast_exp2(ml.x - mn);
+                m[s] = mn;
+                l[s] = l[s] * keep + ml.y * take;
+#pragma unroll
+                for (int e = 0; e < 8; e++) o[s][e] = o[s][e] * keep + x[e] * take;
+            }
+        }
+    }
+    for (; pg < pg_end; pg += W * PB) {
+        Regs nxt;
+        if (pg + W * PB < pg_end) load(pg + W * PB, nxt);
+        if ((pg + PB) * kPage > it.kv_end) {
+            // Rows past the end: their scores are -inf below, and whatever V
+            // holds there may not meet a weight, not even 0.
+#pragma unroll
+            for (int b = 0; b < PB; b++)
+#pragma unroll
+                for (int i = 0; i < LPP; i++)
+                    if ((pg + b) * kPage + i * KPL + kl >= it.kv_end) cur.v[b][i] = u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            float sc[PB][LPP], mx = m[s];
+#pragma unroll
+            for (int b = 0; b < PB; b++)
+#pragma unroll
+                for (int i = 0; i < LPP; i++) {
+                    const half8_t k = __builtin_bit_cast(half8_t, cur.k[b][i]);
+                    float x = 0.f, y = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        x += q[s][e] * (float)k[e];
+                        y += q[s][e + 1] * (float)k[e + 1];
+                    }
+                    x = key_sum<LPK>(x + y);
+                    sc[b][i] = (pg + b) * kPage + i * KPL + kl < it.kv_end ? x : -INFINITY;
+                    mx = fmaxf(mx, sc[b][i]);
+                }
+            const float keep = fast_exp2(m[s] - mx);
+            m[s] = mx;
+            l[s] *= keep;
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[s][e] *= keep;
+#pragma unroll
+            for (int b = 0; b < PB; b++)
+#pragma unroll
+                for (int i = 0; i < LPP; i++) {
+                    const half8_t v = __builtin_bit_cast(half8_t, cur.v[b][i]);
+                    const float p = fast_exp2(sc[b][i] - mx);
+                    l[s] += p;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) o[s][e] += p * (float)v[e];
+                }
+        }
+        if (pg + W * PB < pg_end) cur = nxt;
+    }
+    // The wave's groups, then the waves.
+#pragma unroll
+    for (int s = 0; s < NS; s++) {
+#pragma unroll
+        for (int st = LPK; st < 64; st <<= 1) {
+            const float m2 = __shfl_xor(m[s], st), l2 = __shfl_xor(l[s], st);
+            const float mn = fmaxf(m[s], m2);
+            const float a1 = fast_exp2(m[s] - mn), a2 = fast_exp2(m2 - mn);
+            m[s] = mn;
+            l[s] = l[s] * a1 + l2 * a2;
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[s][e] = o[s][e] * a1 + __shfl_xor(o[s][e], st) * a2;
+        }
+        if (kl == 0) {
+            if (ds == 0) {
+                red[wave][s][0] = m[s];
+                red[wave][s][1] = l[s];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) red[wave][s][2 + ds * 8 + e] = o[s][e];
+        }
+    }
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < it.ns * D; t += 64 * W) {
+        const uint32_t s = t / D, d = t - s * D;
+        float M = red[0][s][0];
+#pragma unroll
+        for (int w = 1; w < W; w++) M = fmaxf(M, red[w][s][0]);
+        float L = 0.f, O = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const float wt = fast_exp2(red[w][s][0] - M);
+            L += red[w][s][1] * wt;
+            O += red[w][s][2 + d] * wt;
+        }
+        if (it.part0 == kNoSlot) {
+            a.out[(int64_t)lay * a.out_layer_stride + (int64_t)it.row0 * a.out_row_stride +
+                  (head * a.group + it.slot0 + s) * D + d] = O / L;
+        } else {
+            const uint64_t part = ((uint64_t)(it.part0 + s) * a.n_lay + lay) * H + head;
+            a.part_o[part * D + d] = O;
+            if (d == 0) {
+                a.part_ml[2 * part] = M;
+                a.part_ml[2 * part + 1] = L;
+            }
+        }
+    }
+}
+
+// Wide items: W waves of 32 slots each, KG times over, over tiles of 32 keys of a
+// prefix.  Each group of W waves takes every KG-th tile: it copies them to LDS by
+// DMA (a ring of four tiles, one barrier a tile), and all its waves read them.  The
+// groups' states are joined at the end.  Of the 32 x 32 x 16 products S^T = K Q^T and O^T += V^T P^T lane l
 // holds slot l % 32: a slot's softmax state lives in two lanes, and S^T's
 // registers are PV's operand as they are (keys 8 (i / 4) + 4 (l / 32) + i % 4 of
 // register i, in V's transposing reads alike).  Every slot sees every key, so
@@ -336,8 +512,8 @@ __device__ __forceinline__ void wait_dma(uint32_t ahead) {  // at most `ahead` t
         __builtin_amdgcn_s_waitcnt(0x0f70);
 }
 
-template <int D, int W, int INL>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : W >= 3 ? 4 : 3, 8))) void prefix_wide_kernel(
+template <int D, int W, int KG, int INL>
+__global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : 3, 8))) void prefix_wide_kernel(
     const PrefixLaunch a, const PlanArg<INL> pa) {
     constexpr int KS = D / 16;                // 16-dim steps of QK
     constexpr int DB = D / 32;                // 32-dim blocks of PV
@@ -347,12 +523,17 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 128
     constexpr int NI = 2 * TB / 1024;         // 1 KB copies of a tile
     constexpr int ND = (NI + W - 1) / W;      // of one wave (the last again, where they do not divide)
     constexpr int WR = 64 / CH;               // rows of one copy
-    constexpr int NS = 3;                     // tiles of the ring
+    constexpr int NS = 4;                     // tiles of the ring
     constexpr float kHi = kWideSlack + kWideLog2;
-    __shared__ __attribute__((aligned(16))) uint8_t ring[NS][2 * TB];
+    constexpr size_t kRing = (size_t)KG * NS * 2 * TB;
+    constexpr int SW = 16 * DB + 2;           // a lane's state: o, then its slot's m and l
+    static_assert((size_t)(KG - 1) * W * SW * 64 * 4 <= kRing, "the groups' states are joined in the ring");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kRing];
 
     const int lane = threadIdx.x & 63;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t kg = wave_all / W, wave = wave_all - kg * W;  // group of keys, wave of slots
+    uint8_t(*const ring)[2 * TB] = reinterpret_cast<uint8_t(*)[2 * TB]>(lds + kg * NS * 2 * TB);
     const uint32_t H = a.pool.n_head, lh = a.n_lay * H;
     const uint8_t* plan = plan_base(pa, a.plan);
     const uint32_t item_i = blockIdx.x / lh;
@@ -366,33 +547,54 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 128
     const uint64_t page_bytes = 2 * a.pool.page_halves;
     const __attribute__((address_space(4))) uint32_t* tab =
         (const __attribute__((address_space(4))) uint32_t*)(plan + a.off_table) + it.tab;
-    const uint32_t pg0 = it.kv_begin / kPage, pg_end = (it.kv_end + kPage - 1) / kPage;
-    const uint32_t n_tiles = (pg_end - pg0 + TP - 1) / TP;
+    // The group's tiles: every KG-th of the item's.
+    const uint32_t pg0 = it.kv_begin / kPage + kg * TP, pg_end = (it.kv_end + kPage - 1) / kPage;
+    const uint32_t all_tiles = (pg_end - it.kv_begin / kPage + TP - 1) / TP;
+    const uint32_t n_tiles = (all_tiles + KG - 1 - kg) / KG;
+    constexpr uint32_t PS = KG * TP;  // pages from a tile of the group to its next
 
     // Copy i of a tile: rows (i % (NI/2)) * WR .. of K (i < NI/2) or V.  Lane
     // l's 16 bytes land at 16 l of the copy's 1 KB: logical chunk (l % CH) ^ sw
     // of row l / CH.  A row past the item's end copies row 0 of its page, a
     // page past it the item's last page: keys of the item, whose weights the
     // last tile makes 0.
+    // (A copy's row and swizzle are bits of their own above the lane's, so its
+    // offsets are the lane's in copy 0 with the copy's bits flipped.)
     const uint32_t lds_ring = (uint32_t)(uintptr_t)NI_LDS(&ring[0][0]);
+    const uint32_t lane_o =
+        (uint32_t)(lane / CH) * D * 2 + ((lane % CH) ^ (tile_chunk<CH>(lane / CH, 0) - lane / CH * CH)) * 16;
+    uint32_t flip[ND], row0[ND], to[ND];  // of this wave's copies (kept in scalars: the same in every tile)
+    uint64_t from[ND];
+#pragma unroll
+    for (int j = 0; j < ND; j++) {
+        const uint32_t i = min(wave + j * W, (uint32_t)NI - 1);
+        row0[j] = (i % (NI / 2)) * WR;
+        const uint32_t rp = row0[j] % kPage;
+        flip[j] = rp * D * 2 | (tile_chunk<CH>(rp, 0) - rp * CH) * 16;
+        to[j] = lds_ring + 1024 * i;
+        from[j] = reinterpret_cast<uint64_t>(i >= NI / 2 ? vbase : kbase);
+        asm volatile("" : "+s"(flip[j]), "+s"(row0[j]), "+s"(to[j]), "+s"(from[j]));
+    }
+    uint32_t pid0 = 0, pid1 = 0;  // the pages of the tile to copy next, asked for a tile ahead
+    auto pages = [&](uint32_t ti) {
+        if (ti < n_tiles) {
+            pid0 = tab[pg0 + ti * PS];
+            pid1 = tab[min(pg0 + ti * PS + 1, pg_end - 1)];
+        }
+    };
     auto issue = [&](uint32_t stage, uint32_t ti) {
-        const uint32_t pg = pg0 + ti * TP;
-        const uint32_t pid0 = tab[pg], pid1 = tab[min(pg + 1, pg_end - 1)];
+        const uint32_t pg = pg0 + ti * PS;
+        const uint64_t pb0 = pid0 * page_bytes, pb1 = pid1 * page_bytes;
+        pages(ti + 1);
         const bool cut = (pg + TP) * kPage > it.kv_end;
 #pragma unroll
         for (int j = 0; j < ND; j++) {
-            const uint32_t i = min(wave + j * W, (uint32_t)NI - 1);  // wave-uniform
-            const uint32_t r0 = (i % (NI / 2)) * WR, row = r0 + lane / CH;
-            const uint32_t chunk = (lane % CH) ^ (tile_chunk<CH>(row, 0) - row * CH);
-            uint32_t o = (row % kPage) * D * 2 + chunk * 16;
-            if (cut && pg * kPage + row >= it.kv_end) o = chunk * 16;
-            const uint64_t pb = (uint64_t)(r0 >= kPage ? pid1 : pid0) * page_bytes;
-            lds_dma16_sbase((i >= NI / 2 ? vbase : kbase) + pb, o, lds_ring + stage * 2 * TB + 1024 * i);
+            uint32_t o = lane_o ^ flip[j];
+            if (cut) o = pg * kPage + row0[j] + lane / CH >= it.kv_end ? o & (D * 2 - 1) : o;  // row 0 of the page
+            lds_dma16_sbase(reinterpret_cast<const void*>(from[j] + (row0[j] >= kPage ? pb1 : pb0)), o,
+                            to[j] + stage * 2 * TB);
         }
     };
-    issue(0u, 0);
-    if (n_tiles > 1) issue(1u, 1);
-
     const uint32_t s0 = wave * kWideSlots;
     const bool mine = s0 < it.ns;  // the wave has slots
     const bool has = s0 + col < it.ns;
@@ -408,8 +610,10 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 128
             xq[2 * c + 1] = reinterpret_cast<const float4*>(qb + c * 16)[1];
         }
     }
-    // The loads have landed (and the first tiles, issued before them) before
-    // any further copy: the loop's waits count copies alone.
+    pages(0);
+    for (uint32_t t = 0; t < min(n_tiles, (uint32_t)NS - 1); t++) issue(t, t);
+    // The loads (and the first tiles, issued after them) have landed before any
+    // further copy: the loop's waits count copies alone.
 #pragma unroll
     for (int c = 0; c < 2 * KS; c++) asm volatile("" : : "v"(xq[c].x), "v"(xq[c].y), "v"(xq[c].z), "v"(xq[c].w));
     half8_t qh[KS], ql[KS];
@@ -449,32 +653,62 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 128
         for (int b = 0; b < DB; b++)
             voff[j][b] = TB + tile_chunk<CH>(8 * j + 4 * g2 + vt, 4 * b + 2 * vh + (va >> 1)) * 16 + (va & 1) * 8;
 
-    // (the stage is a variable: the body instantiated per stage spills 70
-    // registers of 256 at head_dim 128)
-    auto tile = [&](uint32_t stage, uint32_t ti) {
-        wait_dma<ND>(min(n_tiles - 1 - ti, 1u));
-        __syncthreads();  // every wave's part of tile ti is there, and every wave is done with tile ti - 1
-        if (ti + NS - 1 < n_tiles) issue(stage == 0 ? NS - 1 : stage - 1, ti + NS - 1);
-        if (!mine) return;
+    // S^T of the tile at `stage`, relative to the reference, with `between(c)`
+    // written behind the products of step c: work that does not depend on them.
+    auto scores = [&](uint32_t stage, auto between) {
         const uint8_t* const st = &ring[stage][0];
         float16_t sc;
 #pragma unroll
         for (int i = 0; i < 16; i++) sc[i] = -mref;
+        half8_t kh[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) kh[c] = *reinterpret_cast<const half8_t*>(st + koff[c]);
 #pragma unroll
         for (int c = 0; c < KS; c++) {
-            const half8_t kh = *reinterpret_cast<const half8_t*>(st + koff[c]);
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[c], sc, 0, 0, 0);
-            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[c], sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[c % 4], ql[c], sc, 0, 0, 0);
+            sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[c % 4], qh[c], sc, 0, 0, 0);
+            asm volatile("" : "+v"(sc));  // the products stay here, not where their sum is used
+            if (c + 4 < KS) kh[c % 4] = *reinterpret_cast<const half8_t*>(st + koff[c + 4]);
+            between(c);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        const uint32_t key0 = (pg0 + ti * TP) * kPage;
-        if (key0 + TK > it.kv_end) {
-#pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (key0 + 8 * (i / 4) + 4 * g2 + i % 4 >= it.kv_end) sc[i] = -INFINITY;
-        }
+        return sc;
+    };
+    auto largest = [](const float16_t& sc) {
         float lm = sc[0];
 #pragma unroll
         for (int i = 1; i < 16; i++) lm = fmaxf(lm, sc[i]);
+        return lm;
+    };
+    // V's operand for keys of page t of the tile at `st`.
+    auto values = [&](const uint8_t* st, int t, half8_t (&v8)[DB]) {
+#pragma unroll
+        for (int b = 0; b < DB; b++) {
+            half4_t v[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+                v[j] = __builtin_bit_cast(
+                    half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) v4fp16_t*)(
+                                 st + voff[j][b] + t * (int)kPage * D * 2)));
+            v8[b] = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+    };
+    float16_t sc;
+    float lm = 0.f;  // the lane's largest score
+    // Tile ti: its weights are taken while the products of tile ti + 1's scores
+    // run, so that neither the vector nor the matrix units wait for the other.
+    auto tile = [&](auto lastc, uint32_t stage, uint32_t ti) {
+        constexpr bool LAST = decltype(lastc)::value;
+        const uint8_t* const st = &ring[stage][0];
+        if constexpr (LAST) {
+            const uint32_t key0 = (pg0 + ti * PS) * kPage;
+            if (key0 + TK > it.kv_end) {
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (key0 + 8 * (i / 4) + 4 * g2 + i % 4 >= it.kv_end) sc[i] = -INFINITY;
+            }
+        }
+        if constexpr (LAST) lm = largest(sc);
         if (__any(lm > kHi || !set)) {
             const u32x2_t sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(lm), __float_as_uint(lm), false, false);
             const float mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])) - kWideLog2;
@@ -490,44 +724,102 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(D == 128
 #pragma unroll
             for (int i = 0; i < 16; i++) sc[i] -= d;
         }
-        float p[16];
+        float ps[4] = {0.f, 0.f, 0.f, 0.f};
+        u32x4 ph[TP], pl[TP];
+        auto weights = [&](int c) {  // values 16 c / KS .. of the 16, in pairs
+            constexpr int N = 16 / KS;
 #pragma unroll
-        for (int i = 0; i < 16; i++) p[i] = fast_exp2(sc[i]);
-        float ps[4];
+            for (int i = c * N; i < (c + 1) * N; i += 2) {
+                const float p0 = fast_exp2(sc[i]), p1 = fast_exp2(sc[i + 1]);
+                ps[(i / 2) % 4] += p0 + p1;
+                uint32_t h, l;
+                split_w16x2(p0, p1, h, l);
+                ph[i / 8][i % 8 / 2] = h;
+                pl[i / 8][i % 8 / 2] = l;
+            }
+        };
+        float16_t next;
+        half8_t v8[TP][DB];
+        values(st, 0, v8[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (LAST) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) ps[i] = (p[4 * i] + p[4 * i + 1]) + (p[4 * i + 2] + p[4 * i + 3]);
+            for (int c = 0; c < KS; c++) weights(c);
+        } else {
+            next = scores((stage + 1) % NS, weights);
+        }
         lsum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        values(st, 1, v8[1]);
 #pragma unroll
         for (int t = 0; t < TP; t++) {
-            u32x4 h, l;
+            const half8_t p_hi = __builtin_bit_cast(half8_t, ph[t]), p_lo = __builtin_bit_cast(half8_t, pl[t]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                uint32_t hh, ll;
-                split_w16x2(p[8 * t + 2 * e], p[8 * t + 2 * e + 1], hh, ll);
-                h[e] = hh;
-                l[e] = ll;
-            }
-            const half8_t ph = __builtin_bit_cast(half8_t, h), pl = __builtin_bit_cast(half8_t, l);
+            for (int b = 0; b < DB; b++) o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[t][b], p_lo, o[b], 0, 0, 0);
 #pragma unroll
-            for (int b = 0; b < DB; b++) {
-                half4_t v[2];
-#pragma unroll
-                for (int j = 0; j < 2; j++)
-                    v[j] = __builtin_bit_cast(
-                        half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) v4fp16_t*)(
-                                     st + voff[j][b] + t * (int)kPage * D * 2)));
-                const half8_t v8 = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, pl, o[b], 0, 0, 0);
-                o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8, ph, o[b], 0, 0, 0);
-            }
+            for (int b = 0; b < DB; b++) o[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v8[t][b], p_hi, o[b], 0, 0, 0);
+        }
+        static_assert(TP == 2, "two pages of V operands");
+        if constexpr (!LAST) {
+            sc = next;
+            lm = largest(sc);
         }
     };
-    for (uint32_t ti = 0, stage = 0; ti < n_tiles; ti++) {
-        tile(stage, ti);
-        stage = stage == NS - 1 ? 0 : stage + 1;
+    const bool busy = mine && n_tiles > 0;
+    wait_dma<ND>(0);
+    __syncthreads();  // tile 0 is there
+    if (busy) {
+        sc = scores(0, [](int) {});
+        lm = largest(sc);
     }
+    // (the stage is a variable: the body instantiated per stage spills
+    // registers at head_dim 128)
+    uint32_t stage = 0;
+    const uint32_t steps = (all_tiles + KG - 1) / KG;
+    for (uint32_t ti = 0; ti + 1 < steps; ti++) {
+        wait_dma<ND>(ti + 2 < n_tiles ? 1 : 0);
+        __syncthreads();  // every wave's part of tile ti + 1 is there, and every wave is done with tile ti - 1
+        if (ti + NS - 1 < n_tiles) issue((ti + NS - 1) % NS, ti + NS - 1);
+        if (busy && ti + 1 < n_tiles) {
+            tile(std::false_type{}, stage, ti);
+            stage = (stage + 1) % NS;
+        }
+    }
+    // (a group with a tile less has kept its last one for here)
+    if (busy) tile(std::true_type{}, stage, n_tiles - 1);
     const u32x2_t sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(lsum), __float_as_uint(lsum), false, false);
     lsum = __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    if constexpr (KG > 1) {  // the other groups' states through LDS to the first
+        __syncthreads();  // every group is done with the ring
+        float* const box = reinterpret_cast<float*>(lds) + wave * SW * 64 + lane;
+        constexpr int GS = W * SW * 64;  // floats of a group
+        if (kg > 0) {
+            float* p = box + (kg - 1) * GS;
+#pragma unroll
+            for (int b = 0; b < DB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) p[(16 * b + i) * 64] = o[b][i];
+            p[16 * DB * 64] = set ? mref : kMinScore;
+            p[(16 * DB + 1) * 64] = lsum;
+        }
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int g = 0; g < KG - 1; g++) {
+            const float* p = box + g * GS;
+            const float m2 = p[16 * DB * 64];
+            const float m1 = set ? mref : kMinScore, mn = fmaxf(m1, m2);
+            const float w1 = fast_exp2(m1 - mn), w2 = fast_exp2(m2 - mn);
+            if (mn > kMinScore) {
+                mref = mn;
+                set = true;
+            }
+            lsum = lsum * w1 + p[(16 * DB + 1) * 64] * w2;
+#pragma unroll
+            for (int b = 0; b < DB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[b][i] = o[b][i] * w1 + p[(16 * b + i) * 64] * w2;
+        }
+    }
     if (!has) return;
     const uint64_t part = ((uint64_t)(it.part0 + s0 + col) * a.n_lay + lay) * H + head;
     if (g2 == 0) {
@@ -610,24 +902,31 @@ __global__ __launch_bounds__(64 * kMergeWaves) void prefix_merge_kernel(const Pr
     for (int e = 0; e < N; e++) dst[64 * e] = O[e] / L;
 }
 
-template <int D, bool Q8>
-hipError_t attn_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s, const LaunchTiming& t) {
+// One workgroup of kItemWaves per (item, layer, head): prefix_attn_kernel or
+// prefix_rows_kernel.
+template <int D>
+hipError_t items_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s, const LaunchTiming& t) {
+    const uint64_t blocks = (uint64_t)a.n_items * a.n_lay * a.pool.n_head;
     return with_plan(a, ip, ib, [&](auto pa) {
         constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
-        return go(prefix_attn_kernel<D, INL, Q8>, (uint64_t)a.n_items * a.n_lay * a.pool.n_head, 64 * kPW, s, t, a, pa);
+        if (a.pool.q8) return go(prefix_attn_kernel<D, INL, true>, blocks, 64 * kItemWaves, s, t, a, pa);
+        if (a.row_slots == 1) return go(prefix_rows_kernel<D, 1, INL>, blocks, 64 * kItemWaves, s, t, a, pa);
+        if (a.row_slots == 2) return go(prefix_rows_kernel<D, 2, INL>, blocks, 64 * kItemWaves, s, t, a, pa);
+        return go(prefix_attn_kernel<D, INL, false>, blocks, 64 * kItemWaves, s, t, a, pa);
     });
 }
 
 template <int D>
 hipError_t wide_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s, const LaunchTiming& t) {
     const uint64_t blocks = (uint64_t)a.n_items * a.n_lay * a.pool.n_head;
+    constexpr int K1 = wide_groups(D, 1), K2 = wide_groups(D, 2), K3 = wide_groups(D, 3), K4 = wide_groups(D, 4);
     return with_plan(a, ip, ib, [&](auto pa) {
         constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
         switch (a.waves) {
-            case 1: return go(prefix_wide_kernel<D, 1, INL>, blocks, 64, s, t, a, pa);
-            case 2: return go(prefix_wide_kernel<D, 2, INL>, blocks, 128, s, t, a, pa);
-            case 3: return go(prefix_wide_kernel<D, 3, INL>, blocks, 192, s, t, a, pa);
-            case 4: return go(prefix_wide_kernel<D, 4, INL>, blocks, 256, s, t, a, pa);
+            case 1: return go(prefix_wide_kernel<D, 1, K1, INL>, blocks, 64 * K1, s, t, a, pa);
+            case 2: return go(prefix_wide_kernel<D, 2, K2, INL>, blocks, 128 * K2, s, t, a, pa);
+            case 3: return go(prefix_wide_kernel<D, 3, K3, INL>, blocks, 192 * K3, s, t, a, pa);
+            case 4: return go(prefix_wide_kernel<D, 4, K4, INL>, blocks, 256 * K4, s, t, a, pa);
             default: return hipErrorInvalidValue;
         }
     });
@@ -638,15 +937,9 @@ hipError_t wide_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_
 hipError_t launch_prefix_attention(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s,
                                    const LaunchTiming& t) {
     if (a.n_items == 0) return hipSuccess;
-    if (a.waves) {
-        if (a.pool.q8) return hipErrorInvalidValue;
-        if (a.pool.head_dim == 64) return wide_t<64>(a, ip, ib, s, t);
-        if (a.pool.head_dim == 128) return wide_t<128>(a, ip, ib, s, t);
-        return hipErrorInvalidValue;
-    }
-    if (a.pool.head_dim == 64) return a.pool.q8 ? attn_t<64, true>(a, ip, ib, s, t) : attn_t<64, false>(a, ip, ib, s, t);
-    if (a.pool.head_dim == 128)
-        return a.pool.q8 ? attn_t<128, true>(a, ip, ib, s, t) : attn_t<128, false>(a, ip, ib, s, t);
+    if ((a.wide || a.row_slots) && a.pool.q8) return hipErrorInvalidValue;
+    if (a.pool.head_dim == 64) return a.wide ? wide_t<64>(a, ip, ib, s, t) : items_t<64>(a, ip, ib, s, t);
+    if (a.pool.head_dim == 128) return a.wide ? wide_t<128>(a, ip, ib, s, t) : items_t<128>(a, ip, ib, s, t);
     return hipErrorInvalidValue;
 }
 
