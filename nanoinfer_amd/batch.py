@@ -101,10 +101,9 @@ def _stream_ptr(stream) -> int:
 
 
 def _stream_now(device, stream):
-    """The current stream's handle where no stream is given and `device` is the
-    current one: the quick form of _on.  None otherwise."""
-    if stream is None and _raw_stream is not None and _get_device is not None and _tc.cuda.is_initialized() \
-            and _get_device() == device:
+    """The current stream's handle where no stream is given and `device`, a CUDA
+    tensor's, is the current one: the quick form of _on.  None otherwise."""
+    if stream is None and _raw_stream is not None and _get_device is not None and _get_device() == device:
         return _raw_stream(device)
     return None
 
@@ -186,6 +185,10 @@ def _pointer(arr, empty, item):
 
 
 def _rows(rows) -> tuple:
+    if type(rows) is np.ndarray and rows.dtype is _uint32:
+        shape, flags = rows.shape, rows.flags
+        if len(shape) == 2 and shape[1] == 2 and shape[0] and flags.c_contiguous and flags.writeable:
+            return rows, _no_rows.from_buffer(rows), shape[0]
     arr = np.ascontiguousarray(np.asarray(rows, dtype=np.uint32).reshape(-1, 2))
     return arr, _pointer(arr, _no_rows, _abi.ni_row), arr.shape[0]
 
@@ -521,16 +524,18 @@ class PagedKv:
         heads = 0 if q is None else self._query_heads(q)
         cq, pos, pp = heads * self.opts.head_dim, None, None
         if positions is not None:
-            pos = np.asarray(positions)
-            if pos.size != n or (n and pos.dtype is not _uint32 and
-                                 (pos.dtype.kind not in "iu" or pos.min() < 0 or pos.max() > 0xffffffff)):
-                raise ValueError(f"positions must be {n} integers in 0..2^32-1")
-            pos = np.ascontiguousarray(pos.reshape(-1), dtype=np.uint32)
+            pos = positions
+            if not (type(pos) is np.ndarray and pos.dtype is _uint32 and pos.shape == (n,) and pos.flags.c_contiguous):
+                pos = np.asarray(positions)
+                if pos.size != n or (n and (pos.dtype.kind not in "iu" or pos.min() < 0 or pos.max() > 0xffffffff)):
+                    raise ValueError(f"positions must be {n} integers in 0..2^32-1")
+                pos = np.ascontiguousarray(pos.reshape(-1), dtype=np.uint32)
             pp = _pointer(pos, _no_u32, C.c_uint32)
         fits = _fits_layers if layered else _fits_row
         nl, dev = self._n_layer, self.device
-        ks, s = fits(k, n, self._c, nl, dev), _stream_now(dev, stream)
-        if ks is not None and s is not None and fits(v, n, self._c, nl, dev) == ks:
+        ks = fits(k, n, self._c, nl, dev)
+        s = None if ks is None else _stream_now(dev, stream)
+        if s is not None and fits(v, n, self._c, nl, dev) == ks:
             qs = qos = (0, 0)
             if q is not None:
                 qs, qos = fits(q, n, cq, nl, dev), fits(q_out, n, cq, nl, dev)
@@ -583,8 +588,8 @@ class PagedKv:
         cq = heads * self.opts.head_dim
         fits = _fits_layers if layered else _fits_row
         qs, os_ = fits(q, n, cq, self._n_layer, self.device), fits(out, n, cq, self._n_layer, self.device)
-        s = _stream_now(self.device, stream)
-        if qs is not None and os_ is not None and s is not None:
+        s = None if qs is None else _stream_now(self.device, stream)
+        if os_ is not None and s is not None:
             self._check(self._L.ni_kv_prefix_attention(
                 self._h, layer, q.data_ptr(), qs[0], qs[1], heads, rp, n, pre, len(pre), out.data_ptr(), os_[0], os_[1],
                 split_tokens, s))

@@ -1523,12 +1523,6 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
     return NI_OK;
 }
 
-// Heads one thread rotates with the cosines it computes: four once that still
-// gives every CU 2048 threads.
-uint32_t rotary_heads_per(uint64_t threads_per_head, uint32_t heads) {
-    return threads_per_head * heads >= 4ull * 2048 * device_cus() ? 4u : 1u;
-}
-
 void reset_plan(ni_kv* kv) {
     kv->plan.clear();
     kv->qrows.clear();
@@ -2037,8 +2031,11 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
                         rotary->head_dim, D);
     if (rotary->rot_dim == 0 || rotary->rot_dim > D || rotary->rot_dim % 8 != 0)
         return kv->fail(NI_ERR_BAD_ARG, "rot_dim %u: the cache rotates a multiple of 8, at most %u", rotary->rot_dim, D);
-    if ((uint64_t)n_lay * n * (n_q_head + 2ull * kv->o.n_head) * (D / 8) >= (1ull << 37))
+    if (n_q_head > (1u << 20) || (uint64_t)n_lay * n * ((n_q_head + 2ull * kv->o.n_head) * (D / 8) / 256 + 1) >= (1ull << 31))
         return kv->fail(NI_ERR_BAD_ARG, "n_layer * rows * heads too large");
+    if (kv->o.kv_pages > kMaxRotaryPages)
+        return kv->fail(NI_ERR_BAD_ARG, "kv_pages %u: the rotating append takes at most %u", kv->o.kv_pages,
+                        kMaxRotaryPages);
     // Two rows at one position would race on its slot.
     kv->slot_mark.resize((size_t)kv->o.kv_pages * kPage, 0);
     if (++kv->slot_stamp == 0) {
@@ -2046,17 +2043,17 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
         kv->slot_stamp = 1;
     }
     std::vector<uint8_t>& blob = kv->blob;
-    blob.resize(align_up((size_t)n * sizeof(AppendEntry), kAlign));
-    AppendEntry* entries = reinterpret_cast<AppendEntry*>(blob.data());
+    blob.resize(align_up((size_t)n * sizeof(RotaryEntry), kAlign));
+    RotaryEntry* entries = reinterpret_cast<RotaryEntry*>(blob.data());
     for (uint32_t i = 0; i < n; i++) {
         if (int rc = check_row(kv, rows[i])) return rc;
         const ni_row& r = rows[i];
-        const uint32_t page = kv->pages[r.seq][r.pos / kPage], slot = r.pos % kPage;
-        uint32_t& mark = kv->slot_mark[(size_t)page * kPage + slot];
+        const uint32_t place = kv->pages[r.seq][r.pos / kPage] * kPage + r.pos % kPage;
+        uint32_t& mark = kv->slot_mark[place];
         if (mark == kv->slot_stamp)
             return kv->fail(NI_ERR_BAD_ARG, "sequence %u: position %u appears twice", r.seq, r.pos);
         mark = kv->slot_stamp;
-        entries[i] = {i, page, slot, positions ? positions[i] : r.pos};
+        entries[i] = {positions ? positions[i] : r.pos, place};
     }
     DeviceScope device(kv->device);
     const hipStream_t s = (hipStream_t)stream;
@@ -2081,7 +2078,12 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
     a.layer0 = layer0;
     a.n_lay = n_lay;
     a.n_q_head = n_q_head;
-    a.heads_per = rotary_heads_per((uint64_t)n_lay * n * (D / 8), n_q_head + 2 * kv->o.n_head);
+    // A workgroup to each (layer, row); few of them are cut into up to one per 256
+    // chunks, so that every CU gets some.
+    const uint32_t chunks = (n_q_head + 2 * kv->o.n_head) * (D / 8), most = (chunks + 255) / 256;
+    const uint32_t want = (uint32_t)std::min<uint64_t>(2ull * device_cus() / ((uint64_t)n_lay * n) + 1, most);
+    a.share = (most + want - 1) / want * 256;
+    a.parts = (chunks + a.share - 1) / a.share;
     CacheRotary r{};
     r.rot_dim = rotary->rot_dim;
     r.interleaved = rotary->interleaved;

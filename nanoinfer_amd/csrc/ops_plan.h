@@ -37,8 +37,14 @@ struct CacheRotary {
     uint64_t turns[kCachePairs];
 };
 
-// The append with the rotation on the way (ni_kv_append_rotary).  Entry i is
-// input row i; its `pad` holds the row's position.
+// The append with the rotation on the way (ni_kv_append_rotary).  Entry i: where
+// input row i goes.  Eight bytes, so that up to 256 rows travel in the smallest
+// argument block (160 rows in 16-byte entries: 8.4 us of host time a call, 7.0).
+struct RotaryEntry {
+    uint32_t pos;    // position it is rotated to
+    uint32_t place;  // page * kPage + slot
+};
+constexpr uint32_t kMaxRotaryPages = 0xffffffffu / kPage;
 struct AppendRotaryLaunch {
     PoolGeom pool;
     const float* q;  // null: no queries
@@ -53,8 +59,9 @@ struct AppendRotaryLaunch {
     uint32_t n_rows;
     uint32_t layer0;
     uint32_t n_lay;
-    uint32_t n_q_head;   // 0: no queries
-    uint32_t heads_per;  // heads one thread handles with the same cosines
+    uint32_t n_q_head;  // 0: no queries
+    uint32_t parts;     // workgroups of a (layer, row) ...
+    uint32_t share;     // ... of this many chunks of 8 values each (a multiple of 256)
 };
 hipError_t launch_append_rotary(const AppendRotaryLaunch& a, const CacheRotary& r, const void* inline_plan,
                                 uint32_t inline_bytes, hipStream_t s, const LaunchTiming& t = {});
