@@ -120,6 +120,14 @@ __device__ __forceinline__ void split_w16x2(float x0, float x1, uint32_t& hi, ui
     asm("v_fma_mixhi_f16 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "+v"(lo) : "v"(x1), "v"(hi));
 }
 
+// A matrix product may read what a vector instruction wrote two wait states ago
+// at the earliest.  The compiler sees to that for instructions of its own, not
+// for split_w16x2's: operands that go from there into a product pass through here.
+__device__ __forceinline__ void settle(half4_t& a, half4_t& b) { asm volatile("s_nop 1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ void settle(u32x4& a, u32x4& b, u32x4& c, u32x4& d) {
+    asm volatile("s_nop 1" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+}
+
 // Max and sum over lanes l, l ^ 16, l ^ 32, l ^ 48 (the four lanes holding
 // one query column of an MFMA 16x16 output): v_permlane16_swap and
 // v_permlane32_swap of a value with itself leave the two halves of each

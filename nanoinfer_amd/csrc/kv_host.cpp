@@ -1409,12 +1409,23 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
     const uint64_t lh = (uint64_t)n_lay * kv->o.n_head, cus = device_cus();
     auto between = [](uint64_t x, uint64_t lo, uint64_t hi) { return std::min(std::max(x, lo), hi); };
 
-    // The prefixes.  More than kSlotTile slots behind one go through wide items
-    // (f16): the fewest that hold them, of equal waves.
-    uint64_t most = 0;
+    // The prefixes.  Many slots behind long ones go through wide items: the fewest
+    // that hold them, of equal waves.  Those pay for a launch of their own and a long
+    // start with fewer instructions a key, so they are taken from this many (tile of
+    // 16 slots, key, layer, head) on.  Whole calls, wide against narrow, us: head_dim
+    // 64, 48 thousand 13.7 / 13.9, 192 17.0 / 21.3, 768 26.0 / 34.4; 128, 16 thousand
+    // 16.5 / 12.0, 64 20.1 / 20.4, 128 34.9 / 50.0, 384 43.2 / 59.7; the Q8 cache at 64,
+    // 48 thousand 16.0 / 14.0, 180 (runs of five rows) 20.6 / 17.5, 288 39.9 / 38.6,
+    // 768 28.4 / 33.1, at 128 as f16.
+    uint64_t most = 0, work = 0;
     for (uint32_t i = 0; i < n_prefix; i++)
-        if (prefixes[i].len) most = std::max<uint64_t>(most, (uint64_t)prefixes[i].n_rows * group);
-    P.wide = most > kSlotTile && !is_q8(kv->o);
+        if (prefixes[i].len) {
+            const uint64_t slots = (uint64_t)prefixes[i].n_rows * group;
+            most = std::max(most, slots);
+            work += tiles(slots, kSlotTile) * prefixes[i].len * lh;
+        }
+    const uint64_t wide_from = kv->o.head_dim == 128 ? 64000 : is_q8(kv->o) ? 300000 : 40000;
+    P.wide = most > kSlotTile && work >= wide_from;
     P.waves = 0;
     uint64_t p_tile = kSlotTile;
     if (P.wide) {
@@ -1498,7 +1509,7 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
     // Rows of one or two slots leave tiles of 16 nearly empty: vector units (12
     // layers x 64 rows of 1..255 keys, one slot: 64 against 71 us; four slots, 48
     // rows x 8 heads x 128 of 1..511 keys: 17.1 against 16.0).
-    const bool shared = !P.wide && !P.pitems.empty();  // with the prefixes' items
+    const bool shared = !P.wide && !P.pitems.empty();  // a launch, with the prefixes' items
     if (shared) {
         P.items.insert(P.items.end(), P.pitems.begin(), P.pitems.end());
         P.pitems.clear();

@@ -74,8 +74,8 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
 #pragma unroll
         for (int i = 0; i < LD; i++) r.v[i] = load16(vp + 64 * i);
         if constexpr (Q8) {
-            r.ks = *reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(a.pool.k + at) + kPage * D + 16 * rg);
-            r.vs = *reinterpret_cast<const float4*>(reinterpret_cast<const uint8_t*>(a.pool.v + at) + kPage * D + 16 * rg);
+            r.ks = *reinterpret_cast<const float4*>(q8_block(a.pool, false, at) + kPage * D + 16 * rg);
+            r.vs = *reinterpret_cast<const float4*>(q8_block(a.pool, true, at) + kPage * D + 16 * rg);
         }
     };
     Regs cur;
@@ -228,8 +228,9 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
         uint32_t h0, l0, h1, l1;
         split_w16x2(p[0], p[1], h0, l0);
         split_w16x2(p[2], p[3], h1, l1);
-        const half4_t ph = __builtin_bit_cast(half4_t, u32x2_t{h0, h1});
-        const half4_t pl = __builtin_bit_cast(half4_t, u32x2_t{l0, l1});
+        half4_t ph = __builtin_bit_cast(half4_t, u32x2_t{h0, h1});
+        half4_t pl = __builtin_bit_cast(half4_t, u32x2_t{l0, l1});
+        settle(ph, pl);
         if (__any(oalpha != 1.f)) {
 #pragma unroll
             for (int c = 0; c < VC; c++) o[c] *= oalpha;
@@ -345,7 +346,8 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const Pref
     auto load = [&](uint32_t pg, Regs& r) {
 #pragma unroll
         for (int b = 0; b < PB; b++) {
-            const uint64_t at = off + (uint64_t)tab[min(pg + b, pg_end - 1)] * a.pool.page_halves;  // (past the end: masked)
+            // (a page past the end: the last again, its keys masked)
+            const uint64_t at = off + (uint64_t)tab[min(pg + b, pg_end - 1)] * a.pool.page_halves;
             const u32x4* kp = reinterpret_cast<const u32x4*>(a.pool.k + at) + lane;
             const u32x4* vp = reinterpret_cast<const u32x4*>(a.pool.v + at) + lane;
 #pragma unroll
@@ -502,6 +504,12 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const Pref
 // only past kWideSlack (weights up to 2^15 in f16, as hi + lo).
 constexpr float kWideSlack = 8.f, kWideLog2 = 7.f, kWideUnscale = 1.f / 128.f;
 typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef int v2i32_t __attribute__((ext_vector_type(2)));
+
+// 4 bytes per lane from g to LDS at lds + 4 * lane (as lds_dma16).
+__device__ __forceinline__ void lds_dma4(uint64_t g, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(g), "s"(lds) : "memory", "m0");
+}
 
 template <int N>
 __device__ __forceinline__ void wait_dma(uint32_t ahead) {  // at most `ahead` tiles of N copies of this wave in flight
@@ -512,28 +520,35 @@ __device__ __forceinline__ void wait_dma(uint32_t ahead) {  // at most `ahead` t
         __builtin_amdgcn_s_waitcnt(0x0f70);
 }
 
-template <int D, int W, int KG, int INL>
-__global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : 3, 8))) void prefix_wide_kernel(
-    const PrefixLaunch a, const PlanArg<INL> pa) {
+//
+// Q8: the int8 rows are copied as they are, their 64 scales beside them, and
+// become f16 on their way to the products; key scales multiply the scores, value
+// scales the weights (in units of vref, as in prefix_attn_kernel).
+template <int D, int W, int KG, bool Q8, int INL>
+__global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D == 128 ? 2 : 3, 8)))
+void prefix_wide_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
     constexpr int KS = D / 16;                // 16-dim steps of QK
     constexpr int DB = D / 32;                // 32-dim blocks of PV
-    constexpr int CH = D / 8;                 // 16-byte chunks of a row
+    constexpr int RB = Q8 ? D : 2 * D;        // bytes of a row
+    constexpr int CH = RB / 16;               // 16-byte chunks of a row
     constexpr int TP = 2, TK = TP * kPage;    // pages and keys of a tile
-    constexpr int TB = TK * D * 2;            // bytes of a K (or V) tile
+    constexpr int TB = TK * RB;               // bytes of a K (or V) tile
+    constexpr int SB = 2 * TB + (Q8 ? 256 : 0);  // of a stage: K, V, and scales [page][K|V][16]
     constexpr int NI = 2 * TB / 1024;         // 1 KB copies of a tile
     constexpr int ND = (NI + W - 1) / W;      // of one wave (the last again, where they do not divide)
+    constexpr int NW = ND + (Q8 ? 1 : 0);     // loads of one wave: the scales by every wave
     constexpr int WR = 64 / CH;               // rows of one copy
     constexpr int NS = 4;                     // tiles of the ring
     constexpr float kHi = kWideSlack + kWideLog2;
-    constexpr size_t kRing = (size_t)KG * NS * 2 * TB;
-    constexpr int SW = 16 * DB + 2;           // a lane's state: o, then its slot's m and l
-    static_assert((size_t)(KG - 1) * W * SW * 64 * 4 <= kRing, "the groups' states are joined in the ring");
+    constexpr size_t kStates = (size_t)(KG - 1) * W * (16 * DB + 3) * 64 * 4;
+    constexpr size_t kRing = (size_t)KG * NS * SB > kStates ? (size_t)KG * NS * SB : kStates;
+    constexpr int SW = 16 * DB + 3;           // a lane's state: o, then its slot's m, l and vref
     __shared__ __attribute__((aligned(16))) uint8_t lds[kRing];
 
     const int lane = threadIdx.x & 63;
     const uint32_t wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t kg = wave_all / W, wave = wave_all - kg * W;  // group of keys, wave of slots
-    uint8_t(*const ring)[2 * TB] = reinterpret_cast<uint8_t(*)[2 * TB]>(lds + kg * NS * 2 * TB);
+    uint8_t(*const ring)[SB] = reinterpret_cast<uint8_t(*)[SB]>(lds + kg * NS * SB);
     const uint32_t H = a.pool.n_head, lh = a.n_lay * H;
     const uint8_t* plan = plan_base(pa, a.plan);
     const uint32_t item_i = blockIdx.x / lh;
@@ -560,9 +575,16 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
     // last tile makes 0.
     // (A copy's row and swizzle are bits of their own above the lane's, so its
     // offsets are the lane's in copy 0 with the copy's bits flipped.)
+    auto swizzle = [](uint32_t row) -> uint32_t {  // chunk q of a row lies at q ^ swizzle(row)
+        if constexpr (Q8)
+            return D == 64 ? (row >> 2) & 3 : (row >> 1) & 7;  // the 32 rows of a K operand, 16 of V's: distinct banks
+        else
+            return tile_chunk<CH>(row, 0) - row * CH;
+    };
     const uint32_t lds_ring = (uint32_t)(uintptr_t)NI_LDS(&ring[0][0]);
-    const uint32_t lane_o =
-        (uint32_t)(lane / CH) * D * 2 + ((lane % CH) ^ (tile_chunk<CH>(lane / CH, 0) - lane / CH * CH)) * 16;
+    const uint32_t lane_o = (uint32_t)(lane / CH) * RB + ((lane % CH) ^ swizzle(lane / CH)) * 16;
+    // Q8: lane's scale of page lane / 32, K or V (lane / 16 % 2), position lane % 16.
+    const uint64_t scale_from = reinterpret_cast<uint64_t>(lane & 16 ? vbase : kbase) + kPage * D + 4 * (lane & 15);
     uint32_t flip[ND], row0[ND], to[ND];  // of this wave's copies (kept in scalars: the same in every tile)
     uint64_t from[ND];
 #pragma unroll
@@ -570,7 +592,7 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
         const uint32_t i = min(wave + j * W, (uint32_t)NI - 1);
         row0[j] = (i % (NI / 2)) * WR;
         const uint32_t rp = row0[j] % kPage;
-        flip[j] = rp * D * 2 | (tile_chunk<CH>(rp, 0) - rp * CH) * 16;
+        flip[j] = rp * RB | swizzle(rp) * 16;
         to[j] = lds_ring + 1024 * i;
         from[j] = reinterpret_cast<uint64_t>(i >= NI / 2 ? vbase : kbase);
         asm volatile("" : "+s"(flip[j]), "+s"(row0[j]), "+s"(to[j]), "+s"(from[j]));
@@ -590,10 +612,11 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
 #pragma unroll
         for (int j = 0; j < ND; j++) {
             uint32_t o = lane_o ^ flip[j];
-            if (cut) o = pg * kPage + row0[j] + lane / CH >= it.kv_end ? o & (D * 2 - 1) : o;  // row 0 of the page
+            if (cut) o = pg * kPage + row0[j] + lane / CH >= it.kv_end ? o & (RB - 1) : o;  // row 0 of the page
             lds_dma16_sbase(reinterpret_cast<const void*>(from[j] + (row0[j] >= kPage ? pb1 : pb0)), o,
-                            to[j] + stage * 2 * TB);
+                            to[j] + stage * SB);
         }
+        if constexpr (Q8) lds_dma4(scale_from + (lane & 32 ? pb1 : pb0), lds_ring + stage * SB + 2 * TB);
     };
     const uint32_t s0 = wave * kWideSlots;
     const bool mine = s0 < it.ns;  // the wave has slots
@@ -635,6 +658,7 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
         }
     }
     float mref = 0.f, lsum = 0.f;
+    float vref = 1.f, vinv = 1.f;
     bool set = false;  // the reference is a score's (alike in both lanes of a slot)
     float16_t o[DB];
 #pragma unroll
@@ -643,15 +667,47 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
         for (int i = 0; i < 16; i++) o[b][i] = 0.f;
     // Byte offsets in a stage: K chunk 2c + g2 of row col; V keys 8j + 4 g2 +
     // (0..3), dims 32 b + 16 (l / 16 % 2) + (0..15) of a page.
-    uint32_t koff[KS], voff[2][DB];
+    // (Q8: 8 bytes of K's chunk c; V's keys of both j in one 8-bit transposing
+    // read, whose lane 2e + a of 16 reads bytes 8a .. of row e and lane j receives
+    // byte j of the eight rows.)
+    uint32_t koff[KS], voff[Q8 ? 1 : 2][DB];
     const int vt = (lane >> 2) & 3, va = lane & 3, vh = (lane >> 4) & 1;
 #pragma unroll
-    for (int c = 0; c < KS; c++) koff[c] = tile_chunk<CH>(col, 2 * c + g2) * 16;
+    for (int c = 0; c < KS; c++)
+        koff[c] = Q8 ? col * RB + (c ^ swizzle(col)) * 16 + 8 * g2 : col * RB + ((2 * c + g2) ^ swizzle(col)) * 16;
 #pragma unroll
-    for (int j = 0; j < 2; j++)
+    for (int b = 0; b < DB; b++) {
+        if constexpr (Q8) {
+            const uint32_t e = (lane & 15) >> 1, key = (e < 4 ? 0 : 8) + 4 * g2 + (e & 3);
+            voff[0][b] = TB + key * RB + ((2 * b + vh) ^ swizzle(key)) * 16 + 8 * (lane & 1);
+        } else {
 #pragma unroll
-        for (int b = 0; b < DB; b++)
-            voff[j][b] = TB + tile_chunk<CH>(8 * j + 4 * g2 + vt, 4 * b + 2 * vh + (va >> 1)) * 16 + (va & 1) * 8;
+            for (int j = 0; j < 2; j++) {
+                const uint32_t key = 8 * j + 4 * g2 + vt;
+                voff[j][b] = TB + key * RB + ((4 * b + 2 * vh + (va >> 1)) ^ swizzle(key)) * 16 + (va & 1) * 8;
+            }
+        }
+    }
+    auto key_operand = [&](const uint8_t* st, int c) -> half8_t {
+        if constexpr (Q8) {
+            const uint2 w = *reinterpret_cast<const uint2*>(st + koff[c]);
+            return __builtin_shufflevector(i8x4_f16(w.x), i8x4_f16(w.y), 0, 1, 2, 3, 4, 5, 6, 7);
+        } else {
+            return *reinterpret_cast<const half8_t*>(st + koff[c]);
+        }
+    };
+    // Q8: the scales of the lane's 16 keys, K's (which = 0) or V's.
+    auto scales = [&](uint32_t stage, int which, float (&x)[16]) {
+        const uint8_t* p = &ring[stage][0] + 2 * TB + 64 * which + 16 * g2;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4 y = *reinterpret_cast<const float4*>(p + (i / 2) * 128 + (i % 2) * 32);
+            x[4 * i] = y.x;
+            x[4 * i + 1] = y.y;
+            x[4 * i + 2] = y.z;
+            x[4 * i + 3] = y.w;
+        }
+    };
 
     // S^T of the tile at `stage`, relative to the reference, with `between(c)`
     // written behind the products of step c: work that does not depend on them.
@@ -659,18 +715,24 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
         const uint8_t* const st = &ring[stage][0];
         float16_t sc;
 #pragma unroll
-        for (int i = 0; i < 16; i++) sc[i] = -mref;
+        for (int i = 0; i < 16; i++) sc[i] = Q8 ? 0.f : -mref;
         half8_t kh[4];
 #pragma unroll
-        for (int c = 0; c < 4; c++) kh[c] = *reinterpret_cast<const half8_t*>(st + koff[c]);
+        for (int c = 0; c < 4; c++) kh[c] = key_operand(st, c);
 #pragma unroll
         for (int c = 0; c < KS; c++) {
             sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[c % 4], ql[c], sc, 0, 0, 0);
             sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh[c % 4], qh[c], sc, 0, 0, 0);
             asm volatile("" : "+v"(sc));  // the products stay here, not where their sum is used
-            if (c + 4 < KS) kh[c % 4] = *reinterpret_cast<const half8_t*>(st + koff[c + 4]);
+            if (c + 4 < KS) kh[c % 4] = key_operand(st, c + 4);
             between(c);
             __builtin_amdgcn_sched_barrier(0);
+        }
+        if constexpr (Q8) {
+            float ks[16];
+            scales(stage, 0, ks);
+#pragma unroll
+            for (int i = 0; i < 16; i++) sc[i] = fmaf(sc[i], ks[i], -mref);
         }
         return sc;
     };
@@ -684,13 +746,20 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
     auto values = [&](const uint8_t* st, int t, half8_t (&v8)[DB]) {
 #pragma unroll
         for (int b = 0; b < DB; b++) {
-            half4_t v[2];
+            if constexpr (Q8) {
+                const v2i32_t r = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (__attribute__((address_space(3))) v2i32_t*)(st + voff[0][b] + t * (int)kPage * RB));
+                const half4_t lo = i8x4_f16((uint32_t)r.x), hi = i8x4_f16((uint32_t)r.y);
+                v8[b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            } else {
+                half4_t v[2];
 #pragma unroll
-            for (int j = 0; j < 2; j++)
-                v[j] = __builtin_bit_cast(
-                    half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) v4fp16_t*)(
-                                 st + voff[j][b] + t * (int)kPage * D * 2)));
-            v8[b] = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+                for (int j = 0; j < 2; j++)
+                    v[j] = __builtin_bit_cast(
+                        half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) v4fp16_t*)(
+                                     st + voff[j][b] + t * (int)kPage * RB)));
+                v8[b] = __builtin_shufflevector(v[0], v[1], 0, 1, 2, 3, 4, 5, 6, 7);
+            }
         }
     };
     float16_t sc;
@@ -724,14 +793,41 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
 #pragma unroll
             for (int i = 0; i < 16; i++) sc[i] -= d;
         }
+        float vs[Q8 ? 16 : 1];
+        if constexpr (Q8) {
+            scales(stage, 1, vs);
+            if constexpr (LAST) {  // scales past the end may be anything
+                const uint32_t key0 = (pg0 + ti * PS) * kPage;
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (key0 + 8 * (i / 4) + 4 * g2 + i % 4 >= it.kv_end) vs[i] = 0.f;
+            }
+            float vm = vs[0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) vm = fmaxf(vm, vs[i]);
+            if (__any(vm > vref)) {  // (a scale belongs to its key: the same for every slot)
+                const uint32_t bits = __float_as_uint(vm);
+                const u32x2_t sw = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
+                vm = fmaxf(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])), vref);
+                const float shrink = vref / vm;
+                vref = vm;
+                vinv = 1.f / vm;
+#pragma unroll
+                for (int b = 0; b < DB; b++) o[b] *= shrink;
+            }
+        }
         float ps[4] = {0.f, 0.f, 0.f, 0.f};
         u32x4 ph[TP], pl[TP];
         auto weights = [&](int c) {  // values 16 c / KS .. of the 16, in pairs
             constexpr int N = 16 / KS;
 #pragma unroll
             for (int i = c * N; i < (c + 1) * N; i += 2) {
-                const float p0 = fast_exp2(sc[i]), p1 = fast_exp2(sc[i + 1]);
+                float p0 = fast_exp2(sc[i]), p1 = fast_exp2(sc[i + 1]);
                 ps[(i / 2) % 4] += p0 + p1;
+                if constexpr (Q8) {
+                    p0 *= vs[i] * vinv;
+                    p1 *= vs[i + 1] * vinv;
+                }
                 uint32_t h, l;
                 split_w16x2(p0, p1, h, l);
                 ph[i / 8][i % 8 / 2] = h;
@@ -749,6 +845,7 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
             next = scores((stage + 1) % NS, weights);
         }
         lsum += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        settle(ph[0], pl[0], ph[1], pl[1]);
         values(st, 1, v8[1]);
 #pragma unroll
         for (int t = 0; t < TP; t++) {
@@ -765,7 +862,7 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
         }
     };
     const bool busy = mine && n_tiles > 0;
-    wait_dma<ND>(0);
+    wait_dma<NW>(0);
     __syncthreads();  // tile 0 is there
     if (busy) {
         sc = scores(0, [](int) {});
@@ -776,7 +873,7 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
     uint32_t stage = 0;
     const uint32_t steps = (all_tiles + KG - 1) / KG;
     for (uint32_t ti = 0; ti + 1 < steps; ti++) {
-        wait_dma<ND>(ti + 2 < n_tiles ? 1 : 0);
+        wait_dma<NW>(ti + 2 < n_tiles ? 1 : 0);
         __syncthreads();  // every wave's part of tile ti + 1 is there, and every wave is done with tile ti - 1
         if (ti + NS - 1 < n_tiles) issue((ti + NS - 1) % NS, ti + NS - 1);
         if (busy && ti + 1 < n_tiles) {
@@ -800,6 +897,7 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
                 for (int i = 0; i < 16; i++) p[(16 * b + i) * 64] = o[b][i];
             p[16 * DB * 64] = set ? mref : kMinScore;
             p[(16 * DB + 1) * 64] = lsum;
+            p[(16 * DB + 2) * 64] = vref;
         }
         __syncthreads();
         if (kg > 0) return;
@@ -814,10 +912,11 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
                 set = true;
             }
             lsum = lsum * w1 + p[(16 * DB + 1) * 64] * w2;
+            const float u2 = Q8 ? w2 * (p[(16 * DB + 2) * 64] * vinv) : w2;  // in units of this group's vref
 #pragma unroll
             for (int b = 0; b < DB; b++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[b][i] = o[b][i] * w1 + p[(16 * b + i) * 64] * w2;
+                for (int i = 0; i < 16; i++) o[b][i] = o[b][i] * w1 + p[(16 * b + i) * 64] * u2;
         }
     }
     if (!has) return;
@@ -831,10 +930,11 @@ __global__ __launch_bounds__(64 * W * KG) __attribute__((amdgpu_waves_per_eu(D =
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             float4 y;
-            y.x = o[b][4 * i] * kWideUnscale;
-            y.y = o[b][4 * i + 1] * kWideUnscale;
-            y.z = o[b][4 * i + 2] * kWideUnscale;
-            y.w = o[b][4 * i + 3] * kWideUnscale;
+            const float unit = kWideUnscale * vref;
+            y.x = o[b][4 * i] * unit;
+            y.y = o[b][4 * i + 1] * unit;
+            y.z = o[b][4 * i + 2] * unit;
+            y.w = o[b][4 * i + 3] * unit;
             *reinterpret_cast<float4*>(a.part_o + part * D + 32 * b + 8 * i + 4 * g2) = y;
         }
 }
@@ -916,17 +1016,17 @@ hipError_t items_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream
     });
 }
 
-template <int D>
+template <int D, bool Q8>
 hipError_t wide_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s, const LaunchTiming& t) {
     const uint64_t blocks = (uint64_t)a.n_items * a.n_lay * a.pool.n_head;
     constexpr int K1 = wide_groups(D, 1), K2 = wide_groups(D, 2), K3 = wide_groups(D, 3), K4 = wide_groups(D, 4);
     return with_plan(a, ip, ib, [&](auto pa) {
         constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
         switch (a.waves) {
-            case 1: return go(prefix_wide_kernel<D, 1, K1, INL>, blocks, 64 * K1, s, t, a, pa);
-            case 2: return go(prefix_wide_kernel<D, 2, K2, INL>, blocks, 128 * K2, s, t, a, pa);
-            case 3: return go(prefix_wide_kernel<D, 3, K3, INL>, blocks, 192 * K3, s, t, a, pa);
-            case 4: return go(prefix_wide_kernel<D, 4, K4, INL>, blocks, 256 * K4, s, t, a, pa);
+            case 1: return go(prefix_wide_kernel<D, 1, K1, Q8, INL>, blocks, 64 * K1, s, t, a, pa);
+            case 2: return go(prefix_wide_kernel<D, 2, K2, Q8, INL>, blocks, 128 * K2, s, t, a, pa);
+            case 3: return go(prefix_wide_kernel<D, 3, K3, Q8, INL>, blocks, 192 * K3, s, t, a, pa);
+            case 4: return go(prefix_wide_kernel<D, 4, K4, Q8, INL>, blocks, 256 * K4, s, t, a, pa);
             default: return hipErrorInvalidValue;
         }
     });
@@ -937,10 +1037,11 @@ hipError_t wide_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_
 hipError_t launch_prefix_attention(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s,
                                    const LaunchTiming& t) {
     if (a.n_items == 0) return hipSuccess;
-    if ((a.wide || a.row_slots) && a.pool.q8) return hipErrorInvalidValue;
-    if (a.pool.head_dim == 64) return a.wide ? wide_t<64>(a, ip, ib, s, t) : items_t<64>(a, ip, ib, s, t);
-    if (a.pool.head_dim == 128) return a.wide ? wide_t<128>(a, ip, ib, s, t) : items_t<128>(a, ip, ib, s, t);
-    return hipErrorInvalidValue;
+    if ((a.row_slots && a.pool.q8) || (a.pool.head_dim != 64 && a.pool.head_dim != 128)) return hipErrorInvalidValue;
+    if (!a.wide) return a.pool.head_dim == 64 ? items_t<64>(a, ip, ib, s, t) : items_t<128>(a, ip, ib, s, t);
+    if (a.pool.head_dim == 64)
+        return a.pool.q8 ? wide_t<64, true>(a, ip, ib, s, t) : wide_t<64, false>(a, ip, ib, s, t);
+    return a.pool.q8 ? wide_t<128, true>(a, ip, ib, s, t) : wide_t<128, false>(a, ip, ib, s, t);
 }
 
 hipError_t launch_prefix_merge(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s,

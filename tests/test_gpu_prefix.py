@@ -43,7 +43,7 @@ class Cache:
 
     def stored(self, x):
         o = self.opts
-        x = x.view(o.n_layer, -1, o.n_head, o.head_dim).cpu()
+        x = x.reshape(o.n_layer, -1, o.n_head, o.head_dim)
         if not o.q8:
             return x.half().double()
         scale = (x.abs().amax(-1, keepdim=True).double() / 127).float()
@@ -54,16 +54,17 @@ class Cache:
         """q [n_layer, n, heads * hd] -> the result in 64 bits."""
         o = self.opts
         L, n = q.shape[:2]
-        q = q.double().cpu().view(L, n, o.n_head, -1, o.head_dim)
+        q = q.double().view(L, n, o.n_head, -1, o.head_dim)
         out = torch.empty_like(q)
         at = [(s, m) for s, m, c in prefixes for _ in range(c)]
         for i, ((s, p), (ps, m)) in enumerate(zip(rows, at)):
             k, v = self.k[s][:, :p + 1], self.v[s][:, :p + 1]
             if m:
                 k, v = torch.cat([self.k[ps][:, :m], k], 1), torch.cat([self.v[ps][:, :m], v], 1)
-            w = torch.softmax(torch.einsum("lhgd,lkhd->lhgk", q[:, i], k) / math.sqrt(o.head_dim), -1)
-            out[:, i] = torch.einsum("lhgk,lkhd->lhgd", w, v)
-        return out.reshape(L, n, -1)
+            k, v = k.permute(0, 2, 3, 1).contiguous(), v.transpose(1, 2).contiguous()  # [L, heads, hd, keys] and back
+            w = torch.softmax(torch.matmul(q[:, i], k) / math.sqrt(o.head_dim), -1)
+            out[:, i] = torch.matmul(w, v)
+        return out.reshape(L, n, -1).cpu()
 
     def queries(self, n, group=1, seed=1):
         o = self.opts
@@ -106,7 +107,8 @@ def test_runs_of_rows(gpu, d, q8, split):
     """Verify rows and prompt chunks: consecutive rows share their sequence's
     keys and see them causally; rows of one sequence in other orders do not."""
     c = Cache([60, 31, 200, 150], n_layer=2, n_head=3, head_dim=d, q8=q8, seed=7)
-    rows = [(0, p) for p in range(50, 55)] + [(1, p) for p in range(0, 31)] + [(2, 10), (2, 9), (2, 150), (2, 150), (0, 3)]
+    rows = [(0, p) for p in range(50, 55)] + [(1, p) for p in range(0, 31)]
+    rows += [(2, 10), (2, 9), (2, 150), (2, 150), (0, 3)]
     check(c, rows, [(3, 150, 5), (3, 77, 31), (3, 16, 3), (0, 0, 2)], split_tokens=split)
     check(c, rows, [(3, 150, 4), (3, 150, 2), (3, 1, 35)], 2, split_tokens=split)  # a run across two prefixes
 
@@ -127,6 +129,64 @@ def test_many_rows_and_a_long_prefix(gpu, q8):
     rows = [(i, lens[i] - 1) for i in range(70)]
     check(c, rows, [(70, 5000, 40), (71, 2099, 30)], 2)
     check(c, rows, [(70, 4999, 70)], 1, split_tokens=4096)
+
+
+def large(d, q8):
+    """(layers, heads, positions) from which 17 rows behind a prefix take wide tiles."""
+    return (4, 16, 2400) if q8 and d == 64 else (2, 8, 2050)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [16, 17, 33, 65, 97, 129, 200])
+def test_wide_tiles(gpu, n, d, q8):
+    """One to four waves of slots, one workgroup or two, full and not; prefixes
+    that end inside a tile, inside a page and on a border; one of few rows."""
+    layers, heads, m = large(d, q8)
+    c = Cache([n + 4, m + 40, 71], n_layer=layers, n_head=heads, head_dim=d, q8=q8, seed=n)
+    rows = [(0, p) for p in range(4, n + 4)]
+    check(c, rows, [(1, m, n)])
+    check(c, rows, [(1, m + 33, n - 1), (2, 71, 1)], split_tokens=512)
+    check(c, rows[:n // 2 + 1], [(1, m + 14, n // 2 + 1)], 2, split_tokens=352)
+    check(c, rows[:n // 4 + 1], [(1, m + 16, n // 4 + 1)], 4, split_tokens=m // 16 * 16)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_wide_tiles_of_one_row(gpu, d, q8):
+    """Many query heads of a single row, and runs with keys of their own in parts."""
+    layers, heads, m = large(d, q8)
+    c = Cache([700, m], n_layer=layers, n_head=heads, head_dim=d, q8=q8, seed=3)
+    check(c, [(0, 699)], [(1, m, 1)], 20)
+    check(c, [(0, 650), (0, 651), (0, 652)], [(1, m, 3)], 8)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("n,wide", [(3, False), (40, False), (40, True)])
+def test_values_of_many_sizes(gpu, n, wide, q8):
+    """Values that grow along the keys, to thousands: int8 scales past 1."""
+    layers, heads, m = large(64, q8) if wide else (1, 2, 400)
+    c = Cache([n, m], n_layer=layers, n_head=heads, q8=q8, seed=35)
+    size = torch.logspace(-3, 3.5, m, device=gpu)[None, :, None]
+    g = torch.Generator(device="cuda").manual_seed(36)
+    k, v = (torch.randn((layers, m, heads * 64), generator=g, device="cuda") for _ in range(2))
+    for flip in (False, True):
+        k, v = (k.flip(1), v) if flip else (k, v * size)
+        v = v.flip(1) if flip else v
+        c.put(1, k, v)
+        c.k[1], c.v[1] = c.stored(k), c.stored(v)
+        check(c, [(0, p) for p in range(n)], [(1, m, n)])
+        check(c, [(0, 0)] * n, [(1, m - 1, n)], 3, split_tokens=0 if wide else 96)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_what_lies_behind_a_prefix_does_not_matter_to_wide_tiles(gpu, d):
+    layers, heads, m = large(d, False)
+    c = Cache([30, m + 20], n_layer=layers, n_head=heads, head_dim=d, seed=37)
+    bad = torch.full((layers, 17, heads * d), float("nan"), device=gpu)
+    c.put(1, bad, bad, m + 3)
+    check(c, [(0, p) for p in range(30)], [(1, m + 3, 30)])
+    check(c, [(0, p) for p in range(30)], [(1, m, 30)], split_tokens=1024)
 
 
 def test_layers_and_one_layer(gpu):
