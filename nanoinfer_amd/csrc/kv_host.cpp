@@ -1528,8 +1528,9 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
             for (size_t i = round; i < n; i += 2 * round)
                 std::reverse(items->begin() + i, items->begin() + std::min(i + round, n));
     }
-    if (P.n_parts >= (1ull << 31) || std::max(P.items.size(), P.pitems.size()) * lh >= (1ull << 31) ||
-        P.merges.size() * lh * group >= (1ull << 31))
+    // (a launch holds less than 2^32 threads: workgroups of up to 512, merges of 64 a slot)
+    if (P.n_parts >= (1ull << 31) || std::max(P.items.size(), P.pitems.size()) * lh >= (1ull << 23) ||
+        P.merges.size() * lh * group >= (1ull << 26))
         return kv->fail(NI_ERR_BAD_ARG, "rows * layers * heads too large for one call");
     return NI_OK;
 }
@@ -2042,7 +2043,8 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
                         rotary->head_dim, D);
     if (rotary->rot_dim == 0 || rotary->rot_dim > D || rotary->rot_dim % 8 != 0)
         return kv->fail(NI_ERR_BAD_ARG, "rot_dim %u: the cache rotates a multiple of 8, at most %u", rotary->rot_dim, D);
-    if (n_q_head > (1u << 20) || (uint64_t)n_lay * n * ((n_q_head + 2ull * kv->o.n_head) * (D / 8) / 256 + 1) >= (1ull << 31))
+    // (a launch holds less than 2^32 threads, 256 to a workgroup; small rows are cut into several)
+    if (n_q_head > (1u << 16) || (uint64_t)n_lay * n >= (1ull << 23))
         return kv->fail(NI_ERR_BAD_ARG, "n_layer * rows * heads too large");
     if (kv->o.kv_pages > kMaxRotaryPages)
         return kv->fail(NI_ERR_BAD_ARG, "kv_pages %u: the rotating append takes at most %u", kv->o.kv_pages,

@@ -90,7 +90,8 @@ int ni_rotary_apply(const ni_rotary* r, uint32_t dtype, const void* x, int64_t x
     if (n > 1 && out_row_stride < width)
         return call_error(NI_ERR_BAD_ARG, "out's rows overlap: the row stride must be at least %lld", (long long)width);
     if (!aligned(positions, 4)) return call_error(NI_ERR_BAD_ARG, "positions must be 4-byte aligned");
-    if ((uint64_t)n * width >= (1ull << 38)) return call_error(NI_ERR_BAD_ARG, "n * n_head * head_dim too large");
+    // (a launch holds less than 2^32 threads, each of two values or eight)
+    if ((unsigned __int128)n * width >= (1ull << 32)) return call_error(NI_ERR_BAD_ARG, "n * n_head * head_dim too large");
     RotaryLaunch a{};
     a.x = x;
     a.out = out;
@@ -148,6 +149,9 @@ int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stri
     const size_t need = ni_verify_workspace(n_seq, vocab);
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
         return call_error(NI_ERR_BAD_ARG, "workspace must be %zu bytes, 16-byte aligned", need);
+    // (workgroups of one sequence read the drafts while another writes the answer)
+    if (n_draft > 0 && (accepted == n_drafts || tokens == drafted))
+        return call_error(NI_ERR_BAD_ARG, "accepted and tokens may not share memory with n_drafts and drafted");
     VerifyLaunch a{};
     a.target = target;
     a.target_seq_stride = target_seq_stride;

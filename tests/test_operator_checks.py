@@ -107,6 +107,8 @@ def test_rotary_apply_refuses_before_any_launch():
     assert call(r.ref, 0, p, 64, p, 64, 2, 2) == _abi.NI_ERR_BAD_ARG and "overlap" in _err(L)
     assert call(r.ref, 0, p, 64, p, 64, 1, 1, p + 2) == _abi.NI_ERR_BAD_ARG and "positions" in _err(L)
     assert call(r.ref, 0, p, 1 << 33, p, 1 << 33, 1 << 31, 1 << 10) == _abi.NI_ERR_BAD_ARG and "too large" in _err(L)
+    # a launch holds less than 2^32 threads
+    assert call(r.ref, 0, p, 64, p, 1 << 12, 1 << 20, 1 << 6) == _abi.NI_ERR_BAD_ARG and "too large" in _err(L)
     assert call(r.ref, 0, None, 64, None, 64, 0, 1) == _abi.NI_OK
     assert call(r.ref, 0, None, 64, None, 64, 1, 0) == _abi.NI_OK
 
@@ -226,6 +228,14 @@ def test_verify_refuses_misaligned_pointers():
         q = C.addressof(buf) + 2 if name != "work" else C.addressof(buf) // 16 * 16 + 8
         rc, msg, _ = _verify_call(**{name: q})
         assert rc == _abi.NI_ERR_BAD_ARG and "align" in msg, name
+
+
+def test_verify_refuses_answers_over_its_inputs():
+    other = (C.c_int32 * 64)()
+    q = C.addressof(other)
+    for kw in (dict(n_drafts=q, accepted=q), dict(tokens=q, drafted=q)):
+        rc, msg, _ = _verify_call(**kw)
+        assert rc == _abi.NI_ERR_BAD_ARG and "share" in msg
 
 
 def test_verify_workspace_and_nothing_to_do():
