@@ -87,6 +87,9 @@ __device__ __forceinline__ uint32_t q8_byte(float x, float inv) {
     return (uint32_t)(int32_t)fminf(fmaxf(rintf(x * inv), -127.f), 127.f) & 0xffu;
 }
 
+// Byte j of w as a signed integer, in f32.
+__device__ __forceinline__ float i8f(uint32_t w, int j) { return (float)((int32_t)(w << (24 - 8 * j)) >> 24); }
+
 // K/V loads are non-temporal: each byte is streamed once per step (156 -> 140
 // us per config-3 launch against ordinary loads).
 __device__ __forceinline__ u32x4 load16(const u32x4* p) { return __builtin_nontemporal_load(p); }

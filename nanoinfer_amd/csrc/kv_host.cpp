@@ -140,6 +140,7 @@ struct PrefixPlan {
     std::vector<PrefixItem> items;   // over the sequences' own
     uint32_t wide = 0, waves = 0;  // PrefixLaunch::wide and waves of pitems
     uint32_t row_slots = 0;        // PrefixLaunch::row_slots of items
+    uint32_t row_waves = 0;        // and their waves
     std::vector<PrefixMerge> merges;
     std::vector<uint32_t> table;
     uint64_t n_parts = 0;
@@ -1433,11 +1434,16 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
         P.waves = (uint32_t)tiles(most, kWideSlots * n);
         p_tile = (uint64_t)kWideSlots * P.waves;
     }
-    // Keys per partition: wide workgroups fill a CU each, so as many as there are
-    // CUs and no second round; others four to a CU.
+    // Keys per partition.  Wide workgroups fill a CU each, so as many as there are
+    // CUs and no second round.  Of the others one to a CU keeps the memory busy at 8
+    // KB a page, two at 4 KB or less; more only begin and end more often.  Whole
+    // calls at one, two and four to a CU, us: f16 at head_dim 128, 16 rows behind
+    // 32767 keys 101 / 107 / 112, 4 behind 16000 22 / 26 / 35; at 64, 8 behind 16000
+    // 18.7 / 17.7 / 22.7, the 12 layers of 8 behind 8000 94 / 55 / 57; Q8 at 128, 16
+    // behind 32767 83 / 69 / 76; at 64, 32 x 5 behind 2000 20.6 / 17.5 / 21.3.
     uint64_t p_part = split_tokens;
     if (!p_part) {
-        const uint64_t most_units = (P.wide ? 1 : 4) * cus;
+        const uint64_t most_units = (P.wide || (kv->o.head_dim == 128 && !is_q8(kv->o)) ? 1 : 2) * cus;
         auto units = [&](uint64_t part) {
             uint64_t n = 0;
             for (uint32_t i = 0; i < n_prefix; i++)
@@ -1474,10 +1480,24 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
     // else both kinds share a launch and a merge joins them (2 rows x 12 heads
     // behind 515 keys: 7.2 us, joined at once 8.3; 32 x 5 rows of the Q8 cache behind
     // 2001 17.5, 20.2).
-    uint64_t o_keys = 0;
-    for (const Run& u : runs) o_keys += tiles((uint64_t)u.n * group, kSlotTile) * (u.pos0 + u.n);
+    // Partitions: about four items to a CU of 512 keys or more.  Few items leave
+    // CUs idle and are cut smaller, very few into longer ones; many short ones behind
+    // wide items stay whole, which saves the merge.  By these rules and without them,
+    // us: head_dim 64 x 12 heads, 16 rows of up to 1000 keys 10.6 / 12.1, 4 of up to
+    // 4000 12.4 / 13.1, 64 of up to 1023 behind 1000 26.1 / 30.1; 128 x 8 heads, 8 x 4
+    // rows of up to 8000 50.4 / 56.5.
+    uint64_t o_keys = 0, o_units = 0, o_longest = 0;
+    for (const Run& u : runs) {
+        const uint64_t n = tiles((uint64_t)u.n * group, kSlotTile);
+        o_units += n * lh;
+        o_keys += n * lh * (u.pos0 + u.n);
+        o_longest = std::max<uint64_t>(o_longest, u.pos0 + u.n);
+    }
     uint64_t part = split_tokens;
-    if (!part) part = between(align_up(o_keys * lh / (4 * cus), 4 * kPage), 512, 16384);
+    if (!part) {
+        part = between(align_up(o_keys / ((2 * o_units <= cus ? 2 : 4) * cus), 4 * kPage), o_units < cus ? 256 : 512, 16384);
+        if (P.wide && o_units >= 2 * cus && o_longest <= 1024) part = std::max<uint64_t>(part, 1024);
+    }
     for (uint32_t i = 0, r = 0, u0 = 0; i < n_prefix; r += prefixes[i].n_rows, i++) {
         const ni_prefix& p = prefixes[i];
         const uint32_t p_slots = (uint32_t)((uint64_t)p.n_rows * group);
@@ -1506,16 +1526,21 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
             P.n_parts += n_own * slots;
         }
     }
-    // Rows of one or two slots leave tiles of 16 nearly empty: vector units (12
-    // layers x 64 rows of 1..255 keys, one slot: 64 against 71 us; four slots, 48
-    // rows x 8 heads x 128 of 1..511 keys: 17.1 against 16.0).
+    // Rows of one or two slots, on the Q8 cache of one, leave tiles of 16 nearly
+    // empty: vector units (12 layers x 64 rows of 1..255 keys, one slot: 64 against 71
+    // us, Q8 with the prefix's launch 57 / 73; two 53 / 54, Q8 77 / 49; four slots, 48
+    // rows x 8 heads x 128 of 1..511 keys: 17.1 / 16.0).  Launches of several rounds
+    // have two waves to an item in place of four: half as many ends to join (with the
+    // prefix's launch, the same 64 rows 71 / 73 us, Q8 57 / 67; 32 rows of 1..100 keys
+    // 29.4 / 32.2; one layer of 64 rows 14.7 / 14.1, of up to 1023 keys 31.7 / 29.8).
     const bool shared = !P.wide && !P.pitems.empty();  // a launch, with the prefixes' items
     if (shared) {
         P.items.insert(P.items.end(), P.pitems.begin(), P.pitems.end());
         P.pitems.clear();
     }
     const bool rows_alone = std::all_of(runs.begin(), runs.end(), [](const Run& u) { return u.n == 1; });
-    P.row_slots = !is_q8(kv->o) && !shared && group <= 2 && rows_alone ? group : 0;
+    P.row_slots = !shared && group <= (is_q8(kv->o) ? 1u : 2u) && rows_alone ? group : 0;
+    P.row_waves = P.items.size() * lh >= 12 * cus ? 2 : 4;
     // Longest first, so that no launch ends on a long item.  Of a launch whose
     // workgroups are all on the CUs at once, block b shares a CU with blocks b +-
     // CUs, b +- 2 CUs: every second round of CUs runs shortest first.
@@ -2208,8 +2233,9 @@ int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_r
     if (e == hipSuccess) {
         a.off_items = 0;
         a.n_items = (uint32_t)P.items.size();
-        a.wide = a.waves = 0;
+        a.wide = 0;
         a.row_slots = P.row_slots;
+        a.waves = P.row_waves;
         ProfileScope ps(kv, NI_K_ATTN);
         e = launch_prefix_attention(a, ref.inl, ref.inl_bytes, s, ps.t);
     }

@@ -747,9 +747,6 @@ __global__ __launch_bounds__(64 * W) void attn_rows_kernel(const RowsLaunch a) {
 
 // ------------------------------------------------------- Q8 attention
 
-// Byte j of w as a signed integer, in f32.
-__device__ __forceinline__ float i8f(uint32_t w, int j) { return (float)((int32_t)(w << (24 - 8 * j)) >> 24); }
-
 // Pages per wave iteration of attn_q8_kernel: 1 measured 1% faster than 2
 // and 6% faster than 4 on config 3.
 constexpr int kQ8Pages = 1;

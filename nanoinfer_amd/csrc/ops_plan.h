@@ -118,8 +118,8 @@ struct PrefixLaunch {
     uint32_t layer0, n_lay;
     uint32_t group;  // G
     uint32_t wide;       // items of up to kWideSlots * waves slots of a prefix, else of up to kSlotTile
-    uint32_t waves;      // wide: waves of slots
-    uint32_t row_slots;  // 1, 2: every item is one row of at most this many slots (f16); 0: not so
+    uint32_t waves;      // wide: waves of slots; row_slots: waves of an item (2, 4)
+    uint32_t row_slots;  // 1, 2: every item is one row of at most this many slots; 0: not so
     float qscale;    // log2(e) / sqrt(head_dim)
 };
 hipError_t launch_prefix_attention(const PrefixLaunch& a, const void* inline_plan, uint32_t inline_bytes,

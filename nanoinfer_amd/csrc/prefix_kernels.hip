@@ -316,14 +316,17 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
 
 // Items of one row's own keys and up to NS slots (a row's query heads of one
 // cache head), on the vector units: fewer instructions a page than tiles of 16
-// slots that stay nearly empty.  A lane holds 8 dims of a key row (D / 8 lanes a
-// row, KPL rows a load), a group of lanes its own softmax state over the rows it
-// sees; q.k and p.v mix f32 with the f16 of the cache.  Groups and waves start
-// from the prefix's partials, every (W KPL)-th a group, and are joined at the end.
-template <int D, int NS, int INL>
-__global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
-    constexpr int W = kItemWaves;
-    constexpr int LPK = D / 8;               // lanes of a key row
+// slots that stay nearly empty.  A lane holds 16 bytes of a key row (8 dims, of the
+// Q8 cache 16; LPK lanes a row, KPL rows a load), a group of lanes its own softmax
+// state over the rows it sees; q.k and p.v mix f32 with the cache's f16 or int8.
+// Groups and waves start from the prefix's partials, every (W KPL)-th a group, and
+// are joined at the end.
+// Bound by memory: 12 layers x 64 rows of 1..255 keys x 12 heads x 64, 316 MB of
+// f16 in 55 us (5.8 TB/s).
+template <int D, int NS, int W, int INL, bool Q8>
+__global__ __launch_bounds__(64 * W) void prefix_rows_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
+    constexpr int DL = Q8 ? 16 : 8;          // dims of a lane
+    constexpr int LPK = D / DL;              // lanes of a key row
     constexpr int KPL = 64 / LPK;            // rows of a load
     constexpr int LPP = (int)kPage / KPL;    // loads of a page
     constexpr int PB = D == 64 ? 2 : 1;      // pages of an iteration
@@ -342,6 +345,7 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const Pref
     const uint32_t pg_end = (it.kv_end + kPage - 1) / kPage;
     struct Regs {
         u32x4 k[PB][LPP], v[PB][LPP];
+        float ks[Q8 ? PB : 1][LPP], vs[Q8 ? PB : 1][LPP];  // Q8: the rows' scales
     };
     auto load = [&](uint32_t pg, Regs& r) {
 #pragma unroll
@@ -354,27 +358,44 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const Pref
             for (int i = 0; i < LPP; i++) r.k[b][i] = load16(kp + 64 * i);
 #pragma unroll
             for (int i = 0; i < LPP; i++) r.v[b][i] = load16(vp + 64 * i);
+            if constexpr (Q8) {
+#pragma unroll
+                for (int i = 0; i < LPP; i++) {
+                    r.ks[b][i] = reinterpret_cast<const float*>(q8_block(a.pool, false, at) + kPage * D)[i * KPL + kl];
+                    r.vs[b][i] = reinterpret_cast<const float*>(q8_block(a.pool, true, at) + kPage * D)[i * KPL + kl];
+                }
+            }
         }
+    };
+    auto value = [](const u32x4& x, int e) {  // dim e of a lane's 16 bytes
+        if constexpr (Q8)
+            return i8f(x[e / 4], e % 4);
+        else
+            return (float)__builtin_bit_cast(half8_t, x)[e];
     };
     Regs cur;
     uint32_t pg = it.kv_begin / kPage + wave * PB;
     if (pg < pg_end) load(pg, cur);
-    float q[NS][8], m[NS], l[NS], o[NS][8];
+    float q[NS][DL], m[NS], l[NS], o[NS][DL];
     {
         // slot s of a row is query head s of the cache head (past ns: the first again, its result unused)
         const float* qb = a.q + (int64_t)lay * a.q_layer_stride + (int64_t)it.row0 * a.q_row_stride +
-                          (head * a.group + it.slot0) * D + ds * 8;
+                          (head * a.group + it.slot0) * D + ds * DL;
 #pragma unroll
         for (int s = 0; s < NS; s++) {
             const float* p = qb + (s < (int)it.ns ? s : 0) * D;
-            const float4 x0 = reinterpret_cast<const float4*>(p)[0], x1 = reinterpret_cast<const float4*>(p)[1];
-            const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
 #pragma unroll
-            for (int e = 0; e < 8; e++) q[s][e] = x[e] * a.qscale;
+            for (int e = 0; e < DL; e += 4) {
+                const float4 x = *reinterpret_cast<const float4*>(p + e);
+                q[s][e] = x.x * a.qscale;
+                q[s][e + 1] = x.y * a.qscale;
+                q[s][e + 2] = x.z * a.qscale;
+                q[s][e + 3] = x.w * a.qscale;
+            }
             m[s] = kMinScore;
             l[s] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[s][e] = 0.f;
+            for (int e = 0; e < DL; e++) o[s][e] = 0.f;
         }
     }
     if (it.part0 == kNoSlot) {
@@ -384,15 +405,20 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const Pref
                 const uint32_t idx = it.pre0 + (s < (int)it.ns ? s : 0) + j * it.pre_stride;
                 const uint64_t part = ((uint64_t)idx * a.n_lay + lay) * H + head;
                 const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * part);
-                const float4* po = reinterpret_cast<const float4*>(a.part_o + part * D + ds * 8);
-                const float4 x0 = po[0], x1 = po[1];
-                const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+                float4 x[DL / 4];
+#pragma unroll
+                for (int e = 0; e < DL / 4; e++) x[e] = reinterpret_cast<const float4*>(a.part_o + part * D + ds * DL)[e];
                 const float mn = fmaxf(m[s], ml.x);
                 const float keep = fast_exp2(m[s] - mn), take = fast_exp2(ml.x - mn);
                 m[s] = mn;
                 l[s] = l[s] * keep + ml.y * take;
 #pragma unroll
-                for (int e = 0; e < 8; e++) o[s][e] = o[s][e] * keep + x[e] * take;
+                for (int e = 0; e < DL / 4; e++) {
+                    o[s][4 * e] = o[s][4 * e] * keep + x[e].x * take;
+                    o[s][4 * e + 1] = o[s][4 * e + 1] * keep + x[e].y * take;
+                    o[s][4 * e + 2] = o[s][4 * e + 2] * keep + x[e].z * take;
+                    o[s][4 * e + 3] = o[s][4 * e + 3] * keep + x[e].w * take;
+                }
             }
         }
     }
@@ -406,7 +432,12 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const Pref
             for (int b = 0; b < PB; b++)
 #pragma unroll
                 for (int i = 0; i < LPP; i++)
-                    if ((pg + b) * kPage + i * KPL + kl >= it.kv_end) cur.v[b][i] = u32x4{0, 0, 0, 0};
+                    if ((pg + b) * kPage + i * KPL + kl >= it.kv_end) {
+                        if constexpr (Q8)
+                            cur.vs[b][i] = 0.f;
+                        else
+                            cur.v[b][i] = u32x4{0, 0, 0, 0};
+                    }
         }
 #pragma unroll
         for (int s = 0; s < NS; s++) {
@@ -415,14 +446,14 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const Pref
             for (int b = 0; b < PB; b++)
 #pragma unroll
                 for (int i = 0; i < LPP; i++) {
-                    const half8_t k = __builtin_bit_cast(half8_t, cur.k[b][i]);
                     float x = 0.f, y = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        x += q[s][e] * (float)k[e];
-                        y += q[s][e + 1] * (float)k[e + 1];
+                    for (int e = 0; e < DL; e += 2) {
+                        x += q[s][e] * value(cur.k[b][i], e);
+                        y += q[s][e + 1] * value(cur.k[b][i], e + 1);
                     }
                     x = key_sum<LPK>(x + y);
+                    if constexpr (Q8) x *= cur.ks[b][i];
                     sc[b][i] = (pg + b) * kPage + i * KPL + kl < it.kv_end ? x : -INFINITY;
                     mx = fmaxf(mx, sc[b][i]);
                 }
@@ -430,16 +461,16 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const Pref
             m[s] = mx;
             l[s] *= keep;
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[s][e] *= keep;
+            for (int e = 0; e < DL; e++) o[s][e] *= keep;
 #pragma unroll
             for (int b = 0; b < PB; b++)
 #pragma unroll
                 for (int i = 0; i < LPP; i++) {
-                    const half8_t v = __builtin_bit_cast(half8_t, cur.v[b][i]);
-                    const float p = fast_exp2(sc[b][i] - mx);
+                    float p = fast_exp2(sc[b][i] - mx);
                     l[s] += p;
+                    if constexpr (Q8) p *= cur.vs[b][i];
 #pragma unroll
-                    for (int e = 0; e < 8; e++) o[s][e] += p * (float)v[e];
+                    for (int e = 0; e < DL; e++) o[s][e] += p * value(cur.v[b][i], e);
                 }
         }
         if (pg + W * PB < pg_end) cur = nxt;
@@ -455,7 +486,7 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const Pref
             m[s] = mn;
             l[s] = l[s] * a1 + l2 * a2;
 #pragma unroll
-            for (int e = 0; e < 8; e++) o[s][e] = o[s][e] * a1 + __shfl_xor(o[s][e], st) * a2;
+            for (int e = 0; e < DL; e++) o[s][e] = o[s][e] * a1 + __shfl_xor(o[s][e], st) * a2;
         }
         if (kl == 0) {
             if (ds == 0) {
@@ -463,7 +494,7 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_rows_kernel(const Pref
                 red[wave][s][1] = l[s];
             }
 #pragma unroll
-            for (int e = 0; e < 8; e++) red[wave][s][2 + ds * 8 + e] = o[s][e];
+            for (int e = 0; e < DL; e++) red[wave][s][2 + ds * DL + e] = o[s][e];
         }
     }
     __syncthreads();
@@ -1002,17 +1033,26 @@ __global__ __launch_bounds__(64 * kMergeWaves) void prefix_merge_kernel(const Pr
     for (int e = 0; e < N; e++) dst[64 * e] = O[e] / L;
 }
 
-// One workgroup of kItemWaves per (item, layer, head): prefix_attn_kernel or
-// prefix_rows_kernel.
+// One workgroup per (item, layer, head): prefix_attn_kernel or prefix_rows_kernel.
 template <int D>
 hipError_t items_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s, const LaunchTiming& t) {
     const uint64_t blocks = (uint64_t)a.n_items * a.n_lay * a.pool.n_head;
     return with_plan(a, ip, ib, [&](auto pa) {
         constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
-        if (a.pool.q8) return go(prefix_attn_kernel<D, INL, true>, blocks, 64 * kItemWaves, s, t, a, pa);
-        if (a.row_slots == 1) return go(prefix_rows_kernel<D, 1, INL>, blocks, 64 * kItemWaves, s, t, a, pa);
-        if (a.row_slots == 2) return go(prefix_rows_kernel<D, 2, INL>, blocks, 64 * kItemWaves, s, t, a, pa);
-        return go(prefix_attn_kernel<D, INL, false>, blocks, 64 * kItemWaves, s, t, a, pa);
+        auto run = [&](auto q8) {
+            constexpr bool Q8 = decltype(q8)::value;
+            if (a.row_slots == 1) {
+                if (a.waves == 2) return go(prefix_rows_kernel<D, 1, 2, INL, Q8>, blocks, 128, s, t, a, pa);
+                if (a.waves == 4) return go(prefix_rows_kernel<D, 1, 4, INL, Q8>, blocks, 256, s, t, a, pa);
+            }
+            if constexpr (!Q8) {
+                if (a.row_slots == 2 && a.waves == 2) return go(prefix_rows_kernel<D, 2, 2, INL, Q8>, blocks, 128, s, t, a, pa);
+                if (a.row_slots == 2 && a.waves == 4) return go(prefix_rows_kernel<D, 2, 4, INL, Q8>, blocks, 256, s, t, a, pa);
+            }
+            if (a.row_slots) return hipErrorInvalidValue;
+            return go(prefix_attn_kernel<D, INL, Q8>, blocks, 64 * kItemWaves, s, t, a, pa);
+        };
+        return a.pool.q8 ? run(std::true_type{}) : run(std::false_type{});
     });
 }
 
@@ -1037,7 +1077,7 @@ hipError_t wide_t(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_
 hipError_t launch_prefix_attention(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s,
                                    const LaunchTiming& t) {
     if (a.n_items == 0) return hipSuccess;
-    if ((a.row_slots && a.pool.q8) || (a.pool.head_dim != 64 && a.pool.head_dim != 128)) return hipErrorInvalidValue;
+    if (a.pool.head_dim != 64 && a.pool.head_dim != 128) return hipErrorInvalidValue;
     if (!a.wide) return a.pool.head_dim == 64 ? items_t<64>(a, ip, ib, s, t) : items_t<128>(a, ip, ib, s, t);
     if (a.pool.head_dim == 64)
         return a.pool.q8 ? wide_t<64, true>(a, ip, ib, s, t) : wide_t<64, false>(a, ip, ib, s, t);

@@ -189,6 +189,24 @@ def test_what_lies_behind_a_prefix_does_not_matter_to_wide_tiles(gpu, d):
     check(c, [(0, p) for p in range(30)], [(1, m, 30)], split_tokens=1024)
 
 
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_many_short_rows(gpu, d, q8):
+    """A decode batch of every layer: single rows of one key to a few pages, in
+    launches of several rounds, behind a long prefix and behind none; what lies
+    behind their ends, to the last page's, is as bad as can be."""
+    lens = [1 + (i * 7) % 75 for i in range(67)]
+    c = Cache([n + 16 for n in lens] + [700], n_layer=12, n_head=4, head_dim=d, q8=q8, seed=41, spare=3)
+    bad = torch.full((12, 16, 4 * d), float("inf"), device=gpu)
+    for i, n in enumerate(lens):
+        c.put(i, bad, bad, n)
+    rows = [(i, n - 1) for i, n in enumerate(lens)]
+    for group in (1, 2):
+        check(c, rows, [(67, 700, 67)], group)
+        check(c, rows, [(67, 689, 60), (0, 0, 7)], group)
+        check(c, rows, [(0, 0, 67)], group)
+
+
 def test_layers_and_one_layer(gpu):
     c = Cache([20, 50, 64], n_layer=4, n_head=2, head_dim=128, seed=13)
     rows, pre = [(0, 19), (1, 44), (1, 45)], [(2, 63, 3)]
