@@ -360,7 +360,8 @@ typedef struct ni_prefix {
  * all its rows rather than once a row.  prefixes[0..n_prefix) cover the rows
  * in order and in full.  A row of q and out holds n_q_head heads, a multiple
  * of the cache's n_head: query head h reads cache head h / (n_q_head /
- * n_head).  out may be q.  A row's own sequence may not be its prefix.
+ * n_head).  out may be q with the same strides.  A row's own sequence may not
+ * be its prefix.
  * split_tokens: keys per partition, a multiple of 16; 0 = automatic.
  * Under stream capture the call allocates nothing: make the same call once
  * before, so that the handle holds the partials it needs (graphs captured from

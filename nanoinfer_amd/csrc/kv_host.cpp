@@ -2061,6 +2061,9 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
             (all && n_lay > 1 && (uint64_t)q_out_layer_stride < (uint64_t)n_q_head * D))
             return kv->fail(NI_ERR_BAD_ARG, "q_out's rows overlap: strides must be at least %llu",
                             (unsigned long long)n_q_head * D);
+        if (q_out == q && ((n > 1 && q_row_stride != q_out_row_stride) ||
+                           (all && n_lay > 1 && q_layer_stride != q_out_layer_stride)))
+            return kv->fail(NI_ERR_BAD_ARG, "q_out may be q only with q's strides");
     }
     if (!rotary) return kv->fail(NI_ERR_BAD_ARG, "rotary is NULL");
     if (rotary->head_dim != D)
@@ -2164,6 +2167,9 @@ int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_r
         (all && n_lay > 1 && (uint64_t)out_layer_stride < (uint64_t)n_q_head * D))
         return kv->fail(NI_ERR_BAD_ARG, "out's rows overlap: strides must be at least %llu",
                         (unsigned long long)n_q_head * D);
+    if (out == q && ((n > 1 && q_row_stride != out_row_stride) ||
+                     (all && n_lay > 1 && q_layer_stride != out_layer_stride)))
+        return kv->fail(NI_ERR_BAD_ARG, "out may be q only with q's strides");
     for (uint32_t i = 0, r = 0; i < n_prefix; i++) {
         const ni_prefix& p = prefixes[i];
         if (p.len && p.n_rows)

@@ -89,6 +89,8 @@ int ni_rotary_apply(const ni_rotary* r, uint32_t dtype, const void* x, int64_t x
         return call_error(NI_ERR_BAD_ARG, "x and out must be aligned to their type with non-negative row strides");
     if (n > 1 && out_row_stride < width)
         return call_error(NI_ERR_BAD_ARG, "out's rows overlap: the row stride must be at least %lld", (long long)width);
+    if (out == x && n > 1 && x_row_stride != out_row_stride)
+        return call_error(NI_ERR_BAD_ARG, "out may be x only with x's stride");
     if (!aligned(positions, 4)) return call_error(NI_ERR_BAD_ARG, "positions must be 4-byte aligned");
     // (a launch holds less than 2^32 threads, each of two values or eight)
     if ((unsigned __int128)n * width >= (1ull << 32)) return call_error(NI_ERR_BAD_ARG, "n * n_head * head_dim too large");

@@ -20,11 +20,12 @@ pytestmark = pytest.mark.gpu
 class Cache:
     """A PagedKv filled with random rows and what it stores, in 64 bits."""
 
-    def __init__(self, lens, n_layer=1, n_head=2, head_dim=64, q8=False, seed=0, std=1.0, spare=2):
+    def __init__(self, lens, n_layer=1, n_head=2, head_dim=64, q8=False, seed=0, std=1.0, spare=2, far=False):
         pages = sum(-(-n // 16) for n in lens) + spare
+        order = np.random.default_rng(seed).permutation(pages)
         self.opts = na.BatchOpts(n_layer=n_layer, n_head=n_head, head_dim=head_dim, kv_blocks=pages, max_seqs=len(lens),
                                  n_ctx=max(lens), max_rows=4096, q8=q8,
-                                 page_order=np.random.default_rng(seed).permutation(pages))
+                                 page_order=np.sort(order)[::-1].copy() if far else order)
         self.kv = na.PagedKv(self.opts)
         g = torch.Generator(device="cuda").manual_seed(seed)
         self.k, self.v = [], []
@@ -216,6 +217,26 @@ def test_layers_and_one_layer(gpu):
         close(one[None], c.expect(q, rows, pre)[layer:layer + 1])
 
 
+@pytest.mark.parametrize("q8", [False, True])
+def test_offsets_past_32_bits(gpu, q8):
+    """Pages behind 2^32 halves of the pool: every kernel, and the rotating append."""
+    n_head, pages = 32, 68000 if q8 else 33200
+    lens = [1 + 3 * i for i in range(18)] + [2000]
+    c = Cache(lens, n_head=n_head, head_dim=128, q8=q8, seed=43, spare=pages - 200, far=True)
+    page_bytes = n_head * 2 * 16 * (128 + 4 if q8 else 256)
+    assert min(min(c.kv.block_table(s)) for s in range(19)) * page_bytes > 2 ** 33
+    rows = [(i, n - 1) for i, n in enumerate(lens[:18])]
+    g = torch.Generator(device="cuda").manual_seed(44)
+    k, v = (torch.randn((1, 18, n_head * 128), generator=g, device="cuda") for _ in range(2))
+    c.kv.append_rotary(rows, k, v, na.Rotary(128), positions=np.zeros(18, np.uint32))  # (no turn)
+    for i, (s, p) in enumerate(rows):
+        c.k[s][:, p:p + 1], c.v[s][:, p:p + 1] = c.stored(k[:, i:i + 1]), c.stored(v[:, i:i + 1])
+    check(c, rows, [(18, 2000, 18)])  # wide tiles, single rows
+    check(c, rows, [(18, 2000, 18)], 4)
+    check(c, rows[-3:], [(18, 2000, 3)])
+    check(c, rows[-3:], [(18, 2000, 3)], split_tokens=512)
+
+
 def test_strides_in_place_and_rows_behind(gpu):
     c = Cache([20, 50, 64], n_layer=2, n_head=2, seed=15)
     rows, pre = [(0, 19), (1, 44), (1, 45)], [(2, 63, 3)]
@@ -325,6 +346,9 @@ def test_refusals(gpu):
     c.kv.prefix_attention(q, rows, [(2, 0, 2)])  # an empty prefix is not looked at
     assert c.kv.prefix_attention(q[:, :0], [], []).shape == (1, 0, 128)
     assert c.kv.prefix_attention(q[:, :0], [], [(2, 5, 0)]).shape == (1, 0, 128)
+    wide = torch.zeros((1, 2, 256), device=gpu)
+    with pytest.raises(na.KvError, match="q's strides"):  # the same memory, other strides
+        c.kv.prefix_attention(wide[:, :, :128], rows, [(2, 3, 2)], out=wide.view(-1)[:256].view(1, 2, 128))
 
 
 def test_captured_and_replayed(gpu):

@@ -90,3 +90,63 @@ def test_rounds(gpu, n_head, group, d):
         lens = [kv.seq_len(s) - K - 1 for s in seqs]
         assert spec.commit(accepted) == want[0].tolist()
         assert [kv.seq_len(s) for s in seqs] == [n + 1 + a for n, a in zip(lens, want[0].tolist())]
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("d,n_head,P", [(64, 12, 1700), (128, 8, 3000)])
+def test_a_captured_round(gpu, d, n_head, P, q8):
+    """Append, attention over wide tiles and verification in one graph: every
+    replay, over other inputs and between eager calls, gives the eager call's bits."""
+    S, K, V, L = 10, 1, 1234, 1 if d == 128 else 2
+    kv = na.PagedKv(na.BatchOpts(n_layer=L, n_head=n_head, head_dim=d, kv_blocks=P // 16 + 1 + 4 * S, max_seqs=S + 1,
+                                 n_ctx=P, max_rows=P, q8=q8))
+    rot = na.Rotary(d, interleaved=True)
+    g = torch.Generator(device="cuda").manual_seed(d)
+    rand = lambda *shape: torch.randn(shape, generator=g, device="cuda")
+    c = n_head * d
+    lens = [P] + [3 + 5 * i for i in range(S)]
+    seqs = []
+    for n in lens:
+        s = kv.add_seq()
+        kv.reserve(s, n)
+        kv.append([(s, p) for p in range(n)], rand(L, n, c), rand(L, n, c))
+        kv.commit(s, n)
+        seqs.append(s)
+    rows = []
+    for s, n in zip(seqs[1:], lens[1:]):
+        kv.reserve(s, n + K + 1)
+        rows += [(s, n + i) for i in range(K + 1)]
+    n = len(rows)
+    pos = np.array([P + p for _, p in rows], dtype=np.uint32)
+    head = rand(c, V) * 0.2
+    k, v, q = rand(L, n, c), rand(L, n, c), rand(L, n, c)
+    au, su = torch.rand((S, K), generator=g, device="cuda"), torch.rand((S,), generator=g, device="cuda")
+    drafted = torch.randint(0, V, (S, K), generator=g, device="cuda", dtype=torch.int32)
+
+    def round_(to):
+        qr, out, acc, tok = to
+        kv.append_rotary(rows, k, v, rot, q=q, q_out=qr, positions=pos)
+        kv.prefix_attention(qr, rows, [(seqs[0], P, n)], out=out)
+        target = torch.softmax((out[-1] @ head).view(S, K + 1, V), -1)
+        na.verify_drafts(target, drafted, au, su, accepted=acc, tokens=tok)
+
+    def outputs():
+        return (torch.empty((L, n, c), device="cuda"), torch.empty((L, n, c), device="cuda"),
+                torch.empty((S,), dtype=torch.int32, device="cuda"),
+                torch.empty((S, K + 1), dtype=torch.int32, device="cuda"))
+
+    eager, replayed = outputs(), outputs()
+    round_(eager)  # (the handle's partials, the library's workspaces)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        round_(replayed)
+    for i in range(4):
+        for x in (k, v, q):
+            x.copy_(rand(*x.shape))
+        au.copy_(torch.rand((S, K), generator=g, device="cuda"))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in replayed]
+        round_(eager)
+        for a, b in zip(eager, got):
+            assert torch.equal(a, b), i

@@ -107,8 +107,9 @@ def test_rotary_apply_refuses_before_any_launch():
     assert call(r.ref, 0, p, 64, p, 64, 2, 2) == _abi.NI_ERR_BAD_ARG and "overlap" in _err(L)
     assert call(r.ref, 0, p, 64, p, 64, 1, 1, p + 2) == _abi.NI_ERR_BAD_ARG and "positions" in _err(L)
     assert call(r.ref, 0, p, 1 << 33, p, 1 << 33, 1 << 31, 1 << 10) == _abi.NI_ERR_BAD_ARG and "too large" in _err(L)
+    assert call(r.ref, 0, p, 128, p, 64, 2, 1) == _abi.NI_ERR_BAD_ARG and "with x's stride" in _err(L)
     # a launch holds less than 2^32 threads
-    assert call(r.ref, 0, p, 64, p, 1 << 12, 1 << 20, 1 << 6) == _abi.NI_ERR_BAD_ARG and "too large" in _err(L)
+    assert call(r.ref, 0, p, 1 << 12, p, 1 << 12, 1 << 20, 1 << 6) == _abi.NI_ERR_BAD_ARG and "too large" in _err(L)
     assert call(r.ref, 0, None, 64, None, 64, 0, 1) == _abi.NI_OK
     assert call(r.ref, 0, None, 64, None, 64, 1, 0) == _abi.NI_OK
 
