@@ -30,8 +30,9 @@ constexpr float kPUnscale = 1.f / kPScale;
 // parts).  Lane l holds slot l % 16 and keys, then dims, 4 (l / 16) .. + 3.
 // Pages go to LDS row major and come back as operands, V through the
 // transposing read.  The W waves take every W-th page each; their states are joined
-// through LDS.  An item that writes out starts from its prefix's partials, every
-// W-th of them a wave, which arrive while the first pages do.
+// through LDS, four dims of a slot to a thread.  For an item that writes out the
+// thread joins the prefix's partials of its dims first, eight loads at a time,
+// which arrive while the first pages do, and holds the sum to the end.
 template <int D, int INL, bool Q8>
 __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
     constexpr int W = kItemWaves;
@@ -40,10 +41,10 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
     constexpr int CH = D / 8;        // 16-byte chunks of an f16 row
     constexpr int LD = Q8 ? D / 64 : D / 32;  // 16-byte loads a lane makes of a page's K, and of its V
     constexpr size_t kTile = (size_t)kPage * D * 2;
-    constexpr size_t kRed = (size_t)W * kSlotTile * (D + 2) * 4;
+    constexpr size_t kRed = (size_t)W * kSlotTile * (D + 4) * 4;
     constexpr size_t kLds = 2 * W * kTile > kRed ? 2 * W * kTile : kRed;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
-    auto& red = *reinterpret_cast<float(*)[W][kSlotTile][D + 2]>(lds);
+    auto& red = *reinterpret_cast<float(*)[W][kSlotTile][D + 4]>(lds);  // m, l, -, -, o
 
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -114,20 +115,39 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
     float4_t o[VC];
 #pragma unroll
     for (int c = 0; c < VC; c++) o[c] = float4_t{0.f, 0.f, 0.f, 0.f};
-    if (it.part0 == kNoSlot && has) {
-        for (uint32_t j = wave; j < it.n_pre; j += W) {
-            const uint64_t part = ((uint64_t)(it.pre0 + col + j * it.pre_stride) * a.n_lay + lay) * H + head;
-            const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * part);
-            float4_t x[VC];
+    constexpr int PG = kSlotTile * D / 4 / (64 * W);  // (slot, four dims) of a thread
+    float pm[PG], pl[PG];
+    float4_t po[PG];
 #pragma unroll
-            for (int c = 0; c < VC; c++)
-                x[c] = *reinterpret_cast<const float4_t*>(a.part_o + part * D + c * 16 + 4 * rg);
-            const float mn = fmaxf(m, ml.x);
-            const float keep = fast_exp2(m - mn), take = fast_exp2(ml.x - mn) * kPScale;
-            m = mn;
-            lsum = lsum * keep + (rg == 0 ? ml.y * take : 0.f);  // (summed over the slot's four lanes at the end)
+    for (int g = 0; g < PG; g++) {
+        const uint32_t t = threadIdx.x + 64 * W * g, sl = t / (D / 4), d = t % (D / 4) * 4;
+        pm[g] = kMinScore;
+        pl[g] = 0.f;
+        po[g] = float4_t{0.f, 0.f, 0.f, 0.f};
+        if (it.part0 != kNoSlot || sl >= it.ns) continue;
+        constexpr uint32_t N = 8;
+        for (uint32_t j0 = 0; j0 < it.n_pre; j0 += N) {
+            float2 ml[N];
+            float4_t x[N];
 #pragma unroll
-            for (int c = 0; c < VC; c++) o[c] = o[c] * keep + x[c] * take;
+            for (uint32_t i = 0; i < N; i++) {  // (past the last: the last again, of no weight)
+                const uint64_t part = ((uint64_t)(it.pre0 + sl + min(j0 + i, it.n_pre - 1) * it.pre_stride) * a.n_lay + lay) * H + head;
+                ml[i] = *reinterpret_cast<const float2*>(a.part_ml + 2 * part);
+                x[i] = *reinterpret_cast<const float4_t*>(a.part_o + part * D + d);
+            }
+            float mn = pm[g];
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++) mn = fmaxf(mn, ml[i].x);
+            const float keep = fast_exp2(pm[g] - mn);
+            pm[g] = mn;
+            pl[g] *= keep;
+            po[g] *= keep;
+#pragma unroll
+            for (uint32_t i = 0; i < N; i++) {
+                const float w = j0 + i < it.n_pre ? fast_exp2(ml[i].x - mn) : 0.f;
+                pl[g] += ml[i].y * w;
+                po[g] += x[i] * w;
+            }
         }
     }
     // Q8: weights enter PV times scale / vref, so that no f16 overflows: vref
@@ -277,39 +297,36 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
     lsum = rows4_sum(lsum);
     __syncthreads();  // the tiles' LDS becomes `red`
     if (has) {
-        if (rg == 0) {
-            red[wave][col][0] = m;
-            red[wave][col][1] = lsum * kPUnscale;
-        }
+        if (rg == 0) *reinterpret_cast<float2*>(&red[wave][col][0]) = float2{m, lsum * kPUnscale};
 #pragma unroll
         for (int c = 0; c < VC; c++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) red[wave][col][2 + c * 16 + 4 * rg + j] = o[c][j] * (kPUnscale * vref);
+            *reinterpret_cast<float4_t*>(&red[wave][col][4 + c * 16 + 4 * rg]) = o[c] * (kPUnscale * vref);
     }
     __syncthreads();
-    for (uint32_t t = threadIdx.x; t < it.ns * D; t += 64 * W) {
-        const uint32_t sl = t / D, d = t - sl * D;
-        float M = red[0][sl][0];
 #pragma unroll
-        for (int w = 1; w < W; w++) M = fmaxf(M, red[w][sl][0]);
-        float L = 0.f, O = 0.f;
+    for (int g = 0; g < PG; g++) {
+        const uint32_t t = threadIdx.x + 64 * W * g, sl = t / (D / 4), d = t % (D / 4) * 4;
+        if (sl >= it.ns) continue;
+        float M = pm[g];
+#pragma unroll
+        for (int w = 0; w < W; w++) M = fmaxf(M, red[w][sl][0]);
+        const float pw = fast_exp2(pm[g] - M);
+        float L = pl[g] * pw;
+        float4_t O = po[g] * pw;
 #pragma unroll
         for (int w = 0; w < W; w++) {
             const float wt = fast_exp2(red[w][sl][0] - M);
             L += red[w][sl][1] * wt;
-            O += red[w][sl][2 + d] * wt;
+            O += *reinterpret_cast<const float4_t*>(&red[w][sl][4 + d]) * wt;
         }
         if (it.part0 == kNoSlot) {
             const uint32_t r = (it.slot0 + sl) / a.group, gg = it.slot0 + sl - r * a.group;
-            a.out[(int64_t)lay * a.out_layer_stride + (int64_t)(it.row0 + r) * a.out_row_stride +
-                  (head * a.group + gg) * D + d] = O / L;
+            *reinterpret_cast<float4_t*>(a.out + (int64_t)lay * a.out_layer_stride +
+                                         (int64_t)(it.row0 + r) * a.out_row_stride + (head * a.group + gg) * D + d) = O / L;
         } else {
             const uint64_t part = ((uint64_t)(it.part0 + sl) * a.n_lay + lay) * H + head;
-            a.part_o[part * D + d] = O;
-            if (d == 0) {
-                a.part_ml[2 * part] = M;
-                a.part_ml[2 * part + 1] = L;
-            }
+            *reinterpret_cast<float4_t*>(a.part_o + part * D + d) = O;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = float2{M, L};
         }
     }
 }
