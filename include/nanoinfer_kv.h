@@ -322,10 +322,10 @@ int ni_rotary_init(ni_rotary* r, uint32_t head_dim, const ni_rotary_opts* opts);
 
 /* Rotate n rows of n_head heads (row i at x + i * x_row_stride, head_dim
  * values a head) to out.  x and out are of `dtype` (rounded once, to nearest
- * even; computed in f32) and aligned to it (16-byte aligned rows of heads whose
- * head_dim and rot_dim are multiples of 8 are read 16 bytes at a time, others
- * value by value).  Row i is at positions[i] (int32 on the device; negative ones
- * turn backwards), or at pos0 + i where positions is NULL.  out may be x with
+ * even; computed in f32) and aligned to it (calls of many rows are faster where
+ * these are 16-byte aligned and head_dim and rot_dim multiples of 8).  Row i is
+ * at positions[i] (int32 on the device; negative ones turn backwards), or at
+ * pos0 + i where positions is NULL.  out may be x with
  * the same stride; rows that overlap otherwise are undefined.  Enqueued on
  * `stream`; failures are reported by ni_kv_last_error(NULL). */
 int ni_rotary_apply(const ni_rotary* r, uint32_t dtype, const void* x, int64_t x_row_stride, void* out,

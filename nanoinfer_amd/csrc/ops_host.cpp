@@ -104,10 +104,16 @@ int ni_rotary_apply(const ni_rotary* r, uint32_t dtype, const void* x, int64_t x
     a.n_rows = n;
     a.n_head = n_head;
     a.dtype = dtype;
-    a.wide = r->head_dim % 8 == 0 && r->rot_dim % 8 == 0 && aligned(x, 16) && aligned(out, 16) &&
+    // Chunks of eight values, two or four heads' to a thread that turns by the same
+    // angles, where every CU has many; pairs, a thread each, where the chunk's four
+    // angles one after another are what takes the time (or on no 16-byte borders).  us
+    // for pairs and for one, two and four heads: 64 x 12 x 64 f32 2.5, 3.2, 3.8, 4.8;
+    // 512 x 12 x 64 2.7, 3.4, 3.9, 5.0; 4096 x 12 x 64 7.2, 6.2, 6.2, 7.3; bf16, 1024 x 40
+    // x 128 10.5, 9.0, 7.6, 8.4; 2048 17.8, 14.2, 11.3, 11.4; 4095 31.7, 24.0, 17.8, 16.7.
+    const uint64_t per_cu = (uint64_t)n * width / 8 / device_cus();
+    a.wide = per_cu >= 256 && r->head_dim % 8 == 0 && r->rot_dim % 8 == 0 && aligned(x, 16) && aligned(out, 16) &&
              x_row_stride % unit == 0 && out_row_stride % unit == 0;
-    // Four heads to a thread once that still gives every CU 2048 threads.
-    a.heads_per = (uint64_t)n * width / 8 >= 4ull * 2048 * device_cus() ? 4u : 1u;
+    a.heads_per = per_cu >= 4096 ? 4 : per_cu >= 2048 ? 2 : 1;
     const hipError_t e = launch_rotary(a, *r, (hipStream_t)stream);
     if (e != hipSuccess) return call_error(NI_ERR_HIP, "rotary launch failed: %s", hipGetErrorString(e));
     return NI_OK;
@@ -175,7 +181,10 @@ int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stri
     a.n_draft = n_draft;
     a.vocab = vocab;
     a.dtype = dtype;
-    // As many chunks to a workgroup as leave every CU eight of them.
+    // As many chunks to a workgroup as leave every CU eight of them: the chain to the
+    // first rejection is walked once for all, but a run of chunks takes longer.  us at
+    // one, two and eight: 1 sequence of 50257 7.2, 7.9, 12.9; 64 of 131071 19.3, 18.5, 19.9;
+    // 256 of 50257 23.6, 22.5, 22.3.
     const uint64_t chunks = (uint64_t)n_seq * ((vocab + (uint64_t)kVerifyChunk - 1) / kVerifyChunk);
     a.per = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(chunks / (8ull * device_cus()), 1), 16);
     const hipError_t e = launch_verify(a, (hipStream_t)stream);

@@ -32,7 +32,12 @@ constexpr float kPUnscale = 1.f / kPScale;
 // transposing read.  The W waves take every W-th page each; their states are joined
 // through LDS, four dims of a slot to a thread.  For an item that writes out the
 // thread joins the prefix's partials of its dims first, eight loads at a time,
-// which arrive while the first pages do, and holds the sum to the end.
+// which arrive while the first pages do, and holds the sum to the end.  Bound by
+// memory on long prefixes (16 rows x 32 heads x 128 behind 32767 keys, 595 MB with the
+// rows' own keys: 90 us, 6.6 TB/s); by the ~250 vector instructions a page of the Q8
+// cache costs a wave (32 x 5 rows x 12 heads x 64 behind 2001: 13 us); by the start
+// and the chain of pages of its longest items otherwise (48 rows x 32 query heads on 8
+// x 128, 1..511 own keys: 15 us).
 template <int D, int INL, bool Q8>
 __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
     constexpr int W = kItemWaves;
@@ -550,6 +555,10 @@ __global__ __launch_bounds__(64 * W) void prefix_rows_kernel(const PrefixLaunch 
 // register i, in V's transposing reads alike).  Every slot sees every key, so
 // only the last tile masks.  The exponent reference follows the running maximum
 // only past kWideSlack (weights up to 2^15 in f16, as hi + lo).
+// 192 slots x 8 heads x 128 behind 8185 keys (three waves, two groups): 26.5 us, of
+// which ~5 until the first tile is there, ~3 to join and store, ~4 until the
+// partials have left the caches, and between them ~2 us per two tiles, half of it
+// matrix products on the SIMDs that hold two of the six waves.
 constexpr float kWideSlack = 8.f, kWideLog2 = 7.f, kWideUnscale = 1.f / 128.f;
 typedef float float16_t __attribute__((ext_vector_type(16)));
 typedef int v2i32_t __attribute__((ext_vector_type(2)));
@@ -988,7 +997,8 @@ void prefix_wide_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
 }
 
 // One wave per (row, layer, query head): its partials' states weighed by
-// exp2(m - M) and added; lane l holds dims l, l + 64.
+// exp2(m - M) and added; lane l holds dims l, l + 64.  4-5 us, the plan's item, the
+// states and the sums one after another, with little to read.
 template <int D, int INL>
 __global__ __launch_bounds__(64 * kMergeWaves) void prefix_merge_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
     constexpr int N = D / 64;

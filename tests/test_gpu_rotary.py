@@ -57,8 +57,14 @@ CASES = [
     (7, 4, 36, {}, torch.float16),
     (7, 4, 4, dict(rot_dim=2), torch.float32),
     (9, 2, 256, dict(base=1e6), torch.float16),
-    (700, 33, 128, dict(scaling="yarn", factor=8.0, orig_ctx=8192, base=500000.0), torch.float32),  # four heads a thread
+    (700, 33, 128, dict(scaling="yarn", factor=8.0, orig_ctx=8192, base=500000.0), torch.float32),
     (2050, 40, 64, dict(scaling="ntk", factor=5.5, rot_dim=56), torch.bfloat16),
+    # chunks of eight values, one head a thread, two and four
+    (900, 9, 80, dict(rot_dim=72), torch.float16),
+    (500, 11, 128, dict(rot_dim=64, interleaved=True), torch.bfloat16),
+    (300, 7, 256, dict(base=1e6), torch.float32),
+    (1030, 33, 128, dict(interleaved=True), torch.float32),
+    (2100, 41, 128, dict(rot_dim=96), torch.bfloat16),
 ]
 
 
