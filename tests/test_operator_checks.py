@@ -303,7 +303,7 @@ def test_spec_commit_takes_the_callers_numbers():
     with pytest.raises(Exception, match="5 drafts accepted of 4"):
         sp.commit([0, 0, 5])
     assert [kv.seq_len(s) for s in seqs] == [13, 27, 43]  # nothing truncated
-    for bad in ([0, 0], [0, -1, 0]):
+    for bad in ([0, 0], [0, -1, 0], [0, 1 << 32, 0]):
         with pytest.raises(ValueError):
             sp.commit(bad)
     assert sp.commit([0, 0, 0]) == [0, 0, 0]
