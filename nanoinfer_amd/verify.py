@@ -3,6 +3,8 @@
 ``commit`` takes the accepted numbers."""
 from __future__ import annotations
 
+import functools
+
 from . import _abi
 from .batch import KvError, _on, _stream_now, _torch
 from .rotation import dtype_code
@@ -57,7 +59,8 @@ def verify_drafts(target, drafted, accept_u, sample_u, draft=None, n_drafts=None
             and _fits(drafted, i32, (b, k), device) and _fits(accept_u, torch.float32, (b, k), device)
             and _fits(sample_u, torch.float32, (b,), device) and _fits(accepted, i32, (b,), device)
             and _fits(tokens, i32, (b, k + 1), device)):
-        _call(torch, target, drafted, accept_u, sample_u, draft, n_drafts, accepted, tokens, b, k, v, s)
+        _call(torch, target, drafted, accept_u, sample_u, draft, n_drafts, accepted, tokens, b, k, v, s,
+              ((k + 1) * v, v), (k * v, v), k, k, k + 1)
         return accepted, tokens
     if k < 0 or v == 0:
         raise ValueError(f"target is {list(target.shape)}: needs [sequences, drafts + 1, vocabulary]")
@@ -84,24 +87,28 @@ def verify_drafts(target, drafted, accept_u, sample_u, draft=None, n_drafts=None
             accepted = torch.empty((b,), dtype=torch.int32, device=target.device)
         if tokens is None:
             tokens = torch.empty((b, k + 1), dtype=torch.int32, device=target.device)
-        _call(torch, target, drafted, accept_u, sample_u, draft, n_drafts, accepted, tokens, b, k, v, s)
+        _call(torch, target, drafted, accept_u, sample_u, draft, n_drafts, accepted, tokens, b, k, v, s,
+              target.stride(), (0, 0) if draft is None else draft.stride(), drafted.stride(0), accept_u.stride(0),
+              tokens.stride(0))
     return accepted, tokens
 
 
-def _call(torch, target, drafted, accept_u, sample_u, draft, n_drafts, accepted, tokens, b, k, v, s):
+@functools.lru_cache(maxsize=64)
+def _workspace(b, v) -> int:
+    return _abi.lib().ni_verify_workspace(b, v)
+
+
+def _call(torch, target, drafted, accept_u, sample_u, draft, n_drafts, accepted, tokens, b, k, v, s, target_strides,
+          draft_strides, drafted_stride, accept_stride, tokens_stride):
     L = _abi.lib()
-    need = L.ni_verify_workspace(b, v)
+    need = _workspace(b, v)
     # From torch's allocator: of this stream, and of the graph where one is captured.
     work = torch.empty((need,), dtype=torch.uint8, device=target.device)
-    if draft is None or k == 0:
-        dp, ds = None, (0, 0)
-    else:
-        dp, ds = draft.data_ptr(), draft.stride()
-    ts = target.stride()
-    rc = L.ni_verify_drafts(dtype_code(target.dtype), target.data_ptr(), ts[0], ts[1], dp, ds[0], ds[1],
-                            drafted.data_ptr() if k else None, drafted.stride(0),
+    rc = L.ni_verify_drafts(dtype_code(target.dtype), target.data_ptr(), target_strides[0], target_strides[1],
+                            None if draft is None or k == 0 else draft.data_ptr(), draft_strides[0], draft_strides[1],
+                            drafted.data_ptr() if k else None, drafted_stride,
                             None if n_drafts is None else n_drafts.data_ptr(), accept_u.data_ptr() if k else None,
-                            accept_u.stride(0), sample_u.data_ptr(), b, k, v, accepted.data_ptr(), tokens.data_ptr(),
-                            tokens.stride(0), work.data_ptr(), need, s)
+                            accept_stride, sample_u.data_ptr(), b, k, v, accepted.data_ptr(), tokens.data_ptr(),
+                            tokens_stride, work.data_ptr(), need, s)
     if rc != 0:
         raise KvError(rc, (L.ni_kv_last_error(None) or b"").decode())
