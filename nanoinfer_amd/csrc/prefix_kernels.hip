@@ -156,7 +156,7 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
         }
     }
     // Q8: weights enter PV times scale / vref, so that no f16 overflows: vref
-    // starts at 1 and follows the largest value scale past it.
+    // starts at 1 and follows the largest value scale that the slot sees past it.
     float vref = 1.f, vinv = 1.f;
 
     for (; pg < pg_end; pg += W) {
@@ -214,12 +214,14 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
             st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[c], st, 0, 0, 0);
         }
         float s[4], mx = -INFINITY;
+        bool seen[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const uint32_t key = pg * kPage + 4 * rg + j;
+            seen[j] = key < it.kv_end && key <= qpos;
             float x = st[j];
             if constexpr (Q8) x *= cur.ks[j];
-            s[j] = key < it.kv_end && key <= qpos ? x : -INFINITY;
+            s[j] = seen[j] ? x : -INFINITY;
             mx = fmaxf(mx, s[j]);
         }
         mx = rows4_max(mx);
@@ -229,10 +231,12 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
         m = mn;
         float vs[4];
         if constexpr (Q8) {
+            // Scales of keys that the lane's slot sees, each slot by itself: an
+            // infinite or huge one of a later row may not reach the earlier ones.
             float vm = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                vs[j] = pg * kPage + 4 * rg + j < it.kv_end ? cur.vs[j] : 0.f;
+                vs[j] = seen[j] ? cur.vs[j] : 0.f;
                 vm = fmaxf(vm, vs[j]);
             }
             if (__any(vm > vref)) {

@@ -404,3 +404,27 @@ def test_calls_repeat_bit_for_bit(gpu):
     first = c.kv.prefix_attention(q, rows, pre)
     for _ in range(3):
         assert torch.equal(first, c.kv.prefix_attention(q, rows, pre))
+
+
+@pytest.mark.parametrize("bad", [float("inf"), 1e30])
+@pytest.mark.parametrize("d", [64, 128])
+def test_scales_that_only_later_rows_see(gpu, d, bad):
+    """On the Q8 cache an infinite or huge value of a later row makes that
+    row's scale so; the rows before it keep their results."""
+    c = Cache([60, 50], n_head=2, head_dim=d, q8=True, seed=45)
+    v = torch.full((1, 1, 2 * d), bad, device=gpu)
+    for p in (31, 33, 40):
+        k = c.queries(1, seed=p)
+        c.put(0, k, v, p)
+        c.k[0][:, p:p + 1], c.v[0][:, p:p + 1] = c.stored(k), c.stored(v)
+    for group in (2, 5, 9):
+        for n in (3, 4, 5):
+            rows, pre = [(0, p) for p in range(28, 28 + n)], [(1, 50, n)]
+            for split in (0, 16):
+                q = c.queries(n, group)
+                got, want = c.kv.prefix_attention(q, rows, pre, split_tokens=split), c.expect(q, rows, pre)
+                close(got[:, :3], want[:, :3], f"{group} {n} {split}: the rows before the bad value")
+                if n > 3 and math.isfinite(bad):
+                    close(got[:, 3:], want[:, 3:], f"{group} {n} {split}: the rows that see it")
+                elif n > 3:
+                    assert not torch.isfinite(got[:, 3:]).any()
