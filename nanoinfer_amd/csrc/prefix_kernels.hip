@@ -24,6 +24,15 @@ constexpr int kItemWaves = 4;        // waves of an item's workgroup
 constexpr int kMergeWaves = 4;       // slots a merge workgroup joins
 constexpr float kPScale = 16384.f;   // weights enter PV times 2^14: down to 4e-9 they are normal f16
 constexpr float kPUnscale = 1.f / kPScale;
+// Q8: where the value scales' reference starts.  Scales below it (values below
+// 1e-28) lose bits; its inverse and its products with the unscalings are normal.
+constexpr float kMinScale = 0x1p-100f;
+
+// The power of two at or above x (0 of 0): the reference of scales up to x, which those
+// of the pages to come seldom pass, and whose divisions are exact.
+__device__ __forceinline__ float scale_reference(float x) {
+    return __uint_as_float((__float_as_uint(x) + 0x7fffffu) & 0x7f800000u);
+}
 
 // One (item, layer, head): S^T = K Q^T (16 keys x 16 slots; q in f16 hi + lo
 // parts), the online softmax down its columns, O^T += V^T P^T (p in hi + lo
@@ -155,9 +164,10 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
             }
         }
     }
-    // Q8: weights enter PV times scale / vref, so that no f16 overflows: vref
-    // starts at 1 and follows the largest value scale that the slot sees past it.
-    float vref = 1.f, vinv = 1.f;
+    // Q8: weights enter PV times scale / vref, at most 1: vref follows the largest
+    // value scale that the slot has seen, so that the products keep the weights' bits
+    // whatever the values' size.
+    float vref = Q8 ? kMinScale : 1.f, vinv = 1.f / vref;
 
     for (; pg < pg_end; pg += W) {
         Regs nxt;
@@ -240,7 +250,7 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
                 vm = fmaxf(vm, vs[j]);
             }
             if (__any(vm > vref)) {
-                vm = fmaxf(rows4_max(vm), vref);
+                vm = fmaxf(scale_reference(rows4_max(vm)), vref);
                 oalpha *= vref / vm;
                 vref = vm;
                 vinv = 1.f / vm;
@@ -719,7 +729,7 @@ void prefix_wide_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
         }
     }
     float mref = 0.f, lsum = 0.f;
-    float vref = 1.f, vinv = 1.f;
+    float vref = Q8 ? kMinScale : 1.f, vinv = 1.f / vref;
     bool set = false;  // the reference is a score's (alike in both lanes of a slot)
     float16_t o[DB];
 #pragma unroll
@@ -869,7 +879,7 @@ void prefix_wide_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
             if (__any(vm > vref)) {  // (a scale belongs to its key: the same for every slot)
                 const uint32_t bits = __float_as_uint(vm);
                 const u32x2_t sw = __builtin_amdgcn_permlane32_swap(bits, bits, false, false);
-                vm = fmaxf(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])), vref);
+                vm = fmaxf(scale_reference(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]))), vref);
                 const float shrink = vref / vm;
                 vref = vm;
                 vinv = 1.f / vm;
@@ -973,11 +983,17 @@ void prefix_wide_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
                 set = true;
             }
             lsum = lsum * w1 + p[(16 * DB + 1) * 64] * w2;
-            const float u2 = Q8 ? w2 * (p[(16 * DB + 2) * 64] * vinv) : w2;  // in units of this group's vref
+            float u1 = w1, u2 = w2;
+            if constexpr (Q8) {  // in units of the larger vref
+                const float v1 = vref, v2 = p[(16 * DB + 2) * 64];
+                vref = fmaxf(v1, v2);
+                u1 *= v1 / vref;
+                u2 *= v2 / vref;
+            }
 #pragma unroll
             for (int b = 0; b < DB; b++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[b][i] = o[b][i] * w1 + p[(16 * b + i) * 64] * u2;
+                for (int i = 0; i < 16; i++) o[b][i] = o[b][i] * u1 + p[(16 * b + i) * 64] * u2;
         }
     }
     if (!has) return;

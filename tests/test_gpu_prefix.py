@@ -428,3 +428,35 @@ def test_scales_that_only_later_rows_see(gpu, d, bad):
                     close(got[:, 3:], want[:, 3:], f"{group} {n} {split}: the rows that see it")
                 elif n > 3:
                     assert not torch.isfinite(got[:, 3:]).any()
+
+
+@pytest.mark.parametrize("std", [1e-2, 1e-3, 1e-5, 1e-20])
+@pytest.mark.parametrize("d,wide", [(64, False), (128, False), (64, True), (128, True)])
+def test_small_values_on_the_q8_cache(gpu, d, wide, std):
+    """Int8 scales far below 1 cost the weights no bits, in any kernel: values
+    of one small size, and of several, zeros among them, along the keys."""
+    layers, heads, m = large(d, True) if wide else (1, 2, 700)
+    n = 33 if wide else 17
+    c = Cache([n, m], n_layer=layers, n_head=heads, head_dim=d, q8=True, seed=47)
+    g = torch.Generator(device="cuda").manual_seed(48)
+    k, v = (torch.randn((layers, m, heads * d), generator=g, device="cuda") for _ in range(2))
+    own = [torch.randn((layers, n, heads * d), generator=g, device="cuda") for _ in range(2)]
+    c.put(0, own[0], own[1] * std)
+    c.k[0], c.v[0] = c.stored(own[0]), c.stored(own[1] * std)
+    # every 32 keys another size (a group of waves reads every second or fourth such tile)
+    steps = torch.tensor([0.0, 1.0, 0.25, 0.0, 2.0, 1.0, 0.0, 0.5], device=gpu).repeat_interleave(32)
+    for size in (torch.ones(m, device=gpu), steps.repeat(-(-m // 256))[:m], torch.linspace(1, 0, m, device=gpu).square()):
+        c.put(1, k, v * std * size[None, :, None])
+        c.k[1], c.v[1] = c.stored(k), c.stored(v * std * size[None, :, None])
+        check(c, [(0, p) for p in range(n)], [(1, m, n)])
+        check(c, [(0, p) for p in range(n)], [(1, m - 5, n)], 2, split_tokens=0 if wide else 96)
+        check(c, [(0, n - 1)] * 3, [(1, 64, 3)], 5)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_values_of_zero_on_the_q8_cache(gpu, wide):
+    layers, heads, m = large(64, True) if wide else (1, 2, 300)
+    c = Cache([20, m], n_layer=layers, n_head=heads, q8=True, seed=49, std=0.0)
+    rows = [(0, p) for p in range(20)]
+    got = c.kv.prefix_attention(c.queries(20), rows, [(1, m, 20)])
+    assert torch.equal(got, torch.zeros_like(got))
