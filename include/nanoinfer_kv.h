@@ -308,8 +308,8 @@ typedef struct ni_rotary_opts {
 } ni_rotary_opts;
 /* A rotation ready for use: plain data, filled by ni_rotary_init, read during
  * the calls it is passed to and not kept.  turns[i] is f_i / 2 pi in units of
- * 2^-64 turns a position, so angles are exact to 2^-33 turns at any 32-bit
- * position. */
+ * 2^-64 turns a position, within two of them (of a base of at least 1), so
+ * angles are exact to 2^-31 turns at any 32-bit position. */
 typedef struct ni_rotary {
     uint32_t head_dim;
     uint32_t rot_dim;

@@ -35,40 +35,43 @@ int ni_rotary_init(ni_rotary* r, uint32_t head_dim, const ni_rotary_opts* o) {
         return call_error(NI_ERR_BAD_ARG, "factor must be finite and at least 1");
     if (o->attn_scale < 0 || !std::isfinite(o->attn_scale))
         return call_error(NI_ERR_BAD_ARG, "attn_scale must be finite and not negative");
-    const double s = o->scaling == NI_ROTARY_PLAIN ? 1. : o->factor;
-    double base = o->base, lo = 0., hi = 0., scale = 1.;
+    // In 64-bit mantissas: a frequency of 53 bits would put angles 2^-25 turns off at
+    // positions near 2^32.  These are (2 + 4) roundings of 2^-64 of f / 2 pi <= 0.16
+    // turns off, a scaling's included, and half a unit of the table: below two units.
+    const long double s = o->scaling == NI_ROTARY_PLAIN ? 1.L : o->factor;
+    long double base = o->base, lo = 0.L, hi = 0.L, scale = 1.L;
     if (o->scaling == NI_ROTARY_NTK) {
         if (rot <= 2) return call_error(NI_ERR_BAD_ARG, "ntk scaling needs a rot_dim above 2");
-        base *= std::pow(s, (double)rot / (rot - 2));
+        base *= std::pow(s, (long double)rot / (rot - 2));
     } else if (o->scaling == NI_ROTARY_YARN) {
-        const double fast = o->beta_fast > 0 ? o->beta_fast : 32., slow = o->beta_slow > 0 ? o->beta_slow : 1.;
+        const long double fast = o->beta_fast > 0 ? o->beta_fast : 32., slow = o->beta_slow > 0 ? o->beta_slow : 1.;
         if (!(base > 1)) return call_error(NI_ERR_BAD_ARG, "yarn scaling needs a base above 1");
         if (o->orig_ctx == 0) return call_error(NI_ERR_BAD_ARG, "yarn scaling needs orig_ctx");
         if (!(fast >= slow)) return call_error(NI_ERR_BAD_ARG, "beta_fast must be at least beta_slow");
         // The pair that makes `turns` turns over the original context.
-        auto pair = [&](double turns) {
-            return rot * std::log(o->orig_ctx / (turns * 2 * M_PI)) / (2 * std::log(base));
+        auto pair = [&](long double turns) {
+            return rot * std::log(o->orig_ctx / (turns * 2 * M_PIl)) / (2 * std::log(base));
         };
-        lo = std::max(std::floor(pair(fast)), 0.);
-        hi = std::min(std::ceil(pair(slow)), (double)rot - 1);
-        if (s > 1) scale = 0.1 * std::log(s) + 1;
+        lo = std::max(std::floor(pair(fast)), 0.L);
+        hi = std::min(std::ceil(pair(slow)), (long double)rot - 1);
+        if (s > 1) scale = 0.1L * std::log(s) + 1;
     }
     *r = ni_rotary{};
     r->head_dim = head_dim;
     r->rot_dim = rot;
     r->interleaved = o->interleaved;
-    r->scale = (float)(o->attn_scale > 0 ? o->attn_scale : scale);
+    r->scale = (float)(o->attn_scale > 0 ? (long double)o->attn_scale : scale);
     for (uint32_t i = 0; i < rot / 2; i++) {
-        double f = std::pow(base, -2. * i / rot);
+        long double f = std::pow(base, -2.L * i / rot);
         if (o->scaling == NI_ROTARY_LINEAR) f /= s;
         if (o->scaling == NI_ROTARY_YARN) {
             // Pairs that turn often keep their frequency, slow ones take the
             // stretched one, those between a mixture.
-            const double ramp = std::min(std::max((i - lo) / std::max(hi - lo, 0.001), 0.), 1.);
+            const long double ramp = std::min(std::max((i - lo) / std::max(hi - lo, 0.001L), 0.L), 1.L);
             f = f / s * ramp + f * (1 - ramp);
         }
-        const long double turns = (long double)f / (2 * M_PIl);
-        r->turns[i] = (uint64_t)std::ldexp(turns - std::floor(turns), 64);  // 2^-64 of a turn: below 2^64
+        const long double turns = f / (2 * M_PIl);
+        r->turns[i] = (uint64_t)std::round(std::ldexp(turns - std::floor(turns), 64));  // 2^-64 of a turn: below 2^64
     }
     return NI_OK;
 }

@@ -5,9 +5,9 @@
 //                         their pages and queries on their way out
 //
 // Pair i of a head turns by pos * f_i.  A frequency travels as its turns per
-// position in 2^-64 units, so pos * f_i modulo a turn is one 64-bit integer
-// product, exact to pos * 2^-65 turns at any position: no 64-bit floating
-// point and no loss at far positions.
+// position in 2^-64 units, within two of them, so pos * f_i modulo a turn is one
+// 64-bit integer product, exact to pos * 2^-63 turns: no 64-bit floating point, and
+// 2^-31 turns at most at any 32-bit position.
 #include "kv_device.h"
 #include "ops_plan.h"
 
@@ -16,8 +16,9 @@ namespace {
 
 // cos and sin of w * pos turns (w in 2^-64 turns a position), times scale.
 // The turn fraction is reduced to an eighth either way of a quarter turn in
-// integers, so the f32 angle, at most pi/4, is rounded 2^-25 of itself; the
-// Taylor sums end below 2e-9 of the result there.
+// integers, so the f32 angle is at most pi/4; its conversion, constant and product
+// round it by up to 2^-24 of itself each.  The Taylor sums end below 2e-9 of the
+// result there.
 __device__ __forceinline__ void turn(uint64_t w, int64_t pos, float scale, float& c, float& s) {
     const uint64_t f = w * (uint64_t)pos;
     const uint32_t quarter = (uint32_t)((f + (1ull << 61)) >> 62);       // 0..3, to the nearest

@@ -281,3 +281,26 @@ def test_append_refusals(gpu):
         kv.append_rotary([(0, 0)], x, x, rot, layer=1)
     kv.append_rotary([(0, 0), (0, 1)], x, x, rot, layer=0)  # a refused call leaves nothing behind
     kv.append_rotary([], x, x, rot, layer=0)
+
+
+@pytest.mark.parametrize("rows,heads", [(5, 1), (1500, 6)])
+def test_far_positions_against_the_definition(gpu, rows, heads):
+    """Angles from frequencies of the definition, in 50 digits: near 2^32 the
+    table adds 2^-31 turns, 2 pi 2^-31 of |x1| + |x2|, below a twentieth of
+    2^-24 and so within what the tolerance's eight roundings leave."""
+    import decimal
+
+    D = decimal.Decimal
+    pi = D("3.14159265358979323846264338327950288419716939937510582097494459")
+    rot = na.Rotary(64)
+    x = torch.randn((rows, heads, 64), generator=torch.Generator().manual_seed(2))
+    pos = [(1 << 32) - rows + i for i in range(rows)]
+    with decimal.localcontext() as c:
+        c.prec = 50
+        w = [D(10000) ** (-D(2 * i) / 64) / (2 * pi) for i in range(32)]
+        ang = torch.tensor([[float(p * f % 1) for f in w] for p in pos], dtype=torch.float64) * 2 * np.pi
+    c, s = torch.cos(ang)[:, None], torch.sin(ang)[:, None]
+    a, b = x.double()[..., :32], x.double()[..., 32:]
+    want, mag = torch.cat([a * c - b * s, b * c + a * s], 2), (a.abs() + b.abs()).repeat(1, 1, 2)
+    got = na.rotary(x.view(rows, -1).cuda(), rot, heads, pos0=pos[0])
+    close(got.view(rows, heads, 64), want, mag, torch.float32)

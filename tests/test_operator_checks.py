@@ -1,6 +1,7 @@
 """Refusals and host arithmetic of the rotary, shared-prefix and verification
 calls, without a GPU: every check comes before anything touches the device."""
 import ctypes as C
+import decimal
 import math
 
 import numpy as np
@@ -56,6 +57,46 @@ def test_rotary_frequencies(head_dim, rot_dim, kw):
         assert min(diff, (1 << 64) - diff) <= 16 * 2.0 ** -53 * max(x, 1e-300) / (2 * math.pi) * 2.0 ** 64 + 2
     assert r.scale == pytest.approx(want_scale, rel=2.0 ** -23)
     assert r.rot_dim == d
+
+
+PI = decimal.Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899862803")
+
+
+def _decimal_turns(d, base=10000.0, scaling=None, factor=1.0, orig_ctx=0):
+    """f_i / 2 pi modulo a turn, to 50 digits."""
+    with decimal.localcontext() as c:
+        c.prec = 60
+        D = decimal.Decimal
+        b, s = D(base), D(factor)
+        if scaling == "ntk":
+            b *= s ** (D(d) / D(d - 2))
+        f = [b ** (-2 * D(i) / d) for i in range(d // 2)]
+        if scaling == "linear":
+            f = [x / s for x in f]
+        if scaling == "yarn":
+            at = lambda n: d * (D(orig_ctx) / (n * 2 * PI)).ln() / (2 * b.ln())
+            lo = max(at(32).to_integral_value(decimal.ROUND_FLOOR), D(0))
+            hi = min(at(1).to_integral_value(decimal.ROUND_CEILING), D(d - 1))
+            ramp = [min(max((i - lo) / max(hi - lo, D("0.001")), D(0)), D(1)) for i in range(d // 2)]
+            f = [x / s * r + x * (1 - r) for x, r in zip(f, ramp)]
+        return [x / (2 * PI) % 1 for x in f]
+
+
+@pytest.mark.parametrize("head_dim,kw", [
+    (64, {}), (128, {}), (256, dict(base=1e6)), (80, dict(base=500000.0)), (2, {}), (128, dict(base=1.0)),
+    (64, dict(scaling="linear", factor=5.5)), (128, dict(scaling="ntk", factor=8.0, base=500000.0)),
+    (4, dict(scaling="ntk", factor=4.0)),
+    (128, dict(scaling="yarn", factor=8.0, orig_ctx=8192)), (64, dict(scaling="yarn", factor=2.5, orig_ctx=2048)),
+])
+def test_rotary_frequencies_to_the_tables_last_bits(head_dim, kw):
+    """Within two units of 2^-64 turns: the roundings of 2^-64 of f / 2 pi, at
+    most 0.16 turns (2 of the power, 1 of the exponent, which shrinks with f, 2
+    of the quotient by 2 pi, up to 4 of a scaling), and half a unit."""
+    got, want = _turns(na.Rotary(head_dim, **kw)), _decimal_turns(head_dim, **kw)
+    for i, (g, w) in enumerate(zip(got, want)):
+        off = (decimal.Decimal(g) - w * 2 ** 64) % 2 ** 64
+        off = min(off, 2 ** 64 - off)
+        assert off <= 2, f"pair {i}: {off:.1f} units"
 
 
 def test_rotary_attn_scale_replaces_the_scalings_own():
