@@ -125,10 +125,35 @@ __device__ __forceinline__ void split_w16x2(float x0, float x1, uint32_t& hi, ui
 
 // A matrix product may read what a vector instruction wrote two wait states ago
 // at the earliest.  The compiler sees to that for instructions of its own, not
-// for split_w16x2's: operands that go from there into a product pass through here.
-__device__ __forceinline__ void settle(half4_t& a, half4_t& b) { asm volatile("s_nop 1" : "+v"(a), "+v"(b)); }
+// for split_w16x2's: operands that go from there into a product pass through here
+// (split4 and split8 see to it themselves).
+__device__ __forceinline__ void settle(half4_t& a, half4_t& b) { asm("s_nop 1" : "+v"(a), "+v"(b)); }
+__device__ __forceinline__ void settle(half8_t& a, half8_t& b) { asm("s_nop 1" : "+v"(a), "+v"(b)); }
 __device__ __forceinline__ void settle(u32x4& a, u32x4& b, u32x4& c, u32x4& d) {
-    asm volatile("s_nop 1" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+    asm("s_nop 1" : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
+}
+
+// Four or eight values as operands of matrix products, hi and lo parts.
+__device__ __forceinline__ void split4(const float (&x)[4], half4_t& hi, half4_t& lo) {
+    uint32_t h0, l0, h1, l1;
+    split_w16x2(x[0], x[1], h0, l0);
+    split_w16x2(x[2], x[3], h1, l1);
+    hi = __builtin_bit_cast(half4_t, u32x2_t{h0, h1});
+    lo = __builtin_bit_cast(half4_t, u32x2_t{l0, l1});
+    settle(hi, lo);
+}
+__device__ __forceinline__ void split8(const float (&x)[8], half8_t& hi, half8_t& lo) {
+    u32x4 h, l;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t hp, lp;
+        split_w16x2(x[2 * i], x[2 * i + 1], hp, lp);
+        h[i] = hp;
+        l[i] = lp;
+    }
+    hi = __builtin_bit_cast(half8_t, h);
+    lo = __builtin_bit_cast(half8_t, l);
+    settle(hi, lo);
 }
 
 // Max and sum over lanes l, l ^ 16, l ^ 32, l ^ 48 (the four lanes holding

@@ -1723,11 +1723,7 @@ __global__ __launch_bounds__(64 * W, D == 64 ? kMfmaMinWaves : 1) void attn_mfma
 #pragma unroll
                 for (int j = 0; j < 4; j++) p[j] *= cur.vs[b][j] * vinv;
             }
-            uint32_t h0, l0, h1, l1;
-            split_w16x2(p[0], p[1], h0, l0);
-            split_w16x2(p[2], p[3], h1, l1);
-            ph[b] = __builtin_bit_cast(half4_t, u32x2_t{h0, h1});
-            pl[b] = __builtin_bit_cast(half4_t, u32x2_t{l0, l1});
+            split4(p, ph[b], pl[b]);
         }
         lsum = lsum * alpha + ps;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -2414,18 +2410,13 @@ __global__ __launch_bounds__(256) void attn_prefill_q8_kernel(const AttnLaunch a
                 x[0] = x0.x; x[1] = x0.y; x[2] = x0.z; x[3] = x0.w;
                 x[4] = x1.x; x[5] = x1.y; x[6] = x1.z; x[7] = x1.w;
             }
+            float y[8];
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                float x0 = x[e] * a.qscale, x1 = x[e + 1] * a.qscale;
-                asm("" : "+v"(x0), "+v"(x1));  // the f32 products, as the split's residual sees them
-                uint32_t h, l;
-                split_w16x2(x0, x1, h, l);
-                const half2_t hh = __builtin_bit_cast(half2_t, h), ll = __builtin_bit_cast(half2_t, l);
-                qh[c][e] = hh[0];
-                qh[c][e + 1] = hh[1];
-                ql[c][e] = ll[0];
-                ql[c][e + 1] = ll[1];
+            for (int e = 0; e < 8; e++) {
+                y[e] = x[e] * a.qscale;
+                asm("" : "+v"(y[e]));  // the f32 products, as the split's residual sees them
             }
+            split8(y, qh[c], ql[c]);
         }
     }
     // Weights are exp2(s - mref) with mref = m - kLog2PScalePre: p already
@@ -2547,11 +2538,7 @@ __global__ __launch_bounds__(256) void attn_prefill_q8_kernel(const AttnLaunch a
                 p[1] *= vs[b].y * vinv;
                 p[2] *= vs[b].z * vinv;
                 p[3] *= vs[b].w * vinv;
-                uint32_t h0, l0, h1, l1;
-                split_w16x2(p[0], p[1], h0, l0);
-                split_w16x2(p[2], p[3], h1, l1);
-                ph[b] = __builtin_bit_cast(half4_t, u32x2_t{h0, h1});
-                pl[b] = __builtin_bit_cast(half4_t, u32x2_t{l0, l1});
+                split4(p, ph[b], pl[b]);
             }
 #pragma unroll
             for (int b = 0; b < PT; b++) lsum += ps[b];
@@ -2762,18 +2749,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 6
     for (int c = 0; c < QC; c++) {
         const float x[8] = {xq[2 * c].x, xq[2 * c].y, xq[2 * c].z, xq[2 * c].w,
                             xq[2 * c + 1].x, xq[2 * c + 1].y, xq[2 * c + 1].z, xq[2 * c + 1].w};
+        float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            float x0 = qok ? x[e] * a.qscale : 0.f, x1 = qok ? x[e + 1] * a.qscale : 0.f;
-            asm("" : "+v"(x0), "+v"(x1));  // the f32 products, as the split's residual sees them
-            uint32_t h, l;
-            split_w16x2(x0, x1, h, l);
-            const half2_t hh = __builtin_bit_cast(half2_t, h), ll = __builtin_bit_cast(half2_t, l);
-            qh[c][e] = hh[0];
-            qh[c][e + 1] = hh[1];
-            ql[c][e] = ll[0];
-            ql[c][e + 1] = ll[1];
+        for (int e = 0; e < 8; e++) {
+            y[e] = qok ? x[e] * a.qscale : 0.f;
+            asm("" : "+v"(y[e]));  // the f32 products, as the split's residual sees them
         }
+        split8(y, qh[c], ql[c]);
     }
     // Weights are exp2(s - mref): mref = m - kLog2PScalePre for the running
     // reference m, so p enters PV scaled by 2^7 (at most 2^15).  The scores
@@ -2866,11 +2848,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D == 64 ? 6
             float p[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) p[j] = fast_exp2(sc[b][j]);
-            uint32_t h0, l0, h1, l1;
-            split_w16x2(p[0], p[1], h0, l0);
-            split_w16x2(p[2], p[3], h1, l1);
-            ph[b] = __builtin_bit_cast(half4_t, u32x2_t{h0, h1});
-            pl[b] = __builtin_bit_cast(half4_t, u32x2_t{l0, l1});
+            split4(p, ph[b], pl[b]);
         }
         // O^T += V^T P^T, 16 dims per product; pages in pairs through the
         // 32-key product (k-slot 8*rg + 4*i + j of the pair is key 4*rg + j

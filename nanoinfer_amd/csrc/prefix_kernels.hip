@@ -111,18 +111,13 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
             const float4 x0 = reinterpret_cast<const float4*>(qb + c * 32)[0];
             const float4 x1 = reinterpret_cast<const float4*>(qb + c * 32)[1];
             const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+            float y[8];
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                float y0 = has ? x[e] * a.qscale : 0.f, y1 = has ? x[e + 1] * a.qscale : 0.f;
-                asm("" : "+v"(y0), "+v"(y1));  // the f32 products, as the split's residual sees them
-                uint32_t h, l;
-                split_w16x2(y0, y1, h, l);
-                const half2_t hh = __builtin_bit_cast(half2_t, h), ll = __builtin_bit_cast(half2_t, l);
-                qh[c][e] = hh[0];
-                qh[c][e + 1] = hh[1];
-                ql[c][e] = ll[0];
-                ql[c][e + 1] = ll[1];
+            for (int e = 0; e < 8; e++) {
+                y[e] = has ? x[e] * a.qscale : 0.f;
+                asm("" : "+v"(y[e]));  // the f32 products, as the split's residual sees them
             }
+            split8(y, qh[c], ql[c]);
         }
     }
     float m = kMinScore, lsum = 0.f;
@@ -264,12 +259,8 @@ __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const Pref
 #pragma unroll
             for (int j = 0; j < 4; j++) p[j] *= vs[j] * vinv;
         }
-        uint32_t h0, l0, h1, l1;
-        split_w16x2(p[0], p[1], h0, l0);
-        split_w16x2(p[2], p[3], h1, l1);
-        half4_t ph = __builtin_bit_cast(half4_t, u32x2_t{h0, h1});
-        half4_t pl = __builtin_bit_cast(half4_t, u32x2_t{l0, l1});
-        settle(ph, pl);
+        half4_t ph, pl;
+        split4(p, ph, pl);
         if (__any(oalpha != 1.f)) {
 #pragma unroll
             for (int c = 0; c < VC; c++) o[c] *= oalpha;
@@ -715,18 +706,13 @@ void prefix_wide_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
     for (int c = 0; c < KS; c++) {
         const float x[8] = {xq[2 * c].x, xq[2 * c].y, xq[2 * c].z, xq[2 * c].w,
                             xq[2 * c + 1].x, xq[2 * c + 1].y, xq[2 * c + 1].z, xq[2 * c + 1].w};
+        float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            float x0 = has ? x[e] * a.qscale : 0.f, x1 = has ? x[e + 1] * a.qscale : 0.f;
-            asm("" : "+v"(x0), "+v"(x1));  // the f32 products, as the split's residual sees them
-            uint32_t h, l;
-            split_w16x2(x0, x1, h, l);
-            const half2_t hh = __builtin_bit_cast(half2_t, h), ll = __builtin_bit_cast(half2_t, l);
-            qh[c][e] = hh[0];
-            qh[c][e + 1] = hh[1];
-            ql[c][e] = ll[0];
-            ql[c][e + 1] = ll[1];
+        for (int e = 0; e < 8; e++) {
+            y[e] = has ? x[e] * a.qscale : 0.f;
+            asm("" : "+v"(y[e]));  // the f32 products, as the split's residual sees them
         }
+        split8(y, qh[c], ql[c]);
     }
     float mref = 0.f, lsum = 0.f;
     float vref = Q8 ? kMinScale : 1.f, vinv = 1.f / vref;
