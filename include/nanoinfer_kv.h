@@ -364,9 +364,10 @@ typedef struct ni_prefix {
  * be its prefix.
  * split_tokens: keys per partition, a multiple of 16; 0 = automatic.
  * Under stream capture the call allocates nothing: make the same call once
- * before, so that the handle holds the partials it needs (graphs captured from
- * one handle share them, so their replays must not overlap), and the plan
- * must fit the launch arguments (32 KB). */
+ * before, so that the handle holds the partials it needs, and the plan must fit
+ * the launch arguments (32 KB).  Graphs captured from one handle share those
+ * partials, so their replays must not overlap, and come after the work of the
+ * calls made before the capture; calls outside a capture have others. */
 int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_row_stride, int64_t q_layer_stride,
                            uint32_t n_q_head, const ni_row* rows, uint32_t n, const ni_prefix* prefixes,
                            uint32_t n_prefix, float* out, int64_t out_row_stride, int64_t out_layer_stride,

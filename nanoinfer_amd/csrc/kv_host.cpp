@@ -201,9 +201,11 @@ struct ni_kv {
     // retired: launches enqueued before may still use it, so it is freed by
     // the next ni_kv_sync that finds its event complete (or ni_kv_destroy).
     std::vector<std::pair<float*, hipEvent_t>> partials_retired;
-    // A call captured into a graph took `partials`: replays use it whenever
-    // they run, so once outgrown it is kept until ni_kv_destroy.
-    bool partials_captured = false;
+    // The buffer of calls captured into graphs.  Replays use it whenever they
+    // run, unseen by begin_call: eager calls have another, and outgrown ones are
+    // kept until ni_kv_destroy.
+    float* graph_partials = nullptr;
+    size_t graph_partials_bytes = 0;
     std::vector<float*> partials_kept;
     bool capturing = false;  // the current call's stream is capturing (begin_call)
     // ni_kv_step_noalloc: this device's scratch array (null if its address
@@ -1036,6 +1038,29 @@ uint32_t merge_split(const std::vector<MergeItem>& merges, uint32_t D) {
     return split;
 }
 
+// The partials of a call that is captured: those of earlier captures where
+// they are large enough, else the handle's, which the next eager call replaces
+// by new ones (a capture itself can seldom allocate).
+int ensure_graph_partials(ni_kv* kv, size_t bytes, float** out) {
+    if (bytes > kv->graph_partials_bytes) {
+        float* p = kv->partials;
+        size_t cap = kv->partials_bytes;
+        if (bytes > cap) {
+            cap = align_up(bytes + bytes / 2, 1 << 20);
+            hipError_t e = hipMalloc(reinterpret_cast<void**>(&p), cap);
+            if (e != hipSuccess) return kv->hip_fail(e, "hipMalloc(partials)");
+        } else {
+            kv->partials = nullptr;
+            kv->partials_bytes = 0;
+        }
+        if (kv->graph_partials) kv->partials_kept.push_back(kv->graph_partials);
+        kv->graph_partials = p;
+        kv->graph_partials_bytes = cap;
+    }
+    *out = kv->graph_partials;
+    return NI_OK;
+}
+
 int ensure_partials(ni_kv* kv, size_t bytes, hipStream_t s, float** out) {
     if (kv->no_alloc) {
         if (bytes > kScratchBytes)
@@ -1046,11 +1071,9 @@ int ensure_partials(ni_kv* kv, size_t bytes, hipStream_t s, float** out) {
         *out = kv->scratch;
         return NI_OK;
     }
+    if (kv->capturing) return ensure_graph_partials(kv, bytes, out);
     *out = kv->partials;
-    if (bytes <= kv->partials_bytes) {
-        kv->partials_captured |= kv->capturing;
-        return NI_OK;
-    }
+    if (bytes <= kv->partials_bytes) return NI_OK;
     // Launches already enqueued may still use the old buffer: retire it
     // (no host wait here) rather than free it.  Every earlier call's work is
     // ordered before this point of `s` (begin_call), so an event recorded
@@ -1059,9 +1082,7 @@ int ensure_partials(ni_kv* kv, size_t bytes, hipStream_t s, float** out) {
     float* p = nullptr;
     hipError_t e = hipMalloc(reinterpret_cast<void**>(&p), cap);
     if (e != hipSuccess) return kv->hip_fail(e, "hipMalloc(partials)");
-    if (kv->partials && kv->partials_captured) {
-        kv->partials_kept.push_back(kv->partials);
-    } else if (kv->partials) {
+    if (kv->partials) {
         hipEvent_t ev = take_event(kv);
         if (!ev) {
             (void)hipFree(p);
@@ -1077,7 +1098,6 @@ int ensure_partials(ni_kv* kv, size_t bytes, hipStream_t s, float** out) {
     }
     kv->partials = p;
     kv->partials_bytes = cap;
-    kv->partials_captured = kv->capturing;
     *out = p;
     return NI_OK;
 }
@@ -1708,6 +1728,7 @@ void ni_kv_destroy(ni_kv* kv) {
         for (hipEvent_t e : kv->ev_pool) (void)hipEventDestroy(e);
         if (kv->order) (void)hipEventDestroy(kv->order);
         if (kv->partials) (void)hipFree(kv->partials);
+        if (kv->graph_partials) (void)hipFree(kv->graph_partials);
         for (float* p : kv->partials_kept) (void)hipFree(p);
         for (auto& pr : kv->partials_retired) {
             (void)hipFree(pr.first);
@@ -2200,11 +2221,12 @@ int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_r
     const size_t o_bytes = align_up(parts * D * sizeof(float), kAlign), bytes = o_bytes + parts * 2 * sizeof(float);
     float* partials = nullptr;
     if (parts) {
-        if (kv->capturing && bytes > kv->partials_bytes)
+        const size_t held = std::max(kv->partials_bytes, kv->graph_partials_bytes);
+        if (kv->capturing && bytes > held)
             return kv->fail(NI_ERR_BAD_ARG,
                             "the call needs %zu bytes of partials, the handle holds %zu: make it once outside the "
                             "capture",
-                            bytes, kv->partials_bytes);
+                            bytes, held);
         if (int rc = ensure_partials(kv, bytes, s, &partials)) return rc;
     }
     PlanRef ref;

@@ -460,3 +460,51 @@ def test_values_of_zero_on_the_q8_cache(gpu, wide):
     rows = [(0, p) for p in range(20)]
     got = c.kv.prefix_attention(c.queries(20), rows, [(1, m, 20)])
     assert torch.equal(got, torch.zeros_like(got))
+
+
+def test_eager_calls_beside_replays(gpu):
+    """A replay and a call of the same handle on another stream, neither
+    waiting for the other: each has partials of its own."""
+    c = Cache([200, 200, 4000, 3000], n_head=8, head_dim=128, seed=51)
+    rows_a, pre_a = [(0, 184 + i) for i in range(16)], [(2, 4000, 16)]
+    rows_b, pre_b = [(1, 184 + i) for i in range(16)], [(3, 3000, 16)]
+    qa, qb = c.queries(16, seed=2), c.queries(16, seed=3)
+    out_a, out_b = torch.empty_like(qa), torch.empty((20, *qb.shape), device=gpu)
+    want_b = c.kv.prefix_attention(qb, rows_b, pre_b)
+    want_a = c.kv.prefix_attention(qa, rows_a, pre_a)
+    close(want_a, c.expect(qa, rows_a, pre_a))
+    close(want_b, c.expect(qb, rows_b, pre_b))
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.kv.prefix_attention(qa, rows_a, pre_a, out=out_a)
+    c.kv.prefix_attention(qb, rows_b, pre_b, out=out_b[0])
+    torch.cuda.synchronize()
+    for i in range(20):
+        with torch.cuda.stream(a):
+            graph.replay()
+            graph.replay()
+        c.kv.prefix_attention(qb, rows_b, pre_b, out=out_b[i], stream=b)
+    torch.cuda.synchronize()
+    assert torch.equal(out_a, want_a)
+    assert all(torch.equal(x, want_b) for x in out_b)
+    # later captures share the first one's partials, or take the handle's where they need more
+    more = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(more):
+        c.kv.prefix_attention(qb, rows_b, pre_b, out=out_b[0])
+    big = [(0, 199 - i) for i in range(150)]
+    q = c.queries(150, 2)
+    want = c.kv.prefix_attention(q, big, [(2, 4000, 150)], split_tokens=256)
+    out, most = torch.empty_like(want), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(most):
+        c.kv.prefix_attention(q, big, [(2, 4000, 150)], split_tokens=256, out=out)
+    for _ in range(3):
+        for x in (out_a, out_b, out):
+            x.zero_()
+        graph.replay()
+        more.replay()
+        most.replay()
+        c.kv.prefix_attention(qb, rows_b, pre_b, out=out_b[1])
+        torch.cuda.synchronize()
+        assert torch.equal(out_a, want_a) and torch.equal(out, want)
+        assert torch.equal(out_b[0], want_b) and torch.equal(out_b[1], want_b)
