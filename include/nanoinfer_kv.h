@@ -362,6 +362,10 @@ typedef struct ni_prefix {
  * of the cache's n_head: query head h reads cache head h / (n_q_head /
  * n_head).  out may be q with the same strides.  A row's own sequence may not
  * be its prefix.
+ * Range: rows that share tiles hold q / sqrt(head_dim) * log2(e) as two f16
+ * parts, so |q| is at most 3.6e5 (head_dim 64; 5.1e5 at 128); a larger value
+ * may make its row NaN.  On the Q8 cache keys and values that a row sees are
+ * finite; what later rows, or no row, may see does not matter.
  * split_tokens: keys per partition, a multiple of 16; 0 = automatic.
  * Under stream capture the call allocates nothing: make the same call once
  * before, so that the handle holds the partials it needs, and the plan must fit

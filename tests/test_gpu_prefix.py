@@ -508,3 +508,27 @@ def test_eager_calls_beside_replays(gpu):
         torch.cuda.synchronize()
         assert torch.equal(out_a, want_a) and torch.equal(out, want)
         assert torch.equal(out_b[0], want_b) and torch.equal(out_b[1], want_b)
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("d,top", [(64, 3.6e5), (128, 5.1e5)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_queries_at_the_end_of_their_range(gpu, d, top, q8, wide):
+    """The largest q of the contract, against keys that leave ordinary scores."""
+    layers, heads, m = large(d, q8) if wide else (1, 2, 300)
+    n = 33 if wide else 17
+    c = Cache([n, m], n_layer=layers, n_head=heads, head_dim=d, q8=q8, seed=53)
+    g = torch.Generator(device="cuda").manual_seed(54)
+    for s, x in ((0, n), (1, m)):
+        k, v = (torch.randn((layers, x, heads * d), generator=g, device="cuda") for _ in range(2))
+        k *= d ** 0.5 / top  # (f16: halves of 2^-24, as stored)
+        c.put(s, k, v)
+        c.k[s], c.v[s] = c.stored(k), c.stored(v)
+    q = c.queries(n).clamp(-3, 3) * (top / 3)
+    q[..., ::7] = top
+    rows, pre = [(0, p) for p in range(n)], [(1, m, n)]
+    got, want = c.kv.prefix_attention(q, rows, pre), c.expect(q, rows, pre)
+    # A score's products come to 2^6 in magnitude: 2^6 * (2^-22 of the split + up to 2^7 f32 sums of 2^-24) is
+    # 2^-11 of a weight, and as much of the weights' sum.
+    assert torch.isfinite(got).all()
+    assert (got.double().cpu() - want).norm() <= 2.0 ** -10 * want.norm()
