@@ -231,8 +231,13 @@ struct ni_kv {
     // scratch reused across calls
     Plan plan;
     PrefixPlan prefix_plan;
-    std::vector<uint32_t> slot_mark;  // (page, slot) -> stamp of the last ni_kv_append_rotary that wrote it
-    uint32_t slot_stamp = 0;
+    // Places (page * kPage + slot) of one ni_kv_append_rotary: an open-addressed
+    // table of twice its rows at least, an entry in use where it bears the call's stamp.
+    struct PlaceMark {
+        uint32_t place, stamp;
+    };
+    std::vector<PlaceMark> place_marks;
+    uint32_t place_stamp = 0;
     std::vector<uint8_t> blob;  // the serialised plan
     std::vector<QRow> qrows;
     std::vector<int64_t> seq_tab;     // seq -> offset in plan.table, -1 if absent
@@ -2099,11 +2104,19 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
         return kv->fail(NI_ERR_BAD_ARG, "kv_pages %u: the rotating append takes at most %u", kv->o.kv_pages,
                         kMaxRotaryPages);
     // Two rows at one position would race on its slot.
-    kv->slot_mark.resize((size_t)kv->o.kv_pages * kPage, 0);
-    if (++kv->slot_stamp == 0) {
-        std::fill(kv->slot_mark.begin(), kv->slot_mark.end(), 0);
-        kv->slot_stamp = 1;
+    auto& marks = kv->place_marks;
+    if (marks.size() < 2ull * n) marks.resize(2ull * n, {0, 0});
+    if (++kv->place_stamp == 0) {
+        std::fill(marks.begin(), marks.end(), ni_kv::PlaceMark{0, 0});
+        kv->place_stamp = 1;
     }
+    auto taken = [&](uint32_t place) {  // by an earlier row; by this one from now on
+        size_t i = (uint64_t)(place * 0x9e3779b1u) * marks.size() >> 32;
+        for (; marks[i].stamp == kv->place_stamp; i = i + 1 == marks.size() ? 0 : i + 1)
+            if (marks[i].place == place) return true;
+        marks[i] = {place, kv->place_stamp};
+        return false;
+    };
     std::vector<uint8_t>& blob = kv->blob;
     blob.resize(align_up((size_t)n * sizeof(RotaryEntry), kAlign));
     RotaryEntry* entries = reinterpret_cast<RotaryEntry*>(blob.data());
@@ -2111,10 +2124,7 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
         if (int rc = check_row(kv, rows[i])) return rc;
         const ni_row& r = rows[i];
         const uint32_t place = kv->pages[r.seq][r.pos / kPage] * kPage + r.pos % kPage;
-        uint32_t& mark = kv->slot_mark[place];
-        if (mark == kv->slot_stamp)
-            return kv->fail(NI_ERR_BAD_ARG, "sequence %u: position %u appears twice", r.seq, r.pos);
-        mark = kv->slot_stamp;
+        if (taken(place)) return kv->fail(NI_ERR_BAD_ARG, "sequence %u: position %u appears twice", r.seq, r.pos);
         entries[i] = {positions ? positions[i] : r.pos, place};
     }
     DeviceScope device(kv->device);

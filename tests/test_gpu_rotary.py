@@ -304,3 +304,36 @@ def test_far_positions_against_the_definition(gpu, rows, heads):
     want, mag = torch.cat([a * c - b * s, b * c + a * s], 2), (a.abs() + b.abs()).repeat(1, 1, 2)
     got = na.rotary(x.view(rows, -1).cuda(), rot, heads, pos0=pos[0])
     close(got.view(rows, heads, 64), want, mag, torch.float32)
+
+
+def _resident_mb():
+    for line in open("/proc/self/status"):
+        if line.startswith("VmRSS"):
+            return int(line.split()[1]) / 1024
+
+
+def test_a_place_written_twice_among_many_rows(gpu):
+    """Found whichever rows they are, with host memory that follows the rows
+    of a call and not the pages of the pool."""
+    def cache(pages):
+        kv = na.PagedKv(na.BatchOpts(n_layer=1, n_head=1, head_dim=64, kv_blocks=pages, max_seqs=64, n_ctx=64, max_rows=4096))
+        for s in range(64):
+            kv.reserve(kv.add_seq(), 64)
+        return kv
+
+    rot, x = na.Rotary(64), torch.zeros((4096, 64), device=gpu)
+    rows = np.array([(s, p) for s in range(64) for p in range(64)], dtype=np.uint32)
+    rng = np.random.default_rng(5)
+    cache(300).append_rotary(rows, x, x, rot, layer=0)
+    kv = cache(1 << 20)
+    torch.cuda.synchronize()
+    before = _resident_mb()
+    kv.append_rotary(rows[:64], x, x, rot, layer=0)
+    assert _resident_mb() - before < 16
+    for n in (2, 3, 17, 500, 4096):
+        some = rng.permutation(rows)[:n].copy()
+        kv.append_rotary(some, x, x, rot, layer=0)
+        i, j = rng.choice(n, 2, replace=False)
+        some[i] = some[j]
+        with pytest.raises(na.KvError, match="appears twice"):
+            kv.append_rotary(some, x, x, rot, layer=0)
