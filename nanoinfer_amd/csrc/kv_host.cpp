@@ -2056,6 +2056,24 @@ static int check_call(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, 
     return NI_OK;
 }
 
+// Whether two of n x m rows of `width` values share any, row (i, j) beginning at
+// i * a + j * b (strides checked to be non-negative).
+static bool rows_overlap(uint64_t n, uint64_t a, uint64_t m, uint64_t b, uint64_t width) {
+    if (n > 1 && a < width) return true;
+    if (m > 1 && b < width) return true;
+    // One stride steps past all rows of the other, as in any layout of a tensor.
+    if (n == 1 || m == 1) return false;
+    typedef unsigned __int128 u128;
+    if ((u128)(n - 1) * a + width <= b || (u128)(m - 1) * b + width <= a) return false;
+    // Else j steps of b end near i of a for some i, j: the two nearest i of each j.
+    for (uint64_t j = 1; j < m; j++) {
+        const u128 at = (u128)j * b;
+        const u128 i = at / a, past = at - i * a;
+        if ((i < n && past < width) || (i + 1 < n && a - past < width)) return true;
+    }
+    return false;
+}
+
 // A plan too long for the launch arguments is uploaded on another stream,
 // which a capture cannot record.
 static int check_capture(ni_kv* kv, size_t plan_bytes) {
@@ -2083,10 +2101,8 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
     if (n_q_head) {
         if (int rc = check_f32_operand(kv, "q", q, q_row_stride, q_layer_stride, all)) return rc;
         if (int rc = check_f32_operand(kv, "q_out", q_out, q_out_row_stride, q_out_layer_stride, all)) return rc;
-        if ((n > 1 && (uint64_t)q_out_row_stride < (uint64_t)n_q_head * D) ||
-            (all && n_lay > 1 && (uint64_t)q_out_layer_stride < (uint64_t)n_q_head * D))
-            return kv->fail(NI_ERR_BAD_ARG, "q_out's rows overlap: strides must be at least %llu",
-                            (unsigned long long)n_q_head * D);
+        if (rows_overlap(n, q_out_row_stride, all ? n_lay : 1, q_out_layer_stride, (uint64_t)n_q_head * D))
+            return kv->fail(NI_ERR_BAD_ARG, "q_out's rows of %llu values overlap", (unsigned long long)n_q_head * D);
         if (q_out == q && ((n > 1 && q_row_stride != q_out_row_stride) ||
                            (all && n_lay > 1 && q_layer_stride != q_out_layer_stride)))
             return kv->fail(NI_ERR_BAD_ARG, "q_out may be q only with q's strides");
@@ -2194,10 +2210,8 @@ int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_r
     const bool all = layer == NI_ALL_LAYERS;
     if (int rc = check_f32_operand(kv, "q", q, q_row_stride, q_layer_stride, all)) return rc;
     if (int rc = check_f32_operand(kv, "out", out, out_row_stride, out_layer_stride, all)) return rc;
-    if ((n > 1 && (uint64_t)out_row_stride < (uint64_t)n_q_head * D) ||
-        (all && n_lay > 1 && (uint64_t)out_layer_stride < (uint64_t)n_q_head * D))
-        return kv->fail(NI_ERR_BAD_ARG, "out's rows overlap: strides must be at least %llu",
-                        (unsigned long long)n_q_head * D);
+    if (rows_overlap(n, out_row_stride, all ? n_lay : 1, out_layer_stride, (uint64_t)n_q_head * D))
+        return kv->fail(NI_ERR_BAD_ARG, "out's rows of %llu values overlap", (unsigned long long)n_q_head * D);
     if (out == q && ((n > 1 && q_row_stride != out_row_stride) ||
                      (all && n_lay > 1 && q_layer_stride != out_layer_stride)))
         return kv->fail(NI_ERR_BAD_ARG, "out may be q only with q's strides");

@@ -532,3 +532,38 @@ def test_queries_at_the_end_of_their_range(gpu, d, top, q8, wide):
     # 2^-11 of a weight, and as much of the weights' sum.
     assert torch.isfinite(got).all()
     assert (got.double().cpu() - want).norm() <= 2.0 ** -10 * want.norm()
+
+
+def test_outputs_of_every_layout(gpu):
+    """Row and layer strides of any kind: rows that share memory are refused,
+    others hold what rows one after another do."""
+    import random
+
+    c = Cache([20, 50, 64], n_layer=3, n_head=2, seed=55)
+    rows, pre = [(0, 19), (1, 44), (1, 45)], [(2, 63, 3)]
+    q, rot = c.queries(3), na.Rotary(64)
+    want = c.kv.prefix_attention(q, rows, pre)
+    turned = c.kv.append_rotary(rows, q, q, rot, q=q)
+    want_after = c.kv.prefix_attention(q, rows, pre)
+    assert not torch.equal(want, want_after)  # (the keys appended are new; from here on always the same)
+    rng, seen = random.Random(56), set()
+    layouts = [(128, 128), (128, 384), (384, 128), (128, 256), (256, 384), (384, 256), (260, 128), (128, 388)]
+    layouts += [(4 * rng.randint(28, 110), 4 * rng.randint(28, 110)) for _ in range(60)]
+    for a, b in layouts:
+        at = sorted(i * a + j * b for i in range(3) for j in range(3))
+        shared = any(y - x < 128 for x, y in zip(at, at[1:]))
+        seen.add(shared)
+        buf = torch.zeros(2 * a + 2 * b + 128, device=gpu)
+        out = buf.as_strided((3, 3, 128), (b, a, 1))
+        if shared:
+            with pytest.raises(na.KvError, match="overlap"):
+                c.kv.prefix_attention(q, rows, pre, out=out)
+            with pytest.raises(na.KvError, match="overlap"):
+                c.kv.append_rotary(rows, q, q, rot, q=q, q_out=out)
+        else:
+            c.kv.prefix_attention(q, rows, pre, out=out)
+            assert torch.equal(out, want_after), (a, b)
+            buf.zero_()
+            c.kv.append_rotary(rows, q, q, rot, q=q, q_out=out)
+            assert torch.equal(out, turned), (a, b)
+    assert seen == {False, True}
