@@ -184,9 +184,9 @@ class Spec:
         if accepted is not None:
             if hasattr(accepted, "cpu"):
                 accepted = accepted.cpu()
-            arr = np.asarray(accepted, np.int64).reshape(-1)
-            if arr.size != self.n or (arr < 0).any() or (arr > 0xffffffff).any():
-                raise ValueError(f"accepted must be {self.n} numbers in 0..2^32-1")
+            arr = np.asarray(accepted).reshape(-1)
+            if arr.size != self.n or (self.n and (arr.dtype.kind not in "iu" or arr.min() < 0 or arr.max() > 0xffffffff)):
+                raise ValueError(f"accepted must be {self.n} integers in 0..2^32-1")
             arr = np.ascontiguousarray(arr, dtype=np.uint32)
             _check(self._L.ni_spec_commit_accepted(self._h, arr.ctypes.data_as(C.POINTER(_u32))),
                    "ni_spec_commit_accepted")

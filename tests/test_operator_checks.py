@@ -350,3 +350,24 @@ def test_spec_commit_takes_the_callers_numbers():
     assert sp.commit([0, 0, 0]) == [0, 0, 0]
     with pytest.raises(Exception, match="without a planned round"):
         sp.commit([0, 0, 0])
+
+
+def test_spec_commit_refuses_what_is_no_integer():
+    """1.9 accepted drafts are not 1, nor is 2^64 - 1 a small number."""
+    kv = na.PagedKv(na.BatchOpts(kv_blocks=32, max_seqs=2, n_ctx=256, max_rows=64, host_only=True))
+    seqs = [kv.add_seq() for _ in range(2)]
+    for s in seqs:
+        kv.reserve(s, 5)
+        kv.commit(s, 5)
+    sp = drivers.Spec(kv, seqs, 4, 1)
+    work, _ = sp.plan()
+    for s, n, _ in np.asarray(work).tolist():
+        kv.reserve(s, kv.seq_len(s) + n)
+        kv.commit(s, n)
+    for bad in ([0.0, 1.9], [0, float("nan")], torch.tensor([1.0, 2.5]), [False, True], ["0", "1"],
+                np.array([0, 2 ** 64 - 1], dtype=np.uint64)):
+        with pytest.raises(ValueError):
+            sp.commit(bad)
+    assert [kv.seq_len(s) for s in seqs] == [10, 10]
+    assert sp.commit(np.array([0, 4], dtype=np.uint64)) == [0, 4]
+    assert [kv.seq_len(s) for s in seqs] == [6, 10]
