@@ -30,6 +30,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from operator import index
 from typing import Optional, Sequence
 
 import numpy as np
@@ -579,7 +580,7 @@ class PagedKv:
         arr, rp, n = _rows(rows)
         pre = (_abi.ni_prefix * len(prefixes))()
         for p, x in zip(pre, prefixes):
-            seq, length, count = map(int, x)
+            seq, length, count = map(index, x)
             if not (0 <= seq <= 0xffffffff and 0 <= length <= 0xffffffff and 0 <= count <= 0xffffffff):
                 raise ValueError("prefixes must be (seq, length, n_rows) of numbers in 0..2^32-1")
             p.seq, p.len, p.n_rows = seq, length, count

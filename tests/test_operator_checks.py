@@ -371,3 +371,13 @@ def test_spec_commit_refuses_what_is_no_integer():
     assert [kv.seq_len(s) for s in seqs] == [10, 10]
     assert sp.commit(np.array([0, 4], dtype=np.uint64)) == [0, 4]
     assert [kv.seq_len(s) for s in seqs] == [6, 10]
+
+
+def test_prefixes_are_integers():
+    kv = _host_kv()
+    q = torch.zeros((2, 2, 128))
+    for bad in ((0, 1.5, 2), (0, "1", 2), (0, None, 2)):
+        with pytest.raises(TypeError, match="integer"):
+            kv.prefix_attention(q, [(0, 0), (0, 1)], [bad])
+    with pytest.raises(TypeError, match="CUDA"):  # as far as integers of any kind get on the host
+        kv.prefix_attention(q, [(0, 0), (0, 1)], [(np.uint32(0), torch.tensor(0), 2)])
