@@ -111,7 +111,10 @@ def _stream_now(device, stream):
 
 class _on:
     """The device made current where it is not, and `stream` where one is
-    given, for what a call allocates and launches; gives the stream's handle."""
+    given, for what a call allocates and launches; gives the stream's handle.
+    A stream is a torch stream of that device, or another object with its
+    `cuda_stream`: a workspace has to come from the allocator's pool of that
+    stream, or work on another could take it while the call still uses it."""
 
     __slots__ = ("_scopes", "_ptr")
 
@@ -121,7 +124,12 @@ class _on:
         if device is not None and torch.cuda.is_initialized() and \
                 (_get_device() if _get_device is not None else torch.cuda.current_device()) != device:
             scopes.append(torch.cuda.device(device))
-        if stream is not None and hasattr(stream, "stream_id"):
+        if stream is not None:
+            if not hasattr(stream, "stream_id"):
+                at = int(stream.cuda_stream)
+                stream = torch.cuda.ExternalStream(at, device) if at else torch.cuda.default_stream(device)
+            if device is not None and stream.device_index != device:
+                raise ValueError(f"the stream is of cuda:{stream.device_index}, the tensors are on cuda:{device}")
             scopes.append(torch.cuda.stream(stream))
         self._scopes = scopes
         self._ptr = stream

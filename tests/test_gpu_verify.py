@@ -211,3 +211,21 @@ def test_another_stream(gpu):
     s.synchronize()
     want = expect(t, d, au, su, draft=q)
     assert np.array_equal(acc.cpu().numpy(), want[0]) and np.array_equal(tok.cpu().numpy(), want[1])
+
+
+def test_any_object_with_a_streams_handle(gpu):
+    """What the call allocates belongs to the stream it runs on, whatever names it."""
+    from nanoinfer_amd import batch
+
+    t, d, au, su, q = inputs(16, 3, 20001, seed=14)
+    want = expect(t, d, au, su, draft=q)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    for stream in (s, torch.cuda.default_stream()):
+        handle = type("S", (), dict(cuda_stream=stream.cuda_stream))()
+        with batch._on(t.get_device(), handle) as at:
+            assert at == stream.cuda_stream == torch.cuda.current_stream().cuda_stream
+        assert torch.cuda.current_stream() == torch.cuda.default_stream()
+        acc, tok = na.verify_drafts(t, d, au, su, draft=q, stream=handle)
+        stream.synchronize()
+        assert np.array_equal(acc.cpu().numpy(), want[0]) and np.array_equal(tok.cpu().numpy(), want[1])

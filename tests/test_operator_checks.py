@@ -381,3 +381,12 @@ def test_prefixes_are_integers():
             kv.prefix_attention(q, [(0, 0), (0, 1)], [bad])
     with pytest.raises(TypeError, match="CUDA"):  # as far as integers of any kind get on the host
         kv.prefix_attention(q, [(0, 0), (0, 1)], [(np.uint32(0), torch.tensor(0), 2)])
+
+
+def test_a_stream_of_another_device_is_refused():
+    """Its context would make that device the current one, and the launch its."""
+    from nanoinfer_amd import batch
+
+    other = type("S", (), dict(cuda_stream=64, stream_id=3, device_index=1))()
+    with pytest.raises(ValueError, match="the stream is of cuda:1"):
+        batch._on(0, other)
