@@ -43,10 +43,11 @@ __device__ __forceinline__ float scale_reference(float x) {
 // thread joins the prefix's partials of its dims first, eight loads at a time,
 // which arrive while the first pages do, and holds the sum to the end.  Bound by
 // memory on long prefixes (16 rows x 32 heads x 128 behind 32767 keys, 595 MB with the
-// rows' own keys: 90 us, 6.6 TB/s); by the ~250 vector instructions a page of the Q8
-// cache costs a wave (32 x 5 rows x 12 heads x 64 behind 2001: 13 us); by the start
-// and the chain of pages of its longest items otherwise (48 rows x 32 query heads on 8
-// x 128, 1..511 own keys: 15 us).
+// rows' own keys: 90 us, 6.6 TB/s); on the Q8 cache by what a page costs a wave, which
+// is paid once per 16 slots (~250 vector instructions, the f16 page's way into LDS), and by
+// CUs with four workgroups where the mean is 3.4 (32 x 5 rows x 12 heads x 64 behind 2001:
+// 12.7 us, 5.7 of them vector issue); by the start and the chain of pages of its
+// longest items otherwise (48 rows x 32 query heads on 8 x 128, 1..511 own keys: 15 us).
 template <int D, int INL, bool Q8>
 __global__ __launch_bounds__(64 * kItemWaves) void prefix_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
     constexpr int W = kItemWaves;
@@ -925,8 +926,9 @@ void prefix_wide_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
         sc = scores(0, [](int) {});
         lm = largest(sc);
     }
-    // (the stage is a variable: the body instantiated per stage spills
-    // registers at head_dim 128)
+    // (the stage is a variable: the body instantiated per stage spills many
+    // registers at head_dim 128, where three waves of f16 spill 12 bytes a lane as it
+    // is, and two of Q8 8)
     uint32_t stage = 0;
     const uint32_t steps = (all_tiles + KG - 1) / KG;
     for (uint32_t ti = 0; ti + 1 < steps; ti++) {

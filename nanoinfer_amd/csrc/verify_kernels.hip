@@ -118,8 +118,9 @@ __device__ __forceinline__ double wave_sum(double x) {
 
 // Workgroup (run of a.per chunks, sequence): few enough that the chain to the
 // first rejection (draft count, token, probabilities: three loads one after
-// another) is walked once per run.  64 sequences of two rows of 131071 f32, 67 MB:
-// 10.8 us (6.2 TB/s); one of 50257 3.6.
+// another) is walked once per run.  64 sequences of 131071 f32, a third of which end on
+// a rejection and read the drafter's row too, 45 MB: 11 us (4.1 TB/s; a chunk's loads
+// wait for the sums of the one before); one of 50257 3.6.
 template <typename T>
 __global__ __launch_bounds__(kVT) void verify_sums_kernel(const VerifyLaunch a, const uint32_t chunks) {
     __shared__ double2 sh[2][kVT / 64];
