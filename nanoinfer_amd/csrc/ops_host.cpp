@@ -17,6 +17,29 @@ bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p
 
 uint32_t type_bytes(uint32_t dtype) { return dtype == NI_F32 ? 4u : 2u; }
 
+// Rows of `width` 4-byte values (aligned to them), `stride` apart.
+struct Rows {
+    const char* name;
+    const void* p;
+    int64_t stride, width;
+};
+
+// Whether n rows of a and n of b (where it is given) have a value in common.
+bool share(const Rows& a, const Rows& b, uint32_t n) {
+    if (!b.p) return false;
+    typedef __int128 i128;
+    const i128 from = ((i128)reinterpret_cast<uintptr_t>(a.p) - (i128)reinterpret_cast<uintptr_t>(b.p)) / 4;
+    if (from >= (i128)(n - 1) * b.stride + b.width || from + (i128)(n - 1) * a.stride + a.width <= 0) return false;
+    for (uint32_t i = 0; i < n; i++) {
+        // The last row of b that begins at row i of a or before it, and the next.
+        const i128 at = from + (i128)i * a.stride;
+        const i128 j = b.stride > 0 && at > 0 ? std::min<i128>(at / b.stride, n - 1) : 0;
+        for (i128 k = j; k <= j + 1 && k < n; k++)
+            if (at < k * b.stride + b.width && at + a.width > k * b.stride) return true;
+    }
+    return false;
+}
+
 }  // namespace
 
 extern "C" {
@@ -160,9 +183,16 @@ int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stri
     const size_t need = ni_verify_workspace(n_seq, vocab);
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
         return call_error(NI_ERR_BAD_ARG, "workspace must be %zu bytes, 16-byte aligned", need);
-    // (workgroups of one sequence read the drafts while another writes the answer)
-    if (n_draft > 0 && (accepted == n_drafts || tokens == drafted))
-        return call_error(NI_ERR_BAD_ARG, "accepted and tokens may not share memory with n_drafts and drafted");
+    // (workgroups of one sequence read its drafts and numbers while another writes the answer)
+    const Rows acc = {"accepted", accepted, 1, 1}, tok = {"tokens", tokens, tokens_stride, (int64_t)n_draft + 1};
+    const Rows in[] = {{"n_drafts", n_drafts, 1, 1},
+                       {"drafted", n_draft ? drafted : nullptr, drafted_stride, n_draft},
+                       {"accept_u", n_draft ? accept_u : nullptr, accept_stride, n_draft},
+                       {"sample_u", sample_u, 1, 1}};
+    for (const Rows& x : in)
+        for (const Rows& y : {acc, tok})
+            if (share(y, x, n_seq)) return call_error(NI_ERR_BAD_ARG, "%s may not share memory with %s", y.name, x.name);
+    if (share(tok, acc, n_seq)) return call_error(NI_ERR_BAD_ARG, "tokens may not share memory with accepted");
     VerifyLaunch a{};
     a.target = target;
     a.target_seq_stride = target_seq_stride;

@@ -229,3 +229,20 @@ def test_any_object_with_a_streams_handle(gpu):
         acc, tok = na.verify_drafts(t, d, au, su, draft=q, stream=handle)
         stream.synchronize()
         assert np.array_equal(acc.cpu().numpy(), want[0]) and np.array_equal(tok.cpu().numpy(), want[1])
+
+
+def test_answers_beside_their_inputs_in_one_buffer(gpu):
+    """Columns of one buffer share no value: [drafted | tokens | other], any order."""
+    t, d, au, su, q = inputs(9, 4, 700, seed=15)
+    want = expect(t, d, au, su, draft=q)
+    for first, second in ((0, 4), (5, 0)):
+        buf = torch.full((9, 12), -7, dtype=torch.int32, device=gpu)
+        drafted, tokens = buf[:, first:first + 4], buf[:, second:second + 5]
+        drafted.copy_(d)
+        acc, tok = na.verify_drafts(t, drafted, au, su, draft=q, tokens=tokens)
+        assert np.array_equal(acc.cpu().numpy(), want[0]) and np.array_equal(tok.cpu().numpy(), want[1])
+        assert (buf[:, 9:] == -7).all() and torch.equal(drafted, d)
+    for shift in (-4, -1, 0, 1, 3):  # the drafts inside the answer's columns
+        buf = torch.zeros((9, 14), dtype=torch.int32, device=gpu)
+        with pytest.raises(na.KvError, match="tokens may not share memory with drafted"):
+            na.verify_drafts(t, buf[:, 5 + shift:9 + shift], au, su, draft=q, tokens=buf[:, 5:10] if shift != -4 else buf[:, 4:9])

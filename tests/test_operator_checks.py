@@ -390,3 +390,39 @@ def test_a_stream_of_another_device_is_refused():
     other = type("S", (), dict(cuda_stream=64, stream_id=3, device_index=1))()
     with pytest.raises(ValueError, match="the stream is of cuda:1"):
         batch._on(0, other)
+
+
+def test_verify_refuses_answers_that_share_any_value_with_its_inputs():
+    """Views of one buffer, at every shift that overlaps (none of these calls
+    gets as far as a launch)."""
+    names = dict(drafted=("drafted", "ds"), accept_u=("au", "aus"), sample_u=("su", None), n_drafts=("n_drafts", None))
+    n, k = 3, 4
+
+    def buffer():
+        b = (C.c_int32 * 512)()
+        return b, C.addressof(b) + -C.addressof(b) % 16
+
+    keep, at = zip(*[buffer() for _ in range(9)])
+    base = dict(target=at[0], draft=None, drafted=at[1], ds=k, au=at[2], aus=k, su=at[3], n_drafts=at[4],
+                accepted=at[5], tokens=at[6], ts=k + 1, work=at[7], n_seq=n, n_draft=k, vocab=9, tss=45, trs=9)
+    cells = lambda p, stride, width: {p + 4 * (i * stride + j) for i in range(n) for j in range(width)}
+    seen = 0
+    for what, (name, stride_name) in names.items():
+        for shift in range(-24, 25):
+            for ts in (5, 6, 9, 11):
+                for stride in ((0, 4, 6, 11) if stride_name else (1,)):
+                    p = at[8] + 4 * (100 + shift)
+                    kw = dict(base, tokens=at[8] + 400, ts=ts, **{name: p}, **({stride_name: stride} if stride_name else {}))
+                    if not cells(p, stride, k if stride_name else 1) & cells(at[8] + 400, ts, k + 1):
+                        continue
+                    rc, msg, _ = _verify_call(**kw)
+                    assert rc == _abi.NI_ERR_BAD_ARG and f"tokens may not share memory with {what}" in msg, (kw, msg)
+                    seen += 1
+        for shift in (-1, 0, 1):
+            kw = dict(base, accepted=at[8] + 400, **{name: at[8] + 4 * (100 + shift)})
+            if stride_name is None or shift <= 0:
+                rc, msg, _ = _verify_call(**kw)
+                assert rc == _abi.NI_ERR_BAD_ARG and f"accepted may not share memory with {what}" in msg
+    rc, msg, _ = _verify_call(**dict(base, accepted=at[6] + 4))
+    assert rc == _abi.NI_ERR_BAD_ARG and "tokens may not share memory with accepted" in msg
+    assert seen > 500
