@@ -392,7 +392,8 @@ int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_r
  * are taken in 64 bits.  Uniform numbers are in [0, 1).  Probabilities should
  * be finite; negative and NaN ones weigh nothing, and -1 is drawn where none
  * is positive.  target and draft are of `dtype`; strides count elements, rows
- * are dense.  accepted and tokens share no memory with the inputs.
+ * are dense.  accepted and tokens share no memory with the inputs or each
+ * other.
  * workspace: ni_verify_workspace(n_seq, vocab) bytes of device memory,
  * 16-byte aligned, that no other work on the GPU uses meanwhile.  Enqueued on
  * `stream`; failures are reported by ni_kv_last_error(NULL). */

@@ -42,7 +42,7 @@ def verify_drafts(target, drafted, accept_u, sample_u, draft=None, n_drafts=None
     last), the first entry at which the sum passes ``sample_u`` times the whole.
 
     Returns ``(accepted [B], tokens [B, K+1])`` int32 (allocated if not
-    given; they share no memory with the inputs): the accepted drafts, the
+    given; they share no memory with the inputs or each other): the accepted drafts, the
     drawn token, then -1."""
     torch = _torch()
     if not isinstance(target, torch.Tensor) or target.dim() != 3 or dtype_code(target.dtype) is None:
