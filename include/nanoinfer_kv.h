@@ -65,7 +65,8 @@ enum ni_status {
     NI_ERR_EMPTY_WORK = 8,      /* "empty work item" (batch.rs:284-286) */
     NI_ERR_TOO_MANY_ROWS = 9,   /* "{n} rows > max_rows {max}" (batch.rs:300-302) */
     NI_ERR_NOT_RESERVED = 10,   /* a row's position has no page yet (reserve first) */
-    NI_ERR_NO_DEVICE = 11       /* data-path call on a NI_KV_HOST_ONLY handle */
+    NI_ERR_NO_DEVICE = 11,      /* data-path call on a NI_KV_HOST_ONLY handle */
+    NI_ERR_SHARED = 12          /* a write into a page that another sequence holds too (ni_kv_own first) */
 };
 
 /* ni_kv_opts.flags: keep only the host bookkeeping (no device memory); the
@@ -270,6 +271,42 @@ int ni_kv_decode_steps(ni_kv* kv, const uint32_t* seqs, uint32_t n, uint32_t ste
                        const float* v, int64_t row_stride, int64_t layer_stride, int64_t step_stride, float* out,
                        int64_t out_row_stride, int64_t out_layer_stride, int64_t out_step_stride,
                        uint32_t split_tokens, ni_stream stream);
+
+/* ---- pages that sequences share (no counterpart in the reference, whose
+ * sequences own their pages) ----
+ * A page may be held by several sequences; free_seq and truncate return it when
+ * the last lets it go.  Reading is as ever.  A call that would write into a page
+ * held twice (ni_kv_append and its forms; steps, where truncate left the end
+ * inside one) returns NI_ERR_SHARED and writes nothing.  The four calls below
+ * change tables at once and enqueue one launch of copies on `stream`, ordered
+ * as data-path calls are.  They are refused while a step is open and on a
+ * stream that is capturing (a replay would copy again, between pages that have
+ * changed hands); graphs captured before hold the pages of that time.  On error
+ * no table has changed, except after NI_ERR_HIP.  On a NI_KV_HOST_ONLY handle they
+ * keep the books alone. */
+
+/* n new sequences, the i-th (seqs[i], the lowest slots that are not live, in
+ * order) holding the committed positions of parents[i] (live; any of them
+ * several times): the whole pages are shared, the page with the end, if the
+ * length is no multiple of 16, is copied into one of the new sequence's own
+ * (the rows before the end: what lies behind it is undefined). */
+int ni_kv_fork(ni_kv* kv, const uint32_t* parents, uint32_t n, uint32_t* seqs, ni_stream stream);
+/* Sequence seqs[i] (each once) becomes a continuation of what parents[i] (live,
+ * listed or not) held before the call, as beams of a search do: its whole pages
+ * are shared, the page with the end goes to the first that continues a sequence
+ * which is itself replaced, and is copied for all others.  parents[i] ==
+ * seqs[i]: it stays as it is. */
+int ni_kv_reorder(ni_kv* kv, const uint32_t* seqs, const uint32_t* parents, uint32_t n, ni_stream stream);
+/* Pages of its own for positions begin .. end-1 of `seq` (reserved): copies of
+ * those it shares. */
+int ni_kv_own(ni_kv* kv, uint32_t seq, uint32_t begin, uint32_t end, ni_stream stream);
+/* The pages in use become the first ni_kv_blocks_used() of the order in which
+ * pages are handed out (ni_kv_opts.page_order, else 0, 1, 2, ...): those
+ * beyond move to the free ones, both in that order, and the free pages are
+ * handed out in that order again.  *moved (may be NULL): pages moved. */
+int ni_kv_compact(ni_kv* kv, uint32_t* moved, ni_stream stream);
+/* Sequences that hold a page. */
+int ni_kv_page_refs(const ni_kv* kv, uint32_t page, uint32_t* refs);
 
 /* ---- rotary positions, shared prefixes, drafts (no counterpart in the
  * reference, whose model has learned positions, equal head counts and greedy

@@ -31,6 +31,7 @@ NI_ERR_EMPTY_WORK = 8
 NI_ERR_TOO_MANY_ROWS = 9
 NI_ERR_NOT_RESERVED = 10
 NI_ERR_NO_DEVICE = 11
+NI_ERR_SHARED = 12
 
 NI_K_APPEND, NI_K_ATTN, NI_K_MERGE, NI_K_QKV, NI_K_COUNT = 0, 1, 2, 3, 4
 
@@ -149,6 +150,16 @@ def _declare(L):
     L.ni_kv_decode_steps.restype = C.c_int
     L.ni_kv_decode_steps.argtypes = [_vp, C.POINTER(_u32), _u32, _u32, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64,
                                      _i64, _u32, _vp]
+    L.ni_kv_fork.restype = C.c_int
+    L.ni_kv_fork.argtypes = [_vp, C.POINTER(_u32), _u32, C.POINTER(_u32), _vp]
+    L.ni_kv_reorder.restype = C.c_int
+    L.ni_kv_reorder.argtypes = [_vp, C.POINTER(_u32), C.POINTER(_u32), _u32, _vp]
+    L.ni_kv_own.restype = C.c_int
+    L.ni_kv_own.argtypes = [_vp, _u32, _u32, _u32, _vp]
+    L.ni_kv_compact.restype = C.c_int
+    L.ni_kv_compact.argtypes = [_vp, C.POINTER(_u32), _vp]
+    L.ni_kv_page_refs.restype = C.c_int
+    L.ni_kv_page_refs.argtypes = [_vp, _u32, C.POINTER(_u32)]
     L.ni_rotary_init.restype = C.c_int
     L.ni_rotary_init.argtypes = [C.POINTER(ni_rotary), _u32, C.POINTER(ni_rotary_opts)]
     L.ni_rotary_apply.restype = C.c_int

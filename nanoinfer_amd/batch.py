@@ -193,6 +193,14 @@ def _pointer(arr, empty, item):
     return empty.from_buffer(arr) if arr.size and arr.flags.writeable else arr.ctypes.data_as(C.POINTER(item))
 
 
+def _u32_array(x, name) -> np.ndarray:
+    """Host integers of any shape as a flat uint32 array."""
+    a = np.asarray(x)
+    if a.size and (a.dtype.kind not in "iu" or a.min() < 0 or a.max() > 0xffffffff):
+        raise ValueError(f"{name} must be integers in 0..2^32-1")
+    return np.array(a.reshape(-1), dtype=np.uint32)
+
+
 def _rows(rows) -> tuple:
     if type(rows) is np.ndarray and rows.dtype is _uint32:
         shape, flags = rows.shape, rows.flags
@@ -402,6 +410,61 @@ class PagedKv:
 
     def kv_block_bytes(self) -> int:
         return int(self._L.ni_kv_page_bytes(self._h))
+
+    # ---------------------------------------------------------- shared pages
+    def _stream(self, stream) -> int:
+        """The stream that copies of pages are enqueued on: of the cache's device."""
+        if self.device is None:
+            return 0
+        s = _stream_now(self.device, stream)
+        if s is None:
+            with _on(self.device, stream) as s:
+                pass
+        return s
+
+    def fork(self, parents, stream=None) -> list:
+        """New sequences, each holding the committed positions of one of
+        ``parents`` (sequences, any of them several times): whole pages are
+        shared, the page with the end is copied.  Raises :class:`KvError`
+        (nothing has changed then) where slots or pages run out."""
+        p = _u32_array(parents, "parents")
+        out = np.empty_like(p)
+        s = self._stream(stream)
+        self._check(self._L.ni_kv_fork(self._h, _pointer(p, _no_u32, C.c_uint32), p.size,
+                                       _pointer(out, _no_u32, C.c_uint32), s))
+        return out.tolist()
+
+    def reorder(self, seqs, parents, stream=None):
+        """Sequence ``seqs[i]`` becomes a continuation of what ``parents[i]``
+        held, as beams of a search do (``parents[i] == seqs[i]``: it stays as it
+        is).  Both list sequences, each of ``seqs`` once."""
+        q, p = _u32_array(seqs, "seqs"), _u32_array(parents, "parents")
+        if q.size != p.size:
+            raise ValueError(f"{q.size} seqs, {p.size} parents")
+        s = self._stream(stream)
+        self._check(self._L.ni_kv_reorder(self._h, _pointer(q, _no_u32, C.c_uint32), _pointer(p, _no_u32, C.c_uint32),
+                                          q.size, s))
+
+    def own(self, seq: int, begin: int = 0, end: Optional[int] = None, stream=None):
+        """Pages of its own for positions ``begin .. end-1`` (default: the
+        committed ones) of ``seq``: copies of those that it shares."""
+        s = self._stream(stream)
+        self._check(self._L.ni_kv_own(self._h, seq, begin, self.seq_len(seq) if end is None else end, s))
+
+    def compact(self, stream=None) -> int:
+        """Move the pages in use to the front of the order in which pages are
+        handed out; the number that moved."""
+        moved = C.c_uint32()
+        s = self._stream(stream)
+        self._check(self._L.ni_kv_compact(self._h, C.byref(moved), s))
+        return int(moved.value)
+
+    def page_refs(self, page: int) -> int:
+        """Sequences that hold ``page``."""
+        n = C.c_uint32()
+        if self._L.ni_kv_page_refs(self._h, page, C.byref(n)) != 0:
+            raise ValueError(f"page {page} of {self.opts.kv_blocks}")
+        return int(n.value)
 
     # -------------------------------------------------------------- data path
     def append(self, rows, k, v, layer: int = ALL_LAYERS, stream=None):

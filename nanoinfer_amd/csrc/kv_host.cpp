@@ -180,7 +180,9 @@ struct ni_kv {
     std::vector<uint32_t> seq_len;
     std::vector<uint8_t> live;
     std::vector<std::vector<uint32_t>> pages;
-    std::vector<uint32_t> free_pages;  // LIFO stack, back() is handed out next
+    std::vector<uint32_t> free_pages;  // LIFO stack, back() is handed out next (room for every page: a push never throws)
+    std::vector<uint32_t> refs;        // page -> sequences that hold it
+    std::vector<uint32_t> page_order;  // the order in which pages were first handed out
     std::string err;
     bool host_only = false;
     int device = 0;
@@ -300,9 +302,15 @@ int ensure_pages(ni_kv* kv, uint32_t s, uint64_t len) {
     while ((uint64_t)pg.size() * kPage < len) {
         if (kv->free_pages.empty()) return kv->fail(NI_ERR_POOL_EXHAUSTED, "KV cache pool exhausted");
         pg.push_back(kv->free_pages.back());
+        kv->refs[pg.back()] = 1;
         kv->free_pages.pop_back();
     }
     return NI_OK;
+}
+
+// One sequence less holds `page`; the last one frees it.
+void drop_page(ni_kv* kv, uint32_t page) {
+    if (--kv->refs[page] == 0) kv->free_pages.push_back(page);
 }
 
 // Batch::truncate (batch.rs:220-227).
@@ -312,7 +320,7 @@ int truncate_seq(ni_kv* kv, uint32_t s, uint32_t len) {
     const size_t keep = (len + kPage - 1) / kPage;
     auto& pg = kv->pages[s];
     while (pg.size() > keep) {
-        kv->free_pages.push_back(pg.back());
+        drop_page(kv, pg.back());
         pg.pop_back();
     }
     return NI_OK;
@@ -326,6 +334,27 @@ int check_row(ni_kv* kv, const ni_row& r) {
     if ((uint64_t)r.pos >= (uint64_t)kv->pages[r.seq].size() * kPage)
         return kv->fail(NI_ERR_NOT_RESERVED, "sequence %u: position %u has no page (reserved %zu)", r.seq, r.pos,
                         kv->pages[r.seq].size() * kPage);
+    return NI_OK;
+}
+
+int shared_page(ni_kv* kv, uint32_t seq, uint32_t pos) {
+    return kv->fail(NI_ERR_SHARED, "sequence %u: position %u lies in a page that another sequence holds too (ni_kv_own)",
+                    seq, pos);
+}
+
+// check_row of a row that is written.
+int check_write(ni_kv* kv, const ni_row& r) {
+    if (int rc = check_row(kv, r)) return rc;
+    return kv->refs[kv->pages[r.seq][r.pos / kPage]] > 1 ? shared_page(kv, r.seq, r.pos) : NI_OK;
+}
+
+// May sequence `s` grow by n positions in place: no page that they go to, as far
+// as it is reserved, has another holder.
+int check_grow(ni_kv* kv, uint32_t s, uint64_t n) {
+    const auto& pg = kv->pages[s];
+    const uint64_t len = kv->seq_len[s];
+    for (uint64_t i = len / kPage; i < pg.size() && i * kPage < len + n; i++)
+        if (kv->refs[pg[i]] > 1) return shared_page(kv, s, (uint32_t)std::max(len, i * kPage));
     return NI_OK;
 }
 
@@ -1365,7 +1394,11 @@ int run_plan(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const float* k, const f
 // The handle's device current for the scope of a call.
 struct DeviceScope {
     int before = -1, now;
-    explicit DeviceScope(int device) : now(device) {
+    explicit DeviceScope(int device, bool none = false) : now(device) {
+        if (none) {  // a handle without a device
+            before = now;
+            return;
+        }
         if (hipGetDevice(&before) != hipSuccess) before = -1;
         if (before != now) (void)hipSetDevice(now);
     }
@@ -1672,6 +1705,8 @@ int ni_kv_create(const ni_kv_opts* opts, ni_kv** out) {
     } else {
         for (uint32_t i = 0; i < o.kv_pages; i++) kv->free_pages[i] = o.kv_pages - 1 - i;
     }
+    kv->refs.assign(o.kv_pages, 0);
+    kv->page_order.assign(kv->free_pages.rbegin(), kv->free_pages.rend());
     if (!host_only) {
         hipError_t e = hipGetDevice(&kv->device);
         if (e == hipSuccess) {
@@ -1833,6 +1868,238 @@ int ni_kv_pools(const ni_kv* kv, void** k_pool, void** v_pool, size_t* bytes) {
     return NI_OK;
 }
 
+// What ni_kv_fork and its kin check before they look at tables, the call ordered
+// behind the handle's earlier work.
+static int begin_tables(ni_kv* kv, hipStream_t s) {
+    if (kv->step.open) return kv->fail(NI_ERR_BAD_ARG, "a step begun by ni_kv_step_begin is still open");
+    if (kv->host_only) return NI_OK;
+    if (int rc = begin_call(kv, s)) return rc;
+    if (kv->capturing)
+        return kv->fail(NI_ERR_BAD_ARG, "the stream is capturing: tables change once, a replay would copy again");
+    return NI_OK;
+}
+
+static int check_live(ni_kv* kv, uint32_t s) {
+    if (int rc = check_seq(kv, s)) return rc;
+    return kv->live[s] ? NI_OK : kv->fail(NI_ERR_NOT_LIVE, "sequence %u is not live", s);
+}
+
+// Enqueue the copies of pages (their tables have changed already).
+static int copy_pages(ni_kv* kv, const std::vector<PageCopy>& copies, std::vector<uint8_t>& blob, hipStream_t s) {
+    if (copies.empty() || kv->host_only) return NI_OK;
+    memcpy(blob.data(), copies.data(), copies.size() * sizeof(PageCopy));
+    PlanRef ref;
+    if (int rc = place_blob(kv, blob, s, &ref)) return rc;
+    PageCopyLaunch a{};
+    a.pool = kv->geom();
+    a.plan = ref.dev;
+    a.n = (uint32_t)copies.size();
+    a.n_layer = kv->o.n_layer;
+    const hipError_t e = launch_page_copy(a, ref.inl, ref.inl_bytes, s);
+    const int rc = release_plan(kv, ref, s);
+    return e != hipSuccess ? kv->hip_fail(e, "page copy kernel") : rc;
+}
+
+static size_t copies_bytes(size_t n) { return align_up(n * sizeof(PageCopy), kAlign); }
+
+int ni_kv_page_refs(const ni_kv* kv, uint32_t page, uint32_t* refs) {
+    if (!kv || !refs || page >= kv->o.kv_pages) return NI_ERR_BAD_ARG;
+    *refs = kv->refs[page];
+    return NI_OK;
+}
+
+int ni_kv_fork(ni_kv* kv, const uint32_t* parents, uint32_t n, uint32_t* seqs, ni_stream stream) try {
+    if (!kv) return NI_ERR_BAD_ARG;
+    if (n == 0) return NI_OK;
+    if (!parents || !seqs) return kv->fail(NI_ERR_BAD_ARG, "%s is NULL", parents ? "seqs" : "parents");
+    if (n > kv->o.max_seqs) return kv->fail(NI_ERR_NO_SLOT, "no sequence slot");
+    DeviceScope device(kv->device, kv->host_only);
+    if (int rc = begin_tables(kv, (hipStream_t)stream)) return rc;
+    std::vector<std::vector<uint32_t>> tables(n);
+    std::vector<PageCopy> copies;
+    std::vector<uint32_t> slots;
+    for (uint32_t i = 0; i < n; i++) {
+        if (int rc = check_live(kv, parents[i])) return rc;
+        const uint32_t len = kv->seq_len[parents[i]];
+        const auto& pg = kv->pages[parents[i]];
+        tables[i].reserve(len / kPage + 1);
+        tables[i].assign(pg.begin(), pg.begin() + len / kPage);
+        if (len % kPage) copies.push_back({pg[len / kPage], i, len % kPage});  // (dst: the fork, for now)
+    }
+    for (uint32_t s = 0; s < kv->o.max_seqs && slots.size() < n; s++)
+        if (!kv->live[s]) slots.push_back(s);
+    if (slots.size() < n) return kv->fail(NI_ERR_NO_SLOT, "no sequence slot");
+    if (copies.size() > kv->free_pages.size()) return kv->fail(NI_ERR_POOL_EXHAUSTED, "KV cache pool exhausted");
+    std::vector<uint8_t> blob(copies_bytes(copies.size()));
+    // Nothing below throws.
+    for (PageCopy& c : copies) {
+        auto& table = tables[c.dst];
+        c.dst = kv->free_pages.back();
+        kv->free_pages.pop_back();
+        table.push_back(c.dst);
+    }
+    for (uint32_t i = 0; i < n; i++) {
+        kv->live[slots[i]] = 1;
+        kv->seq_len[slots[i]] = kv->seq_len[parents[i]];
+        seqs[i] = slots[i];  // (seqs may be parents)
+        for (uint32_t p : tables[i]) kv->refs[p]++;
+        kv->pages[slots[i]].swap(tables[i]);
+    }
+    return copy_pages(kv, copies, blob, (hipStream_t)stream);
+} catch (const std::bad_alloc&) {
+    return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
+}
+
+int ni_kv_reorder(ni_kv* kv, const uint32_t* seqs, const uint32_t* parents, uint32_t n, ni_stream stream) try {
+    if (!kv) return NI_ERR_BAD_ARG;
+    if (n == 0) return NI_OK;
+    if (!parents || !seqs) return kv->fail(NI_ERR_BAD_ARG, "%s is NULL", parents ? "seqs" : "parents");
+    DeviceScope device(kv->device, kv->host_only);
+    if (int rc = begin_tables(kv, (hipStream_t)stream)) return rc;
+    // Sequences that others replace: whose end page one of its continuations may take over.
+    enum : uint8_t { kStays = 0, kReplaced = 1, kTaken = 2 };
+    std::vector<uint8_t> state(kv->o.max_seqs, kStays);
+    std::vector<uint8_t> listed(kv->o.max_seqs, 0);
+    for (uint32_t i = 0; i < n; i++) {
+        if (int rc = check_live(kv, seqs[i])) return rc;
+        if (int rc = check_live(kv, parents[i])) return rc;
+        if (listed[seqs[i]]) return kv->fail(NI_ERR_BAD_ARG, "sequence %u appears twice in one call", seqs[i]);
+        listed[seqs[i]] = 1;
+        if (parents[i] != seqs[i]) state[seqs[i]] = kReplaced;
+    }
+    constexpr uint32_t kNone = 0xffffffffu;
+    struct Change {
+        uint32_t seq, len;
+        uint32_t copy;  // index into copies of its last page, or kNone
+        std::vector<uint32_t> table;
+    };
+    std::vector<Change> changes;
+    std::vector<PageCopy> copies;
+    for (uint32_t i = 0; i < n; i++) {
+        if (parents[i] == seqs[i]) continue;
+        const uint32_t len = kv->seq_len[parents[i]];
+        const auto& pg = kv->pages[parents[i]];
+        Change c{seqs[i], len, kNone, {}};
+        c.table.reserve(len / kPage + 1);
+        c.table.assign(pg.begin(), pg.begin() + len / kPage);
+        if (len % kPage) {
+            if (state[parents[i]] == kReplaced) {
+                state[parents[i]] = kTaken;
+                c.table.push_back(pg[len / kPage]);
+            } else {
+                c.copy = (uint32_t)copies.size();
+                copies.push_back({pg[len / kPage], kNone, len % kPage});
+            }
+        }
+        changes.push_back(std::move(c));
+    }
+    if (changes.empty()) return NI_OK;
+    std::vector<uint8_t> blob(copies_bytes(copies.size()));
+    // Nothing below throws.  The new holds before the old ones go, so that what
+    // reaches 0 is free: no page that is copied from does.
+    size_t released = 0;
+    for (const Change& c : changes)
+        for (uint32_t p : c.table) kv->refs[p]++;
+    for (const Change& c : changes)
+        for (uint32_t p : kv->pages[c.seq]) released += --kv->refs[p] == 0;
+    if (copies.size() > kv->free_pages.size() + released) {
+        for (const Change& c : changes)
+            for (uint32_t p : kv->pages[c.seq]) kv->refs[p]++;
+        for (const Change& c : changes)
+            for (uint32_t p : c.table) kv->refs[p]--;
+        return kv->fail(NI_ERR_POOL_EXHAUSTED, "KV cache pool exhausted");
+    }
+    // A copy goes to the last page that its sequence held before, if nothing holds
+    // that any more: a search whose beams keep their order keeps its pages.
+    for (const Change& c : changes) {
+        const auto& old = kv->pages[c.seq];
+        if (c.copy == kNone || old.empty() || kv->refs[old.back()] != 0) continue;
+        copies[c.copy].dst = old.back();
+        kv->refs[old.back()] = 1;
+    }
+    for (const Change& c : changes) {
+        const auto& old = kv->pages[c.seq];
+        for (size_t i = old.size(); i-- > 0;)
+            if (kv->refs[old[i]] == 0) {
+                kv->refs[old[i]] = kNone;  // (once, however many of the changed held it)
+                kv->free_pages.push_back(old[i]);
+            }
+    }
+    for (const Change& c : changes)
+        for (uint32_t p : kv->pages[c.seq])
+            if (kv->refs[p] == kNone) kv->refs[p] = 0;
+    for (Change& c : changes) {
+        if (c.copy != kNone) {
+            uint32_t& dst = copies[c.copy].dst;
+            if (dst == kNone) {
+                dst = kv->free_pages.back();
+                kv->free_pages.pop_back();
+                kv->refs[dst] = 1;
+            }
+            c.table.push_back(dst);  // (room was made)
+        }
+        kv->pages[c.seq].swap(c.table);
+    }
+    for (const Change& c : changes) kv->seq_len[c.seq] = c.len;
+    return copy_pages(kv, copies, blob, (hipStream_t)stream);
+} catch (const std::bad_alloc&) {
+    return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
+}
+
+int ni_kv_own(ni_kv* kv, uint32_t seq, uint32_t begin, uint32_t end, ni_stream stream) try {
+    if (!kv) return NI_ERR_BAD_ARG;
+    DeviceScope device(kv->device, kv->host_only);
+    if (int rc = begin_tables(kv, (hipStream_t)stream)) return rc;
+    if (int rc = check_live(kv, seq)) return rc;
+    auto& pg = kv->pages[seq];
+    if (begin > end || end > (uint64_t)pg.size() * kPage)
+        return kv->fail(NI_ERR_BAD_ARG, "sequence %u: positions %u..%u are not all reserved (%zu are)", seq, begin, end,
+                        pg.size() * kPage);
+    std::vector<PageCopy> copies;
+    for (uint64_t i = begin / kPage; i * kPage < end && begin < end; i++)
+        if (kv->refs[pg[i]] > 1) copies.push_back({pg[i], (uint32_t)i, kPage});
+    if (copies.size() > kv->free_pages.size()) return kv->fail(NI_ERR_POOL_EXHAUSTED, "KV cache pool exhausted");
+    std::vector<uint8_t> blob(copies_bytes(copies.size()));
+    for (PageCopy& c : copies) {
+        const uint32_t i = c.dst;
+        c.dst = kv->free_pages.back();
+        kv->free_pages.pop_back();
+        kv->refs[c.src]--;
+        kv->refs[c.dst] = 1;
+        pg[i] = c.dst;
+    }
+    return copy_pages(kv, copies, blob, (hipStream_t)stream);
+} catch (const std::bad_alloc&) {
+    return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
+}
+
+int ni_kv_compact(ni_kv* kv, uint32_t* moved, ni_stream stream) try {
+    if (!kv) return NI_ERR_BAD_ARG;
+    if (moved) *moved = 0;
+    DeviceScope device(kv->device, kv->host_only);
+    if (int rc = begin_tables(kv, (hipStream_t)stream)) return rc;
+    const uint32_t n = kv->o.kv_pages, used = n - (uint32_t)kv->free_pages.size();
+    std::vector<PageCopy> copies;
+    std::vector<uint32_t> now(n);  // page -> where it lies afterwards
+    for (uint32_t p = 0; p < n; p++) now[p] = p;
+    const auto& order = kv->page_order;
+    for (uint32_t from = used, to = 0; from < n; from++) {
+        if (kv->refs[order[from]] == 0) continue;
+        while (kv->refs[order[to]] != 0) to++;  // (as many are free before `used` as are in use behind it)
+        copies.push_back({order[from], order[to], kPage});
+        now[order[from]] = order[to++];
+    }
+    std::vector<uint8_t> blob(copies_bytes(copies.size()));
+    for (const PageCopy& c : copies) std::swap(kv->refs[c.src], kv->refs[c.dst]);
+    for (auto& pg : kv->pages)
+        for (uint32_t& p : pg) p = now[p];
+    for (uint32_t i = used; i < n; i++) kv->free_pages[n - 1 - i] = order[i];
+    if (moved) *moved = (uint32_t)copies.size();
+    return copy_pages(kv, copies, blob, (hipStream_t)stream);
+} catch (const std::bad_alloc&) {
+    return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
+}
+
 int ni_kv_append(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, const float* k, const float* v,
                  int64_t row_stride, int64_t layer_stride, ni_stream stream) {
     if (!kv) return NI_ERR_BAD_ARG;
@@ -1847,7 +2114,7 @@ int ni_kv_append(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, const
     if (int rc = check_f32_operand(kv, "v", v, row_stride, layer_stride, all)) return rc;
     reset_plan(kv);
     for (uint32_t i = 0; i < n; i++) {
-        if (int rc = check_row(kv, rows[i])) return rc;
+        if (int rc = check_write(kv, rows[i])) return rc;
         const ni_row& r = rows[i];
         kv->plan.app.push_back({i, kv->pages[r.seq][r.pos / kPage], r.pos % kPage, 0});
     }
@@ -1885,7 +2152,7 @@ static int qkv_run(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, con
     reset_plan(kv);
     if (fused)
         for (uint32_t i = 0; i < n; i++) {
-            if (int rc = check_row(kv, rows[i])) return rc;
+            if (int rc = check_write(kv, rows[i])) return rc;
             const ni_row& r = rows[i];
             kv->plan.app.push_back({i, kv->pages[r.seq][r.pos / kPage], r.pos % kPage, 0});
         }
@@ -2137,7 +2404,7 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
     blob.resize(align_up((size_t)n * sizeof(RotaryEntry), kAlign));
     RotaryEntry* entries = reinterpret_cast<RotaryEntry*>(blob.data());
     for (uint32_t i = 0; i < n; i++) {
-        if (int rc = check_row(kv, rows[i])) return rc;
+        if (int rc = check_write(kv, rows[i])) return rc;
         const ni_row& r = rows[i];
         const uint32_t place = kv->pages[r.seq][r.pos / kPage] * kPage + r.pos % kPage;
         if (taken(place)) return kv->fail(NI_ERR_BAD_ARG, "sequence %u: position %u appears twice", r.seq, r.pos);
@@ -2448,6 +2715,7 @@ int ni_kv_decode_steps(ni_kv* kv, const uint32_t* seqs, uint32_t n, uint32_t ste
         if (kv->step_mark[s] == kv->step_stamp)
             return kv->fail(NI_ERR_BAD_ARG, "sequence %u appears twice in one call", s);
         kv->step_mark[s] = kv->step_stamp;
+        if (int rc = check_grow(kv, s, steps)) return rc;
         if (int rc = ensure_pages(kv, s, (uint64_t)kv->seq_len[s] + steps)) return rc;
     }
     // batch.rs:351-357: every step enqueued at once; step t appends and
@@ -2485,6 +2753,7 @@ static int prepare_step(ni_kv* kv, const ni_work* work, uint32_t n_work) {
             return kv->fail(NI_ERR_BAD_ARG, "sequence %u appears twice in one step", it.seq);
         kv->step_mark[it.seq] = kv->step_stamp;
         const uint32_t len = kv->seq_len[it.seq];
+        if (int rc = check_grow(kv, it.seq, it.n_new)) return rc;
         if (int rc = ensure_pages(kv, it.seq, (uint64_t)len + it.n_new)) return rc;
         n_rows += it.n_new;
     }

@@ -124,6 +124,18 @@ struct PoolGeom {
     uint32_t q8;
 };
 
+// A page to copy, over all layers: its first `rows` positions (kPage: the whole page).
+struct PageCopy {
+    uint32_t src, dst, rows;
+};
+
+struct PageCopyLaunch {
+    PoolGeom pool;
+    const uint8_t* plan;  // PageCopy[n] (unused when inline)
+    uint32_t n;
+    uint32_t n_layer;
+};
+
 struct AppendLaunch {
     PoolGeom pool;
     const float* k;
@@ -268,6 +280,8 @@ struct LaunchTiming {
 
 hipError_t launch_append(const AppendLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s,
                          const LaunchTiming& t = {});
+// (no source is a destination of the same launch)
+hipError_t launch_page_copy(const PageCopyLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s);
 hipError_t launch_gather(const GatherLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s);
 hipError_t launch_gather_q8(const GatherQ8Launch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s);
 hipError_t launch_attention(const AttnLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s,

@@ -1,0 +1,86 @@
+// page_kernels.hip -- gfx950 kernel of page copies (ni_kv_fork, ni_kv_reorder,
+// ni_kv_own, ni_kv_compact).
+//
+// A page is one contiguous run of bytes in each layer, so a whole page is copied
+// as it lies, in 16-byte units.  Of a page that a sequence ends in, only the rows
+// before the end are: of each (head, K|V) block the units of those rows, which lie
+// together, and their scales.
+#include "kv_device.h"
+
+namespace ni {
+namespace {
+
+constexpr int kCT = 256;        // threads
+constexpr int kUnits = 4;       // 16-byte units of a thread, loaded before the first is stored
+constexpr uint32_t kTileUnits = kCT * kUnits;
+
+// A page's layout in 16-byte units.
+struct PageShape {
+    uint32_t page;        // of one layer
+    uint32_t block;       // of one (head, K|V) block
+    uint32_t values;      // of its values, 16 rows
+    uint32_t blocks;      // 2 * heads
+};
+
+// Workgroup (copy from `first` on, layer, tile of kTileUnits units).
+template <int INL>
+__global__ __launch_bounds__(kCT) void page_copy_kernel(const PageCopyLaunch a, const PageShape g, const uint32_t tiles,
+                                                        const uint32_t first, const PlanArg<INL> pa) {
+    const uint32_t unit = blockIdx.x / tiles, tile = blockIdx.x - unit * tiles;
+    const uint32_t i = unit / a.n_layer, layer = unit - i * a.n_layer;
+    const PageCopy c = reinterpret_cast<const PageCopy*>(plan_base(pa, a.plan))[first + i];
+    uint8_t* const base = reinterpret_cast<uint8_t*>(a.pool.k + (uint64_t)layer * a.pool.layer_halves);
+    const u32x4* const src = reinterpret_cast<const u32x4*>(base + (uint64_t)c.src * g.page * 16);
+    u32x4* const dst = reinterpret_cast<u32x4*>(base + (uint64_t)c.dst * g.page * 16);
+    const uint32_t scales = c.rows < kPage && a.pool.q8 ? (c.rows + 3) / 4 : 0;  // units with scales of a block's rows
+    const uint32_t values = c.rows < kPage ? g.values / kPage * c.rows : g.values;
+    const uint32_t per = values + scales;
+    const uint32_t n = c.rows < kPage ? per * g.blocks : g.page;
+    u32x4 x[kUnits];
+    uint32_t at[kUnits], words[kUnits];  // unit of the page; words of it to copy
+#pragma unroll
+    for (int j = 0; j < kUnits; j++) {
+        const uint32_t u = tile * kTileUnits + j * kCT + threadIdx.x;
+        at[j] = u;
+        words[j] = u < n ? 4 : 0;
+        if (c.rows < kPage && u < n) {
+            const uint32_t b = u / per, w = u - b * per;
+            at[j] = b * g.block + (w < values ? w : g.values + w - values);
+            if (w >= values) words[j] = min(4u, c.rows - 4 * (w - values));
+        }
+        if (words[j]) x[j] = __builtin_nontemporal_load(src + at[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < kUnits; j++) {
+        if (words[j] == 4) {
+            __builtin_nontemporal_store(x[j], dst + at[j]);
+        } else if (words[j]) {
+            uint32_t* p = reinterpret_cast<uint32_t*>(dst + at[j]);
+            for (uint32_t w = 0; w < words[j]; w++) p[w] = x[j][w];
+        }
+    }
+}
+
+}  // namespace
+
+hipError_t launch_page_copy(const PageCopyLaunch& a, const void* ip, uint32_t ib, hipStream_t s) {
+    PageShape g;
+    g.page = (uint32_t)(a.pool.page_halves / 8);
+    g.block = a.pool.head_halves / 16;
+    g.values = kPage * a.pool.head_dim / (a.pool.q8 ? 16 : 8);
+    g.blocks = 2 * a.pool.n_head;
+    const uint32_t tiles = (g.page + kTileUnits - 1) / kTileUnits;
+    // (a launch holds less than 2^32 threads)
+    const uint32_t most = (uint32_t)((1ull << 23) / ((uint64_t)a.n_layer * tiles));
+    if (most == 0) return hipErrorInvalidValue;
+    return with_plan(a, ip, ib, [&](auto pa) {
+        constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
+        hipError_t e = hipSuccess;
+        for (uint32_t first = 0; first < a.n && e == hipSuccess; first += most)
+            e = go(page_copy_kernel<INL>, (uint64_t)(a.n - first < most ? a.n - first : most) * a.n_layer * tiles, kCT, s,
+                   LaunchTiming{}, a, g, tiles, first, pa);
+        return e;
+    });
+}
+
+}  // namespace ni
