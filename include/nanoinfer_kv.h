@@ -79,6 +79,21 @@ enum ni_status {
  * (attn_decode_split_q8, :50-95); ni_kv_gather and ni_kv_qkv_append are
  * refused (ni_kv_gather_q8 returns the stored bytes). */
 #define NI_KV_Q8 2u
+/* ni_kv_opts.flags: the block-scaled cache (no counterpart in the reference;
+ * device handles, not with NI_KV_Q8): 8-bit floats (e4m3: 3 bits of mantissa, up to 448) and
+ * one scale for the 16 positions of a page, each head, K and V by themselves:
+ * 64.5 bytes per 64 values.  A scale is the smallest power of two in
+ * 2^-117..2^120 that brings the block's values to at most 448, so that scaling
+ * is exact and a value is rounded once, to nearest even (half a step: 2^-4 of
+ * itself, or 2^-10 of the scale where that is more).  It grows when an appended row needs it,
+ * the block's other values being rounded again (which loses nothing above 2^-6 of the new scale),
+ * begins anew when the block's first position is written, whatever is then
+ * in the positions that the call does not write, and never shrinks else.  Inputs
+ * must be finite: a NaN is stored as 0, an infinity as the block's largest value.
+ * The append, steps (not ni_kv_step_noalloc, not one layer at a time), decode
+ * steps, both attention calls and ni_kv_gather_values take such handles, the
+ * others refuse them. */
+#define NI_KV_B8 4u
 
 /* Sizes and policies (the KV fields of BatchOpts, batch.rs:44-76, plus the
  * model shape the reference takes from Config, crates/core/src/config.rs:23). */
@@ -193,6 +208,14 @@ int ni_kv_gather(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, uint1
  * k_out/v_out 16-byte aligned. */
 int ni_kv_gather_q8(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, int8_t* k_out, int8_t* v_out,
                     float* k_scale, float* v_scale, ni_stream stream);
+
+/* What the cache stands for at each row, in f32, in the reference's row
+ * layout: f16 widened, Q8 and block-scaled values times their scales (exact but
+ * for Q8, whose products are rounded once).
+ * k_out and v_out 16-byte aligned with strides that are multiples of 4
+ * floats; their rows do not overlap. */
+int ni_kv_gather_values(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, float* k_out, float* v_out,
+                        int64_t row_stride, int64_t layer_stride, ni_stream stream);
 
 /* Paged decode attention (b_attn_split + b_attn_merge, batch.metal:349-424;
  * math of kv16.rs:144-164): row i attends causally to keys 0..rows[i].pos
@@ -401,7 +424,8 @@ typedef struct ni_prefix {
  * be its prefix.
  * Range: rows that share tiles hold q / sqrt(head_dim) * log2(e) as two f16
  * parts, so |q| is at most 3.6e5 (head_dim 64; 5.1e5 at 128); a larger value
- * may make its row NaN.  On the Q8 cache keys and values that a row sees are
+ * may make its row NaN (on the block-scaled cache every row's are so held, in
+ * ni_paged_decode_attention and steps too).  On the Q8 cache keys and values that a row sees are
  * finite; what later rows, or no row, may see does not matter.
  * split_tokens: keys per partition, a multiple of 16; 0 = automatic.
  * Under stream capture the call allocates nothing: make the same call once
@@ -448,7 +472,11 @@ int ni_kv_sync(ni_kv* kv, ni_stream stream);
 /* The device pool, for inspection: one allocation of `bytes`, laid out
  * [n_layer][kv_pages][n_head][K block][V block]; *k_pool is its start and
  * *v_pool the first V block.  f16: a block is [16][head_dim] f16.  Q8: a
- * block is [16][head_dim] int8 then 16 f32 scales. */
+ * block is [16][head_dim] int8 then 16 f32 scales.  Block-scaled: a block is
+ * [head_dim/64] runs of 1024 bytes, in which value (position p, dim d % 64 = x)
+ * lies at x/16*256 + p*16 + x%16 of K and p/4*256 + x%16*16 + x/16*4 + p%4 of V
+ * (the order in which lanes take them to matrix products), and a page ends
+ * in [n_head][K, V] f32 scales, padded to 128 bytes. */
 int ni_kv_pools(const ni_kv* kv, void** k_pool, void** v_pool, size_t* bytes);
 
 /* Contiguous causal attention over f32 K/V rows, the CPU engine's op

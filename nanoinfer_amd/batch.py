@@ -65,6 +65,7 @@ class BatchOpts:
     host_only: bool = False
     page_order: Optional[Sequence[int]] = None  # order in which pages are handed out
     q8: bool = False  # int8 K/V + f32 scale per (position, head) (kv8.metal)
+    block8: bool = False  # 8-bit floats + a power-of-two scale per (page, head)
 
     @property
     def n_embd(self) -> int:
@@ -294,7 +295,8 @@ class PagedKv:
         o = _abi.ni_kv_opts()
         o.n_layer, o.n_head, o.head_dim = opts.n_layer, opts.n_head, opts.head_dim
         o.kv_pages, o.max_seqs, o.max_ctx, o.max_rows = opts.kv_blocks, opts.max_seqs, opts.n_ctx, opts.max_rows
-        o.flags = (_abi.NI_KV_HOST_ONLY if opts.host_only else 0) | (_abi.NI_KV_Q8 if opts.q8 else 0)
+        o.flags = (_abi.NI_KV_HOST_ONLY if opts.host_only else 0) | (_abi.NI_KV_Q8 if opts.q8 else 0) | (
+            _abi.NI_KV_B8 if opts.block8 else 0)
         self._order = None
         if opts.page_order is not None:
             self._order = np.ascontiguousarray(np.asarray(opts.page_order, dtype=np.uint32))
@@ -557,6 +559,19 @@ class PagedKv:
         self._check(self._L.ni_kv_gather_q8(self._h, layer, rp, n, ko.data_ptr(), vo.data_ptr(), ks.data_ptr(),
                                             vs.data_ptr(), _stream_ptr(stream)))
         return (ko, vo), (ks, vs)
+
+    def gather_values(self, rows, layer: int = ALL_LAYERS, stream=None):
+        """What the cache stands for at each (seq, pos) row: (k, v) float32
+        [n_layer, n, C], or [n, C] of one layer, on any cache."""
+        torch = _torch()
+        arr, rp, n = _rows(rows)
+        c, layered = self._c, layer == ALL_LAYERS
+        with _on(self.device, stream) as s:
+            k, v = (torch.empty((self._n_layer, n, c) if layered else (n, c), dtype=torch.float32, device="cuda")
+                    for _ in range(2))
+            self._check(self._L.ni_kv_gather_values(self._h, layer, rp, n, k.data_ptr(), v.data_ptr(), c,
+                                                    n * c if layered else 0, s))
+        return k, v
 
     def attention(self, q, rows, out=None, layer: int = ALL_LAYERS, split_tokens: int = 0, stream=None):
         """Paged decode attention of each row over keys 0..pos of its sequence."""

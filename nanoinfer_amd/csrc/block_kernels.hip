@@ -1,0 +1,451 @@
+// block_kernels.hip -- gfx950 kernels of the block-scaled cache (NI_KV_B8): e4m3
+// values, one power-of-two scale for each (page, head) of K and of V.
+//
+//   block_append_kernel   f32 rows into the pages, scales grown where they must
+//   block_attn_kernel     16 slots (query heads of rows that read the same cache
+//                         head) over a run of keys, on the matrix cores
+//   values_kernel         what the cache stands for, in f32 (any pool)
+//
+// A block's bytes lie in the order in which the lanes of block_attn_kernel take
+// them to matrix products, so that a page needs no LDS on its way: lane l loads the
+// 16 bytes at 16 l of each KB.  Of K they are dims 16 (l / 16) .. + 15 of
+// position l % 16; of V positions 4 (l / 16) .. + 3 of dims l % 16 + 16 (0..3).
+#include "kv_device.h"
+#include "ops_plan.h"
+
+namespace ni {
+namespace {
+
+constexpr float kTop = 448.f;  // the largest e4m3 value
+constexpr int kMinExp = -117, kMaxExp = 120;
+
+// Bytes of value (position p, dim d) within its block.
+__device__ __forceinline__ uint32_t k_byte(uint32_t p, uint32_t d) {
+    return d / 64 * 1024 + d % 64 / 16 * 256 + p * 16 + d % 16;
+}
+__device__ __forceinline__ uint32_t v_byte(uint32_t p, uint32_t d) {
+    return d / 64 * 1024 + p / 4 * 256 + d % 16 * 16 + d % 64 / 16 * 4 + p % 4;
+}
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+// The exponent of the scale that values up to `top` (finite, not negative) need:
+// top <= 448 * 2^e = 1.75 * 2^(e + 8).
+__device__ __forceinline__ int scale_exp(float top) {
+    const uint32_t b = __float_as_uint(top);
+    const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return min(max(e, kMinExp), kMaxExp);
+}
+// The exponent of a stored scale; below every other where nothing was stored yet.
+__device__ __forceinline__ int exp_of(float scale) { return (int)(__float_as_uint(scale) >> 23) - 127; }
+
+__device__ __forceinline__ float wave_max(float x) {
+    x = fmaxf(x, dpp_move<0xb1>(x));
+    x = fmaxf(x, dpp_move<0x4e>(x));
+    x = fmaxf(x, dpp_move<0x141>(x));
+    x = fmaxf(x, dpp_move<0x140>(x));
+    return rows4_max(x);
+}
+
+// Four values times `inv` as e4m3, to nearest even.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float inv) {
+    const auto in = [&](float x) { return fminf(fmaxf(x * inv, -kTop), kTop); };
+    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(in(a), in(b), 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(in(c), in(d), lo, true);
+}
+// Four stored values times `by` (a power of two, at most 1), rounded again.
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float by) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    return e4m3x4(lo[0], lo[1], hi[0], hi[1], by);
+}
+// An input as it is stored: a NaN as 0 (an infinity ends at the largest value).
+__device__ __forceinline__ float number(float x) { return x == x ? x : 0.f; }
+__device__ __forceinline__ float finite_size(float x) {
+    const float y = fabsf(x);
+    return y < INFINITY ? y : 0.f;
+}
+
+// One wave per (page of the call, layer, head) and K or V.  A lane holds the 16
+// bytes that it loads in block_attn_kernel: of K a position's 16 dims (those of
+// positions that are not new only where the scale grows), of V four positions
+// of four dims, merged with what is there where not all of them are new.
+template <int D, int INL>
+__global__ __launch_bounds__(256) void block_append_kernel(const BlockAppendLaunch a, const PlanArg<INL> pa) {
+    constexpr int NB = D / 64;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t H = a.pool.n_head;
+    const uint64_t unit = (uint64_t)blockIdx.x * 4 + wave;  // ((entry, layer), head, K | V)
+    const uint32_t is_v = (uint32_t)(unit & 1), head = (uint32_t)(unit / 2 % H);
+    const uint32_t el = (uint32_t)(unit / 2 / H);
+    if (el >= a.n * a.n_lay) return;
+    const uint32_t entry = el / a.n_lay, lay = el - entry * a.n_lay;
+    const uint8_t* plan = plan_base(pa, a.plan);
+    const BlockAppend e = reinterpret_cast<const BlockAppend*>(plan)[entry];
+    const uint32_t* list = reinterpret_cast<const uint32_t*>(plan + a.off_list);
+    uint8_t* const page = reinterpret_cast<uint8_t*>(a.pool.k + (uint64_t)(a.layer0 + lay) * a.pool.layer_halves +
+                                                     (uint64_t)e.page * a.pool.page_halves);
+    uint8_t* const block = page + ((uint64_t)head * 2 + is_v) * kPage * D;
+    float* const scale = reinterpret_cast<float*>(page + a.pool.b8) + 2 * head + is_v;
+    const float before = *scale;
+    const uint32_t slots = e.slots & 0xffffu;
+    const float* const in = (is_v ? a.v : a.k) + (int64_t)lay * a.layer_stride + head * D;
+    auto row_of = [&](uint32_t p) {  // input row of new position p
+        const uint32_t i = e.src + __popc(slots & ((1u << p) - 1u));
+        return (int64_t)(e.slots & kListed ? list[i] : i) * a.row_stride;
+    };
+    const uint32_t hi = lane >> 4, lo = lane & 15u;
+    // x[i][4 w + b]: the value of byte 4 w + b of the lane's 16 of run i
+    float x[NB][16];
+    bool mine[4];  // of V position 4 hi + b is new; of K all alike
+    float top = 0.f;
+    if (!is_v) {
+#pragma unroll
+        for (int b = 0; b < 4; b++) mine[b] = slots >> lo & 1;
+        const float* p = in + (mine[0] ? row_of(lo) : 0) + 16 * hi;
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                float4 y = {0.f, 0.f, 0.f, 0.f};
+                if (mine[0]) y = *reinterpret_cast<const float4*>(p + 64 * i + 4 * w);
+                x[i][4 * w] = y.x;
+                x[i][4 * w + 1] = y.y;
+                x[i][4 * w + 2] = y.z;
+                x[i][4 * w + 3] = y.w;
+            }
+    } else {
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            mine[b] = slots >> (4 * hi + b) & 1;
+            const float* p = in + (mine[b] ? row_of(4 * hi + b) : 0) + lo;
+#pragma unroll
+            for (int i = 0; i < NB; i++)
+#pragma unroll
+                for (int w = 0; w < 4; w++) x[i][4 * w + b] = mine[b] ? p[64 * i + 16 * w] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            top = fmaxf(top, finite_size(x[i][j]));
+            x[i][j] = number(x[i][j]);
+        }
+    top = wave_max(top);
+    const bool anew = slots & 1u;  // the block begins with this call
+    const int old = exp_of(before), need = scale_exp(top), now = anew ? need : max(old, need);
+    const float inv = pow2(-now);
+    // Old values that stay: by how much they shrink (nothing is there yet below kMinExp).
+    const bool grown = !anew && now > old;
+    const float by = old < kMinExp ? 0.f : pow2(max(old - now, -126));
+    const bool any = mine[0] || mine[1] || mine[2] || mine[3], all = mine[0] && mine[1] && mine[2] && mine[3];
+    if (any || grown) {
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            u32x4* at = reinterpret_cast<u32x4*>(block + 1024 * i) + lane;
+            u32x4 y = {0, 0, 0, 0};
+            if (!all) y = *at;
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const uint32_t fresh = e4m3x4(x[i][4 * w], x[i][4 * w + 1], x[i][4 * w + 2], x[i][4 * w + 3], inv);
+                const uint32_t kept = grown ? rescale4(y[w], by) : y[w];
+                const uint32_t take = (mine[0] ? 0xffu : 0u) | (mine[1] ? 0xff00u : 0u) | (mine[2] ? 0xff0000u : 0u) |
+                                      (mine[3] ? 0xff000000u : 0u);
+                y[w] = (fresh & take) | (kept & ~take);
+            }
+            *at = y;
+        }
+    }
+    if (lane == 0 && (anew || grown)) *scale = pow2(now);
+}
+
+// Eight stored values as f16, exactly (e4m3 lies within f16).
+__device__ __forceinline__ half8_t e4m3_f16x8(uint32_t a, uint32_t b) {
+    const half2_t x0 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false));
+    const half2_t x1 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true));
+    const half2_t x2 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, false));
+    const half2_t x3 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.f, true));
+    return half8_t{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+}
+__device__ __forceinline__ half4_t e4m3_f16x4(uint32_t a) {
+    const half2_t x0 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, false));
+    const half2_t x1 = __builtin_bit_cast(half2_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.f, true));
+    return half4_t{x0[0], x0[1], x1[0], x1[1]};
+}
+
+constexpr int kBlockWaves = 4;
+// Weights are exp2(score - reference), the reference the running maximum less
+// kRefLog2, raised when a score passes it by kRefLog2 + kRefSlack: at most 2^15 in f16
+// (as hi + lo), normal down to 2^-27 of the largest.
+constexpr float kRefLog2 = 13.f, kRefSlack = 2.f, kRefUnscale = 1.f / 8192.f;
+
+// One (item, layer, head): S^T = K Q^T (16 keys x 16 slots; q in f16 hi + lo
+// parts, keys as stored, their page's scale on the sums), the online softmax down
+// its columns, O^T += (V^T P^T of a page) times its value scale.  Lane l holds slot
+// l % 16 and keys, then dims, 4 (l / 16) .. + 3: S^T's registers are P^T's operand
+// as they are.  The four waves take PB pages in turn, the next ones' loads
+// issued before the products of these; their states are joined through LDS.
+template <int D, int INL>
+__global__ __launch_bounds__(64 * kBlockWaves) void block_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
+    constexpr int W = kBlockWaves, NB = D / 64, PB = 2;
+    __shared__ float red[W][kSlotTile][D + 4];  // m, l, -, -, o
+    const int lane = threadIdx.x & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t H = a.pool.n_head, lh = a.n_lay * H;
+    const uint8_t* plan = plan_base(pa, a.plan);
+    const uint32_t item_i = blockIdx.x / lh;
+    const uint32_t rem = blockIdx.x - item_i * lh;
+    const uint32_t lay = rem / H, head = rem - lay * H;
+    const PrefixItem it = reinterpret_cast<const PrefixItem*>(plan + a.off_items)[item_i];
+    const int col = lane & 15, rg = lane >> 4;
+    typedef const __attribute__((address_space(4))) uint32_t* Words;
+    typedef const __attribute__((address_space(4))) float* Scales;
+    const Words tab = (Words)(plan + a.off_table) + it.tab;
+    const uint8_t* const layer = reinterpret_cast<const uint8_t*>(a.pool.k + (uint64_t)(a.layer0 + lay) * a.pool.layer_halves);
+    const uint64_t page_bytes = 2 * a.pool.page_halves;
+    const uint32_t at_block = head * 2 * kPage * D, at_scale = a.pool.b8 + 8 * head;
+    const uint32_t pg_end = (it.kv_end + kPage - 1) / kPage;
+
+    struct Regs {
+        u32x4 k[PB][NB], v[PB][NB];
+        float ks[PB], vs[PB];
+    };
+    auto load = [&](uint32_t pg, Regs& r) {
+#pragma unroll
+        for (int b = 0; b < PB; b++) {
+            // (a page past the end: the last again, its keys masked)
+            const uint8_t* page = layer + (uint64_t)tab[min(pg + b, pg_end - 1)] * page_bytes;
+            const u32x4* p = reinterpret_cast<const u32x4*>(page + at_block) + lane;
+#pragma unroll
+            for (int i = 0; i < NB; i++) r.k[b][i] = load16(p + 64 * i);
+#pragma unroll
+            for (int i = 0; i < NB; i++) r.v[b][i] = load16(p + 64 * (NB + i));
+            const Scales sc = (Scales)(page + at_scale);
+            r.ks[b] = sc[0];
+            r.vs[b] = sc[1];
+        }
+    };
+    Regs cur;
+    uint32_t pg = it.kv_begin / kPage + wave * PB;
+    if (pg < pg_end) load(pg, cur);
+
+    const bool has = col < (int)it.ns;
+    const uint32_t slot = it.slot0 + (has ? (uint32_t)col : 0u);
+    const uint32_t row = slot / a.group, g = slot - row * a.group;
+    const uint32_t qpos = min(it.pos0 + row, kWholePos);
+    const uint32_t first_pos = min(it.pos0 + it.slot0 / a.group, kWholePos);  // of the item's first slot
+    const uint32_t plain_end = min(it.kv_end, first_pos + 1);                 // every slot sees the keys before it
+    half8_t qh[NB][2], ql[NB][2];
+    {
+        // step (i, j) of QK: dims 64 i + 16 rg + 8 j .. + 7, as the lane's bytes of K
+        const float* qb = a.q + (int64_t)lay * a.q_layer_stride + (int64_t)(it.row0 + row) * a.q_row_stride +
+                          (head * a.group + g) * D + 16 * rg;
+#pragma unroll
+        for (int i = 0; i < NB; i++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float4 x0 = reinterpret_cast<const float4*>(qb + 64 * i + 8 * j)[0];
+                const float4 x1 = reinterpret_cast<const float4*>(qb + 64 * i + 8 * j)[1];
+                const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    y[e] = has ? x[e] * a.qscale : 0.f;
+                    asm("" : "+v"(y[e]));  // the f32 products, as the split's residual sees them
+                }
+                split8(y, qh[i][j], ql[i][j]);
+            }
+    }
+    float mref = 0.f, lsum = 0.f;
+    bool set = false;  // the reference is a score's (alike in the four lanes of a slot)
+    float4_t o[4 * NB];
+#pragma unroll
+    for (int c = 0; c < 4 * NB; c++) o[c] = float4_t{0.f, 0.f, 0.f, 0.f};
+
+    for (; pg < pg_end; pg += W * PB) {
+        Regs nxt;
+        if (pg + W * PB < pg_end) load(pg + W * PB, nxt);
+        float s[PB][4];
+#pragma unroll
+        for (int b = 0; b < PB; b++) {
+            float4_t st = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < NB; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const half8_t kh = e4m3_f16x8(cur.k[b][i][2 * j], cur.k[b][i][2 * j + 1]);
+                    st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[i][j], st, 0, 0, 0);
+                    st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[i][j], st, 0, 0, 0);
+                }
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[b][j] = fmaf(st[j], cur.ks[b], -mref);
+        }
+        if ((pg + PB) * kPage > plain_end) {
+#pragma unroll
+            for (int b = 0; b < PB; b++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t key = (pg + b) * kPage + 4 * rg + j;
+                    if (key >= it.kv_end || key > qpos) s[b][j] = -INFINITY;
+                }
+        }
+        float lm = s[0][0];
+#pragma unroll
+        for (int b = 0; b < PB; b++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) lm = fmaxf(lm, s[b][j]);
+        if (__any(lm > kRefLog2 + kRefSlack || !set)) {
+            const float mx = rows4_max(lm) - kRefLog2;
+            // The first finite maximum sets the reference, later ones only raise it.
+            const bool none = mx == -INFINITY;
+            const float d = set ? fmaxf(mx, 0.f) : none ? 0.f : mx;
+            const float alpha = set ? fast_exp2(-d) : 1.f;  // (nothing is summed yet)
+            set = set || !none;
+            lsum *= alpha;
+#pragma unroll
+            for (int c = 0; c < 4 * NB; c++) o[c] *= alpha;
+            mref += d;
+#pragma unroll
+            for (int b = 0; b < PB; b++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[b][j] -= d;
+        }
+#pragma unroll
+        for (int b = 0; b < PB; b++) {
+            float p[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) p[j] = fast_exp2(s[b][j]);
+            lsum += (p[0] + p[1]) + (p[2] + p[3]);
+            half4_t ph, pl;
+            split4(p, ph, pl);
+#pragma unroll
+            for (int i = 0; i < NB; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const half4_t v4 = e4m3_f16x4(cur.v[b][i][c]);
+                    float4_t t = __builtin_amdgcn_mfma_f32_16x16x16f16(v4, pl, float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    t = __builtin_amdgcn_mfma_f32_16x16x16f16(v4, ph, t, 0, 0, 0);
+                    o[4 * i + c] += t * cur.vs[b];
+                }
+        }
+        if (pg + W * PB < pg_end) cur = nxt;
+    }
+    lsum = rows4_sum(lsum);
+    if (has) {
+        if (rg == 0) *reinterpret_cast<float2*>(&red[wave][col][0]) = float2{set ? mref + kRefLog2 : kMinScore, lsum * kRefUnscale};
+#pragma unroll
+        for (int c = 0; c < 4 * NB; c++)
+            *reinterpret_cast<float4_t*>(&red[wave][col][4 + c * 16 + 4 * rg]) = o[c] * kRefUnscale;
+    }
+    __syncthreads();
+    for (uint32_t t = threadIdx.x; t < it.ns * (D / 4); t += 64 * W) {
+        const uint32_t sl = t / (D / 4), d = t % (D / 4) * 4;
+        float M = red[0][sl][0];
+#pragma unroll
+        for (int w = 1; w < W; w++) M = fmaxf(M, red[w][sl][0]);
+        float L = 0.f;
+        float4_t O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const float wt = fast_exp2(red[w][sl][0] - M);
+            L += red[w][sl][1] * wt;
+            O += *reinterpret_cast<const float4_t*>(&red[w][sl][4 + d]) * wt;
+        }
+        if (it.part0 == kNoSlot) {
+            const uint32_t r = (it.slot0 + sl) / a.group, gg = it.slot0 + sl - r * a.group;
+            *reinterpret_cast<float4_t*>(a.out + (int64_t)lay * a.out_layer_stride +
+                                         (int64_t)(it.row0 + r) * a.out_row_stride + (head * a.group + gg) * D + d) = O / L;
+        } else {
+            const uint64_t part = ((uint64_t)(it.part0 + sl) * a.n_lay + lay) * H + head;
+            *reinterpret_cast<float4_t*>(a.part_o + part * D + d) = O;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = float2{M, L};
+        }
+    }
+}
+
+// A thread takes four dims of a row and head of K or V: dims d .. + 3, of a
+// block-scaled V dims d, d + 16, d + 32, d + 48 (one word of four positions each).
+template <int INL>
+__global__ __launch_bounds__(256) void values_kernel(const ValuesLaunch a, const PlanArg<INL> pa) {
+    const uint32_t D = a.pool.head_dim, quads = D / 4, per_row = 2 * a.pool.n_head * quads;
+    const uint64_t gid = (uint64_t)blockIdx.x * 256u + threadIdx.x;
+    const uint64_t lr = gid / per_row;
+    if (lr >= (uint64_t)a.n_lay * a.n_rows) return;
+    uint32_t u = (uint32_t)(gid - lr * per_row);
+    const uint32_t lay = (uint32_t)(lr / a.n_rows), row = (uint32_t)(lr - (uint64_t)lay * a.n_rows);
+    const uint32_t is_v = u / (a.pool.n_head * quads);
+    u -= is_v * a.pool.n_head * quads;
+    const uint32_t head = u / quads, x = u - head * quads;
+    const AppendEntry e = reinterpret_cast<const AppendEntry*>(plan_base(pa, a.plan) + a.off_entries)[row];
+    const uint16_t* const page = a.pool.k + (uint64_t)(a.layer0 + lay) * a.pool.layer_halves + (uint64_t)e.page * a.pool.page_halves;
+    float* const out = (is_v ? a.v_out : a.k_out) + (int64_t)lay * a.layer_stride + (int64_t)e.src_row * a.row_stride + head * D;
+    float4 y;
+    if (a.pool.b8) {
+        const uint8_t* block = reinterpret_cast<const uint8_t*>(page) + (head * 2 + is_v) * kPage * D;
+        const float scale = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(page) + a.pool.b8)[2 * head + is_v];
+        if (!is_v) {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(block + k_byte(e.slot, 4 * x));
+            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+            y = float4{lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
+        } else {
+            const uint32_t d = x / 16 * 64 + x % 16;
+            const u32x4 w = *reinterpret_cast<const u32x4*>(block + (v_byte(e.slot, d) & ~15u));
+            float z[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                z[i] = __builtin_amdgcn_cvt_f32_fp8((int)(w[i] >> (8 * (e.slot % 4))), 0) * scale;
+                out[d + 16 * i] = z[i];
+            }
+            return;
+        }
+    } else {
+        const uint16_t* block = page + (uint64_t)head * a.pool.head_halves + (is_v ? a.pool.head_halves / 2 : 0);
+        if (a.pool.q8) {
+            const uint8_t* b = reinterpret_cast<const uint8_t*>(block);
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(b + e.slot * D + 4 * x);
+            const float scale = reinterpret_cast<const float*>(b + kPage * D)[e.slot];
+            y = float4{i8f(w, 0) * scale, i8f(w, 1) * scale, i8f(w, 2) * scale, i8f(w, 3) * scale};
+        } else {
+            const half4_t h = *reinterpret_cast<const half4_t*>(block + e.slot * D + 4 * x);
+            y = float4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
+        }
+    }
+    reinterpret_cast<float4*>(out)[x] = y;
+}
+
+}  // namespace
+
+hipError_t launch_block_append(const BlockAppendLaunch& a, const void* ip, uint32_t ib, hipStream_t s,
+                               const LaunchTiming& t) {
+    const uint64_t units = (uint64_t)a.n * a.n_lay * a.pool.n_head * 2;
+    if (units == 0) return hipSuccess;
+    return with_plan(a, ip, ib, [&](auto pa) {
+        constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
+        if (a.pool.head_dim == 64) return go(block_append_kernel<64, INL>, (units + 3) / 4, 256, s, t, a, pa);
+        if (a.pool.head_dim == 128) return go(block_append_kernel<128, INL>, (units + 3) / 4, 256, s, t, a, pa);
+        return hipErrorInvalidValue;
+    });
+}
+
+hipError_t launch_block_attention(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s,
+                                  const LaunchTiming& t) {
+    const uint64_t blocks = (uint64_t)a.n_items * a.n_lay * a.pool.n_head;
+    if (blocks == 0) return hipSuccess;
+    return with_plan(a, ip, ib, [&](auto pa) {
+        constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
+        if (a.pool.head_dim == 64) return go(block_attn_kernel<64, INL>, blocks, 64 * kBlockWaves, s, t, a, pa);
+        if (a.pool.head_dim == 128) return go(block_attn_kernel<128, INL>, blocks, 64 * kBlockWaves, s, t, a, pa);
+        return hipErrorInvalidValue;
+    });
+}
+
+hipError_t launch_gather_values(const ValuesLaunch& a, const void* ip, uint32_t ib, hipStream_t s) {
+    const uint64_t threads = (uint64_t)a.n_lay * a.n_rows * 2 * a.pool.n_head * (a.pool.head_dim / 4);
+    if (threads == 0) return hipSuccess;
+    return with_plan(a, ip, ib, [&](auto pa) {
+        constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
+        return go(values_kernel<INL>, (threads + 255) / 256, 256, s, {}, a, pa);
+    });
+}
+
+}  // namespace ni

@@ -240,6 +240,15 @@ struct ni_kv {
     };
     std::vector<PlaceMark> place_marks;
     uint32_t place_stamp = 0;
+    // ni_kv_append on a block-scaled pool: entries, their list, and the stamp of
+    // the last call that wrote to a page.
+    std::vector<BlockAppend> block_entries;
+    std::vector<uint32_t> block_list;
+    std::vector<uint32_t> page_stamps;
+    uint32_t page_stamp = 0;
+    std::vector<std::pair<uint32_t, uint32_t>> block_rows;  // (page * 16 + slot, row), where they are sorted
+    std::vector<ni_row> step_rows;     // ni_kv_step on such a pool
+    std::vector<uint32_t> step_at;
     std::vector<uint8_t> blob;  // the serialised plan
     std::vector<QRow> qrows;
     std::vector<int64_t> seq_tab;     // seq -> offset in plan.table, -1 if absent
@@ -282,6 +291,7 @@ struct ni_kv {
         g.n_head = o.n_head;
         g.head_dim = o.head_dim;
         g.q8 = (o.flags & NI_KV_Q8) ? 1u : 0u;
+        g.b8 = (o.flags & NI_KV_B8) ? o.n_head * 2 * kPage * o.head_dim : 0u;
         return g;
     }
 };
@@ -361,6 +371,7 @@ int check_grow(ni_kv* kv, uint32_t s, uint64_t n) {
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 bool is_q8(const ni_kv_opts& o) { return (o.flags & NI_KV_Q8) != 0; }
+bool is_b8(const ni_kv_opts& o) { return (o.flags & NI_KV_B8) != 0; }
 
 // Rows of one sequence that share one pass over the keys (the matrix-core
 // tile, f16 and Q8 pools alike).
@@ -368,7 +379,13 @@ uint32_t max_group_rows(const ni_kv*) { return kMaxGroupRows; }
 
 // Halves of one K (or V) block of a (page, head).
 uint64_t kv_block_halves(const ni_kv_opts& o) {
+    if (is_b8(o)) return (uint64_t)kPage * o.head_dim / 2;
     return is_q8(o) ? (uint64_t)kPage * o.head_dim / 2 + kPage * 2 : (uint64_t)kPage * o.head_dim;
+}
+
+// Halves of one page of one layer (block-scaled: its scales at the end).
+uint64_t kv_page_halves(const ni_kv_opts& o) {
+    return 2 * kv_block_halves(o) * o.n_head + (is_b8(o) ? align_up(8ull * o.n_head, 128) / 2 : 0);
 }
 
 int check_f32_operand(ni_kv* kv, const char* name, const void* p, int64_t row_stride, int64_t layer_stride,
@@ -1410,9 +1427,10 @@ struct DeviceScope {
 // Cut a ni_kv_prefix_attention call into items.  Queries travel as slots (the
 // `group` query heads of a row that read one cache head).  A prefix is read by
 // its rows' slots together, each sequence's own keys by its rows' (consecutive
-// rows of one sequence at consecutive positions form a run).
-int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32_t n_prefix, uint32_t group,
-                uint32_t n_lay, uint32_t split_tokens, PrefixPlan& P) {
+// rows of one sequence at consecutive positions form a run).  at: the input row of
+// each (NULL: its index; given only without prefixes).
+int plan_prefix(ni_kv* kv, const ni_row* rows, const uint32_t* at, const ni_prefix* prefixes, uint32_t n_prefix,
+                uint32_t group, uint32_t n_lay, uint32_t split_tokens, PrefixPlan& P) {
     P.pitems.clear();
     P.items.clear();
     P.merges.clear();
@@ -1421,18 +1439,20 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
     struct Run {
         uint32_t seq, row0, pos0, n;
         uint32_t prefix;  // index into prefixes
+        uint32_t first;   // index into rows
     };
     std::vector<Run> runs;
     for (uint32_t i = 0, r = 0; i < n_prefix; i++)
         for (uint32_t e = r + prefixes[i].n_rows; r < e; r++) {
+            const uint32_t row = at ? at[r] : r;
             if (!runs.empty()) {
                 Run& u = runs.back();
-                if (u.prefix == i && u.seq == rows[r].seq && u.pos0 + u.n == rows[r].pos) {
+                if (u.prefix == i && u.seq == rows[r].seq && u.pos0 + u.n == rows[r].pos && u.row0 + u.n == row) {
                     u.n++;
                     continue;
                 }
             }
-            runs.push_back({rows[r].seq, r, rows[r].pos, 1, i});
+            runs.push_back({rows[r].seq, row, rows[r].pos, 1, i, r});
         }
     // Page lists, one per sequence: as many pages as any of its runs reads.
     struct Scratch {  // seq_need and seq_tab as they were, whatever happens
@@ -1484,7 +1504,7 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
             work += tiles(slots, kSlotTile) * prefixes[i].len * lh;
         }
     const uint64_t wide_from = kv->o.head_dim == 128 ? 64000 : is_q8(kv->o) ? 300000 : 40000;
-    P.wide = most > kSlotTile && work >= wide_from;
+    P.wide = most > kSlotTile && work >= wide_from && !is_b8(kv->o);
     P.waves = 0;
     uint64_t p_tile = kSlotTile;
     if (P.wide) {
@@ -1563,7 +1583,7 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
         for (; u0 < runs.size() && runs[u0].prefix == i; u0++) {
             const Run& u = runs[u0];
             const uint64_t slots = (uint64_t)u.n * group, n_own = (u.pos0 + u.n + part - 1) / part;
-            const uint64_t pre = pre0[i] + (uint64_t)(u.row0 - r) * group;  // the run's first partial of the prefix
+            const uint64_t pre = pre0[i] + (uint64_t)(u.first - r) * group;  // the run's first partial of the prefix
             const uint32_t tab = tab_of(u.seq);
             const bool whole = n_own == 1 && (P.wide || n_pre == 0);
             for (uint64_t j = 0; j < n_own; j++)
@@ -1597,7 +1617,7 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const ni_prefix* prefixes, uint32
         P.pitems.clear();
     }
     const bool rows_alone = std::all_of(runs.begin(), runs.end(), [](const Run& u) { return u.n == 1; });
-    P.row_slots = !shared && group <= (is_q8(kv->o) ? 1u : 2u) && rows_alone ? group : 0;
+    P.row_slots = !shared && !is_b8(kv->o) && group <= (is_q8(kv->o) ? 1u : 2u) && rows_alone ? group : 0;
     P.row_waves = P.items.size() * lh >= 12 * cus ? 2 : 4;
     // Longest first, so that no launch ends on a long item.  Of a launch whose
     // workgroups are all on the CUs at once, block b shares a CU with blocks b +-
@@ -1663,8 +1683,12 @@ int ni_kv_create(const ni_kv_opts* opts, ni_kv** out) {
         g_create_error = "n_layer, n_head, kv_pages, max_seqs, max_ctx and max_rows must be > 0; head_dim a multiple of 8";
         return NI_ERR_BAD_ARG;
     }
-    if (o.flags & ~(NI_KV_HOST_ONLY | NI_KV_Q8)) {
+    if (o.flags & ~(NI_KV_HOST_ONLY | NI_KV_Q8 | NI_KV_B8)) {
         g_create_error = "unknown flags";
+        return NI_ERR_BAD_ARG;
+    }
+    if (is_q8(o) && is_b8(o)) {
+        g_create_error = "a cache is either Q8 or block-scaled";
         return NI_ERR_BAD_ARG;
     }
     const bool host_only = (o.flags & NI_KV_HOST_ONLY) != 0;
@@ -1716,7 +1740,7 @@ int ni_kv_create(const ni_kv_opts* opts, ni_kv** out) {
             // 16 f32 scales, 16 * head_dim + 64 bytes (kv_block_halves()).
             const uint64_t block = kv_block_halves(o);
             kv->head_halves = (uint32_t)(2 * block);
-            kv->page_halves = 2 * block * o.n_head;
+            kv->page_halves = kv_page_halves(o);
             kv->layer_halves = kv->page_halves * o.kv_pages;
             kv->pool_bytes = (size_t)(kv->layer_halves * o.n_layer * sizeof(uint16_t));
             e = hipMalloc(reinterpret_cast<void**>(&kv->kpool), kv->pool_bytes);
@@ -1782,7 +1806,7 @@ void ni_kv_destroy(ni_kv* kv) {
 }
 
 size_t ni_kv_page_bytes(const ni_kv* kv) {
-    return kv ? (size_t)2 * kv->o.n_layer * kv->o.n_head * kv_block_halves(kv->o) * 2 : 0;
+    return kv ? (size_t)kv->o.n_layer * kv_page_halves(kv->o) * 2 : 0;
 }
 
 int ni_kv_add_seq(ni_kv* kv, uint32_t* seq) {
@@ -1866,6 +1890,132 @@ int ni_kv_pools(const ni_kv* kv, void** k_pool, void** v_pool, size_t* bytes) {
     if (v_pool) *v_pool = kv->vpool;
     if (bytes) *bytes = kv->pool_bytes;
     return NI_OK;
+}
+
+// A plan too long for the launch arguments is uploaded on another stream,
+// which a capture cannot record.
+static int check_capture(ni_kv* kv, size_t plan_bytes) {
+    if (kv->capturing && plan_bytes > kInlinePlanBytes)
+        return kv->fail(NI_ERR_BAD_ARG,
+                        "the call's plan is %zu bytes; under stream capture it travels with the launch, at most %u "
+                        "(fewer rows or shorter contexts per call)",
+                        plan_bytes, kInlinePlanBytes);
+    return NI_OK;
+}
+
+static int block_unsupported(ni_kv* kv, const char* what) {
+    return kv->fail(NI_ERR_BAD_ARG, "%s does not take a block-scaled cache", what);
+}
+
+// Sort a call's rows into the pages they go to (block_entries, block_list).
+static int plan_block_append(ni_kv* kv, const ni_row* rows, uint32_t n) {
+    auto& entries = kv->block_entries;
+    auto& list = kv->block_list;
+    entries.clear();
+    list.clear();
+    if (kv->page_stamps.empty()) kv->page_stamps.assign(kv->o.kv_pages, 0);
+    if (++kv->page_stamp == 0) {
+        std::fill(kv->page_stamps.begin(), kv->page_stamps.end(), 0u);
+        kv->page_stamp = 1;
+    }
+    // Rows mostly come page by page, in the order of their positions.
+    bool sorted = true;
+    uint32_t last_slot = 0;
+    for (uint32_t i = 0; i < n; i++) {
+        if (int rc = check_write(kv, rows[i])) return rc;
+        const uint32_t page = kv->pages[rows[i].seq][rows[i].pos / kPage], slot = rows[i].pos % kPage;
+        if (!entries.empty() && entries.back().page == page && slot > last_slot) {
+            entries.back().slots |= 1u << slot;
+        } else {
+            sorted &= kv->page_stamps[page] != kv->page_stamp;
+            kv->page_stamps[page] = kv->page_stamp;
+            entries.push_back({page, i, 1u << slot});
+        }
+        last_slot = slot;
+    }
+    if (sorted) return NI_OK;
+    auto& order = kv->block_rows;
+    order.clear();
+    for (uint32_t i = 0; i < n; i++)
+        order.push_back({0, i});
+    // (page and slot compared apart: their product may pass 32 bits)
+    auto page_of = [&](uint32_t i) { return kv->pages[rows[i].seq][rows[i].pos / kPage]; };
+    for (auto& o : order) o.first = page_of(o.second);
+    std::sort(order.begin(), order.end(), [&](const auto& a, const auto& b) {
+        if (a.first != b.first) return a.first < b.first;
+        return rows[a.second].pos % kPage < rows[b.second].pos % kPage;
+    });
+    entries.clear();
+    for (uint32_t i = 0; i < n; i++) {
+        const uint32_t page = order[i].first;
+        const ni_row& r = rows[order[i].second];
+        const uint32_t slot = 1u << r.pos % kPage;
+        if (i == 0 || order[i - 1].first != page) entries.push_back({page, i, kListed});
+        if (entries.back().slots & slot)
+            return kv->fail(NI_ERR_BAD_ARG, "sequence %u: position %u appears twice", r.seq, r.pos);
+        entries.back().slots |= slot;
+        list.push_back(order[i].second);
+    }
+    return NI_OK;
+}
+
+// ni_kv_append on a block-scaled pool.
+static int block_append(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const ni_row* rows, uint32_t n, const float* k,
+                        const float* v, int64_t row_stride, int64_t layer_stride, hipStream_t s) try {
+    if (int rc = plan_block_append(kv, rows, n)) return rc;
+    const auto& entries = kv->block_entries;
+    const auto& list = kv->block_list;
+    // (a launch holds less than 2^32 threads, a wave to each of K and V of a head)
+    if ((uint64_t)entries.size() * n_lay * kv->o.n_head >= (1ull << 24))
+        return kv->fail(NI_ERR_BAD_ARG, "rows * layers * heads too large for one call");
+    std::vector<uint8_t>& blob = kv->blob;
+    const size_t off_list = align_up(entries.size() * sizeof(BlockAppend), 16);
+    blob.resize(align_up(off_list + list.size() * sizeof(uint32_t), kAlign));
+    memcpy(blob.data(), entries.data(), entries.size() * sizeof(BlockAppend));
+    if (!list.empty()) memcpy(blob.data() + off_list, list.data(), list.size() * sizeof(uint32_t));
+    DeviceScope device(kv->device);
+    if (int rc = begin_call(kv, s)) return rc;
+    if (int rc = check_capture(kv, blob.size())) return rc;
+    PlanRef ref;
+    if (int rc = place_blob(kv, blob, s, &ref)) return rc;
+    BlockAppendLaunch a{};
+    a.pool = kv->geom();
+    a.k = k;
+    a.v = v;
+    a.row_stride = row_stride;
+    a.layer_stride = layer_stride;
+    a.plan = ref.dev;
+    a.off_list = (uint32_t)off_list;
+    a.n = (uint32_t)entries.size();
+    a.layer0 = layer0;
+    a.n_lay = n_lay;
+    hipError_t e;
+    {
+        ProfileScope ps(kv, NI_K_APPEND);
+        e = launch_block_append(a, ref.inl, ref.inl_bytes, s, ps.t);
+    }
+    const int rc = release_plan(kv, ref, s);
+    return e != hipSuccess ? kv->hip_fail(e, "block append kernel") : rc;
+} catch (const std::bad_alloc&) {
+    return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
+}
+
+static int run_prefix(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const float* q, int64_t q_row_stride,
+                      int64_t q_layer_stride, uint32_t n_q_head, const ni_row* rows, const uint32_t* at,
+                      const ni_prefix* prefixes, uint32_t n_prefix, float* out, int64_t out_row_stride, int64_t out_layer_stride,
+                      uint32_t split_tokens, hipStream_t s);
+
+// Attention of n rows (checked) over a block-scaled pool, query heads as the cache's.
+static int block_attention(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const float* q, int64_t q_row_stride,
+                           int64_t q_layer_stride, const ni_row* rows, const uint32_t* at, uint32_t n, float* out,
+                           int64_t out_row_stride, int64_t out_layer_stride, uint32_t split_tokens, hipStream_t s) try {
+    if (split_tokens % kPage != 0)
+        return kv->fail(NI_ERR_BAD_ARG, "split_tokens %u must be a multiple of %u", split_tokens, kPage);
+    const ni_prefix none{0, 0, n};
+    return run_prefix(kv, layer0, n_lay, q, q_row_stride, q_layer_stride, kv->o.n_head, rows, at, &none, 1, out,
+                      out_row_stride, out_layer_stride, split_tokens, s);
+} catch (const std::bad_alloc&) {
+    return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
 }
 
 // What ni_kv_fork and its kin check before they look at tables, the call ordered
@@ -2112,6 +2262,8 @@ int ni_kv_append(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, const
     const bool all = layer == NI_ALL_LAYERS;
     if (int rc = check_f32_operand(kv, "k", k, row_stride, layer_stride, all)) return rc;
     if (int rc = check_f32_operand(kv, "v", v, row_stride, layer_stride, all)) return rc;
+    if (is_b8(kv->o))
+        return block_append(kv, layer0, n_lay, rows, n, k, v, row_stride, all ? layer_stride : 0, (hipStream_t)stream);
     reset_plan(kv);
     for (uint32_t i = 0; i < n; i++) {
         if (int rc = check_write(kv, rows[i])) return rc;
@@ -2131,6 +2283,7 @@ static int qkv_run(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, con
     const bool fused = rows != nullptr;
     if (fused && is_q8(kv->o))
         return kv->fail(NI_ERR_BAD_ARG, "Q8 cache: project with ni_kv_qkv_project and append with ni_kv_append");
+    if (fused && is_b8(kv->o)) return block_unsupported(kv, "ni_kv_qkv_append");
     const uint32_t C = kv->o.n_head * kv->o.head_dim, n_feat = 3 * C;
     if (fused && (layer < 0 || (uint32_t)layer >= kv->o.n_layer))
         return kv->fail(NI_ERR_BAD_ARG, "layer %d out of range (%u layers)", layer, kv->o.n_layer);
@@ -2220,6 +2373,7 @@ int ni_kv_gather(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, uint1
     if (!rows) return kv->fail(NI_ERR_BAD_ARG, "rows is NULL");
     if (n > kv->o.max_rows) return kv->fail(NI_ERR_TOO_MANY_ROWS, "%u rows > max_rows %u", n, kv->o.max_rows);
     if (is_q8(kv->o)) return kv->fail(NI_ERR_BAD_ARG, "Q8 cache: use ni_kv_gather_q8");
+    if (is_b8(kv->o)) return kv->fail(NI_ERR_BAD_ARG, "block-scaled cache: use ni_kv_gather_values");
     const bool all = layer == NI_ALL_LAYERS;
     if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out) || row_stride % 8 != 0 || row_stride < 0 ||
         (all && (layer_stride % 8 != 0 || layer_stride < 0)))
@@ -2303,6 +2457,12 @@ int ni_paged_decode_attention(ni_kv* kv, int32_t layer, const float* q, int64_t 
     const bool all = layer == NI_ALL_LAYERS;
     if (int rc = check_f32_operand(kv, "q", q, q_row_stride, q_layer_stride, all)) return rc;
     if (int rc = check_f32_operand(kv, "out", out, out_row_stride, out_layer_stride, all)) return rc;
+    if (is_b8(kv->o)) {
+        for (uint32_t i = 0; i < n; i++)
+            if (int rc = check_row(kv, rows[i])) return rc;
+        return block_attention(kv, layer0, n_lay, q, q_row_stride, all ? q_layer_stride : 0, rows, nullptr, n, out, out_row_stride,
+                               all ? out_layer_stride : 0, split_tokens, (hipStream_t)stream);
+    }
     reset_plan(kv);
     for (uint32_t i = 0; i < n; i++) {
         if (int rc = check_row(kv, rows[i])) return rc;
@@ -2341,15 +2501,46 @@ static bool rows_overlap(uint64_t n, uint64_t a, uint64_t m, uint64_t b, uint64_
     return false;
 }
 
-// A plan too long for the launch arguments is uploaded on another stream,
-// which a capture cannot record.
-static int check_capture(ni_kv* kv, size_t plan_bytes) {
-    if (kv->capturing && plan_bytes > kInlinePlanBytes)
-        return kv->fail(NI_ERR_BAD_ARG,
-                        "the call's plan is %zu bytes; under stream capture it travels with the launch, at most %u "
-                        "(fewer rows or shorter contexts per call)",
-                        plan_bytes, kInlinePlanBytes);
-    return NI_OK;
+int ni_kv_gather_values(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, float* k_out, float* v_out,
+                        int64_t row_stride, int64_t layer_stride, ni_stream stream) try {
+    if (!kv) return NI_ERR_BAD_ARG;
+    uint32_t layer0, n_lay;
+    if (int rc = check_call(kv, layer, rows, n, &layer0, &n_lay)) return rc;
+    if (n == 0) return NI_OK;
+    const bool all = layer == NI_ALL_LAYERS;
+    if (int rc = check_f32_operand(kv, "k_out", k_out, row_stride, layer_stride, all)) return rc;
+    if (int rc = check_f32_operand(kv, "v_out", v_out, row_stride, layer_stride, all)) return rc;
+    const uint64_t C = (uint64_t)kv->o.n_head * kv->o.head_dim;
+    if (rows_overlap(n, row_stride, all ? n_lay : 1, layer_stride, C))
+        return kv->fail(NI_ERR_BAD_ARG, "k_out's rows of %llu values overlap", (unsigned long long)C);
+    std::vector<uint8_t>& blob = kv->blob;
+    blob.resize(align_up((size_t)n * sizeof(AppendEntry), kAlign));
+    AppendEntry* entries = reinterpret_cast<AppendEntry*>(blob.data());
+    for (uint32_t i = 0; i < n; i++) {
+        if (int rc = check_row(kv, rows[i])) return rc;
+        entries[i] = {i, kv->pages[rows[i].seq][rows[i].pos / kPage], rows[i].pos % kPage, 0};
+    }
+    DeviceScope device(kv->device);
+    const hipStream_t s = (hipStream_t)stream;
+    if (int rc = begin_call(kv, s)) return rc;
+    if (int rc = check_capture(kv, blob.size())) return rc;
+    PlanRef ref;
+    if (int rc = place_blob(kv, blob, s, &ref)) return rc;
+    ValuesLaunch a{};
+    a.pool = kv->geom();
+    a.k_out = k_out;
+    a.v_out = v_out;
+    a.row_stride = row_stride;
+    a.layer_stride = all ? layer_stride : 0;
+    a.plan = ref.dev;
+    a.n_rows = n;
+    a.layer0 = layer0;
+    a.n_lay = n_lay;
+    const hipError_t e = launch_gather_values(a, ref.inl, ref.inl_bytes, s);
+    const int rc = release_plan(kv, ref, s);
+    return e != hipSuccess ? kv->hip_fail(e, "gather kernel") : rc;
+} catch (const std::bad_alloc&) {
+    return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
 }
 
 int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n, const ni_rotary* rotary,
@@ -2360,6 +2551,7 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
     if (!kv) return NI_ERR_BAD_ARG;
     uint32_t layer0, n_lay;
     if (int rc = check_call(kv, layer, rows, n, &layer0, &n_lay)) return rc;
+    if (is_b8(kv->o)) return block_unsupported(kv, "ni_kv_append_rotary");
     if (n == 0) return NI_OK;
     const bool all = layer == NI_ALL_LAYERS;
     const uint32_t D = kv->o.head_dim;
@@ -2455,6 +2647,87 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
     return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
 }
 
+// Plan and enqueue a call of ni_kv_prefix_attention (checked), or any attention
+// over a block-scaled pool.
+static int run_prefix(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const float* q, int64_t q_row_stride,
+                      int64_t q_layer_stride, uint32_t n_q_head, const ni_row* rows, const uint32_t* at,
+                      const ni_prefix* prefixes, uint32_t n_prefix, float* out, int64_t out_row_stride, int64_t out_layer_stride,
+                      uint32_t split_tokens, hipStream_t s) {
+    PrefixPlan& P = kv->prefix_plan;
+    if (int rc = plan_prefix(kv, rows, at, prefixes, n_prefix, n_q_head / kv->o.n_head, n_lay, split_tokens, P)) return rc;
+    std::vector<uint8_t>& blob = kv->blob;
+    const size_t off_pitems = align_up(P.items.size() * sizeof(PrefixItem), kAlign);
+    const size_t off_merges = align_up(off_pitems + P.pitems.size() * sizeof(PrefixItem), kAlign);
+    const size_t off_table = align_up(off_merges + P.merges.size() * sizeof(PrefixMerge), kAlign);
+    blob.resize(align_up(off_table + P.table.size() * sizeof(uint32_t), kAlign));
+    memcpy(blob.data(), P.items.data(), P.items.size() * sizeof(PrefixItem));
+    if (!P.pitems.empty()) memcpy(blob.data() + off_pitems, P.pitems.data(), P.pitems.size() * sizeof(PrefixItem));
+    if (!P.merges.empty()) memcpy(blob.data() + off_merges, P.merges.data(), P.merges.size() * sizeof(PrefixMerge));
+    memcpy(blob.data() + off_table, P.table.data(), P.table.size() * sizeof(uint32_t));
+
+    const uint32_t D = kv->o.head_dim, H = kv->o.n_head;
+    DeviceScope device(kv->device);
+    if (int rc = begin_call(kv, s)) return rc;
+    if (int rc = check_capture(kv, blob.size())) return rc;
+    const size_t parts = (size_t)P.n_parts * n_lay * H;
+    const size_t o_bytes = align_up(parts * D * sizeof(float), kAlign), bytes = o_bytes + parts * 2 * sizeof(float);
+    float* partials = nullptr;
+    if (parts) {
+        const size_t held = std::max(kv->partials_bytes, kv->graph_partials_bytes);
+        if (kv->capturing && bytes > held)
+            return kv->fail(NI_ERR_BAD_ARG,
+                            "the call needs %zu bytes of partials, the handle holds %zu: make it once outside the "
+                            "capture",
+                            bytes, held);
+        if (int rc = ensure_partials(kv, bytes, s, &partials)) return rc;
+    }
+    PlanRef ref;
+    if (int rc = place_blob(kv, blob, s, &ref)) return rc;
+    PrefixLaunch a{};
+    a.pool = kv->geom();
+    a.q = q;
+    a.out = out;
+    a.q_row_stride = q_row_stride;
+    a.q_layer_stride = q_layer_stride;
+    a.out_row_stride = out_row_stride;
+    a.out_layer_stride = out_layer_stride;
+    a.plan = ref.dev;
+    a.off_merges = (uint32_t)off_merges;
+    a.off_table = (uint32_t)off_table;
+    a.part_o = partials;
+    a.part_ml = partials ? partials + o_bytes / sizeof(float) : nullptr;
+    a.n_merges = (uint32_t)P.merges.size();
+    a.layer0 = layer0;
+    a.n_lay = n_lay;
+    a.group = n_q_head / H;
+    a.qscale = (float)(1.4426950408889634 / std::sqrt((double)D));
+    hipError_t e = hipSuccess;
+    if (!P.pitems.empty()) {
+        a.off_items = (uint32_t)off_pitems;
+        a.n_items = (uint32_t)P.pitems.size();
+        a.wide = P.wide;
+        a.waves = P.waves;
+        ProfileScope ps(kv, NI_K_ATTN);
+        e = launch_prefix_attention(a, ref.inl, ref.inl_bytes, s, ps.t);
+    }
+    if (e == hipSuccess) {
+        a.off_items = 0;
+        a.n_items = (uint32_t)P.items.size();
+        a.wide = 0;
+        a.row_slots = P.row_slots;
+        a.waves = P.row_waves;
+        ProfileScope ps(kv, NI_K_ATTN);
+        e = is_b8(kv->o) ? launch_block_attention(a, ref.inl, ref.inl_bytes, s, ps.t)
+                         : launch_prefix_attention(a, ref.inl, ref.inl_bytes, s, ps.t);
+    }
+    if (e == hipSuccess && a.n_merges) {
+        ProfileScope ps(kv, NI_K_MERGE);
+        e = launch_prefix_merge(a, ref.inl, ref.inl_bytes, s, ps.t);
+    }
+    const int rc2 = release_plan(kv, ref, s);
+    return e != hipSuccess ? kv->hip_fail(e, is_b8(kv->o) ? "block-scaled attention kernel" : "shared-prefix attention kernel") : rc2;
+}
+
 int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_row_stride, int64_t q_layer_stride,
                            uint32_t n_q_head, const ni_row* rows, uint32_t n, const ni_prefix* prefixes,
                            uint32_t n_prefix, float* out, int64_t out_row_stride, int64_t out_layer_stride,
@@ -2492,78 +2765,8 @@ int ni_kv_prefix_attention(ni_kv* kv, int32_t layer, const float* q, int64_t q_r
                 return kv->fail(NI_ERR_BAD_ARG, "row %u: sequence %u is its own prefix", r, p.seq);
         }
     }
-    PrefixPlan& P = kv->prefix_plan;
-    if (int rc = plan_prefix(kv, rows, prefixes, n_prefix, n_q_head / H, n_lay, split_tokens, P)) return rc;
-    std::vector<uint8_t>& blob = kv->blob;
-    const size_t off_pitems = align_up(P.items.size() * sizeof(PrefixItem), kAlign);
-    const size_t off_merges = align_up(off_pitems + P.pitems.size() * sizeof(PrefixItem), kAlign);
-    const size_t off_table = align_up(off_merges + P.merges.size() * sizeof(PrefixMerge), kAlign);
-    blob.resize(align_up(off_table + P.table.size() * sizeof(uint32_t), kAlign));
-    memcpy(blob.data(), P.items.data(), P.items.size() * sizeof(PrefixItem));
-    if (!P.pitems.empty()) memcpy(blob.data() + off_pitems, P.pitems.data(), P.pitems.size() * sizeof(PrefixItem));
-    if (!P.merges.empty()) memcpy(blob.data() + off_merges, P.merges.data(), P.merges.size() * sizeof(PrefixMerge));
-    memcpy(blob.data() + off_table, P.table.data(), P.table.size() * sizeof(uint32_t));
-
-    DeviceScope device(kv->device);
-    const hipStream_t s = (hipStream_t)stream;
-    if (int rc = begin_call(kv, s)) return rc;
-    if (int rc = check_capture(kv, blob.size())) return rc;
-    const size_t parts = (size_t)P.n_parts * n_lay * H;
-    const size_t o_bytes = align_up(parts * D * sizeof(float), kAlign), bytes = o_bytes + parts * 2 * sizeof(float);
-    float* partials = nullptr;
-    if (parts) {
-        const size_t held = std::max(kv->partials_bytes, kv->graph_partials_bytes);
-        if (kv->capturing && bytes > held)
-            return kv->fail(NI_ERR_BAD_ARG,
-                            "the call needs %zu bytes of partials, the handle holds %zu: make it once outside the "
-                            "capture",
-                            bytes, held);
-        if (int rc = ensure_partials(kv, bytes, s, &partials)) return rc;
-    }
-    PlanRef ref;
-    if (int rc = place_blob(kv, blob, s, &ref)) return rc;
-    PrefixLaunch a{};
-    a.pool = kv->geom();
-    a.q = q;
-    a.out = out;
-    a.q_row_stride = q_row_stride;
-    a.q_layer_stride = all ? q_layer_stride : 0;
-    a.out_row_stride = out_row_stride;
-    a.out_layer_stride = all ? out_layer_stride : 0;
-    a.plan = ref.dev;
-    a.off_merges = (uint32_t)off_merges;
-    a.off_table = (uint32_t)off_table;
-    a.part_o = partials;
-    a.part_ml = partials ? partials + o_bytes / sizeof(float) : nullptr;
-    a.n_merges = (uint32_t)P.merges.size();
-    a.layer0 = layer0;
-    a.n_lay = n_lay;
-    a.group = n_q_head / H;
-    a.qscale = (float)(1.4426950408889634 / std::sqrt((double)D));
-    hipError_t e = hipSuccess;
-    if (!P.pitems.empty()) {
-        a.off_items = (uint32_t)off_pitems;
-        a.n_items = (uint32_t)P.pitems.size();
-        a.wide = P.wide;
-        a.waves = P.waves;
-        ProfileScope ps(kv, NI_K_ATTN);
-        e = launch_prefix_attention(a, ref.inl, ref.inl_bytes, s, ps.t);
-    }
-    if (e == hipSuccess) {
-        a.off_items = 0;
-        a.n_items = (uint32_t)P.items.size();
-        a.wide = 0;
-        a.row_slots = P.row_slots;
-        a.waves = P.row_waves;
-        ProfileScope ps(kv, NI_K_ATTN);
-        e = launch_prefix_attention(a, ref.inl, ref.inl_bytes, s, ps.t);
-    }
-    if (e == hipSuccess && a.n_merges) {
-        ProfileScope ps(kv, NI_K_MERGE);
-        e = launch_prefix_merge(a, ref.inl, ref.inl_bytes, s, ps.t);
-    }
-    const int rc2 = release_plan(kv, ref, s);
-    return e != hipSuccess ? kv->hip_fail(e, "shared-prefix attention kernel") : rc2;
+    return run_prefix(kv, layer0, n_lay, q, q_row_stride, all ? q_layer_stride : 0, n_q_head, rows, nullptr, prefixes, n_prefix,
+                      out, out_row_stride, all ? out_layer_stride : 0, split_tokens, (hipStream_t)stream);
 } catch (const std::bad_alloc&) {
     return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
 }
@@ -2594,6 +2797,7 @@ int ni_kv_step_noalloc(ni_kv* kv, const ni_work* work, uint32_t n_work, const fl
                        int64_t out_layer_stride, uint32_t split_tokens, ni_stream stream) {
     if (!kv) return NI_ERR_BAD_ARG;
     if (kv->host_only) return kv->fail(NI_ERR_NO_DEVICE, "host-only handle has no device pools");
+    if (is_b8(kv->o)) return block_unsupported(kv, "ni_kv_step_noalloc");
     if (!kv->scratch)
         return kv->fail(NI_ERR_HIP, "ni_kv_step_noalloc: no scratch on this device (hipGetSymbolAddress: %s)",
                         hipGetErrorString(kv->scratch_err));
@@ -2614,6 +2818,7 @@ int ni_kv_step_noalloc(ni_kv* kv, const ni_work* work, uint32_t n_work, const fl
 int ni_kv_step_begin(ni_kv* kv, const ni_work* work, uint32_t n_work, uint32_t split_tokens) {
     if (!kv) return NI_ERR_BAD_ARG;
     if (kv->step.open) return kv->fail(NI_ERR_BAD_ARG, "a step is already open");
+    if (is_b8(kv->o)) return block_unsupported(kv, "ni_kv_step_begin");
     if (n_work && !work) return kv->fail(NI_ERR_BAD_ARG, "work is NULL");
     if (int rc = prepare_step(kv, work, n_work)) return rc;
     // Partitions and launch shape for one layer per launch.
@@ -2841,9 +3046,44 @@ static int build_step_plan(ni_kv* kv, const ni_work* work, uint32_t n_work, uint
     return plan_attention(kv, split_tokens, n_lay);
 }
 
+// The launch half of ni_kv_step on a block-scaled pool: all rows appended, then
+// the queried ones attended.
+static int block_step(ni_kv* kv, const ni_work* work, uint32_t n_work, const float* q, const float* k, const float* v,
+                      int64_t row_stride, int64_t layer_stride, float* out, int64_t out_row_stride,
+                      int64_t out_layer_stride, uint32_t split_tokens, hipStream_t stream) try {
+    if (split_tokens % kPage != 0)
+        return kv->fail(NI_ERR_BAD_ARG, "split_tokens %u must be a multiple of %u", split_tokens, kPage);
+    const uint32_t n_lay = kv->o.n_layer;
+    auto& rows = kv->step_rows;
+    auto& at = kv->step_at;
+    rows.clear();
+    for (uint32_t w = 0; w < n_work; w++)
+        for (uint32_t i = 0; i < work[w].n_new; i++) rows.push_back({work[w].seq, kv->seq_len[work[w].seq] + i});
+    if (int rc = block_append(kv, 0, n_lay, rows.data(), (uint32_t)rows.size(), k, v, row_stride, layer_stride, stream))
+        return rc;
+    at.clear();
+    for (uint32_t w = 0, row = 0; w < n_work; row += work[w++].n_new)
+        for (uint32_t i = work[w].n_new - work[w].n_query; i < work[w].n_new; i++) {
+            rows[at.size()] = rows[row + i];
+            at.push_back(row + i);
+        }
+    if (at.empty()) return NI_OK;
+    return block_attention(kv, 0, n_lay, q, row_stride, layer_stride, rows.data(), at.data(), (uint32_t)at.size(), out,
+                           out_row_stride, out_layer_stride, split_tokens, stream);
+} catch (const std::bad_alloc&) {
+    return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
+}
+
 static int enqueue_step(ni_kv* kv, const ni_work* work, uint32_t n_work, const float* q, const float* k,
                         const float* v, int64_t row_stride, int64_t layer_stride, float* out, int64_t out_row_stride,
                         int64_t out_layer_stride, uint32_t split_tokens, hipStream_t stream) {
+    if (is_b8(kv->o)) {
+        if (int rc = block_step(kv, work, n_work, q, k, v, row_stride, layer_stride, out, out_row_stride, out_layer_stride,
+                                split_tokens, stream))
+            return rc;
+        for (uint32_t w = 0; w < n_work; w++) kv->seq_len[work[w].seq] += work[w].n_new;
+        return NI_OK;
+    }
     if (int rc = build_step_plan(kv, work, n_work, split_tokens, kv->o.n_layer)) return rc;
     int rc = run_plan(kv, 0, kv->o.n_layer, k, v, row_stride, layer_stride, q, row_stride, layer_stride, out,
                       out_row_stride, out_layer_stride, stream);

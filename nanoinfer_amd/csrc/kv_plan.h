@@ -122,6 +122,9 @@ struct PoolGeom {
     // Q8 blocks (kv8.metal:15-48): [16][head_dim] int8, then 16 f32 scales
     // (amax / 127 per position) at byte 16 * head_dim.
     uint32_t q8;
+    // Block-scaled pools: the byte of a page where its scales begin
+    // ([n_head][K, V] f32); 0 for the others.
+    uint32_t b8;
 };
 
 // A page to copy, over all layers: its first `rows` positions (kPage: the whole page).
@@ -134,6 +137,37 @@ struct PageCopyLaunch {
     const uint8_t* plan;  // PageCopy[n] (unused when inline)
     uint32_t n;
     uint32_t n_layer;
+};
+
+// Rows that one call appends to one page of a block-scaled pool: the slots set
+// in the low 16 bits of `slots`, taken in order from input rows src, src + 1,
+// ..., or (kListed) from those at list[src], list[src + 1], ....
+struct BlockAppend {
+    uint32_t page, src, slots;
+};
+constexpr uint32_t kListed = 1u << 16;
+
+struct BlockAppendLaunch {
+    PoolGeom pool;
+    const float* k;
+    const float* v;
+    int64_t row_stride, layer_stride;
+    const uint8_t* plan;  // BlockAppend[n], then the list at off_list
+    uint32_t off_list;
+    uint32_t n;
+    uint32_t layer0, n_lay;
+};
+
+// f32 values of rows (AppendEntry, src_row = output row), any pool.
+struct ValuesLaunch {
+    PoolGeom pool;
+    float* k_out;
+    float* v_out;
+    int64_t row_stride, layer_stride;
+    const uint8_t* plan;
+    uint32_t off_entries;
+    uint32_t n_rows;
+    uint32_t layer0, n_lay;
 };
 
 struct AppendLaunch {
@@ -280,6 +314,9 @@ struct LaunchTiming {
 
 hipError_t launch_append(const AppendLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s,
                          const LaunchTiming& t = {});
+hipError_t launch_block_append(const BlockAppendLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s,
+                               const LaunchTiming& t = {});
+hipError_t launch_gather_values(const ValuesLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s);
 // (no source is a destination of the same launch)
 hipError_t launch_page_copy(const PageCopyLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s);
 hipError_t launch_gather(const GatherLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s);

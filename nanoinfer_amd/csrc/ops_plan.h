@@ -124,6 +124,9 @@ struct PrefixLaunch {
 };
 hipError_t launch_prefix_attention(const PrefixLaunch& a, const void* inline_plan, uint32_t inline_bytes,
                                    hipStream_t s, const LaunchTiming& t = {});
+// The same items (never wide, never joining partials) over a block-scaled pool.
+hipError_t launch_block_attention(const PrefixLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s,
+                                  const LaunchTiming& t = {});
 hipError_t launch_prefix_merge(const PrefixLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s,
                                const LaunchTiming& t = {});
 

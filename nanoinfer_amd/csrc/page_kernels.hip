@@ -3,8 +3,8 @@
 //
 // A page is one contiguous run of bytes in each layer, so a whole page is copied
 // as it lies, in 16-byte units.  Of a page that a sequence ends in, only the rows
-// before the end are: of each (head, K|V) block the units of those rows, which lie
-// together, and their scales.
+// before the end are: of each (head, K|V) block the units of those rows and their
+// scales.
 #include "kv_device.h"
 
 namespace ni {
@@ -32,10 +32,13 @@ __global__ __launch_bounds__(kCT) void page_copy_kernel(const PageCopyLaunch a, 
     uint8_t* const base = reinterpret_cast<uint8_t*>(a.pool.k + (uint64_t)layer * a.pool.layer_halves);
     const u32x4* const src = reinterpret_cast<const u32x4*>(base + (uint64_t)c.src * g.page * 16);
     u32x4* const dst = reinterpret_cast<u32x4*>(base + (uint64_t)c.dst * g.page * 16);
-    const uint32_t scales = c.rows < kPage && a.pool.q8 ? (c.rows + 3) / 4 : 0;  // units with scales of a block's rows
-    const uint32_t values = c.rows < kPage ? g.values / kPage * c.rows : g.values;
-    const uint32_t per = values + scales;
-    const uint32_t n = c.rows < kPage ? per * g.blocks : g.page;
+    const bool part = c.rows < kPage;
+    // Of a part: units of a block's rows, and those with their scales (block-scaled: of
+    // a run of 64 dims of K and of V, four positions of V to a unit; its scales end the page).
+    const uint32_t values = part ? a.pool.b8 ? 4 * c.rows + 16 * ((c.rows + 3) / 4) : g.values / kPage * c.rows : 0;
+    const uint32_t scales = part && a.pool.q8 ? (c.rows + 3) / 4 : 0;
+    const uint32_t per = values + scales, runs = a.pool.b8 ? g.blocks / 2 * (g.block / 64) : g.blocks;
+    const uint32_t n = part ? per * runs + (a.pool.b8 ? (a.pool.n_head + 1) / 2 : 0) : g.page;
     u32x4 x[kUnits];
     uint32_t at[kUnits], words[kUnits];  // unit of the page; words of it to copy
 #pragma unroll
@@ -43,10 +46,17 @@ __global__ __launch_bounds__(kCT) void page_copy_kernel(const PageCopyLaunch a, 
         const uint32_t u = tile * kTileUnits + j * kCT + threadIdx.x;
         at[j] = u;
         words[j] = u < n ? 4 : 0;
-        if (c.rows < kPage && u < n) {
+        if (part && u < n) {
             const uint32_t b = u / per, w = u - b * per;
-            at[j] = b * g.block + (w < values ? w : g.values + w - values);
-            if (w >= values) words[j] = min(4u, c.rows - 4 * (w - values));
+            if (!a.pool.b8) {
+                at[j] = b * g.block + (w < values ? w : g.values + w - values);
+                if (w >= values) words[j] = min(4u, c.rows - 4 * (w - values));
+            } else if (b < runs) {
+                const uint32_t nb = g.block / 64, head = b / nb, x16 = w / c.rows;
+                at[j] = (2 * head * nb + b % nb) * 64 + (w < 4 * c.rows ? x16 * 16 + w - x16 * c.rows : nb * 64 + w - 4 * c.rows);
+            } else {
+                at[j] = a.pool.b8 / 16 + u - per * runs;
+            }
         }
         if (words[j]) x[j] = __builtin_nontemporal_load(src + at[j]);
     }
