@@ -131,7 +131,7 @@ typedef struct ni_work {
 int ni_kv_create(const ni_kv_opts* opts, ni_kv** out);
 void ni_kv_destroy(ni_kv* kv);
 /* Text of the last failure on this handle; with kv == NULL, of the last
- * failed ni_kv_create, ni_attention, ni_rotary_* or ni_verify_* on this thread. */
+ * failed ni_kv_create, ni_attention, ni_rotary_*, ni_verify_* or ni_beam_* on this thread. */
 const char* ni_kv_last_error(const ni_kv* kv);
 /* Bytes of one page over all layers, K and V (BatchEngine::kv_block_bytes, batch.rs:107-109). */
 size_t ni_kv_page_bytes(const ni_kv* kv);
@@ -464,6 +464,34 @@ int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stri
                      int64_t drafted_stride, const int32_t* n_drafts, const float* accept_u, int64_t accept_stride,
                      const float* sample_u, uint32_t n_seq, uint32_t n_draft, uint32_t vocab, int32_t* accepted,
                      int32_t* tokens, int64_t tokens_stride, void* workspace, size_t workspace_bytes, ni_stream stream);
+
+/* Beam search's selection: the k best continuations of each search over its
+ * beams and the vocabulary, best first.  The total of beam w and token v is
+ * scores[b][w] + logits[b][w][v] - log(sum over u of exp(logits[b][w][u])); totals
+ * are compared in 64 bits (the logarithm is 2e-6 off at most, ~1e-8 as a rule), equal ones go to
+ * the lowest (beam, token).  A beam that is finished (finished[b][w] != 0; NULL:
+ * none is) has one candidate, pad_token, of total scores[b][w]; its logits are
+ * not read, nor are those of a beam whose score is -infinity.  Totals of -infinity (banned
+ * tokens) and NaN are no candidates; a NaN logit weighs nothing in the sum, and
+ * a beam with a logit of +infinity has no candidates.  Answer i of search b:
+ * out_scores[b][i], parents[b][i] (the beam) and tokens[b][i]; where there
+ * are fewer candidates -infinity, -1 and -1.  out_history (NULL: none): row b *
+ * k + i is the n_history entries of the parent's row of history (row b * n_beam +
+ * w) and the token (-1 throughout where there is none).
+ * logits are of `dtype`, strides count elements, rows are dense; history_stride
+ * and out_history_stride lie between rows; scores, finished, out_scores, parents and tokens are dense.
+ * n_beam and k are at most 64, vocab 2^26.  The outputs' extents share no memory with those of
+ * the inputs or each other.
+ * workspace: ni_beam_workspace(n_search, n_beam, vocab) bytes of device memory,
+ * 16-byte aligned, that no other work on the GPU uses meanwhile.  Enqueued on
+ * `stream`; failures are reported by ni_kv_last_error(NULL).  The cache follows by
+ * ni_kv_reorder. */
+size_t ni_beam_workspace(uint32_t n_search, uint32_t n_beam, uint32_t vocab);
+int ni_beam_select(uint32_t dtype, const void* logits, int64_t search_stride, int64_t beam_stride, const float* scores,
+                   const int32_t* finished, uint32_t pad_token, uint32_t n_search, uint32_t n_beam, uint32_t vocab,
+                   uint32_t k, float* out_scores, int32_t* parents, int32_t* tokens, const int32_t* history,
+                   int64_t history_stride, uint32_t n_history, int32_t* out_history, int64_t out_history_stride,
+                   void* workspace, size_t workspace_bytes, ni_stream stream);
 
 /* Wait for all work this handle enqueued on `stream`; afterwards no call of
  * the handle waits for that work, and `stream` may be destroyed. */

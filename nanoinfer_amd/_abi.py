@@ -178,6 +178,11 @@ def _declare(L):
     L.ni_verify_drafts.restype = C.c_int
     L.ni_verify_drafts.argtypes = [_u32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _u32, _u32,
                                    _u32, _vp, _vp, _i64, _vp, C.c_size_t, _vp]
+    L.ni_beam_workspace.restype = C.c_size_t
+    L.ni_beam_workspace.argtypes = [_u32, _u32, _u32]
+    L.ni_beam_select.restype = C.c_int
+    L.ni_beam_select.argtypes = [_u32, _vp, _i64, _i64, _vp, _vp, _u32, _u32, _u32, _u32, _u32, _vp, _vp, _vp, _vp, _i64,
+                                 _u32, _vp, _i64, _vp, C.c_size_t, _vp]
     L.ni_kv_sync.restype = C.c_int
     L.ni_kv_sync.argtypes = [_vp, _vp]
     L.ni_kv_pools.restype = C.c_int

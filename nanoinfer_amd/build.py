@@ -25,7 +25,7 @@ DRIVE_EXE = os.path.join(HERE, "ni_drive")
 
 SOURCES = [os.path.join(CSRC, f) for f in ("kv_kernels.hip", "rotary_kernels.hip", "prefix_kernels.hip",
                                            "verify_kernels.hip", "page_kernels.hip",
-                                           "block_kernels.hip", "kv_host.cpp", "ops_host.cpp")]
+                                           "block_kernels.hip", "beam_kernels.hip", "kv_host.cpp", "ops_host.cpp")]
 HEADERS = [os.path.join(CSRC, f) for f in ("kv_plan.h", "kv_device.h", "ops_plan.h")] + \
     [os.path.join(INCLUDE, "nanoinfer_kv.h")]
 DRIVER_SOURCES = [os.path.join(CSRC, "drivers.cpp")]

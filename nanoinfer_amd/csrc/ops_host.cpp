@@ -1,6 +1,6 @@
 // ops_host.cpp -- C ABI of the operators that need no cache handle: rotary
-// positions over contiguous rows (ni_rotary_*) and the verification of drafted
-// tokens (ni_verify_*).  Checks come before anything touches the device.
+// positions over contiguous rows (ni_rotary_*), the verification of drafted
+// tokens (ni_verify_*) and beam search's selection (ni_beam_*).  Checks come before anything touches the device.
 #include <hip/hip_runtime_api.h>
 
 #include <algorithm>
@@ -39,6 +39,13 @@ bool share(const Rows& a, const Rows& b, uint32_t n) {
     }
     return false;
 }
+
+// The bytes from an array's first value to its last.
+struct Span {
+    const char* p;
+    uint64_t n;
+    bool meets(const Span& o) const { return n && o.n && p < o.p + o.n && o.p < p + n; }
+};
 
 }  // namespace
 
@@ -222,6 +229,108 @@ int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stri
     a.per = (uint32_t)std::min<uint64_t>(std::max<uint64_t>(chunks / (8ull * device_cus()), 1), 16);
     const hipError_t e = launch_verify(a, (hipStream_t)stream);
     if (e != hipSuccess) return call_error(NI_ERR_HIP, "verification launch failed: %s", hipGetErrorString(e));
+    return NI_OK;
+}
+
+size_t ni_beam_workspace(uint32_t n_search, uint32_t n_beam, uint32_t vocab) {
+    const uint64_t rows = (uint64_t)n_search * n_beam;
+    return rows * (((uint64_t)vocab + kBeamChunk - 1) / kBeamChunk * sizeof(BeamSum) +
+                   ((uint64_t)vocab + kBeamGroup - 1) / kBeamGroup * sizeof(float));
+}
+
+int ni_beam_select(uint32_t dtype, const void* logits, int64_t search_stride, int64_t beam_stride, const float* scores,
+                   const int32_t* finished, uint32_t pad_token, uint32_t n_search, uint32_t n_beam, uint32_t vocab,
+                   uint32_t k, float* out_scores, int32_t* parents, int32_t* tokens, const int32_t* history,
+                   int64_t history_stride, uint32_t n_history, int32_t* out_history, int64_t out_history_stride,
+                   void* workspace, size_t workspace_bytes, ni_stream stream) {
+    if (dtype > NI_BF16) return call_error(NI_ERR_BAD_ARG, "unknown type %u", dtype);
+    if (n_search == 0 || k == 0) return NI_OK;
+    if (n_beam == 0 || n_beam > kBeamMax) return call_error(NI_ERR_BAD_ARG, "%u beams: 1..%u", n_beam, kBeamMax);
+    if (k > kBeamMax) return call_error(NI_ERR_BAD_ARG, "k %u: at most %u", k, kBeamMax);
+    if (vocab == 0 || vocab > (1u << kBeamTokenBits))
+        return call_error(NI_ERR_BAD_ARG, "vocab %u must be 1..2^%u", vocab, kBeamTokenBits);
+    if (finished && pad_token >= vocab) return call_error(NI_ERR_BAD_ARG, "pad_token %u is not in the vocabulary", pad_token);
+    const uint64_t chunks = ((uint64_t)vocab + kBeamChunk - 1) / kBeamChunk, rows = (uint64_t)n_search * n_beam;
+    const bool hist = out_history != nullptr;
+    if (n_history > (1u << 30)) return call_error(NI_ERR_BAD_ARG, "n_history %u too large", n_history);
+    const struct {
+        const char* name;
+        const void* p;
+        bool needed;
+        uintptr_t align;
+        int64_t stride;
+    } args[] = {{"logits", logits, true, type_bytes(dtype), std::min(search_stride, beam_stride)},
+                {"scores", scores, true, 4, 0},
+                {"finished", finished, false, 4, 0},
+                {"out_scores", out_scores, true, 4, 0},
+                {"parents", parents, true, 4, 0},
+                {"tokens", tokens, true, 4, 0},
+                {"history", history, hist && n_history > 0, 4, hist ? history_stride : 0},
+                {"out_history", out_history, false, 4, hist ? out_history_stride : 0}};
+    for (const auto& x : args) {
+        if (x.needed && !x.p) return call_error(NI_ERR_BAD_ARG, "%s is NULL", x.name);
+        if (!aligned(x.p, x.align)) return call_error(NI_ERR_BAD_ARG, "%s is not aligned to its type", x.name);
+        if (x.stride < 0) return call_error(NI_ERR_BAD_ARG, "%s must have non-negative strides", x.name);
+    }
+    const uint64_t outs = (uint64_t)n_search * k;
+    if (hist && outs > 1 && out_history_stride < (int64_t)n_history + 1)
+        return call_error(NI_ERR_BAD_ARG, "out_history's rows overlap: the stride must be at least %u", n_history + 1);
+    const size_t need = ni_beam_workspace(n_search, n_beam, vocab);
+    if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
+        return call_error(NI_ERR_BAD_ARG, "workspace must be %zu bytes, 16-byte aligned", need);
+    // (the workgroup of one search reads its beams while another's writes its answers)
+    const uint64_t per = std::min<uint64_t>(std::max<uint64_t>(rows * chunks / (8ull * device_cus()), 1), 16);
+    const uint64_t runs = (chunks + per - 1) / per;
+    // (a launch holds less than 2^32 threads)
+    if (rows * runs >= (1ull << 24) || n_search >= (1u << 22))
+        return call_error(NI_ERR_BAD_ARG, "%u searches of %u beams: too many for one call", n_search, n_beam);
+    const auto span = [](const void* p, uint64_t n, int64_t stride, uint64_t width) {
+        return Span{static_cast<const char*>(p), p ? 4 * ((n - 1) * (uint64_t)stride + width) : 0};
+    };
+    typedef unsigned __int128 u128;
+    const u128 read = (u128)(n_search - 1) * (uint64_t)search_stride + (u128)(n_beam - 1) * (uint64_t)beam_stride + vocab;
+    if (read >= (u128)1 << 60) return call_error(NI_ERR_BAD_ARG, "logits' strides are too large");
+    const Span in[] = {span(scores, 1, 0, rows), span(finished, 1, 0, rows),
+                       span(hist && n_history ? history : nullptr, rows, history_stride, n_history),
+                       Span{static_cast<const char*>(logits), (uint64_t)read * type_bytes(dtype)}};
+    const Span out[] = {span(out_scores, 1, 0, outs), span(parents, 1, 0, outs), span(tokens, 1, 0, outs),
+                        span(out_history, outs, out_history_stride, (uint64_t)n_history + 1)};
+    const char* const in_name[] = {"scores", "finished", "history", "logits"};
+    const char* const out_name[] = {"out_scores", "parents", "tokens", "out_history"};
+    for (int i = 0; i < 4; i++) {
+        for (int j = 0; j < 4; j++)
+            if (out[i].meets(in[j]))
+                return call_error(NI_ERR_BAD_ARG, "%s may not share memory with %s", out_name[i], in_name[j]);
+        for (int j = 0; j < i; j++)
+            if (out[i].meets(out[j]))
+                return call_error(NI_ERR_BAD_ARG, "%s may not share memory with %s", out_name[i], out_name[j]);
+    }
+    BeamLaunch a{};
+    a.logits = logits;
+    a.search_stride = search_stride;
+    a.beam_stride = beam_stride;
+    a.scores = scores;
+    a.finished = finished;
+    a.history = history;
+    a.history_stride = history_stride;
+    a.out_history_stride = out_history_stride;
+    a.out_scores = out_scores;
+    a.parents = parents;
+    a.tokens = tokens;
+    a.out_history = out_history;
+    a.sums = static_cast<BeamSum*>(workspace);
+    a.groups = reinterpret_cast<float*>(a.sums + rows * chunks);
+    a.n_search = n_search;
+    a.n_beam = n_beam;
+    a.vocab = vocab;
+    a.k = k;
+    a.pad = pad_token;
+    a.n_history = n_history;
+    a.n_groups = (vocab + kBeamGroup - 1) / kBeamGroup;
+    a.dtype = dtype;
+    a.per = (uint32_t)per;
+    const hipError_t e = launch_beam(a, (hipStream_t)stream);
+    if (e != hipSuccess) return call_error(NI_ERR_HIP, "beam selection launch failed: %s", hipGetErrorString(e));
     return NI_OK;
 }
 

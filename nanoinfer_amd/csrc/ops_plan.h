@@ -1,6 +1,6 @@
-// ops_plan.h -- what the host hands to the kernels of the rotary, shared-prefix
-// and verification operators (rotary_kernels.hip, prefix_kernels.hip,
-// verify_kernels.hip).  The host checks every index and size before it
+// ops_plan.h -- what the host hands to the kernels of the rotary, shared-prefix,
+// verification and beam operators (rotary_kernels.hip, prefix_kernels.hip,
+// verify_kernels.hip, beam_kernels.hip).  The host checks every index and size before it
 // launches; the kernels check what only the device can see (token ids, draft
 // counts).
 #pragma once
@@ -153,6 +153,35 @@ struct VerifyLaunch {
     uint32_t per;  // chunks one workgroup of the sums adds up
 };
 hipError_t launch_verify(const VerifyLaunch& a, hipStream_t s);
+
+// -------------------------------------------------------- beam selection
+
+constexpr uint32_t kBeamChunk = 2048;      // vocabulary entries a workgroup takes at a time
+constexpr uint32_t kBeamGroup = 128;       // entries whose largest is kept
+constexpr uint32_t kBeamMax = 64;          // beams of a search, and answers
+constexpr uint32_t kBeamTokenBits = 26;    // (beam, token) in 32 bits
+
+struct BeamSum {  // of the run of chunks of one workgroup: sum of exp(logit - top)
+    float top, sum;
+};
+
+struct BeamLaunch {
+    const void* logits;
+    int64_t search_stride, beam_stride;
+    const float* scores;
+    const int32_t* finished;  // null: none is
+    const int32_t* history;
+    int64_t history_stride, out_history_stride;
+    float* out_scores;
+    int32_t* parents;
+    int32_t* tokens;
+    int32_t* out_history;  // null: no histories
+    float* groups;         // [n_search * n_beam][n_groups]: the largest logit of each group
+    BeamSum* sums;         // [n_search * n_beam][chunks]: one of each run, first
+    uint32_t n_search, n_beam, vocab, k, pad, n_history, n_groups, dtype;
+    uint32_t per;  // chunks to a workgroup
+};
+hipError_t launch_beam(const BeamLaunch& a, hipStream_t s);
 
 // ------------------------------------------------------------------ errors
 
