@@ -480,7 +480,7 @@ int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stri
  * w) and the token (-1 throughout where there is none).
  * logits are of `dtype`, strides count elements, rows are dense; history_stride
  * and out_history_stride lie between rows; scores, finished, out_scores, parents and tokens are dense.
- * n_beam and k are at most 64, vocab 2^26.  The outputs' extents share no memory with those of
+ * n_beam and k are at most 64, vocab 2^25.  The outputs' extents share no memory with those of
  * the inputs or each other.
  * workspace: ni_beam_workspace(n_search, n_beam, vocab) bytes of device memory,
  * 16-byte aligned, that no other work on the GPU uses meanwhile.  Enqueued on

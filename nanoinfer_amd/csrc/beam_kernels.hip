@@ -15,6 +15,9 @@
 // running maximum (1.6e-7 of a term that counts), eight terms are added in f32 (2^-21),
 // all other sums and the logarithm run in 64 bits: with the maximum's few raises, 1e-7
 // each, a normaliser is 2e-6 off at most, ~1e-8 as a rule.
+#include <cfloat>
+#include <type_traits>
+
 #include "kv_device.h"
 #include "ops_plan.h"
 
@@ -68,8 +71,8 @@ __global__ __launch_bounds__(kBT) void beam_scan_kernel(const BeamLaunch a, cons
     double s = 0.;
     for (uint32_t chunk = chunk0; chunk < chunk1; chunk++) {
         Eight<T> next = cur;
-        const uint32_t v = chunk * kBeamChunk + threadIdx.x * kBE;
-        if (chunk + 1 < chunk1) next.load(x, v + kBeamChunk, a.vocab);
+        const uint32_t p = chunk * kBeamChunk + threadIdx.x * kBE;
+        if (chunk + 1 < chunk1) next.load(x, p + kBeamChunk, a.vocab);
         float y[kBE], top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < (int)kBE; i++) {
@@ -88,7 +91,7 @@ __global__ __launch_bounds__(kBT) void beam_scan_kernel(const BeamLaunch a, cons
         top = fmaxf(top, dpp_move<0x4e>(top));
         top = fmaxf(top, dpp_move<0x141>(top));
         top = fmaxf(top, dpp_move<0x140>(top));
-        if (lane % kGroupLanes == 0 && v < a.vocab) groups[v / kBeamGroup] = top;
+        if (lane % kGroupLanes == 0 && p / kBeamGroup < a.n_groups) groups[p / kBeamGroup] = top;
         cur = next;
     }
     // The workgroup's maximum and sum.
@@ -116,186 +119,292 @@ struct Cand {
     __device__ __forceinline__ bool before(double t, uint32_t i) const { return total > t || (total == t && index < i); }
 };
 
-__device__ __forceinline__ Cand read_lane(const Cand& c, int l) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, c.total);
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, l), hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), l);
-    return Cand{__builtin_bit_cast(double, (uint64_t)hi << 32 | lo), (uint32_t)__builtin_amdgcn_readlane((int)c.index, l)};
-}
-// The lane before's value (lane 0: its own).
-__device__ __forceinline__ uint32_t lane_before(uint32_t x) {
-    return (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x138, 0xf, 0xf, false);  // wave_shr:1
-}
+constexpr uint32_t kPT = 1024;          // threads of a pick
+constexpr uint32_t kPU = 8;             // candidates a thread holds at a time
+constexpr uint32_t kList = 1024;        // candidates that are ranked at once
+constexpr uint32_t kSetLanes = 8, kSets = kPT / kSetLanes;  // sets of candidates whose best are compared
+static_assert(kPT * kPU == kBeamMax * kBeamGroup, "the entries of the chosen groups are looked at once");
 
-// A wave's best candidates so far, best first, one a lane (the first k are right).
-struct Best {
-    Cand c = {-INFINITY, 0xffffffffu};
-    Cand last = {-INFINITY, 0xffffffffu};  // the k-th
-    // Every lane offers one.
-    __device__ __forceinline__ void offer(const Cand& x, uint32_t k) {
-        uint64_t in = __ballot(x.total > -INFINITY && x.before(last.total, last.index));
-        const uint32_t lane = threadIdx.x & 63u;
-        while (in) {
-            const int l = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)in) - 1);
-            in &= in - 1;
-            const Cand y = read_lane(x, l);
-            if (!y.before(last.total, last.index)) continue;
-            const uint32_t at = (uint32_t)__popcll(__ballot(c.before(y.total, y.index)));
-            const uint64_t bits = __builtin_bit_cast(uint64_t, c.total);
-            const uint64_t up = (uint64_t)lane_before((uint32_t)(bits >> 32)) << 32 | lane_before((uint32_t)bits);
-            const uint32_t up_i = lane_before(c.index);
-            if (lane > at) {
-                c.total = __builtin_bit_cast(double, up);
-                c.index = up_i;
-            } else if (lane == at) {
-                c = y;
-            }
-            last = read_lane(c, (int)k - 1);
-        }
-    }
+struct Pick {
+    double totals[kList];
+    uint32_t indices[kList];
+    float tops[kSets];
+    double best[kBeamMax];  // the answer so far, best first
+    uint32_t best_index[kBeamMax];
+    uint32_t bound;  // as an integer of the same order
+    uint32_t n, counts[3];
 };
 
-constexpr uint32_t kPT = 1024;          // threads of a pick
-constexpr uint32_t kPW = kPT / 64;
+// Sum over groups of `lanes` lanes, a power of two up to 16.
+__device__ __forceinline__ uint32_t lanes_sum(uint32_t x, uint32_t lanes) {
+    const auto moved = [&](auto c) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(c)::value, 0xf, 0xf, false); };
+    if (lanes >= 2) x += moved(std::integral_constant<int, 0xb1>{});
+    if (lanes >= 4) x += moved(std::integral_constant<int, 0x4e>{});
+    if (lanes >= 8) x += moved(std::integral_constant<int, 0x141>{});
+    if (lanes >= 16) x += moved(std::integral_constant<int, 0x140>{});
+    return x;
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
+    x = lanes_sum(x, 16);
+    return (uint32_t)(__builtin_amdgcn_readlane((int)x, 0) + __builtin_amdgcn_readlane((int)x, 16) +
+                      __builtin_amdgcn_readlane((int)x, 32) + __builtin_amdgcn_readlane((int)x, 48));
+}
+__device__ __forceinline__ float wave_top(float x) {
+    x = fmaxf(x, dpp_move<0xb1>(x));
+    x = fmaxf(x, dpp_move<0x4e>(x));
+    x = fmaxf(x, dpp_move<0x141>(x));
+    x = fmaxf(x, dpp_move<0x140>(x));
+    return rows4_max(x);
+}
+// Floats as integers of the same order.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b >> 31 ? ~b : b | 1u << 31;
+}
+__device__ __forceinline__ float from_order(uint32_t o) { return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o); }
 
-// Where candidate sits among all waves' first k (those without a total behind the others): every thread of the
-// workgroup takes part.  totals, indices: kPW * k entries; ranks as many counters, zeroed.
-__device__ __forceinline__ void rank_all(const double* totals, const uint32_t* indices, uint32_t* ranks, uint32_t n) {
-    // 2^j threads to a candidate, each against its share of the others
-    uint32_t parts = 1;
-    while (parts * 2 * n <= kPT) parts *= 2;
-    const uint32_t i = threadIdx.x / parts, part = threadIdx.x - i * parts;
-    if (i < n) {
-        const Cand me = {totals[i], indices[i]};
-        uint32_t before = 0;
-        for (uint32_t j = part; j < n; j += parts) before += Cand{totals[j], indices[j]}.before(me.total, me.index) ? 1u : 0u;
-        if (before) atomicAdd(&ranks[i], before);
+// The first k of the n listed candidates into sh.best, in order: a candidate's place
+// is the number of those before it.
+__device__ __forceinline__ void rank_list(Pick& sh, uint32_t n, uint32_t k) {
+    uint32_t parts = 1;  // threads to a candidate, each against its share of the others
+    while (parts < 16 && parts * 2 * n <= kPT) parts *= 2;
+    const uint32_t i = threadIdx.x / parts, part = threadIdx.x % parts;
+    const Cand me = i < n ? Cand{sh.totals[i], sh.indices[i]} : Cand{0., 0u};
+    uint32_t rank = 0;
+    if (i < n)
+        for (uint32_t j = part; j < n; j += parts) rank += Cand{sh.totals[j], sh.indices[j]}.before(me.total, me.index) ? 1u : 0u;
+    rank = lanes_sum(rank, parts);
+    if (i < n && part == 0 && rank < k) {
+        sh.best[rank] = me.total;
+        sh.best_index[rank] = me.index;
     }
+}
+
+// How many candidates of the workgroup are counted; turn: the number of the call.
+__device__ __forceinline__ uint32_t count_all(Pick& sh, uint32_t mine, uint32_t turn) {
+    const uint32_t at = turn % 3;  // (the counter of the call after next is cleared while this one's is read)
+    if (threadIdx.x == 0) sh.counts[(turn + 1) % 3] = 0;
+    mine = wave_sum(mine);
+    if ((threadIdx.x & 63u) == 0 && mine) atomicAdd(&sh.counts[at], mine);
+    __syncthreads();
+    return sh.counts[at];
+}
+
+// Doubles as integers of the same order.
+__device__ __forceinline__ uint64_t order_of(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x + 0.);  // (-0 as 0)
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+
+// The first k of the workgroup's candidates into the list, where more are left than it
+// holds: the k-th total bit by bit, then the last index among its equals.
+__device__ __forceinline__ void pick_equal(Pick& sh, const double (&t)[kPU], const uint32_t (&index)[kPU], uint32_t k) {
+    uint64_t key[kPU], kth = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < kPU; j++) key[j] = t[j] > -INFINITY ? order_of(t[j]) : 0;
+    if (threadIdx.x < 3) sh.counts[threadIdx.x] = 0;
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    uint32_t turn = 0;
+    for (int bit = 63; bit >= 0; bit--) {
+        const uint64_t trial = kth | 1ull << bit;
+        uint32_t mine = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kPU; j++) mine += key[j] >= trial ? 1u : 0u;
+        if (count_all(sh, mine, turn++) >= k) kth = trial;
+    }
+    uint32_t above = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < kPU; j++) above += key[j] > kth ? 1u : 0u;
+    const uint32_t equals = k - count_all(sh, above, turn++);
+    uint32_t last = 0xffffffffu;  // the lowest index up to which there are as many
+    for (int bit = 31; bit >= 0; bit--) {
+        const uint32_t trial = last & ~(1u << bit);
+        uint32_t mine = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kPU; j++) mine += key[j] == kth && index[j] <= trial ? 1u : 0u;
+        if (count_all(sh, mine, turn++) >= equals) last = trial;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kPU; j++)
+        if (key[j] > kth || (key[j] == kth && index[j] <= last)) {
+            const uint32_t at = atomicAdd(&sh.n, 1u);
+            sh.totals[at] = t[j];
+            sh.indices[at] = index[j];
+        }
+    __syncthreads();
+}
+
+// Bring the threads' candidates (-infinity: none) into the k best of sh.best, of which
+// `have` are there; gives how many are then.  What lies below the k-th best of the
+// bests of 256 sets of candidates is out; the few others are ranked with the best so
+// far.  Every thread of the workgroup calls it.
+__device__ __forceinline__ uint32_t pick_more(Pick& sh, const double (&t)[kPU], const uint32_t (&index)[kPU], uint32_t k,
+                                              uint32_t have) {
+    double high = t[0];
+#pragma unroll
+    for (uint32_t j = 1; j < kPU; j++) high = fmax(high, t[j]);
+    float top = fminf((float)high, FLT_MAX);
+    top -= fabsf(top) * 0x1p-23f;  // in f32, not above it
+    top = fmaxf(top, dpp_move<0xb1>(top));
+    top = fmaxf(top, dpp_move<0x4e>(top));
+    top = fmaxf(top, dpp_move<0x141>(top));
+    static_assert(kSetLanes == 8 && kSets % (4 * kSetLanes) == 0, "a set is half a row of lanes, each of which compares fours");
+    const uint32_t set = threadIdx.x / kSetLanes, part = threadIdx.x % kSetLanes;
+    if (part == 0) sh.tops[set] = top;
+    if (threadIdx.x == 0) {
+        sh.n = 0;
+        sh.bound = 0;
+    }
+    __syncthreads();
+    uint32_t reach = 0;  // sets whose best is no lower than this one's
+#pragma unroll
+    for (uint32_t j = 0; j < kSets / kSetLanes; j += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(&sh.tops[part * (kSets / kSetLanes) + j]);
+        reach += (x.x >= top ? 1u : 0u) + (x.y >= top ? 1u : 0u) + (x.z >= top ? 1u : 0u) + (x.w >= top ? 1u : 0u);
+    }
+    reach = lanes_sum(reach, kSetLanes);
+    if (part == 0 && reach >= k) atomicMax(&sh.bound, order_of(top));  // at least k candidates lie there or above
+    __syncthreads();
+    double bound = (double)from_order(sh.bound);
+    if (have == k) bound = fmax(bound, sh.best[k - 1]);
+    constexpr uint32_t kRoom = kList - kBeamMax;
+#pragma unroll
+    for (uint32_t j = 0; j < kPU; j++)
+        if (t[j] > -INFINITY && t[j] >= bound) {
+            const uint32_t at = atomicAdd(&sh.n, 1u);
+            if (at < kRoom) {
+                sh.totals[at] = t[j];
+                sh.indices[at] = index[j];
+            }
+        }
+    __syncthreads();
+    if (sh.n > kRoom) {
+        __syncthreads();  // (everyone has seen it)
+        pick_equal(sh, t, index, k);
+    }
+    const uint32_t n = sh.n + have;
+    if (threadIdx.x < have) {
+        sh.totals[n - have + threadIdx.x] = sh.best[threadIdx.x];
+        sh.indices[n - have + threadIdx.x] = sh.best_index[threadIdx.x];
+    }
+    __syncthreads();
+    rank_list(sh, n, k);
+    __syncthreads();
+    return min(n, k);
 }
 
 // One workgroup a search.
 template <typename T>
 __global__ __launch_bounds__(kPT) void beam_pick_kernel(const BeamLaunch a, const uint32_t chunks, const uint32_t runs) {
-    __shared__ double offset[kBeamMax];           // score - normaliser: what a logit is added to
-    __shared__ double totals[kPW * kBeamMax];
-    __shared__ uint32_t indices[kPW * kBeamMax], ranks[kPW * kBeamMax];
-    __shared__ uint32_t chosen[kBeamMax];         // groups, then (beam, token) of the answers
-    __shared__ double best[kBeamMax];
+    __shared__ Pick sh;
+    __shared__ double offset[kBeamMax];    // score - normaliser: what a logit is added to
+    __shared__ uint32_t chosen[kBeamMax];  // groups
     __shared__ uint8_t done[kBeamMax];
-    const uint32_t b = blockIdx.x, W = a.n_beam, k = a.k, row0 = b * W;
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    for (uint32_t w = wave; w < W; w += kPW) {
+    const uint32_t b = blockIdx.x, W = a.n_beam, k = a.k, row0 = b * W, G = a.n_groups, all = W * G;
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // (G is a multiple of 64: the 64 groups of a wave are of one beam)
+    auto beam_of = [&](uint32_t i) { return (uint32_t)(((uint64_t)(i / 64) * a.beam_magic) >> 32); };
+    auto row_of = [&](uint32_t w) {
+        return static_cast<const T*>(a.logits) + (int64_t)b * a.search_stride + (int64_t)w * a.beam_stride;
+    };
+    // The first groups' largest logits come while the normalisers are found.
+    const float* const groups = a.groups + (uint64_t)row0 * G;
+    float x[kPU];
+    auto load = [&](uint32_t i0) {
+#pragma unroll
+        for (uint32_t j = 0; j < kPU; j++) {
+            const uint32_t i = i0 + j * kPT + threadIdx.x;
+            x[j] = i < all ? groups[i] : -INFINITY;
+        }
+    };
+    load(0);
+    for (uint32_t w = wave; w < W; w += kPT / 64) {
         const float score = a.scores[row0 + w];
         const bool fin = is_finished(a, row0 + w);
         double off = -INFINITY;
         if (!fin && score > -INFINITY) {
             const BeamSum* p = a.sums + (uint64_t)(row0 + w) * chunks;
-            float M = -INFINITY;
-            for (uint32_t r = lane; r < runs; r += 64) M = fmaxf(M, p[r].top);
-            for (int o = 32; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-            double S = 0.;
-            if (fabsf(M) < INFINITY)
-                for (uint32_t r = lane; r < runs; r += 64)
+            const BeamSum none = {-INFINITY, 0.f}, mine = lane < runs ? p[lane] : none;  // the first 64
+            float M = mine.top;
+            for (uint32_t r = lane + 64; r < runs; r += 64) M = fmaxf(M, p[r].top);
+            M = wave_top(M);
+            if (fabsf(M) < INFINITY) {
+                double S = mine.top > -INFINITY ? (double)mine.sum * exp((double)mine.top - (double)M) : 0.;
+                for (uint32_t r = lane + 64; r < runs; r += 64)
                     if (p[r].top > -INFINITY) S += (double)p[r].sum * exp((double)p[r].top - (double)M);
-            for (int o = 32; o > 0; o >>= 1) S += __shfl_xor(S, o);
-            if (fabsf(M) < INFINITY) off = (double)score - ((double)M + log(S));
+                for (int o = 32; o > 0; o >>= 1) S += __shfl_xor(S, o);
+                off = (double)score - ((double)M + log(S));
+            }
         }
         if (lane == 0) {
             offset[w] = fin ? (double)score : off;
             done[w] = fin;
         }
     }
-    for (uint32_t i = threadIdx.x; i < kPW * k; i += kPT) ranks[i] = 0;
-    if (threadIdx.x < k) {
-        chosen[threadIdx.x] = 0xffffffffu;
-        best[threadIdx.x] = -INFINITY;
-    }
     __syncthreads();
-    // The groups.
-    const uint32_t G = a.n_groups;
-    {
-        Best mine;
-        // Of all beams one after another, eight loads at a time; a finished beam has one
-        // candidate, in the pad token's group.
-        const float* g = a.groups + (uint64_t)row0 * G;
-        constexpr int U = 8;
-        for (uint32_t i0 = threadIdx.x; i0 < W * G + threadIdx.x; i0 += U * kPT) {
-            float x[U];
+    uint32_t have = 0;
+    double t[kPU];
+    uint32_t index[kPU];
+    for (uint32_t i0 = 0; i0 < all; i0 += kPT * kPU) {
+        if (i0 > 0) load(i0);
 #pragma unroll
-            for (int j = 0; j < U; j++) x[j] = i0 + j * kPT < W * G ? g[i0 + j * kPT] : -INFINITY;
-#pragma unroll
-            for (int j = 0; j < U; j++) {
-                const uint32_t i = i0 + j * kPT, w = min(i / G, W - 1);
+        for (uint32_t j = 0; j < kPU; j++) {
+            const uint32_t at = i0 + j * kPT + wave * 64, i = at + lane;
+            index[j] = i;
+            t[j] = -INFINITY;
+            if (at < all) {
+                const uint32_t w = beam_of(at);
                 const double off = offset[w];
-                double t = off > -INFINITY ? off + (double)x[j] : -INFINITY;  // (the groups of others were not written)
-                if (done[w]) t = i - w * G == a.pad / kBeamGroup ? off : -INFINITY;
-                if (i >= W * G) t = -INFINITY;
-                mine.offer(Cand{t, i}, k);
+                // (what was not written -- groups past a row, of a beam that is finished or has no
+                // score -- may hold anything; a finished beam has one candidate, in its first)
+                double y = i - w * G < a.n_filled ? off + (double)x[j] : -INFINITY;
+                if (done[w]) y = i == w * G ? off : -INFINITY;
+                if (off > -INFINITY && y > -INFINITY) t[j] = y;
             }
         }
-        if (lane < k) {
-            totals[wave * k + lane] = mine.c.total;
-            indices[wave * k + lane] = mine.c.index;
-        }
+        have = pick_more(sh, t, index, k, have);
     }
+    if (threadIdx.x < k) chosen[threadIdx.x] = threadIdx.x < have ? sh.best_index[threadIdx.x] : 0xffffffffu;
     __syncthreads();
-    rank_all(totals, indices, ranks, kPW * k);
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kPW * k; i += kPT) {
-        if (ranks[i] < k && totals[i] > -INFINITY) chosen[ranks[i]] = indices[i];
-        ranks[i] = 0;
-    }
-    __syncthreads();
-    // Their entries.
-    {
-        Best mine;
-        for (uint32_t c = wave; c < k; c += kPW) {
-            const uint32_t gi = chosen[c];
-            if (gi == 0xffffffffu) continue;
-            const uint32_t w = gi / G, v0 = (gi - w * G) * kBeamGroup;
-            const T* const x = static_cast<const T*>(a.logits) + (int64_t)b * a.search_stride + (int64_t)w * a.beam_stride;
-            const double off = offset[w];
-            T y[kBeamGroup / 64];
+    // The chosen groups' entries, half a group to a wave.
+    static_assert(kBeamGroup == 128, "two waves to a group");
+    T y[kPU];
 #pragma unroll
-            for (uint32_t j = 0; j < kBeamGroup / 64; j++) {
-                const uint32_t v = v0 + 64 * j + lane;
-                y[j] = !done[w] && v < a.vocab ? x[v] : (T)-INFINITY;
-            }
-#pragma unroll
-            for (uint32_t j = 0; j < kBeamGroup / 64; j++) {
-                const uint32_t v = v0 + 64 * j + lane;
-                double t = v < a.vocab ? off + (double)(float)y[j] : -INFINITY;
-                if (done[w]) t = v == a.pad ? off : -INFINITY;
-                mine.offer(Cand{t, w << kBeamTokenBits | v}, k);
-            }
-        }
-        if (lane < k) {
-            totals[wave * k + lane] = mine.c.total;
-            indices[wave * k + lane] = mine.c.index;
+    for (uint32_t j = 0; j < kPU; j++) {
+        const uint32_t c = (j * kPT / 64 + wave) / 2, e = wave % 2 * 64 + lane;
+        y[j] = (T)-INFINITY;
+        index[j] = 0xffffffffu;
+        if (c < have) {
+            const uint32_t g = __builtin_amdgcn_readfirstlane(chosen[c]), w = beam_of(g);
+            const T* const row = row_of(w);
+            const uint32_t v = (g - w * G) * kBeamGroup + e;
+            const bool fin = done[w], in = !fin && v < a.vocab;
+            if (in) y[j] = row[v];
+            if (in || (fin && e == 0)) index[j] = w << kBeamTokenBits | (fin ? a.pad : v);
         }
     }
-    __syncthreads();
-    if (threadIdx.x < k) chosen[threadIdx.x] = 0xffffffffu;
-    rank_all(totals, indices, ranks, kPW * k);
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kPW * k; i += kPT)
-        if (ranks[i] < k && totals[i] > -INFINITY) {
-            chosen[ranks[i]] = indices[i];
-            best[ranks[i]] = totals[i];
-        }
-    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < kPU; j++) {
+        const uint32_t w = index[j] >> kBeamTokenBits;
+        double z = -INFINITY;
+        if (index[j] != 0xffffffffu) z = done[w] ? offset[w] : offset[w] + (double)(float)y[j];
+        t[j] = z > -INFINITY ? z : -INFINITY;
+    }
+    have = pick_more(sh, t, index, k, 0);
     if (threadIdx.x < k) {
-        const uint32_t c = chosen[threadIdx.x];
-        const bool none = best[threadIdx.x] == -INFINITY;
+        const bool none = threadIdx.x >= have;
+        const uint32_t c = sh.best_index[threadIdx.x];
         const uint64_t o = (uint64_t)b * k + threadIdx.x;
-        a.out_scores[o] = (float)best[threadIdx.x];
+        a.out_scores[o] = none ? -INFINITY : (float)sh.best[threadIdx.x];
         a.parents[o] = none ? -1 : (int32_t)(c >> kBeamTokenBits);
         a.tokens[o] = none ? -1 : (int32_t)(c & ((1u << kBeamTokenBits) - 1u));
     }
     if (a.out_history) {
-        for (uint32_t i = wave; i < k; i += kPW) {
-            const uint32_t c = chosen[i];
-            const bool none = best[i] == -INFINITY;
-            const int32_t* src = a.history + (int64_t)(row0 + (none ? 0 : c >> kBeamTokenBits)) * a.history_stride;
+        for (uint32_t i = wave; i < k; i += kPT / 64) {
+            const bool none = i >= have;
+            const uint32_t c = none ? 0 : sh.best_index[i];
+            const int32_t* src = a.history + (int64_t)(row0 + (c >> kBeamTokenBits)) * a.history_stride;
             int32_t* dst = a.out_history + (int64_t)((uint64_t)b * k + i) * a.out_history_stride;
             for (uint32_t j = lane; j < a.n_history; j += 64) dst[j] = none ? -1 : src[j];
             if (lane == 0) dst[a.n_history] = none ? -1 : (int32_t)(c & ((1u << kBeamTokenBits) - 1u));
@@ -305,7 +414,7 @@ __global__ __launch_bounds__(kPT) void beam_pick_kernel(const BeamLaunch a, cons
 
 template <typename T>
 hipError_t beam_t(const BeamLaunch& a, hipStream_t s) {
-    const uint32_t chunks = (a.vocab + kBeamChunk - 1) / kBeamChunk, runs = (chunks + a.per - 1) / a.per;
+    const uint32_t chunks = beam_chunks(a.vocab), runs = (chunks + a.per - 1) / a.per;
     hipLaunchKernelGGL(beam_scan_kernel<T>, dim3(a.n_search * a.n_beam * runs), dim3(kBT), 0, s, a, chunks, runs);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

@@ -40,6 +40,8 @@ bool share(const Rows& a, const Rows& b, uint32_t n) {
     return false;
 }
 
+uint32_t align64(uint32_t x) { return (x + 63) / 64 * 64; }
+
 // The bytes from an array's first value to its last.
 struct Span {
     const char* p;
@@ -234,8 +236,8 @@ int ni_verify_drafts(uint32_t dtype, const void* target, int64_t target_seq_stri
 
 size_t ni_beam_workspace(uint32_t n_search, uint32_t n_beam, uint32_t vocab) {
     const uint64_t rows = (uint64_t)n_search * n_beam;
-    return rows * (((uint64_t)vocab + kBeamChunk - 1) / kBeamChunk * sizeof(BeamSum) +
-                   ((uint64_t)vocab + kBeamGroup - 1) / kBeamGroup * sizeof(float));
+    if (vocab > kBeamVocab) return 0;
+    return rows * (beam_chunks(vocab) * sizeof(BeamSum) + align64(beam_groups(vocab)) * sizeof(float));
 }
 
 int ni_beam_select(uint32_t dtype, const void* logits, int64_t search_stride, int64_t beam_stride, const float* scores,
@@ -247,10 +249,10 @@ int ni_beam_select(uint32_t dtype, const void* logits, int64_t search_stride, in
     if (n_search == 0 || k == 0) return NI_OK;
     if (n_beam == 0 || n_beam > kBeamMax) return call_error(NI_ERR_BAD_ARG, "%u beams: 1..%u", n_beam, kBeamMax);
     if (k > kBeamMax) return call_error(NI_ERR_BAD_ARG, "k %u: at most %u", k, kBeamMax);
-    if (vocab == 0 || vocab > (1u << kBeamTokenBits))
-        return call_error(NI_ERR_BAD_ARG, "vocab %u must be 1..2^%u", vocab, kBeamTokenBits);
+    if (vocab == 0 || vocab > kBeamVocab)
+        return call_error(NI_ERR_BAD_ARG, "vocab %u must be 1..%u", vocab, kBeamVocab);
     if (finished && pad_token >= vocab) return call_error(NI_ERR_BAD_ARG, "pad_token %u is not in the vocabulary", pad_token);
-    const uint64_t chunks = ((uint64_t)vocab + kBeamChunk - 1) / kBeamChunk, rows = (uint64_t)n_search * n_beam;
+    const uint64_t chunks = beam_chunks(vocab), rows = (uint64_t)n_search * n_beam;
     const bool hist = out_history != nullptr;
     if (n_history > (1u << 30)) return call_error(NI_ERR_BAD_ARG, "n_history %u too large", n_history);
     const struct {
@@ -326,7 +328,12 @@ int ni_beam_select(uint32_t dtype, const void* logits, int64_t search_stride, in
     a.k = k;
     a.pad = pad_token;
     a.n_history = n_history;
-    a.n_groups = (vocab + kBeamGroup - 1) / kBeamGroup;
+    a.n_filled = beam_groups(vocab);
+    a.n_groups = align64(a.n_filled);
+    // m = 2^32 / g rounded up, g = n_groups / 64 at most 2^12 + 1: x * m is x / g * 2^32 and less than x * g / g
+    // more, which for x below 64 g, and so x * g below 2^31, never reaches the next whole.
+    const uint64_t g = a.n_groups / 64;
+    a.beam_magic = ((1ull << 32) + g - 1) / g;
     a.dtype = dtype;
     a.per = (uint32_t)per;
     const hipError_t e = launch_beam(a, (hipStream_t)stream);

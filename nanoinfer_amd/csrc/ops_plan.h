@@ -160,6 +160,10 @@ constexpr uint32_t kBeamChunk = 2048;      // vocabulary entries a workgroup tak
 constexpr uint32_t kBeamGroup = 128;       // entries whose largest is kept
 constexpr uint32_t kBeamMax = 64;          // beams of a search, and answers
 constexpr uint32_t kBeamTokenBits = 26;    // (beam, token) in 32 bits
+constexpr uint32_t kBeamVocab = 1u << 25;
+
+constexpr uint32_t beam_chunks(uint32_t vocab) { return (vocab + kBeamChunk - 1) / kBeamChunk; }
+constexpr uint32_t beam_groups(uint32_t vocab) { return (vocab + kBeamGroup - 1) / kBeamGroup; }
 
 struct BeamSum {  // of the run of chunks of one workgroup: sum of exp(logit - top)
     float top, sum;
@@ -178,8 +182,11 @@ struct BeamLaunch {
     int32_t* out_history;  // null: no histories
     float* groups;         // [n_search * n_beam][n_groups]: the largest logit of each group
     BeamSum* sums;         // [n_search * n_beam][chunks]: one of each run, first
-    uint32_t n_search, n_beam, vocab, k, pad, n_history, n_groups, dtype;
-    uint32_t per;  // chunks to a workgroup
+    uint32_t n_search, n_beam, vocab, k, pad, n_history, dtype;
+    uint32_t n_filled;    // beam_groups(vocab)
+    uint32_t n_groups;    // and the next multiple of 64: the groups' stride
+    uint64_t beam_magic;  // i / 64 * beam_magic >> 32 is i / n_groups, for i below n_beam * n_groups
+    uint32_t per;         // chunks to a workgroup
 };
 hipError_t launch_beam(const BeamLaunch& a, hipStream_t s);
 

@@ -204,3 +204,15 @@ def test_refusals(gpu):
     with pytest.raises(na.KvError):
         na.beam_select(logits, scores, 3, history=h[:, :, :4].contiguous(), tokens=h.view(-1)[:6].view(2, 3),
                        out_history=h)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("w,v,k", [(8, 131071, 16), (64, 40000, 64), (3, 2000, 33)])
+def test_more_equal_totals_than_are_ranked_at_once(gpu, dtype, w, v, k):
+    g = torch.Generator("cuda").manual_seed(6)
+    logits = torch.randint(0, 2, (2, w, v), generator=g, device="cuda").to(dtype)
+    logits[1] = logits[1, :1]
+    logits[1, -1, v // 2:] = 2
+    scores = torch.zeros((2, w), device="cuda")
+    logits[0] = logits[0, 0].sort().values  # the best at the end of every row
+    _check(na.beam_select(logits, scores, k), logits, scores, k, exact=True)
