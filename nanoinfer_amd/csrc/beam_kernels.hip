@@ -33,6 +33,47 @@ constexpr float kLog2e = 1.44269504088896340736f;
 // Whether anything of beam w of search b is read: it is alive, and goes on.
 __device__ __forceinline__ bool is_finished(const BeamLaunch& a, uint32_t row) { return a.finished && a.finished[row] != 0; }
 
+// Sum over groups of `lanes` lanes, a power of two up to 16.
+__device__ __forceinline__ uint32_t lanes_sum(uint32_t x, uint32_t lanes) {
+    const auto moved = [&](auto c) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(c)::value, 0xf, 0xf, false); };
+    if (lanes >= 2) x += moved(std::integral_constant<int, 0xb1>{});
+    if (lanes >= 4) x += moved(std::integral_constant<int, 0x4e>{});
+    if (lanes >= 8) x += moved(std::integral_constant<int, 0x141>{});
+    if (lanes >= 16) x += moved(std::integral_constant<int, 0x140>{});
+    return x;
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
+    x = lanes_sum(x, 16);
+    return (uint32_t)(__builtin_amdgcn_readlane((int)x, 0) + __builtin_amdgcn_readlane((int)x, 16) +
+                      __builtin_amdgcn_readlane((int)x, 32) + __builtin_amdgcn_readlane((int)x, 48));
+}
+__device__ __forceinline__ float wave_top(float x) {
+    x = fmaxf(x, dpp_move<0xb1>(x));
+    x = fmaxf(x, dpp_move<0x4e>(x));
+    x = fmaxf(x, dpp_move<0x141>(x));
+    x = fmaxf(x, dpp_move<0x140>(x));
+    return rows4_max(x);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_move64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xf, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double lane_of(double v, int l) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), l) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, l));
+}
+__device__ __forceinline__ double wave_sum(double x) {
+    x += dpp_move64<0xb1>(x);
+    x += dpp_move64<0x4e>(x);
+    x += dpp_move64<0x141>(x);
+    x += dpp_move64<0x140>(x);
+    return (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
+}
+
 // Eight neighbouring entries of a row from entry v on, those past the
 // vocabulary -infinity.  Rows begin anywhere, so the wide loads ask for no more
 // than an entry's alignment (which the memory system takes).
@@ -44,7 +85,7 @@ struct Eight {
     __device__ __forceinline__ void load(const T* row, uint32_t v, uint32_t vocab) {
         if (v + kBE <= vocab) {
 #pragma unroll
-            for (int i = 0; i < (int)kBE / N; i++) w[i] = __builtin_nontemporal_load(reinterpret_cast<const V*>(row + v + N * i));
+            for (int i = 0; i < (int)kBE / N; i++) w[i] = *reinterpret_cast<const V*>(row + v + N * i);
         } else {
 #pragma unroll
             for (int i = 0; i < (int)kBE; i++) w[i / N][i % N] = v + i < vocab ? row[v + i] : (T)-INFINITY;
@@ -95,14 +136,12 @@ __global__ __launch_bounds__(kBT) void beam_scan_kernel(const BeamLaunch a, cons
         cur = next;
     }
     // The workgroup's maximum and sum.
-    float M = m;
-    for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off));
+    float M = wave_top(m);
     if (lane == 0) tops[threadIdx.x >> 6] = M;
     __syncthreads();
     M = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
     const float ref = fabsf(M) == INFINITY ? 0.f : M;
-    double sum = s * (double)fast_exp2((m - ref) * kLog2e);
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
+    const double sum = wave_sum(s * (double)fast_exp2((m - ref) * kLog2e));
     if (lane == 0) sums[threadIdx.x >> 6] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -122,46 +161,18 @@ struct Cand {
 constexpr uint32_t kPT = 1024;          // threads of a pick
 constexpr uint32_t kPU = 8;             // candidates a thread holds at a time
 constexpr uint32_t kList = 1024;        // candidates that are ranked at once
-constexpr uint32_t kSetLanes = 8, kSets = kPT / kSetLanes;  // sets of candidates whose best are compared
+constexpr uint32_t kSetLanes = 16, kSets = kPT / kSetLanes;  // sets of candidates whose best are compared
 static_assert(kPT * kPU == kBeamMax * kBeamGroup, "the entries of the chosen groups are looked at once");
 
 struct Pick {
     double totals[kList];
     uint32_t indices[kList];
-    float tops[kSets];
+    __attribute__((aligned(16))) float tops[kSets];
     double best[kBeamMax];  // the answer so far, best first
     uint32_t best_index[kBeamMax];
-    uint32_t bound;  // as an integer of the same order
+    float bound;
     uint32_t n, counts[3];
 };
-
-// Sum over groups of `lanes` lanes, a power of two up to 16.
-__device__ __forceinline__ uint32_t lanes_sum(uint32_t x, uint32_t lanes) {
-    const auto moved = [&](auto c) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(c)::value, 0xf, 0xf, false); };
-    if (lanes >= 2) x += moved(std::integral_constant<int, 0xb1>{});
-    if (lanes >= 4) x += moved(std::integral_constant<int, 0x4e>{});
-    if (lanes >= 8) x += moved(std::integral_constant<int, 0x141>{});
-    if (lanes >= 16) x += moved(std::integral_constant<int, 0x140>{});
-    return x;
-}
-__device__ __forceinline__ uint32_t wave_sum(uint32_t x) {
-    x = lanes_sum(x, 16);
-    return (uint32_t)(__builtin_amdgcn_readlane((int)x, 0) + __builtin_amdgcn_readlane((int)x, 16) +
-                      __builtin_amdgcn_readlane((int)x, 32) + __builtin_amdgcn_readlane((int)x, 48));
-}
-__device__ __forceinline__ float wave_top(float x) {
-    x = fmaxf(x, dpp_move<0xb1>(x));
-    x = fmaxf(x, dpp_move<0x4e>(x));
-    x = fmaxf(x, dpp_move<0x141>(x));
-    x = fmaxf(x, dpp_move<0x140>(x));
-    return rows4_max(x);
-}
-// Floats as integers of the same order.
-__device__ __forceinline__ uint32_t order_of(float x) {
-    const uint32_t b = __float_as_uint(x);
-    return b >> 31 ? ~b : b | 1u << 31;
-}
-__device__ __forceinline__ float from_order(uint32_t o) { return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o); }
 
 // The first k of the n listed candidates into sh.best, in order: a candidate's place
 // is the number of those before it.
@@ -196,14 +207,33 @@ __device__ __forceinline__ uint64_t order_of(double x) {
     return b >> 63 ? ~b : b | 1ull << 63;
 }
 
-// The first k of the workgroup's candidates into the list, where more are left than it
-// holds: the k-th total bit by bit, then the last index among its equals.
-__device__ __forceinline__ void pick_equal(Pick& sh, const double (&t)[kPU], const uint32_t (&index)[kPU], uint32_t k) {
+// Candidates j of bit j of `in` into the list, as far as `room` goes; sh.n counts them all.
+__device__ __forceinline__ void take(Pick& sh, const double (&t)[kPU], const uint32_t (&index)[kPU], uint32_t in, uint32_t room) {
+    if (in == 0) return;
+    // (few lanes have any: each adds for itself, which the compiler makes of an address that it cannot see to be one)
+    uint32_t zero = 0;
+    asm("" : "+v"(zero));
+    uint32_t at = atomicAdd(&sh.n + zero, (uint32_t)__popc(in));
+#pragma unroll
+    for (uint32_t j = 0; j < kPU; j++)
+        if (in >> j & 1u) {
+            if (at < room) {
+                sh.totals[at] = t[j];
+                sh.indices[at] = index[j];
+            }
+            at++;
+        }
+}
+
+// The first k of the workgroup's candidates into the list, behind the best so far, where
+// more are left than it holds: the k-th total bit by bit, then the last index among its equals.
+__device__ __forceinline__ void pick_equal(Pick& sh, const double (&t)[kPU], const uint32_t (&index)[kPU], uint32_t k,
+                                           uint32_t have) {
     uint64_t key[kPU], kth = 0;
 #pragma unroll
     for (uint32_t j = 0; j < kPU; j++) key[j] = t[j] > -INFINITY ? order_of(t[j]) : 0;
     if (threadIdx.x < 3) sh.counts[threadIdx.x] = 0;
-    if (threadIdx.x == 0) sh.n = 0;
+    if (threadIdx.x == 0) sh.n = have;
     __syncthreads();
     uint32_t turn = 0;
     for (int bit = 63; bit >= 0; bit--) {
@@ -225,13 +255,10 @@ __device__ __forceinline__ void pick_equal(Pick& sh, const double (&t)[kPU], con
         for (uint32_t j = 0; j < kPU; j++) mine += key[j] == kth && index[j] <= trial ? 1u : 0u;
         if (count_all(sh, mine, turn++) >= equals) last = trial;
     }
+    uint32_t in = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < kPU; j++)
-        if (key[j] > kth || (key[j] == kth && index[j] <= last)) {
-            const uint32_t at = atomicAdd(&sh.n, 1u);
-            sh.totals[at] = t[j];
-            sh.indices[at] = index[j];
-        }
+    for (uint32_t j = 0; j < kPU; j++) in |= (key[j] > kth || (key[j] == kth && index[j] <= last) ? 1u : 0u) << j;
+    take(sh, t, index, in, kList);
     __syncthreads();
 }
 
@@ -249,46 +276,39 @@ __device__ __forceinline__ uint32_t pick_more(Pick& sh, const double (&t)[kPU], 
     top = fmaxf(top, dpp_move<0xb1>(top));
     top = fmaxf(top, dpp_move<0x4e>(top));
     top = fmaxf(top, dpp_move<0x141>(top));
-    static_assert(kSetLanes == 8 && kSets % (4 * kSetLanes) == 0, "a set is half a row of lanes, each of which compares fours");
+    top = fmaxf(top, dpp_move<0x140>(top));
+    static_assert(kSetLanes == 16 && kSets == 4 * kSetLanes, "a set is a row of lanes, each of which compares four");
     const uint32_t set = threadIdx.x / kSetLanes, part = threadIdx.x % kSetLanes;
     if (part == 0) sh.tops[set] = top;
-    if (threadIdx.x == 0) {
-        sh.n = 0;
-        sh.bound = 0;
+    if (threadIdx.x == 0) sh.n = have;
+    if (threadIdx.x < have) {  // the best so far begin the list
+        sh.totals[threadIdx.x] = sh.best[threadIdx.x];
+        sh.indices[threadIdx.x] = sh.best_index[threadIdx.x];
     }
     __syncthreads();
-    uint32_t reach = 0;  // sets whose best is no lower than this one's
+    uint32_t reach = 0;  // sets whose best is higher, and (16 bits up) no lower than this one's
+    const float4 others = *reinterpret_cast<const float4*>(&sh.tops[4 * part]);
 #pragma unroll
-    for (uint32_t j = 0; j < kSets / kSetLanes; j += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(&sh.tops[part * (kSets / kSetLanes) + j]);
-        reach += (x.x >= top ? 1u : 0u) + (x.y >= top ? 1u : 0u) + (x.z >= top ? 1u : 0u) + (x.w >= top ? 1u : 0u);
+    for (int e = 0; e < 4; e++) {
+        const float y = e == 0 ? others.x : e == 1 ? others.y : e == 2 ? others.z : others.w;
+        reach += (y > top ? 1u : 0u) + (y >= top ? 1u << 16 : 0u);
     }
     reach = lanes_sum(reach, kSetLanes);
-    if (part == 0 && reach >= k) atomicMax(&sh.bound, order_of(top));  // at least k candidates lie there or above
+    // The k-th best: at least k candidates lie there or above.  (Equals write the same.)
+    if (part == 0 && (reach & 0xffffu) < k && reach >> 16 >= k) sh.bound = top;
     __syncthreads();
-    double bound = (double)from_order(sh.bound);
+    double bound = (double)sh.bound;
     if (have == k) bound = fmax(bound, sh.best[k - 1]);
-    constexpr uint32_t kRoom = kList - kBeamMax;
+    uint32_t in = 0;  // bit j: candidate j is not out
 #pragma unroll
-    for (uint32_t j = 0; j < kPU; j++)
-        if (t[j] > -INFINITY && t[j] >= bound) {
-            const uint32_t at = atomicAdd(&sh.n, 1u);
-            if (at < kRoom) {
-                sh.totals[at] = t[j];
-                sh.indices[at] = index[j];
-            }
-        }
+    for (uint32_t j = 0; j < kPU; j++) in |= (t[j] > -INFINITY && t[j] >= bound ? 1u : 0u) << j;
+    take(sh, t, index, in, kList);
     __syncthreads();
-    if (sh.n > kRoom) {
+    if (sh.n > kList) {
         __syncthreads();  // (everyone has seen it)
-        pick_equal(sh, t, index, k);
+        pick_equal(sh, t, index, k, have);
     }
-    const uint32_t n = sh.n + have;
-    if (threadIdx.x < have) {
-        sh.totals[n - have + threadIdx.x] = sh.best[threadIdx.x];
-        sh.indices[n - have + threadIdx.x] = sh.best_index[threadIdx.x];
-    }
-    __syncthreads();
+    const uint32_t n = sh.n;
     rank_list(sh, n, k);
     __syncthreads();
     return min(n, k);
@@ -330,11 +350,12 @@ __global__ __launch_bounds__(kPT) void beam_pick_kernel(const BeamLaunch a, cons
             for (uint32_t r = lane + 64; r < runs; r += 64) M = fmaxf(M, p[r].top);
             M = wave_top(M);
             if (fabsf(M) < INFINITY) {
-                double S = mine.top > -INFINITY ? (double)mine.sum * exp((double)mine.top - (double)M) : 0.;
-                for (uint32_t r = lane + 64; r < runs; r += 64)
-                    if (p[r].top > -INFINITY) S += (double)p[r].sum * exp((double)p[r].top - (double)M);
-                for (int o = 32; o > 0; o >>= 1) S += __shfl_xor(S, o);
-                off = (double)score - ((double)M + log(S));
+                auto part = [&](const BeamSum& x) {
+                    return x.top > -INFINITY ? (double)x.sum * (double)fast_exp2((x.top - M) * kLog2e) : 0.;
+                };
+                double S = part(mine);
+                for (uint32_t r = lane + 64; r < runs; r += 64) S += part(p[r]);
+                off = (double)score - ((double)M + log(wave_sum(S)));
             }
         }
         if (lane == 0) {
@@ -343,55 +364,60 @@ __global__ __launch_bounds__(kPT) void beam_pick_kernel(const BeamLaunch a, cons
         }
     }
     __syncthreads();
+    // The groups, kPT * kPU at a time, then the chosen ones' entries.  (One body for
+    // both: the code is fetched anew for every launch.)
     uint32_t have = 0;
-    double t[kPU];
-    uint32_t index[kPU];
-    for (uint32_t i0 = 0; i0 < all; i0 += kPT * kPU) {
-        if (i0 > 0) load(i0);
+    for (uint32_t i0 = 0;; i0 += kPT * kPU) {
+        const bool last = i0 >= all;
+        double t[kPU];
+        uint32_t index[kPU];
+        if (!last) {
+            if (i0 > 0) load(i0);
 #pragma unroll
-        for (uint32_t j = 0; j < kPU; j++) {
-            const uint32_t at = i0 + j * kPT + wave * 64, i = at + lane;
-            index[j] = i;
-            t[j] = -INFINITY;
-            if (at < all) {
-                const uint32_t w = beam_of(at);
-                const double off = offset[w];
-                // (what was not written -- groups past a row, of a beam that is finished or has no
-                // score -- may hold anything; a finished beam has one candidate, in its first)
-                double y = i - w * G < a.n_filled ? off + (double)x[j] : -INFINITY;
-                if (done[w]) y = i == w * G ? off : -INFINITY;
-                if (off > -INFINITY && y > -INFINITY) t[j] = y;
+            for (uint32_t j = 0; j < kPU; j++) {
+                const uint32_t at = i0 + j * kPT + wave * 64, i = at + lane;
+                index[j] = i;
+                t[j] = -INFINITY;
+                if (at < all) {
+                    const uint32_t w = beam_of(at);
+                    const double off = offset[w];
+                    // (what was not written -- groups past a row, of a beam that is finished or has no
+                    // score -- may hold anything; a finished beam has one candidate, in its first)
+                    double y = i - w * G < a.n_filled ? off + (double)x[j] : -INFINITY;
+                    if (done[w]) y = i == w * G ? off : -INFINITY;
+                    if (off > -INFINITY && y > -INFINITY) t[j] = y;
+                }
             }
+        } else {
+            if (threadIdx.x < k) chosen[threadIdx.x] = threadIdx.x < have ? sh.best_index[threadIdx.x] : 0xffffffffu;
+            __syncthreads();
+            static_assert(kBeamGroup == 128, "two waves to a group");
+            T y[kPU];
+#pragma unroll
+            for (uint32_t j = 0; j < kPU; j++) {
+                const uint32_t c = (j * kPT / 64 + wave) / 2, e = wave % 2 * 64 + lane;
+                y[j] = (T)-INFINITY;
+                index[j] = 0xffffffffu;
+                if (c < have) {
+                    const uint32_t g = __builtin_amdgcn_readfirstlane(chosen[c]), w = beam_of(g);
+                    const uint32_t v = (g - w * G) * kBeamGroup + e;
+                    const bool fin = done[w], in = !fin && v < a.vocab;
+                    if (in) y[j] = row_of(w)[v];
+                    if (in || (fin && e == 0)) index[j] = w << kBeamTokenBits | (fin ? a.pad : v);
+                }
+            }
+#pragma unroll
+            for (uint32_t j = 0; j < kPU; j++) {
+                const uint32_t w = index[j] >> kBeamTokenBits;
+                double z = -INFINITY;
+                if (index[j] != 0xffffffffu) z = done[w] ? offset[w] : offset[w] + (double)(float)y[j];
+                t[j] = z > -INFINITY ? z : -INFINITY;
+            }
+            have = 0;
         }
         have = pick_more(sh, t, index, k, have);
+        if (last) break;
     }
-    if (threadIdx.x < k) chosen[threadIdx.x] = threadIdx.x < have ? sh.best_index[threadIdx.x] : 0xffffffffu;
-    __syncthreads();
-    // The chosen groups' entries, half a group to a wave.
-    static_assert(kBeamGroup == 128, "two waves to a group");
-    T y[kPU];
-#pragma unroll
-    for (uint32_t j = 0; j < kPU; j++) {
-        const uint32_t c = (j * kPT / 64 + wave) / 2, e = wave % 2 * 64 + lane;
-        y[j] = (T)-INFINITY;
-        index[j] = 0xffffffffu;
-        if (c < have) {
-            const uint32_t g = __builtin_amdgcn_readfirstlane(chosen[c]), w = beam_of(g);
-            const T* const row = row_of(w);
-            const uint32_t v = (g - w * G) * kBeamGroup + e;
-            const bool fin = done[w], in = !fin && v < a.vocab;
-            if (in) y[j] = row[v];
-            if (in || (fin && e == 0)) index[j] = w << kBeamTokenBits | (fin ? a.pad : v);
-        }
-    }
-#pragma unroll
-    for (uint32_t j = 0; j < kPU; j++) {
-        const uint32_t w = index[j] >> kBeamTokenBits;
-        double z = -INFINITY;
-        if (index[j] != 0xffffffffu) z = done[w] ? offset[w] : offset[w] + (double)(float)y[j];
-        t[j] = z > -INFINITY ? z : -INFINITY;
-    }
-    have = pick_more(sh, t, index, k, 0);
     if (threadIdx.x < k) {
         const bool none = threadIdx.x >= have;
         const uint32_t c = sh.best_index[threadIdx.x];
