@@ -173,22 +173,39 @@ __device__ __forceinline__ half4_t e4m3_f16x4(uint32_t a) {
     return half4_t{x0[0], x0[1], x1[0], x1[1]};
 }
 
-constexpr int kBlockWaves = 4;
 // Weights are exp2(score - reference), the reference the running maximum less
 // kRefLog2, raised when a score passes it by kRefLog2 + kRefSlack: at most 2^15 in f16
-// (as hi + lo), normal down to 2^-27 of the largest.
-constexpr float kRefLog2 = 13.f, kRefSlack = 2.f, kRefUnscale = 1.f / 8192.f;
+// (as hi + lo), normal down to 2^-24 of the largest.
+constexpr float kRefLog2 = 10.f, kRefSlack = 5.f, kRefUnscale = 1.f / 1024.f;
+// Weights of a page whose value scale is 2^-k of the outputs' unit enter a product 2^k
+// smaller up to this k: what that costs them lies 2^-32 below the page's largest.
+constexpr int kNear = 6;
 
-// One (item, layer, head): S^T = K Q^T (16 keys x 16 slots; q in f16 hi + lo
-// parts, keys as stored, their page's scale on the sums), the online softmax down
-// its columns, O^T += (V^T P^T of a page) times its value scale.  Lane l holds slot
-// l % 16 and keys, then dims, 4 (l / 16) .. + 3: S^T's registers are P^T's operand
-// as they are.  The four waves take PB pages in turn, the next ones' loads
-// issued before the products of these; their states are joined through LDS.
-template <int D, int INL>
-__global__ __launch_bounds__(64 * kBlockWaves) void block_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
-    constexpr int W = kBlockWaves, NB = D / 64, PB = 2;
-    __shared__ float red[W][kSlotTile][D + 4];  // m, l, -, -, o
+// (in place: the compiler would keep both and copy where the multiplication is passed by.  A
+// matrix product may still be writing x: its 16 passes are waited for; and one may read it next.)
+__device__ __forceinline__ void scale_in_place(float4_t& x, float by) {
+    asm volatile("s_nop 15\n\ts_nop 3\n\tv_mul_f32 %0, %4, %0\n\tv_mul_f32 %1, %4, %1\n\tv_mul_f32 %2, %4, %2\n\tv_mul_f32 %3, %4, %3\n\ts_nop 1"
+                 : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]) : "v"(by));
+}
+
+// One (item, layer, head), NT tiles of 16 slots: S^T = K Q^T (16 keys x 16 slots; q
+// in f16 hi + lo parts, keys as stored, their page's scale on the sums), the online
+// softmax down its columns, O^T += V^T P^T of two pages, in units of a value scale.  Lane l
+// holds slot l % 16 of each tile and keys, then dims, 4 (l / 16) .. + 3: S^T's registers
+// are P^T's operand as they are.  The W waves take two pages each in turn, the next
+// ones' loads issued before the products of these; their states are joined through
+// LDS.
+template <int D, int NT, int W, bool MANY, int INL>
+__global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
+    constexpr int NB = D / 64, PB = 2, NC = 4 * NB;  // runs of 64 dims; pages of an iteration; 16-dim chunks
+    // MANY: the queries are held once for all waves, in LDS, as each lane's operands.
+    constexpr bool kShared = MANY;
+    __shared__ union Lds {
+        float red[W][NT * kSlotTile][D + 4];  // m, l, -, -, o
+        half8_t q[NT][NB][2][kShared ? 2 : 1][64];
+        __device__ Lds() {}
+    } lds;
+    auto& red = lds.red;
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t H = a.pool.n_head, lh = a.n_lay * H;
@@ -208,134 +225,278 @@ __global__ __launch_bounds__(64 * kBlockWaves) void block_attn_kernel(const Pref
 
     struct Regs {
         u32x4 k[PB][NB], v[PB][NB];
-        float ks[PB], vs[PB];
     };
-    auto load = [&](uint32_t pg, Regs& r) {
+    // (runs of many slots read each page many times, from the caches; others once)
+    auto load16 = [](const u32x4* p) { return MANY ? *p : __builtin_nontemporal_load(p); };
+    // (page ids are asked for a turn ahead of the pages: one that waited for its id would wait twice)
+    auto pages = [&](uint32_t pg, uint32_t (&id)[PB]) {
+#pragma unroll
+        for (int b = 0; b < PB; b++) id[b] = tab[min(pg + b, pg_end - 1)];  // (past the end: the last again, its keys masked)
+    };
+    auto load = [&](const uint32_t (&id)[PB], Regs& r, bool k, bool v) {
 #pragma unroll
         for (int b = 0; b < PB; b++) {
-            // (a page past the end: the last again, its keys masked)
-            const uint8_t* page = layer + (uint64_t)tab[min(pg + b, pg_end - 1)] * page_bytes;
-            const u32x4* p = reinterpret_cast<const u32x4*>(page + at_block) + lane;
+            const u32x4* p = reinterpret_cast<const u32x4*>(layer + id[b] * page_bytes + at_block) + lane;
 #pragma unroll
-            for (int i = 0; i < NB; i++) r.k[b][i] = load16(p + 64 * i);
+            for (int i = 0; i < NB; i++)
+                if (k) r.k[b][i] = load16(p + 64 * i);
 #pragma unroll
-            for (int i = 0; i < NB; i++) r.v[b][i] = load16(p + 64 * (NB + i));
-            const Scales sc = (Scales)(page + at_scale);
-            r.ks[b] = sc[0];
-            r.vs[b] = sc[1];
+            for (int i = 0; i < NB; i++)
+                if (v) r.v[b][i] = load16(p + 64 * (NB + i));
+        }
+    };
+    auto scales = [&](const uint32_t (&id)[PB], float (&ks)[PB], float (&vs)[PB]) {
+#pragma unroll
+        for (int b = 0; b < PB; b++) {
+            const Scales sc = (Scales)(layer + id[b] * page_bytes + at_scale);
+            ks[b] = sc[0];
+            vs[b] = sc[1];
         }
     };
     Regs cur;
     uint32_t pg = it.kv_begin / kPage + wave * PB;
-    if (pg < pg_end) load(pg, cur);
+    uint32_t id[PB];  // of the next turn's pages
+    float ks[PB], vs[PB];
+    pages(pg, id);
+    if (pg < pg_end) load(id, cur, true, true);
+    scales(id, ks, vs);
+    pages(pg + W * PB, id);
 
-    const bool has = col < (int)it.ns;
-    const uint32_t slot = it.slot0 + (has ? (uint32_t)col : 0u);
-    const uint32_t row = slot / a.group, g = slot - row * a.group;
-    const uint32_t qpos = min(it.pos0 + row, kWholePos);
     const uint32_t first_pos = min(it.pos0 + it.slot0 / a.group, kWholePos);  // of the item's first slot
     const uint32_t plain_end = min(it.kv_end, first_pos + 1);                 // every slot sees the keys before it
-    half8_t qh[NB][2], ql[NB][2];
-    {
+    uint32_t qpos[NT];
+    half8_t qh[kShared ? 1 : NB][2], ql[kShared ? 1 : NB][2];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const bool has = t * (int)kSlotTile + col < (int)it.ns;
+        const uint32_t slot = it.slot0 + (has ? t * kSlotTile + col : 0u);
+        const uint32_t row = slot / a.group, g = slot - row * a.group;
+        qpos[t] = min(it.pos0 + row, kWholePos);
         // step (i, j) of QK: dims 64 i + 16 rg + 8 j .. + 7, as the lane's bytes of K
         const float* qb = a.q + (int64_t)lay * a.q_layer_stride + (int64_t)(it.row0 + row) * a.q_row_stride +
                           (head * a.group + g) * D + 16 * rg;
+        auto operand = [&](int i, int j, half8_t& hi, half8_t& lo) {
+            const float4 x0 = reinterpret_cast<const float4*>(qb + 64 * i + 8 * j)[0];
+            const float4 x1 = reinterpret_cast<const float4*>(qb + 64 * i + 8 * j)[1];
+            const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                y[e] = has ? x[e] * a.qscale : 0.f;
+                asm("" : "+v"(y[e]));  // the f32 products, as the split's residual sees them
+            }
+            split8(y, hi, lo);
+        };
+        if constexpr (kShared) {
+            static_assert(W == 4, "a step of every tile to a wave, or two");
+            if (NB == 2 || wave / 2 == t) {  // (one tile of 64 dims: two waves have none)
+                const int i = NB == 2 ? wave / 2 : 0, j = wave % 2;
+                half8_t hi, lo;
+                operand(i, j, hi, lo);
+                lds.q[t][i][j][0][lane] = hi;
+                lds.q[t][i][j][1][lane] = lo;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NB; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) operand(i, j, qh[i][j], ql[i][j]);
+        }
+    }
+    if constexpr (kShared) __syncthreads();
+    float mref[NT], lsum[NT];
+    bool set[NT];  // the reference is a score's (alike in the four lanes of a slot)
+    float4_t o[NT][NC];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        mref[t] = lsum[t] = 0.f;
+        set[t] = false;
+#pragma unroll
+        for (int c = 0; c < NC; c++) o[t][c] = float4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    int unit = kMinExp - 1;  // log2 of the largest value scale so far
+    for (; pg < pg_end; pg += W * PB) {
+        // One tile: the next pages' registers beside these.  Two leave no room for that: keys
+        // follow the products that read the last ones, values likewise.
+        constexpr bool kBeside = !MANY;
+        const bool more = pg + W * PB < pg_end;
+        Regs nxt;
+        if (kBeside && more) load(id, nxt, true, true);
+        if constexpr (kShared) asm volatile("" : : : "memory");  // (the queries stay in LDS: not kept from one turn to the next)
+        float4_t st[NT][PB];
+        // (products that add to one sum stand apart, here and below: each waits for the one before)
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int b = 0; b < PB; b++) st[t][b] = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NB; i++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const float4 x0 = reinterpret_cast<const float4*>(qb + 64 * i + 8 * j)[0];
-                const float4 x1 = reinterpret_cast<const float4*>(qb + 64 * i + 8 * j)[1];
-                const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-                float y[8];
+                half8_t kh[PB], q_hi[NT], q_lo[NT];
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    y[e] = has ? x[e] * a.qscale : 0.f;
-                    asm("" : "+v"(y[e]));  // the f32 products, as the split's residual sees them
+                for (int t = 0; t < NT; t++) {
+                    if constexpr (kShared) {
+                        q_hi[t] = lds.q[t][i][j][0][lane];
+                        q_lo[t] = lds.q[t][i][j][1][lane];
+                    } else {
+                        q_hi[t] = qh[i][j];
+                        q_lo[t] = ql[i][j];
+                    }
                 }
-                split8(y, qh[i][j], ql[i][j]);
+#pragma unroll
+                for (int b = 0; b < PB; b++) kh[b] = e4m3_f16x8(cur.k[b][i][2 * j], cur.k[b][i][2 * j + 1]);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int b = 0; b < PB; b++)
+                        st[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[b], q_lo[t], st[t][b], 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int b = 0; b < PB; b++)
+                        st[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh[b], q_hi[t], st[t][b], 0, 0, 0);
             }
-    }
-    float mref = 0.f, lsum = 0.f;
-    bool set = false;  // the reference is a score's (alike in the four lanes of a slot)
-    float4_t o[4 * NB];
+        if (!kBeside && more) load(id, cur, true, false);
+        float next_ks[PB], next_vs[PB];
+        uint32_t next_id[PB];
+        scales(id, next_ks, next_vs);
+        pages(pg + 2 * W * PB, next_id);
+        // Outputs are kept in units of the largest value scale so far, 2^unit: exact, down to
+        // 2^-126 of it.  The weights of pages whose scale is no more than 2^kNear smaller
+        // are taken in those units too, and both pages enter one product.
+        const int e0 = exp_of(vs[0]), e1 = exp_of(vs[1]);
+        if (max(e0, e1) > unit) {
+            if (unit >= kMinExp) {  // (else nothing is summed yet)
+                const float down = pow2(max(unit - max(e0, e1), -126));
 #pragma unroll
-    for (int c = 0; c < 4 * NB; c++) o[c] = float4_t{0.f, 0.f, 0.f, 0.f};
-
-    for (; pg < pg_end; pg += W * PB) {
-        Regs nxt;
-        if (pg + W * PB < pg_end) load(pg + W * PB, nxt);
-        float s[PB][4];
+                for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int b = 0; b < PB; b++) {
-            float4_t st = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < NB; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const half8_t kh = e4m3_f16x8(cur.k[b][i][2 * j], cur.k[b][i][2 * j + 1]);
-                    st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, ql[i][j], st, 0, 0, 0);
-                    st = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, qh[i][j], st, 0, 0, 0);
-                }
-#pragma unroll
-            for (int j = 0; j < 4; j++) s[b][j] = fmaf(st[j], cur.ks[b], -mref);
+                    for (int c = 0; c < NC; c++) scale_in_place(o[t][c], down);
+            }
+            unit = max(e0, e1);
         }
-        if ((pg + PB) * kPage > plain_end) {
+        const int below[PB] = {unit - e0, unit - e1};
+        const bool near = max(below[0], below[1]) <= kNear;
+        half4_t ph[NT][PB], pl[NT][PB];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            float s[PB][4];
+#pragma unroll
+            for (int b = 0; b < PB; b++) {
+                const float ref = mref[t] + (near ? (float)below[b] : 0.f);
+#pragma unroll
+                for (int j = 0; j < 4; j++) s[b][j] = fmaf(st[t][b][j], ks[b], -ref);
+            }
+            if ((pg + PB) * kPage > plain_end) {
+#pragma unroll
+                for (int b = 0; b < PB; b++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t key = (pg + b) * kPage + 4 * rg + j;
+                        if (key >= it.kv_end || key > qpos[t]) s[b][j] = -INFINITY;
+                    }
+            }
+            float lm = s[0][0];
 #pragma unroll
             for (int b = 0; b < PB; b++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const uint32_t key = (pg + b) * kPage + 4 * rg + j;
-                    if (key >= it.kv_end || key > qpos) s[b][j] = -INFINITY;
+                for (int j = 0; j < 4; j++) lm = fmaxf(lm, s[b][j]);
+            if (__any(lm > kRefLog2 + kRefSlack || !set[t])) {
+                const float mx = rows4_max(lm) - kRefLog2;
+                // The first finite maximum sets the reference, later ones only raise it.
+                const bool none = mx == -INFINITY;
+                const float d = set[t] ? fmaxf(mx, 0.f) : none ? 0.f : mx;
+                const float alpha = set[t] ? fast_exp2(-d) : 1.f;  // (nothing is summed yet)
+                set[t] = set[t] || !none;
+                if (__any(alpha != 1.f)) {
+                    lsum[t] *= alpha;
+#pragma unroll
+                    for (int c = 0; c < NC; c++) scale_in_place(o[t][c], alpha);
                 }
+                mref[t] += d;
+#pragma unroll
+                for (int b = 0; b < PB; b++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) s[b][j] -= d;
+            }
+#pragma unroll
+            for (int b = 0; b < PB; b++) {
+                float p[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) p[j] = fast_exp2(s[b][j]);
+                lsum[t] += ((p[0] + p[1]) + (p[2] + p[3])) * (near ? pow2(below[b]) : 1.f);
+                split4(p, ph[t][b], pl[t][b]);
+            }
         }
-        float lm = s[0][0];
+        if (near) {
+            half8_t wh[NT], wl[NT];
 #pragma unroll
-        for (int b = 0; b < PB; b++)
+            for (int t = 0; t < NT; t++) {
+                wh[t] = __builtin_shufflevector(ph[t][0], ph[t][1], 0, 1, 2, 3, 4, 5, 6, 7);
+                wl[t] = __builtin_shufflevector(pl[t][0], pl[t][1], 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            constexpr int G = 4 / NT;  // chunks at a time
 #pragma unroll
-            for (int j = 0; j < 4; j++) lm = fmaxf(lm, s[b][j]);
-        if (__any(lm > kRefLog2 + kRefSlack || !set)) {
-            const float mx = rows4_max(lm) - kRefLog2;
-            // The first finite maximum sets the reference, later ones only raise it.
-            const bool none = mx == -INFINITY;
-            const float d = set ? fmaxf(mx, 0.f) : none ? 0.f : mx;
-            const float alpha = set ? fast_exp2(-d) : 1.f;  // (nothing is summed yet)
-            set = set || !none;
-            lsum *= alpha;
+            for (int c0 = 0; c0 < NC; c0 += G) {
+                half8_t v8[G];
 #pragma unroll
-            for (int c = 0; c < 4 * NB; c++) o[c] *= alpha;
-            mref += d;
+                for (int g = 0; g < G; g++) {
+                    const int i = (c0 + g) / 4, c = (c0 + g) % 4;
+                    v8[g] = e4m3_f16x8(cur.v[0][i][c], cur.v[1][i][c]);
+                }
 #pragma unroll
-            for (int b = 0; b < PB; b++)
+                for (int g = 0; g < G; g++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[b][j] -= d;
+                    for (int t = 0; t < NT; t++)
+                        o[t][c0 + g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8[g], wl[t], o[t][c0 + g], 0, 0, 0);
+#pragma unroll
+                for (int g = 0; g < G; g++)
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+                        o[t][c0 + g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8[g], wh[t], o[t][c0 + g], 0, 0, 0);
+            }
+        } else {
+            // Each page's sums by themselves, then in those units.
+#pragma unroll 1
+            for (int b = 0; b < PB; b++) {
+                const float down = pow2(max(-(b ? below[1] : below[0]), -126));
+#pragma unroll
+                for (int i = 0; i < NB; i++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        const half4_t v4 = e4m3_f16x4(b ? cur.v[1][i][c] : cur.v[0][i][c]);
+#pragma unroll
+                        for (int t = 0; t < NT; t++) {
+                            float4_t x = {0.f, 0.f, 0.f, 0.f};
+                            x = __builtin_amdgcn_mfma_f32_16x16x16f16(v4, b ? pl[t][1] : pl[t][0], x, 0, 0, 0);
+                            x = __builtin_amdgcn_mfma_f32_16x16x16f16(v4, b ? ph[t][1] : ph[t][0], x, 0, 0, 0);
+                            o[t][4 * i + c] += x * down;
+                        }
+                    }
+            }
         }
+        if (kBeside && more) cur = nxt;
+        if (!kBeside && more) load(id, cur, false, true);
 #pragma unroll
         for (int b = 0; b < PB; b++) {
-            float p[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) p[j] = fast_exp2(s[b][j]);
-            lsum += (p[0] + p[1]) + (p[2] + p[3]);
-            half4_t ph, pl;
-            split4(p, ph, pl);
-#pragma unroll
-            for (int i = 0; i < NB; i++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const half4_t v4 = e4m3_f16x4(cur.v[b][i][c]);
-                    float4_t t = __builtin_amdgcn_mfma_f32_16x16x16f16(v4, pl, float4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                    t = __builtin_amdgcn_mfma_f32_16x16x16f16(v4, ph, t, 0, 0, 0);
-                    o[4 * i + c] += t * cur.vs[b];
-                }
+            ks[b] = next_ks[b];
+            vs[b] = next_vs[b];
+            id[b] = next_id[b];
         }
-        if (pg + W * PB < pg_end) cur = nxt;
     }
-    lsum = rows4_sum(lsum);
-    if (has) {
-        if (rg == 0) *reinterpret_cast<float2*>(&red[wave][col][0]) = float2{set ? mref + kRefLog2 : kMinScore, lsum * kRefUnscale};
+    if constexpr (kShared) __syncthreads();  // the queries' LDS becomes `red`
 #pragma unroll
-        for (int c = 0; c < 4 * NB; c++)
-            *reinterpret_cast<float4_t*>(&red[wave][col][4 + c * 16 + 4 * rg]) = o[c] * kRefUnscale;
+    for (int t = 0; t < NT; t++) {
+        const float l = rows4_sum(lsum[t]);
+        const int sl = t * (int)kSlotTile + col;
+        if (sl < (int)it.ns) {
+            if (rg == 0) *reinterpret_cast<float2*>(&red[wave][sl][0]) = float2{set[t] ? mref[t] + kRefLog2 : kMinScore, l * kRefUnscale};
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+                *reinterpret_cast<float4_t*>(&red[wave][sl][4 + c * 16 + 4 * rg]) = o[t][c] * (kRefUnscale * pow2(max(unit, kMinExp)));
+        }
     }
     __syncthreads();
     for (uint32_t t = threadIdx.x; t < it.ns * (D / 4); t += 64 * W) {
@@ -427,14 +588,22 @@ hipError_t launch_block_append(const BlockAppendLaunch& a, const void* ip, uint3
     });
 }
 
+template <int D, int INL>
+static hipError_t block_attn_t(const PrefixLaunch& a, uint64_t blocks, hipStream_t s, const LaunchTiming& t, const PlanArg<INL>& pa) {
+    if (a.wide == 2) return go(block_attn_kernel<D, 2, 4, true, INL>, blocks, 256, s, t, a, pa);
+    if (a.wide == 1) return go(block_attn_kernel<D, 1, 4, true, INL>, blocks, 256, s, t, a, pa);
+    if (a.waves == 8) return go(block_attn_kernel<D, 1, 8, false, INL>, blocks, 512, s, t, a, pa);
+    return go(block_attn_kernel<D, 1, 4, false, INL>, blocks, 256, s, t, a, pa);
+}
+
 hipError_t launch_block_attention(const PrefixLaunch& a, const void* ip, uint32_t ib, hipStream_t s,
                                   const LaunchTiming& t) {
     const uint64_t blocks = (uint64_t)a.n_items * a.n_lay * a.pool.n_head;
     if (blocks == 0) return hipSuccess;
     return with_plan(a, ip, ib, [&](auto pa) {
         constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
-        if (a.pool.head_dim == 64) return go(block_attn_kernel<64, INL>, blocks, 64 * kBlockWaves, s, t, a, pa);
-        if (a.pool.head_dim == 128) return go(block_attn_kernel<128, INL>, blocks, 64 * kBlockWaves, s, t, a, pa);
+        if (a.pool.head_dim == 64) return block_attn_t<64, INL>(a, blocks, s, t, pa);
+        if (a.pool.head_dim == 128) return block_attn_t<128, INL>(a, blocks, s, t, pa);
         return hipErrorInvalidValue;
     });
 }

@@ -141,6 +141,7 @@ struct PrefixPlan {
     uint32_t wide = 0, waves = 0;  // PrefixLaunch::wide and waves of pitems
     uint32_t row_slots = 0;        // PrefixLaunch::row_slots of items
     uint32_t row_waves = 0;        // and their waves
+    uint32_t block_tiles = 0, block_waves = 4;  // block-scaled: PrefixLaunch::wide and waves
     std::vector<PrefixMerge> merges;
     std::vector<uint32_t> table;
     uint64_t n_parts = 0;
@@ -1564,9 +1565,27 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const uint32_t* at, const ni_pref
     // us: head_dim 64 x 12 heads, 16 rows of up to 1000 keys 10.6 / 12.1, 4 of up to
     // 4000 12.4 / 13.1, 64 of up to 1023 behind 1000 26.1 / 30.1; 128 x 8 heads, 8 x 4
     // rows of up to 8000 50.4 / 56.5.
+    const bool b8 = is_b8(kv->o);
+    // Block-scaled: runs of more slots than a tile, where there are two items to a CU,
+    // share their queries and pages through LDS and caches; from eight of two tiles on they
+    // take two at a time.  us, one tile and two: 512 rows x 16 x 12 heads x 64, 12 layers, 520 /
+    // 449; 2041 rows x 32 query heads on 8 x 128 99 / 99; 2 x 300 of those 17.8 / 22.2.
+    uint64_t o_tile = kSlotTile;
+    bool many = false;
+    if (b8) {
+        uint64_t ones = 0, twos = 0, most_slots = 0;
+        for (const Run& u : runs) {
+            const uint64_t slots = (uint64_t)u.n * group;
+            ones += tiles(slots, kSlotTile);
+            twos += tiles(slots, 2 * kSlotTile);
+            most_slots = std::max(most_slots, slots);
+        }
+        many = most_slots > kSlotTile && ones * lh >= 2 * cus;
+        if (many && twos * lh >= 8 * cus) o_tile = 2 * kSlotTile;
+    }
     uint64_t o_keys = 0, o_units = 0, o_longest = 0;
     for (const Run& u : runs) {
-        const uint64_t n = tiles((uint64_t)u.n * group, kSlotTile);
+        const uint64_t n = tiles((uint64_t)u.n * group, o_tile);
         o_units += n * lh;
         o_keys += n * lh * (u.pos0 + u.n);
         o_longest = std::max<uint64_t>(o_longest, u.pos0 + u.n);
@@ -1576,6 +1595,11 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const uint32_t* at, const ni_pref
         part = between(align_up(o_keys / ((2 * o_units <= cus ? 2 : 4) * cus), 4 * kPage), o_units < cus ? 256 : 512, 16384);
         if (P.wide && o_units >= 2 * cus && o_longest <= 1024) part = std::max<uint64_t>(part, 1024);
     }
+    // Block-scaled: where every item has a CU (or half of one) to itself, eight waves hold
+    // up to 2048 keys, without partials to merge.
+    const bool eight = b8 && !many && o_units <= 2 * cus && o_longest > 128 && o_longest <= 2048 && !split_tokens;
+    if (eight) part = 2048;
+    if (many && !split_tokens) part = std::max<uint64_t>(part, 2048);
     for (uint32_t i = 0, r = 0, u0 = 0; i < n_prefix; r += prefixes[i].n_rows, i++) {
         const ni_prefix& p = prefixes[i];
         const uint32_t p_slots = (uint32_t)((uint64_t)p.n_rows * group);
@@ -1587,8 +1611,8 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const uint32_t* at, const ni_pref
             const uint32_t tab = tab_of(u.seq);
             const bool whole = n_own == 1 && (P.wide || n_pre == 0);
             for (uint64_t j = 0; j < n_own; j++)
-                for (uint64_t s0 = 0; s0 < slots; s0 += kSlotTile) {
-                    const uint32_t ns = (uint32_t)std::min<uint64_t>(kSlotTile, slots - s0);
+                for (uint64_t s0 = 0; s0 < slots; s0 += o_tile) {
+                    const uint32_t ns = (uint32_t)std::min<uint64_t>(o_tile, slots - s0);
                     const uint64_t end = u.pos0 + (s0 + ns - 1) / group + 1;  // of the tile's last row
                     if (j * part >= end) continue;
                     P.items.push_back({tab, u.row0, (uint32_t)s0, ns, u.pos0, (uint32_t)(j * part),
@@ -1611,6 +1635,8 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const uint32_t* at, const ni_pref
     // have two waves to an item in place of four: half as many ends to join (with the
     // prefix's launch, the same 64 rows 71 / 73 us, Q8 57 / 67; 32 rows of 1..100 keys
     // 29.4 / 32.2; one layer of 64 rows 14.7 / 14.1, of up to 1023 keys 31.7 / 29.8).
+    P.block_tiles = many ? (uint32_t)(o_tile / kSlotTile) : 0;
+    P.block_waves = eight ? 8 : 4;
     const bool shared = !P.wide && !P.pitems.empty();  // a launch, with the prefixes' items
     if (shared) {
         P.items.insert(P.items.end(), P.pitems.begin(), P.pitems.end());
@@ -2716,6 +2742,10 @@ static int run_prefix(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const float* q
         a.wide = 0;
         a.row_slots = P.row_slots;
         a.waves = P.row_waves;
+        if (is_b8(kv->o)) {
+            a.wide = P.block_tiles;
+            a.waves = P.block_waves;
+        }
         ProfileScope ps(kv, NI_K_ATTN);
         e = is_b8(kv->o) ? launch_block_attention(a, ref.inl, ref.inl_bytes, s, ps.t)
                          : launch_prefix_attention(a, ref.inl, ref.inl_bytes, s, ps.t);
