@@ -89,11 +89,22 @@ __global__ __launch_bounds__(256) void block_append_kernel(const BlockAppendLaun
     const float before = *scale;
     const uint32_t slots = e.slots & 0xffffu;
     const float* const in = (is_v ? a.v : a.k) + (int64_t)lay * a.layer_stride + head * D;
-    auto row_of = [&](uint32_t p) {  // input row of new position p
-        const uint32_t i = e.src + __popc(slots & ((1u << p) - 1u));
+    // Input row of position p; of one that is not new the first row, whose values are
+    // dropped (loads that no branch parts are in flight together).
+    auto row_of = [&](uint32_t p, bool mine) {
+        const uint32_t i = e.src + (mine ? __popc(slots & ((1u << p) - 1u)) : 0);
         return (int64_t)(e.slots & kListed ? list[i] : i) * a.row_stride;
     };
     const uint32_t hi = lane >> 4, lo = lane & 15u;
+    // What a lane's bytes hold beside new ones is asked for with the rows, not behind them.
+    const uint32_t four = slots >> (4 * hi) & 15u;
+    const bool beside = is_v && four != 0 && four != 15u;
+    u32x4 held[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        held[i] = u32x4{0, 0, 0, 0};
+        if (beside) held[i] = reinterpret_cast<const u32x4*>(block + 1024 * i)[lane];
+    }
     // x[i][4 w + b]: the value of byte 4 w + b of the lane's 16 of run i
     float x[NB][16];
     bool mine[4];  // of V position 4 hi + b is new; of K all alike
@@ -101,13 +112,12 @@ __global__ __launch_bounds__(256) void block_append_kernel(const BlockAppendLaun
     if (!is_v) {
 #pragma unroll
         for (int b = 0; b < 4; b++) mine[b] = slots >> lo & 1;
-        const float* p = in + (mine[0] ? row_of(lo) : 0) + 16 * hi;
+        const float* p = in + row_of(lo, mine[0]) + 16 * hi;
 #pragma unroll
         for (int i = 0; i < NB; i++)
 #pragma unroll
             for (int w = 0; w < 4; w++) {
-                float4 y = {0.f, 0.f, 0.f, 0.f};
-                if (mine[0]) y = *reinterpret_cast<const float4*>(p + 64 * i + 4 * w);
+                const float4 y = *reinterpret_cast<const float4*>(p + 64 * i + 4 * w);
                 x[i][4 * w] = y.x;
                 x[i][4 * w + 1] = y.y;
                 x[i][4 * w + 2] = y.z;
@@ -117,17 +127,18 @@ __global__ __launch_bounds__(256) void block_append_kernel(const BlockAppendLaun
 #pragma unroll
         for (int b = 0; b < 4; b++) {
             mine[b] = slots >> (4 * hi + b) & 1;
-            const float* p = in + (mine[b] ? row_of(4 * hi + b) : 0) + lo;
+            const float* p = in + row_of(4 * hi + b, mine[b]) + lo;
 #pragma unroll
             for (int i = 0; i < NB; i++)
 #pragma unroll
-                for (int w = 0; w < 4; w++) x[i][4 * w + b] = mine[b] ? p[64 * i + 16 * w] : 0.f;
+                for (int w = 0; w < 4; w++) x[i][4 * w + b] = p[64 * i + 16 * w];
         }
     }
 #pragma unroll
     for (int i = 0; i < NB; i++)
 #pragma unroll
         for (int j = 0; j < 16; j++) {
+            x[i][j] = mine[j % 4] ? x[i][j] : 0.f;
             top = fmaxf(top, finite_size(x[i][j]));
             x[i][j] = number(x[i][j]);
         }
@@ -143,8 +154,8 @@ __global__ __launch_bounds__(256) void block_append_kernel(const BlockAppendLaun
 #pragma unroll
         for (int i = 0; i < NB; i++) {
             u32x4* at = reinterpret_cast<u32x4*>(block + 1024 * i) + lane;
-            u32x4 y = {0, 0, 0, 0};
-            if (!all) y = *at;
+            u32x4 y = held[i];
+            if (!all && !beside) y = *at;
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 const uint32_t fresh = e4m3x4(x[i][4 * w], x[i][4 * w + 1], x[i][4 * w + 2], x[i][4 * w + 3], inv);
@@ -157,6 +168,85 @@ __global__ __launch_bounds__(256) void block_append_kernel(const BlockAppendLaun
         }
     }
     if (lane == 0 && (anew || grown)) *scale = pow2(now);
+}
+
+// The same where every page takes one row, as in a decode step: 16 lanes per (page,
+// layer, head) and K or V, 4 D / 64 dims of the row to a lane (with a wave each, whose
+// lanes had little to do, 64 rows x 12 layers x 12 heads took 12.5 us).  Of K a lane stores its own
+// bytes, of V it merges them with the 16 that hold three other positions.  Where the scale
+// grows the lanes go over the block, 16 bytes each in turn.
+template <int D, int INL>
+__global__ __launch_bounds__(256) void block_append_row_kernel(const BlockAppendLaunch a, const PlanArg<INL> pa) {
+    constexpr int NB = D / 64;
+    const uint32_t x16 = threadIdx.x & 15u;
+    const uint32_t H = a.pool.n_head;
+    const uint64_t unit = ((uint64_t)blockIdx.x * 256 + threadIdx.x) / 16;  // ((entry, layer), head, K | V)
+    const uint32_t is_v = (uint32_t)(unit & 1), eh = (uint32_t)(unit / 2), el = eh / H, head = eh - el * H;
+    if (el >= a.n * a.n_lay) return;
+    const uint32_t entry = el / a.n_lay, lay = el - entry * a.n_lay;
+    const uint8_t* plan = plan_base(pa, a.plan);
+    const BlockAppend e = reinterpret_cast<const BlockAppend*>(plan)[entry];
+    uint8_t* const page = reinterpret_cast<uint8_t*>(a.pool.k + (uint64_t)(a.layer0 + lay) * a.pool.layer_halves +
+                                                     (uint64_t)e.page * a.pool.page_halves);
+    uint8_t* const block = page + ((uint64_t)head * 2 + is_v) * kPage * D;
+    float* const scale = reinterpret_cast<float*>(page + a.pool.b8) + 2 * head + is_v;
+    const float before = *scale;
+    const uint32_t slot = (uint32_t)__ffs(e.slots & 0xffffu) - 1u;
+    const uint32_t src = e.slots & kListed ? reinterpret_cast<const uint32_t*>(plan + a.off_list)[e.src] : e.src;
+    const float* const in = (is_v ? a.v : a.k) + (int64_t)lay * a.layer_stride + (int64_t)src * a.row_stride + head * D;
+    // dim of value (i, w): 64 i + 4 x16 + w of K, 64 i + 16 w + x16 of V
+    const float* const mine = in + (is_v ? x16 : 4 * x16);
+    const uint32_t step = is_v ? 16 : 1;
+    u32x4 held[NB];
+    float x[NB][4], top = 0.f;
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        held[i] = reinterpret_cast<const u32x4*>(block + 1024 * i + slot / 4 * 256)[x16];  // (V: beside the new bytes)
+#pragma unroll
+        for (int w = 0; w < 4; w++) x[i][w] = mine[64 * i + step * w];
+    }
+#pragma unroll
+    for (int i = 0; i < NB; i++)
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            top = fmaxf(top, finite_size(x[i][w]));
+            x[i][w] = number(x[i][w]);
+        }
+    top = fmaxf(top, dpp_move<0xb1>(top));
+    top = fmaxf(top, dpp_move<0x4e>(top));
+    top = fmaxf(top, dpp_move<0x141>(top));
+    top = fmaxf(top, dpp_move<0x140>(top));
+    const bool anew = slot == 0;  // the block begins with this row
+    const int old = exp_of(before), need = scale_exp(top), now = anew ? need : max(old, need);
+    const float inv = pow2(-now);
+    const bool grown = !anew && now > old;
+    const float by = old < kMinExp ? 0.f : pow2(max(old - now, -126));
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        u32x4* const words = reinterpret_cast<u32x4*>(block + 1024 * i);
+        const uint32_t fresh = e4m3x4(x[i][0], x[i][1], x[i][2], x[i][3], inv);
+        if (grown)
+            for (uint32_t hi = 0; hi < 4; hi++) {
+                if (is_v ? hi == slot / 4 : x16 == slot) continue;  // (K: the row itself)
+                u32x4 y = words[16 * hi + x16];
+#pragma unroll
+                for (int w = 0; w < 4; w++) y[w] = rescale4(y[w], by);
+                words[16 * hi + x16] = y;
+            }
+        if (is_v) {
+            u32x4 y = held[i];
+            const uint32_t at = 8 * (slot % 4);
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                if (grown) y[w] = rescale4(y[w], by);
+                y[w] = (y[w] & ~(0xffu << at)) | (fresh >> (8 * w) & 0xffu) << at;
+            }
+            words[16 * (slot / 4) + x16] = y;
+        } else {
+            *reinterpret_cast<uint32_t*>(block + k_byte(slot, 64 * i + 4 * x16)) = fresh;
+        }
+    }
+    if (x16 == 0 && (anew || grown)) *scale = pow2(now);
 }
 
 // Eight stored values as f16, exactly (e4m3 lies within f16).
@@ -582,6 +672,11 @@ hipError_t launch_block_append(const BlockAppendLaunch& a, const void* ip, uint3
     if (units == 0) return hipSuccess;
     return with_plan(a, ip, ib, [&](auto pa) {
         constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
+        if (a.single) {
+            if (a.pool.head_dim == 64) return go(block_append_row_kernel<64, INL>, (units + 15) / 16, 256, s, t, a, pa);
+            if (a.pool.head_dim == 128) return go(block_append_row_kernel<128, INL>, (units + 15) / 16, 256, s, t, a, pa);
+            return hipErrorInvalidValue;
+        }
         if (a.pool.head_dim == 64) return go(block_append_kernel<64, INL>, (units + 3) / 4, 256, s, t, a, pa);
         if (a.pool.head_dim == 128) return go(block_append_kernel<128, INL>, (units + 3) / 4, 256, s, t, a, pa);
         return hipErrorInvalidValue;

@@ -2015,6 +2015,7 @@ static int block_append(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const ni_row
     a.n = (uint32_t)entries.size();
     a.layer0 = layer0;
     a.n_lay = n_lay;
+    a.single = entries.size() == n;
     hipError_t e;
     {
         ProfileScope ps(kv, NI_K_APPEND);

@@ -156,6 +156,7 @@ struct BlockAppendLaunch {
     uint32_t off_list;
     uint32_t n;
     uint32_t layer0, n_lay;
+    uint32_t single;  // every page takes one row
 };
 
 // f32 values of rows (AppendEntry, src_row = output row), any pool.
