@@ -29,6 +29,7 @@ library and fails if it cannot.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
 from dataclasses import dataclass
 from operator import index
 from typing import Optional, Sequence
@@ -196,6 +197,11 @@ def _pointer(arr, empty, item):
 
 def _u32_array(x, name) -> np.ndarray:
     """Host integers of any shape as a flat uint32 array."""
+    if type(x) is list:
+        try:
+            return np.frombuffer(array("I", x), dtype=np.uint32)  # (refuses what is no integer of 32 bits)
+        except (TypeError, OverflowError):
+            pass  # lists of lists, or what is said below
     a = np.asarray(x)
     if a.size and (a.dtype.kind not in "iu" or a.min() < 0 or a.max() > 0xffffffff):
         raise ValueError(f"{name} must be integers in 0..2^32-1")
@@ -473,11 +479,15 @@ class PagedKv:
         """Write f32 K/V rows as f16 into their pages (b_kv_write)."""
         arr, rp, n = _rows(rows)
         layered = layer == ALL_LAYERS
-        rs, ls = self._f32(k, "k", layered, n)
-        rs2, ls2 = self._f32(v, "v", layered, n)
-        if (rs, ls) != (rs2, ls2):
-            raise ValueError("k and v must share strides")
-        self._on_device(k=k, v=v)
+        _torch()
+        fits = _fits_layers if layered else _fits_row
+        s = fits(k, n, self._c, self._n_layer, self.device)
+        if s is None or fits(v, n, self._c, self._n_layer, self.device) != s:
+            s = self._f32(k, "k", layered, n)
+            if s != self._f32(v, "v", layered, n):
+                raise ValueError("k and v must share strides")
+            self._on_device(k=k, v=v)
+        rs, ls = s
         self._check(self._L.ni_kv_append(self._h, layer, rp, n, k.data_ptr(), v.data_ptr(), rs, ls,
                                          _stream_ptr(stream)))
 
@@ -566,12 +576,20 @@ class PagedKv:
         torch = _torch()
         arr, rp, n = _rows(rows)
         c, layered = self._c, layer == ALL_LAYERS
-        with _on(self.device, stream) as s:
-            k, v = (torch.empty((self._n_layer, n, c) if layered else (n, c), dtype=torch.float32, device="cuda")
-                    for _ in range(2))
-            self._check(self._L.ni_kv_gather_values(self._h, layer, rp, n, k.data_ptr(), v.data_ptr(), c,
+        shape = (2, self._n_layer, n, c) if layered else (2, n, c)
+        s = None if self.device is None else _stream_now(self.device, stream)
+        if s is not None:
+            both = torch.empty(shape, dtype=_float32, device="cuda")
+            at = both.data_ptr()
+            self._check(self._L.ni_kv_gather_values(self._h, layer, rp, n, at, at + both.nbytes // 2, c,
                                                     n * c if layered else 0, s))
-        return k, v
+            return both.unbind(0)
+        with _on(self.device, stream) as s:
+            both = torch.empty(shape, dtype=_float32, device="cuda")
+            at = both.data_ptr()
+            self._check(self._L.ni_kv_gather_values(self._h, layer, rp, n, at, at + both.nbytes // 2, c,
+                                                    n * c if layered else 0, s))
+        return both.unbind(0)
 
     def attention(self, q, rows, out=None, layer: int = ALL_LAYERS, split_tokens: int = 0, stream=None):
         """Paged decode attention of each row over keys 0..pos of its sequence."""

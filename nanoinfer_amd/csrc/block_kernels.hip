@@ -627,24 +627,25 @@ __global__ __launch_bounds__(256) void values_kernel(const ValuesLaunch a, const
     const uint32_t is_v = u / (a.pool.n_head * quads);
     u -= is_v * a.pool.n_head * quads;
     const uint32_t head = u / quads, x = u - head * quads;
-    const AppendEntry e = reinterpret_cast<const AppendEntry*>(plan_base(pa, a.plan) + a.off_entries)[row];
-    const uint16_t* const page = a.pool.k + (uint64_t)(a.layer0 + lay) * a.pool.layer_halves + (uint64_t)e.page * a.pool.page_halves;
-    float* const out = (is_v ? a.v_out : a.k_out) + (int64_t)lay * a.layer_stride + (int64_t)e.src_row * a.row_stride + head * D;
+    const uint32_t place = reinterpret_cast<const uint32_t*>(plan_base(pa, a.plan) + a.off_entries)[row], slot = place % kPage;
+    const uint16_t* const page = a.pool.k + (uint64_t)(a.layer0 + lay) * a.pool.layer_halves +
+                                 (uint64_t)(place / kPage) * a.pool.page_halves;
+    float* const out = (is_v ? a.v_out : a.k_out) + (int64_t)lay * a.layer_stride + (int64_t)row * a.row_stride + head * D;
     float4 y;
     if (a.pool.b8) {
         const uint8_t* block = reinterpret_cast<const uint8_t*>(page) + (head * 2 + is_v) * kPage * D;
         const float scale = reinterpret_cast<const float*>(reinterpret_cast<const uint8_t*>(page) + a.pool.b8)[2 * head + is_v];
         if (!is_v) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(block + k_byte(e.slot, 4 * x));
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(block + k_byte(slot, 4 * x));
             const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
             y = float4{lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
         } else {
             const uint32_t d = x / 16 * 64 + x % 16;
-            const u32x4 w = *reinterpret_cast<const u32x4*>(block + (v_byte(e.slot, d) & ~15u));
+            const u32x4 w = *reinterpret_cast<const u32x4*>(block + (v_byte(slot, d) & ~15u));
             float z[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                z[i] = __builtin_amdgcn_cvt_f32_fp8((int)(w[i] >> (8 * (e.slot % 4))), 0) * scale;
+                z[i] = __builtin_amdgcn_cvt_f32_fp8((int)(w[i] >> (8 * (slot % 4))), 0) * scale;
                 out[d + 16 * i] = z[i];
             }
             return;
@@ -653,11 +654,11 @@ __global__ __launch_bounds__(256) void values_kernel(const ValuesLaunch a, const
         const uint16_t* block = page + (uint64_t)head * a.pool.head_halves + (is_v ? a.pool.head_halves / 2 : 0);
         if (a.pool.q8) {
             const uint8_t* b = reinterpret_cast<const uint8_t*>(block);
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(b + e.slot * D + 4 * x);
-            const float scale = reinterpret_cast<const float*>(b + kPage * D)[e.slot];
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(b + slot * D + 4 * x);
+            const float scale = reinterpret_cast<const float*>(b + kPage * D)[slot];
             y = float4{i8f(w, 0) * scale, i8f(w, 1) * scale, i8f(w, 2) * scale, i8f(w, 3) * scale};
         } else {
-            const half4_t h = *reinterpret_cast<const half4_t*>(block + e.slot * D + 4 * x);
+            const half4_t h = *reinterpret_cast<const half4_t*>(block + slot * D + 4 * x);
             y = float4{(float)h[0], (float)h[1], (float)h[2], (float)h[3]};
         }
     }

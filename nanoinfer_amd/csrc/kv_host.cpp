@@ -2541,11 +2541,11 @@ int ni_kv_gather_values(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
     if (rows_overlap(n, row_stride, all ? n_lay : 1, layer_stride, C))
         return kv->fail(NI_ERR_BAD_ARG, "k_out's rows of %llu values overlap", (unsigned long long)C);
     std::vector<uint8_t>& blob = kv->blob;
-    blob.resize(align_up((size_t)n * sizeof(AppendEntry), kAlign));
-    AppendEntry* entries = reinterpret_cast<AppendEntry*>(blob.data());
+    blob.resize(align_up((size_t)n * sizeof(uint32_t), kAlign));
+    uint32_t* entries = reinterpret_cast<uint32_t*>(blob.data());
     for (uint32_t i = 0; i < n; i++) {
         if (int rc = check_row(kv, rows[i])) return rc;
-        entries[i] = {i, kv->pages[rows[i].seq][rows[i].pos / kPage], rows[i].pos % kPage, 0};
+        entries[i] = kv->pages[rows[i].seq][rows[i].pos / kPage] * kPage + rows[i].pos % kPage;
     }
     DeviceScope device(kv->device);
     const hipStream_t s = (hipStream_t)stream;

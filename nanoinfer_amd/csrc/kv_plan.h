@@ -159,7 +159,8 @@ struct BlockAppendLaunch {
     uint32_t single;  // every page takes one row
 };
 
-// f32 values of rows (AppendEntry, src_row = output row), any pool.
+// f32 values of rows, any pool; entry i: page * kPage + slot of row i (32 bits: a
+// device holds no pool of 2^28 pages, of 2 KB at least).
 struct ValuesLaunch {
     PoolGeom pool;
     float* k_out;
