@@ -266,7 +266,6 @@ def _prepare_pages(case, seed):
         kv = _cache(case, n_pages, order, 2 * case["seqs"] * case["beams"] + case["seqs"], max(ctx) + case["grown"],
                     q8=case["fmt"] == "int8")
         pool = torch.as_tensor(_Pool(kv), device="cuda").view(contents.shape)
-        pool.copy_(contents)
         state = dict(case=case, kv=kv, pool=pool, ctx=ctx, live=[])
         for n in ctx:
             state["live"].append(kv.add_seq())
@@ -280,6 +279,7 @@ def _prepare_pages(case, seed):
                     kv.commit(s, case["grown"])
             state["beams"] = [s for beams in groups for s in beams]
             state["parents"] = [beams[w] for beams, p in zip(groups, _parents(case)) for w in p]
+        pool.copy_(contents)  # (behind the copies that forks have made)
         return state
     state = dict(case=case, pool=contents)
     if case["op"] == "compact":
