@@ -389,7 +389,8 @@ struct DeviceBufs {
 
 // Algorithmic bytes of one step: each KV byte once, append and q/out rows.
 // kvb = stored bytes of one position's K (or V) in one layer: 2C for f16,
-// C + 4 * n_head for Q8 (int8 values and a scale per head).
+// C + 4 * n_head for Q8 (int8 values and a scale per head), C + n_head / 4 for the
+// block-scaled cache (a scale per head of 16 positions).
 double step_bytes(const ni_work* w, uint32_t n, const uint32_t* ctx, uint32_t n_layer, uint32_t c, double kvb) {
     double b = 0;
     for (uint32_t i = 0; i < n; i++) {
@@ -417,7 +418,9 @@ struct Runner {
 
     explicit Runner(const ni_drive_opts& opts) : o(opts), C(opts.kv.n_head * opts.kv.head_dim), L(opts.kv.n_layer) {
         ls = (int64_t)opts.kv.max_rows * C;
-        kvb = (opts.kv.flags & NI_KV_Q8) ? (double)C + 4.0 * opts.kv.n_head : 2.0 * C;
+        kvb = opts.kv.flags & NI_KV_Q8   ? (double)C + 4.0 * opts.kv.n_head
+              : opts.kv.flags & NI_KV_B8 ? (double)C + 0.25 * opts.kv.n_head
+                                         : 2.0 * C;
     }
     ~Runner() {
         if (stream) (void)hipStreamDestroy(stream);

@@ -4,7 +4,7 @@
 // one JSON line.
 //
 //   ni_drive [serve|spec|qkv|prefill] [--per-layer|--step-layers] [--steps K] [--warmup W]
-//            [--ramp R] [--split T] [--all-prompt-rows] [--seed S] [--rows N] [--q8]
+//            [--ramp R] [--split T] [--all-prompt-rows] [--seed S] [--rows N] [--q8|--block8]
 //            [--wfmt f32|f16|q8_0|q4_0]
 //
 // --ramp: R append-only iterations (no attention) before the warmup.
@@ -15,6 +15,9 @@
 //
 // prefill: 16 sequences append and attend N-row prompts (default 512) from
 // empty, every row queried, rolled back each iteration.
+//
+// --block8: the block-scaled cache, one ni_kv_step per iteration or --per-layer
+// (it has no --step-layers and no qkv).
 //
 // qkv: the QKV projection of N rows per layer with K/V appended in its
 // epilogue, weights in --wfmt; --per-layer runs the unfused path (f32
@@ -32,7 +35,7 @@ static uint32_t pages(uint32_t n) { return (n + NI_KV_BLOCK - 1) / NI_KV_BLOCK; 
 int main(int argc, char** argv) {
     ni_drive_opts o{};
     std::string workload = "serve";
-    bool q8 = false;  // the Q8 cache (NI_KV_Q8)
+    bool q8 = false, block8 = false;  // the Q8 cache (NI_KV_Q8), the block-scaled one (NI_KV_B8)
     o.launch = NI_DRIVE_STEP;
     o.steps = 2000;
     o.warmup = 300;
@@ -50,6 +53,7 @@ int main(int argc, char** argv) {
         if (!strcmp(a, "serve") || !strcmp(a, "spec") || !strcmp(a, "qkv") || !strcmp(a, "prefill")) workload = a;
         else if (!strcmp(a, "--rows")) o.qkv_rows = (uint32_t)atoi(val(a));
         else if (!strcmp(a, "--q8")) q8 = true;
+        else if (!strcmp(a, "--block8")) block8 = true;
         else if (!strcmp(a, "--wfmt")) {  // qkv: f32 (default), f16, q8_0, q4_0
             const char* f = val(a);
             if (!strcmp(f, "f32")) o.qkv_wformat = NI_W_F32;
@@ -71,7 +75,7 @@ int main(int argc, char** argv) {
         else if (!strcmp(a, "--seed")) o.data_seed = o.serve.seed = strtoull(val(a), nullptr, 10);
         else {
             fprintf(stderr, "usage: ni_drive [serve|spec|qkv|prefill] [--per-layer|--step-layers] [--steps K] [--warmup W] "
-                            "[--ramp R] [--split T] [--all-prompt-rows] [--seed S] [--rows N] [--q8] [--wfmt F]\n");
+                            "[--ramp R] [--split T] [--all-prompt-rows] [--seed S] [--rows N] [--q8|--block8] [--wfmt F]\n");
             return 2;
         }
     }
@@ -119,6 +123,7 @@ int main(int argc, char** argv) {
         o.kv.max_rows = 512;
     }
     if (q8) o.kv.flags |= NI_KV_Q8;
+    if (block8) o.kv.flags |= NI_KV_B8;
     ni_drive_result r{};
     if (int rc = ni_drive_run(&o, &r)) {
         fprintf(stderr, "ni_drive: %s (status %d)\n", ni_drive_last_error(), rc);
@@ -138,7 +143,7 @@ int main(int argc, char** argv) {
            "\"mean_context\": %.1f, \"kv\": \"%s\", \"idle_us_plan_call\": %.2f, \"idle_us_layer_call\": %.2f}\n",
            workload.c_str(), o.launch == NI_DRIVE_STEP ? "step" : o.launch == NI_DRIVE_PER_LAYER ? "per-layer" : "step-layers", r.steps, o.ramp, o.warmup, gbs,
            100.0 * gbs / 8000.0, r.seconds / r.steps * 1e3, r.gpu_seconds / r.steps * 1e3, r.host_us_per_step,
-           (double)r.launches / r.steps, r.seq_tokens / r.seconds, r.bytes / r.steps, r.mean_live, r.mean_context, q8 ? "q8" : "f16",
+           (double)r.launches / r.steps, r.seq_tokens / r.seconds, r.bytes / r.steps, r.mean_live, r.mean_context, q8 ? "q8" : block8 ? "block8" : "f16",
            r.idle_us_plan_call, r.idle_us_layer_call);
     return 0;
 }
