@@ -378,7 +378,7 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
             split8(y, hi, lo);
         };
         if constexpr (kShared) {
-            static_assert(W == 4, "a step of every tile to a wave, or two");
+            static_assert(!kShared || W == 4, "a step of every tile to a wave, or two");
             if (NB == 2 || wave / 2 == t) {  // (one tile of 64 dims: two waves have none)
                 const int i = NB == 2 ? wave / 2 : 0, j = wave % 2;
                 half8_t hi, lo;
@@ -689,6 +689,7 @@ static hipError_t block_attn_t(const PrefixLaunch& a, uint64_t blocks, hipStream
     if (a.wide == 2) return go(block_attn_kernel<D, 2, 4, true, INL>, blocks, 256, s, t, a, pa);
     if (a.wide == 1) return go(block_attn_kernel<D, 1, 4, true, INL>, blocks, 256, s, t, a, pa);
     if (a.waves == 8) return go(block_attn_kernel<D, 1, 8, false, INL>, blocks, 512, s, t, a, pa);
+    if (a.waves == 2) return go(block_attn_kernel<D, 1, 2, false, INL>, blocks, 128, s, t, a, pa);
     return go(block_attn_kernel<D, 1, 4, false, INL>, blocks, 256, s, t, a, pa);
 }
 

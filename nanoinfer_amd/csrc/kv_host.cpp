@@ -1636,7 +1636,6 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const uint32_t* at, const ni_pref
     // prefix's launch, the same 64 rows 71 / 73 us, Q8 57 / 67; 32 rows of 1..100 keys
     // 29.4 / 32.2; one layer of 64 rows 14.7 / 14.1, of up to 1023 keys 31.7 / 29.8).
     P.block_tiles = many ? (uint32_t)(o_tile / kSlotTile) : 0;
-    P.block_waves = eight ? 8 : 4;
     const bool shared = !P.wide && !P.pitems.empty();  // a launch, with the prefixes' items
     if (shared) {
         P.items.insert(P.items.end(), P.pitems.begin(), P.pitems.end());
@@ -1645,6 +1644,8 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const uint32_t* at, const ni_pref
     const bool rows_alone = std::all_of(runs.begin(), runs.end(), [](const Run& u) { return u.n == 1; });
     P.row_slots = !shared && !is_b8(kv->o) && group <= (is_q8(kv->o) ? 1u : 2u) && rows_alone ? group : 0;
     P.row_waves = P.items.size() * lh >= 12 * cus ? 2 : 4;
+    // (block-scaled: 64 rows of 1..767 keys, 12 layers x 12 heads, 82 / 77)
+    P.block_waves = eight ? 8 : P.row_waves;
     // Longest first, so that no launch ends on a long item.  Of a launch whose
     // workgroups are all on the CUs at once, block b shares a CU with blocks b +-
     // CUs, b +- 2 CUs: every second round of CUs runs shortest first.
