@@ -1,7 +1,8 @@
 // block_kernels.hip -- gfx950 kernels of the block-scaled cache (NI_KV_B8): e4m3
 // values, one power-of-two scale for each (page, head) of K and of V.
 //
-//   block_append_kernel   f32 rows into the pages, scales grown where they must
+//   block_append_kernel, block_append_row_kernel   f32 rows into the pages, scales
+//                         grown where they must
 //   block_attn_kernel     16 slots (query heads of rows that read the same cache
 //                         head) over a run of keys, on the matrix cores
 //   values_kernel         what the cache stands for, in f32 (any pool)
@@ -69,6 +70,9 @@ __device__ __forceinline__ float finite_size(float x) {
 // bytes that it loads in block_attn_kernel: of K a position's 16 dims (those of
 // positions that are not new only where the scale grows), of V four positions
 // of four dims, merged with what is there where not all of them are new.
+// Bound by memory, from some thousand waves on (84 MB 21 us, 4.0 TB/s); of 2047 rows of 8 heads x
+// 128, 21 MB in 2064 waves, 9.1 us, the launch's start and each wave's loads, maximum and stores,
+// one after another, are half.
 template <int D, int INL>
 __global__ __launch_bounds__(256) void block_append_kernel(const BlockAppendLaunch a, const PlanArg<INL> pa) {
     constexpr int NB = D / 64;
@@ -172,7 +176,8 @@ __global__ __launch_bounds__(256) void block_append_kernel(const BlockAppendLaun
 
 // The same where every page takes one row, as in a decode step: 16 lanes per (page,
 // layer, head) and K or V, 4 D / 64 dims of the row to a lane (with a wave each, whose
-// lanes had little to do, 64 rows x 12 layers x 12 heads took 12.5 us).  Of K a lane stores its own
+// lanes had little to do, 64 rows x 12 layers x 12 heads took 12.5 us, so 5.4; of one layer 3.6,
+// a launch).  Of K a lane stores its own
 // bytes, of V it merges them with the 16 that hold three other positions.  Where the scale
 // grows the lanes go over the block, 16 bytes each in turn.
 template <int D, int INL>
@@ -285,6 +290,12 @@ __device__ __forceinline__ void scale_in_place(float4_t& x, float by) {
 // are P^T's operand as they are.  The W waves take two pages each in turn, the next
 // ones' loads issued before the products of these; their states are joined through
 // LDS.
+//   Bound by memory for one tile: 16 sequences of 32 k keys, 4 query heads to each of 8 cache
+// heads x 128, 1.03 GB, 159 us, 6.5 TB/s; 64 rows of 1..767 keys, 12 layers x 12 heads x 64, 0.41 GB,
+// 77 us, 5.3 TB/s (short items: a start and a join to each 2 to 24 turns).  Two tiles are bound by
+// what their waves issue: a prompt of 2041 rows x 32 query heads on 8 x 128, 34 GFLOP (69 with hi
+// + lo), 101 us, of which the matrix cores are busy 28 and vector instructions (157 of a wave for
+// two tiles of a page, 32 of them conversions) issue for 34.
 template <int D, int NT, int W, bool MANY, int INL>
 __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
     constexpr int NB = D / 64, PB = 2, NC = 4 * NB;  // runs of 64 dims; pages of an iteration; 16-dim chunks
@@ -614,6 +625,7 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
     }
 }
 
+// Bound by the launch and its stores: 2047 rows of 8 heads x 128, 21 MB, 8.3 us; 64 rows 3.7.
 // A thread takes four dims of a row and head of K or V: dims d .. + 3, of a
 // block-scaled V dims d, d + 16, d + 32, d + 48 (one word of four positions each).
 template <int INL>
@@ -708,6 +720,7 @@ hipError_t launch_block_attention(const PrefixLaunch& a, const void* ip, uint32_
 hipError_t launch_gather_values(const ValuesLaunch& a, const void* ip, uint32_t ib, hipStream_t s) {
     const uint64_t threads = (uint64_t)a.n_lay * a.n_rows * 2 * a.pool.n_head * (a.pool.head_dim / 4);
     if (threads == 0) return hipSuccess;
+    if (threads > 0xffffff00ull) return hipErrorInvalidValue;  // (handles allow 2^32 - 32)
     return with_plan(a, ip, ib, [&](auto pa) {
         constexpr int INL = sizeof(pa.b) > 4 ? (int)sizeof(pa.b) : 0;
         return go(values_kernel<INL>, (threads + 255) / 256, 256, s, {}, a, pa);

@@ -1,5 +1,6 @@
 // kv_device.h -- device helpers the gfx950 kernels share (kv_kernels.hip,
-// rotary_kernels.hip, prefix_kernels.hip, verify_kernels.hip): vector types,
+// rotary_kernels.hip, prefix_kernels.hip, verify_kernels.hip, page_kernels.hip,
+// block_kernels.hip, beam_kernels.hip): vector types,
 // f32 -> f16 and Q8 conversions, plans passed with the launch arguments, LDS
 // tiles and DMA, and the launch helpers.
 #pragma once

@@ -1,7 +1,7 @@
 // kv_plan.h -- the per-call plan the host builds and the kernels read.
 //
 // Shared by the host side (kv_host.cpp) and the gfx950 kernels
-// (kv_kernels.hip).  A data-path call turns its rows into a compact plan
+// (kv_kernels.hip, page_kernels.hip).  A data-path call turns its rows into a compact plan
 // (append destinations, attention work items, merge items and the block-table
 // segments those items read), uploads it with one async copy and launches the
 // kernels over it.  The device never sees the host's full block tables.
