@@ -90,6 +90,8 @@ enum ni_status {
  * begins anew when the block's first position is written, whatever is then
  * in the positions that the call does not write, and never shrinks else.  Inputs
  * must be finite: a NaN is stored as 0, an infinity as the block's largest value.
+ * In attention, values of a block whose scale lies more than 2^83 below the
+ * largest that the row has met so far add nothing.
  * The append, steps (not ni_kv_step_noalloc, not one layer at a time), decode
  * steps, both attention calls and ni_kv_gather_values take such handles, the
  * others refuse them. */

@@ -275,13 +275,9 @@ constexpr float kRefLog2 = 10.f, kRefSlack = 5.f, kRefUnscale = 1.f / 1024.f;
 // Weights of a page whose value scale is 2^-k of the outputs' unit enter a product 2^k
 // smaller up to this k: what that costs them lies 2^-32 below the page's largest.
 constexpr int kNear = 6;
-
-// (in place: the compiler would keep both and copy where the multiplication is passed by.  A
-// matrix product may still be writing x: its 16 passes are waited for; and one may read it next.)
-__device__ __forceinline__ void scale_in_place(float4_t& x, float by) {
-    asm volatile("s_nop 15\n\ts_nop 3\n\tv_mul_f32 %0, %4, %0\n\tv_mul_f32 %1, %4, %1\n\tv_mul_f32 %2, %4, %2\n\tv_mul_f32 %3, %4, %3\n\ts_nop 1"
-                 : "+v"(x[0]), "+v"(x[1]), "+v"(x[2]), "+v"(x[3]) : "v"(by));
-}
+// Others are added with the outputs brought to their units, where these stay finite: weights
+// below 2^15, values below 2^9, a million keys to a wave.  Smaller scales add nothing.
+constexpr int kFar = 83;
 
 // One (item, layer, head), NT tiles of 16 slots: S^T = K Q^T (16 keys x 16 slots; q
 // in f16 hi + lo parts, keys as stored, their page's scale on the sums), the online
@@ -294,15 +290,16 @@ __device__ __forceinline__ void scale_in_place(float4_t& x, float by) {
 // heads x 128, 1.03 GB, 159 us, 6.5 TB/s; 64 rows of 1..767 keys, 12 layers x 12 heads x 64, 0.41 GB,
 // 77 us, 5.3 TB/s (short items: a start and a join to each 2 to 24 turns).  Two tiles are bound by
 // what their waves issue: a prompt of 2041 rows x 32 query heads on 8 x 128, 34 GFLOP (69 with hi
-// + lo), 101 us, of which the matrix cores are busy 28 and vector instructions (157 of a wave for
-// two tiles of a page, 32 of them conversions) issue for 34.
+// + lo), 84 us, of which the matrix cores are busy 28 and vector instructions (some 160 of a wave
+// for two tiles of a page, 32 of them conversions) issue for 35; 512 rows x 16 x 12 heads x 64, 12
+// layers, 380 us.
 template <int D, int NT, int W, bool MANY, int INL>
 __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
     constexpr int NB = D / 64, PB = 2, NC = 4 * NB;  // runs of 64 dims; pages of an iteration; 16-dim chunks
     // MANY: the queries are held once for all waves, in LDS, as each lane's operands.
     constexpr bool kShared = MANY;
     __shared__ union Lds {
-        float red[W][NT * kSlotTile][D + 4];  // m, l, -, -, o
+        float red[W][kSlotTile][D + 4];  // of a tile: m, l, -, -, o
         half8_t q[NT][NB][2][kShared ? 2 : 1][64];
         __device__ Lds() {}
     } lds;
@@ -464,8 +461,8 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
         uint32_t next_id[PB];
         scales(id, next_ks, next_vs);
         pages(pg + 2 * W * PB, next_id);
-        // Outputs are kept in units of the largest value scale so far, 2^unit: exact, down to
-        // 2^-126 of it.  The weights of pages whose scale is no more than 2^kNear smaller
+        // Outputs are kept in units of the largest value scale so far, 2^unit: exact, as far as
+        // f32 reaches.  The weights of pages whose scale is no more than 2^kNear smaller
         // are taken in those units too, and both pages enter one product.
         const int e0 = exp_of(vs[0]), e1 = exp_of(vs[1]);
         if (max(e0, e1) > unit) {
@@ -474,13 +471,13 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
 #pragma unroll
                 for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int c = 0; c < NC; c++) scale_in_place(o[t][c], down);
+                    for (int c = 0; c < NC; c++) o[t][c] *= down;
             }
             unit = max(e0, e1);
         }
         const int below[PB] = {unit - e0, unit - e1};
         const bool near = max(below[0], below[1]) <= kNear;
-        half4_t ph[NT][PB], pl[NT][PB];
+        half8_t wh[NT], wl[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             float s[PB][4];
@@ -514,7 +511,7 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
                 if (__any(alpha != 1.f)) {
                     lsum[t] *= alpha;
 #pragma unroll
-                    for (int c = 0; c < NC; c++) scale_in_place(o[t][c], alpha);
+                    for (int c = 0; c < NC; c++) o[t][c] *= alpha;
                 }
                 mref[t] += d;
 #pragma unroll
@@ -522,21 +519,31 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
 #pragma unroll
                     for (int j = 0; j < 4; j++) s[b][j] -= d;
             }
+            half4_t ph[PB], pl[PB];
 #pragma unroll
             for (int b = 0; b < PB; b++) {
                 float p[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) p[j] = fast_exp2(s[b][j]);
                 lsum[t] += ((p[0] + p[1]) + (p[2] + p[3])) * (near ? pow2(below[b]) : 1.f);
-                split4(p, ph[t][b], pl[t][b]);
+                split4(p, ph[b], pl[b]);
             }
+            wh[t] = __builtin_shufflevector(ph[0], ph[1], 0, 1, 2, 3, 4, 5, 6, 7);
+            wl[t] = __builtin_shufflevector(pl[0], pl[1], 0, 1, 2, 3, 4, 5, 6, 7);
         }
-        if (near) {
-            half8_t wh[NT], wl[NT];
+        // Both pages at once, or one at a time, the outputs in its units meanwhile.  (One body for
+        // both, which drops the other page's values: with one of its own for pages by themselves
+        // the compiler kept the outputs twice, 220 registers and two waves to a SIMD in place of 154
+        // and three: the prompt below 102 us.)
+#pragma unroll 1
+        for (int b = 0; b < (near ? 1 : PB); b++) {
+            const int by = near ? 0 : min(b ? below[1] : below[0], kFar + 1);
+            const uint32_t with0 = near || (b == 0 && by <= kFar) ? ~0u : 0u, with1 = near || (b == 1 && by <= kFar) ? ~0u : 0u;
+            if (by) {
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                wh[t] = __builtin_shufflevector(ph[t][0], ph[t][1], 0, 1, 2, 3, 4, 5, 6, 7);
-                wl[t] = __builtin_shufflevector(pl[t][0], pl[t][1], 0, 1, 2, 3, 4, 5, 6, 7);
+                for (int t = 0; t < NT; t++)
+#pragma unroll
+                    for (int c = 0; c < NC; c++) o[t][c] *= by <= kFar ? pow2(by) : 1.f;
             }
             constexpr int G = 4 / NT;  // chunks at a time
 #pragma unroll
@@ -545,7 +552,7 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
 #pragma unroll
                 for (int g = 0; g < G; g++) {
                     const int i = (c0 + g) / 4, c = (c0 + g) % 4;
-                    v8[g] = e4m3_f16x8(cur.v[0][i][c], cur.v[1][i][c]);
+                    v8[g] = e4m3_f16x8(cur.v[0][i][c] & with0, cur.v[1][i][c] & with1);
                 }
 #pragma unroll
                 for (int g = 0; g < G; g++)
@@ -558,24 +565,11 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
                     for (int t = 0; t < NT; t++)
                         o[t][c0 + g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v8[g], wh[t], o[t][c0 + g], 0, 0, 0);
             }
-        } else {
-            // Each page's sums by themselves, then in those units.
-#pragma unroll 1
-            for (int b = 0; b < PB; b++) {
-                const float down = pow2(max(-(b ? below[1] : below[0]), -126));
+            if (by) {
 #pragma unroll
-                for (int i = 0; i < NB; i++)
+                for (int t = 0; t < NT; t++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        const half4_t v4 = e4m3_f16x4(b ? cur.v[1][i][c] : cur.v[0][i][c]);
-#pragma unroll
-                        for (int t = 0; t < NT; t++) {
-                            float4_t x = {0.f, 0.f, 0.f, 0.f};
-                            x = __builtin_amdgcn_mfma_f32_16x16x16f16(v4, b ? pl[t][1] : pl[t][0], x, 0, 0, 0);
-                            x = __builtin_amdgcn_mfma_f32_16x16x16f16(v4, b ? ph[t][1] : ph[t][0], x, 0, 0, 0);
-                            o[t][4 * i + c] += x * down;
-                        }
-                    }
+                    for (int c = 0; c < NC; c++) o[t][c] *= by <= kFar ? pow2(-by) : 1.f;
             }
         }
         if (kBeside && more) cur = nxt;
@@ -587,40 +581,43 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
             id[b] = next_id[b];
         }
     }
-    if constexpr (kShared) __syncthreads();  // the queries' LDS becomes `red`
+    // The waves' states of a tile at a time, through LDS.
 #pragma unroll
     for (int t = 0; t < NT; t++) {
+        if (kShared || t) __syncthreads();  // (the queries, or the last tile's states, are read)
+        const uint32_t first = t * kSlotTile;
         const float l = rows4_sum(lsum[t]);
-        const int sl = t * (int)kSlotTile + col;
-        if (sl < (int)it.ns) {
-            if (rg == 0) *reinterpret_cast<float2*>(&red[wave][sl][0]) = float2{set[t] ? mref[t] + kRefLog2 : kMinScore, l * kRefUnscale};
+        if (first + col < it.ns) {
+            if (rg == 0) *reinterpret_cast<float2*>(&red[wave][col][0]) = float2{set[t] ? mref[t] + kRefLog2 : kMinScore, l * kRefUnscale};
 #pragma unroll
             for (int c = 0; c < NC; c++)
-                *reinterpret_cast<float4_t*>(&red[wave][sl][4 + c * 16 + 4 * rg]) = o[t][c] * (kRefUnscale * pow2(max(unit, kMinExp)));
+                *reinterpret_cast<float4_t*>(&red[wave][col][4 + c * 16 + 4 * rg]) = o[t][c] * (kRefUnscale * pow2(max(unit, kMinExp)));
         }
-    }
-    __syncthreads();
-    for (uint32_t t = threadIdx.x; t < it.ns * (D / 4); t += 64 * W) {
-        const uint32_t sl = t / (D / 4), d = t % (D / 4) * 4;
-        float M = red[0][sl][0];
+        __syncthreads();
+        const uint32_t slots = it.ns > first ? min(it.ns - first, kSlotTile) : 0u;
+        for (uint32_t u = threadIdx.x; u < slots * (D / 4); u += 64 * W) {
+            const uint32_t sl = u / (D / 4), d = u % (D / 4) * 4;
+            float M = red[0][sl][0];
 #pragma unroll
-        for (int w = 1; w < W; w++) M = fmaxf(M, red[w][sl][0]);
-        float L = 0.f;
-        float4_t O = {0.f, 0.f, 0.f, 0.f};
+            for (int w = 1; w < W; w++) M = fmaxf(M, red[w][sl][0]);
+            float L = 0.f;
+            float4_t O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int w = 0; w < W; w++) {
-            const float wt = fast_exp2(red[w][sl][0] - M);
-            L += red[w][sl][1] * wt;
-            O += *reinterpret_cast<const float4_t*>(&red[w][sl][4 + d]) * wt;
-        }
-        if (it.part0 == kNoSlot) {
-            const uint32_t r = (it.slot0 + sl) / a.group, gg = it.slot0 + sl - r * a.group;
-            *reinterpret_cast<float4_t*>(a.out + (int64_t)lay * a.out_layer_stride +
-                                         (int64_t)(it.row0 + r) * a.out_row_stride + (head * a.group + gg) * D + d) = O / L;
-        } else {
-            const uint64_t part = ((uint64_t)(it.part0 + sl) * a.n_lay + lay) * H + head;
-            *reinterpret_cast<float4_t*>(a.part_o + part * D + d) = O;
-            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = float2{M, L};
+            for (int w = 0; w < W; w++) {
+                const float wt = fast_exp2(red[w][sl][0] - M);
+                L += red[w][sl][1] * wt;
+                O += *reinterpret_cast<const float4_t*>(&red[w][sl][4 + d]) * wt;
+            }
+            const uint32_t slot = first + sl;
+            if (it.part0 == kNoSlot) {
+                const uint32_t r = (it.slot0 + slot) / a.group, gg = it.slot0 + slot - r * a.group;
+                *reinterpret_cast<float4_t*>(a.out + (int64_t)lay * a.out_layer_stride +
+                                             (int64_t)(it.row0 + r) * a.out_row_stride + (head * a.group + gg) * D + d) = O / L;
+            } else {
+                const uint64_t part = ((uint64_t)(it.part0 + slot) * a.n_lay + lay) * H + head;
+                *reinterpret_cast<float4_t*>(a.part_o + part * D + d) = O;
+                if (d == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = float2{M, L};
+            }
         }
     }
 }

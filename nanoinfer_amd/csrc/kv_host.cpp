@@ -1569,7 +1569,7 @@ int plan_prefix(ni_kv* kv, const ni_row* rows, const uint32_t* at, const ni_pref
     // Block-scaled: runs of more slots than a tile, where there are two items to a CU,
     // share their queries and pages through LDS and caches; from eight of two tiles on they
     // take two at a time.  us, one tile and two: 512 rows x 16 x 12 heads x 64, 12 layers, 520 /
-    // 449; 2041 rows x 32 query heads on 8 x 128 99 / 99; 2 x 300 of those 17.8 / 22.2.
+    // 380; 2041 rows x 32 query heads on 8 x 128 99 / 84; 2 x 300 of those 16.4 / 22.2.
     uint64_t o_tile = kSlotTile;
     bool many = false;
     if (b8) {

@@ -338,6 +338,39 @@ def test_scales_far_apart_and_rows_not_seen(gpu):
     assert torch.equal(kv.attention(q[:, :4], ask[:4]), again)
 
 
+@pytest.mark.parametrize("n_layer,n_head,head_dim", [(4, 16, 128), (4, 16, 64), (1, 8, 128)])
+def test_prompts_over_scales_far_apart(gpu, n_layer, n_head, head_dim):
+    """Pages whose value scales lie up to 2^80 apart, in tiles of many rows (two at a time, and one)."""
+    g = torch.Generator("cuda").manual_seed(19)
+    n, c = 1056, n_head * head_dim
+    kv = _kv(n_layer, n_head, head_dim, pages=n // PAGE, seqs=1, ctx=n, max_rows=n)
+    s = kv.add_seq()
+    kv.reserve(s, n)
+    rows = [(s, p) for p in range(n)]
+    k = torch.randn((n_layer, n, c), generator=g, device="cuda")
+    v = torch.randn((n_layer, n, c), generator=g, device="cuda")
+    sizes = torch.tensor([1.0, 1e-9, 1e12, 1e-12, 3.0, 1e6, 1e-3], device="cuda")
+    v *= sizes[torch.arange(n, device="cuda") // PAGE % 7][None, :, None]
+    kv.append(rows, k, v)
+    q = torch.randn((n_layer, n, c), generator=g, device="cuda") * 3
+    out = kv.attention(q, rows)
+    kk, vv = kv.gather_values(rows)
+    past = torch.ones((n, n), dtype=torch.bool, device="cuda").tril()
+    for layer, head in ((0, 0), (n_layer - 1, n_head - 1)):
+        at = slice(head * head_dim, (head + 1) * head_dim)
+        qh, kh, vh = (x[layer, :, at].double().cpu() for x in (q, kk, vv))
+        parts = (qh.abs() @ kh.abs().T) / math.sqrt(head_dim)
+        w = torch.softmax(((qh @ kh.T) / math.sqrt(head_dim)).masked_fill(~past.cpu(), -math.inf), -1)
+        # the scores' error (q's parts 2^-21, head_dim + 8 sums of 2^-24), weights and sums as for single rows
+        ds = (parts * past.cpu()).amax(-1, keepdim=True) * (2.0 ** -21 + (head_dim + 8) * 2.0 ** -24) + 2e-6
+        # (a weight is 2^10 and more at the largest key, f16 in steps of 2^-24 at the least, 2^6 smaller in the units of
+        # a near page: half a step is 2^-29 of the largest weight)
+        small = w.amax(-1, keepdim=True) * 2.0 ** -28 * (past.cpu().double() @ vh.abs())
+        bound = (w @ vh.abs()) * (2 * ds + 2.0 ** -17) + small + 1e-30
+        want = w @ vh
+        assert bool(((out[layer, :, at].double().cpu() - want).abs() <= bound + want.abs() * 2.0 ** -20).all()), (layer, head)
+
+
 def test_steps(gpu):
     """ni_kv_step and decode steps: the append, then the queried rows' attention."""
     rng, g = random.Random(1), torch.Generator("cuda").manual_seed(10)
