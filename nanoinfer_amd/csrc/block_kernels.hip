@@ -290,8 +290,8 @@ constexpr int kFar = 83;
 // heads x 128, 1.03 GB, 159 us, 6.5 TB/s; 64 rows of 1..767 keys, 12 layers x 12 heads x 64, 0.41 GB,
 // 77 us, 5.3 TB/s (short items: a start and a join to each 2 to 24 turns).  Two tiles are bound by
 // what their waves issue: a prompt of 2041 rows x 32 query heads on 8 x 128, 34 GFLOP (69 with hi
-// + lo), 84 us, of which the matrix cores are busy 28 and vector instructions (some 160 of a wave
-// for two tiles of a page, 32 of them conversions) issue for 35; 512 rows x 16 x 12 heads x 64, 12
+// + lo), 84 us, of which the matrix cores are busy 28 and vector instructions (some 150 of a wave
+// for two tiles of a page, 32 of them conversions) issue for 31; 512 rows x 16 x 12 heads x 64, 12
 // layers, 380 us.
 template <int D, int NT, int W, bool MANY, int INL>
 __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
