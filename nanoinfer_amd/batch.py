@@ -476,7 +476,7 @@ class PagedKv:
 
     # -------------------------------------------------------------- data path
     def append(self, rows, k, v, layer: int = ALL_LAYERS, stream=None):
-        """Write f32 K/V rows as f16 into their pages (b_kv_write)."""
+        """Write f32 K/V rows into their pages, in the cache's format (b_kv_write)."""
         arr, rp, n = _rows(rows)
         layered = layer == ALL_LAYERS
         _torch()

@@ -147,7 +147,7 @@ __global__ __launch_bounds__(256) void block_append_kernel(const BlockAppendLaun
             x[i][j] = number(x[i][j]);
         }
     top = wave_max(top);
-    const bool anew = slots & 1u;  // the block begins with this call
+    const bool anew = e.slots & kAnew;  // the block begins with this call, whatever its scale was
     const int old = exp_of(before), need = scale_exp(top), now = anew ? need : max(old, need);
     const float inv = pow2(-now);
     // Old values that stay: by how much they shrink (nothing is there yet below kMinExp).
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(256) void block_append_row_kernel(const BlockAppend
     top = fmaxf(top, dpp_move<0x4e>(top));
     top = fmaxf(top, dpp_move<0x141>(top));
     top = fmaxf(top, dpp_move<0x140>(top));
-    const bool anew = slot == 0;  // the block begins with this row
+    const bool anew = e.slots & kAnew;  // the block begins with this row, whatever its scale was
     const int old = exp_of(before), need = scale_exp(top), now = anew ? need : max(old, need);
     const float inv = pow2(-now);
     const bool grown = !anew && now > old;

@@ -183,6 +183,12 @@ struct ni_kv {
     std::vector<std::vector<uint32_t>> pages;
     std::vector<uint32_t> free_pages;  // LIFO stack, back() is handed out next (room for every page: a push never throws)
     std::vector<uint32_t> refs;        // page -> sequences that hold it
+    // Block-scaled: (page, layer) -> which of its rows were written (by calls made or
+    // captured) since the page was handed out, and not rolled back.  Its scales begin anew
+    // with a call that writes them all: a page keeps nothing of who held it before.  One
+    // for all layers until a call takes a single one.
+    std::vector<uint16_t> written;
+    uint32_t written_layers = 1;
     std::vector<uint32_t> page_order;  // the order in which pages were first handed out
     std::string err;
     bool host_only = false;
@@ -304,6 +310,13 @@ int check_seq(ni_kv* kv, uint32_t s) {
     return NI_OK;
 }
 
+// Block-scaled: page `dst` holds the first `rows` rows of `src` (itself: the others are gone).
+void keep_written(ni_kv* kv, uint32_t dst, uint32_t src, uint32_t rows) {
+    if (kv->written.empty()) return;
+    const size_t L = kv->written_layers;
+    for (size_t l = 0; l < L; l++) kv->written[dst * L + l] = kv->written[src * L + l] & ((1u << rows) - 1u);
+}
+
 // Batch::ensure_blocks (batch.rs:243-254).
 int ensure_pages(ni_kv* kv, uint32_t s, uint64_t len) {
     if (len > kv->o.max_ctx)
@@ -314,6 +327,7 @@ int ensure_pages(ni_kv* kv, uint32_t s, uint64_t len) {
         if (kv->free_pages.empty()) return kv->fail(NI_ERR_POOL_EXHAUSTED, "KV cache pool exhausted");
         pg.push_back(kv->free_pages.back());
         kv->refs[pg.back()] = 1;
+        keep_written(kv, pg.back(), pg.back(), 0);
         kv->free_pages.pop_back();
     }
     return NI_OK;
@@ -334,6 +348,7 @@ int truncate_seq(ni_kv* kv, uint32_t s, uint32_t len) {
         drop_page(kv, pg.back());
         pg.pop_back();
     }
+    if (len % kPage && kv->refs[pg.back()] == 1) keep_written(kv, pg.back(), pg.back(), len % kPage);
     return NI_OK;
 }
 
@@ -1757,6 +1772,7 @@ int ni_kv_create(const ni_kv_opts* opts, ni_kv** out) {
         for (uint32_t i = 0; i < o.kv_pages; i++) kv->free_pages[i] = o.kv_pages - 1 - i;
     }
     kv->refs.assign(o.kv_pages, 0);
+    if (is_b8(o)) kv->written.assign(o.kv_pages, 0);
     kv->page_order.assign(kv->free_pages.rbegin(), kv->free_pages.rend());
     if (!host_only) {
         hipError_t e = hipGetDevice(&kv->device);
@@ -1986,10 +2002,47 @@ static int plan_block_append(ni_kv* kv, const ni_row* rows, uint32_t n) {
     return NI_OK;
 }
 
+// Mark the entries that begin their page's scales in layers layer0 .. layer0 + n_lay - 1;
+// false where the layers differ in that.
+static bool mark_anew(ni_kv* kv, uint32_t layer0, uint32_t n_lay) {
+    const uint32_t L = kv->written_layers;
+    for (BlockAppend& e : kv->block_entries) {
+        const uint16_t* w = &kv->written[(size_t)e.page * L + (L > 1 ? layer0 : 0)];
+        const bool anew = (w[0] & ~e.slots) == 0;
+        for (uint32_t l = 1; l < (L > 1 ? n_lay : 1); l++)
+            if (((w[l] & ~e.slots) == 0) != anew) return false;
+        e.slots = anew ? e.slots | kAnew : e.slots & ~kAnew;
+    }
+    return true;
+}
+
+// The entries' rows are written in these layers.
+static void mark_written(ni_kv* kv, uint32_t layer0, uint32_t n_lay) {
+    const uint32_t L = kv->written_layers;
+    for (const BlockAppend& e : kv->block_entries) {
+        uint16_t* w = &kv->written[(size_t)e.page * L + (L > 1 ? layer0 : 0)];
+        for (uint32_t l = 0; l < (L > 1 ? n_lay : 1); l++) w[l] |= (uint16_t)e.slots;
+    }
+}
+
 // ni_kv_append on a block-scaled pool.
 static int block_append(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const ni_row* rows, uint32_t n, const float* k,
                         const float* v, int64_t row_stride, int64_t layer_stride, hipStream_t s) try {
     if (int rc = plan_block_append(kv, rows, n)) return rc;
+    if (kv->written_layers == 1 && n_lay < kv->o.n_layer) {  // (from here on the layers are told apart)
+        const uint32_t L = kv->o.n_layer;
+        std::vector<uint16_t> each(kv->written.size() * L);
+        for (size_t i = 0; i < each.size(); i++) each[i] = kv->written[i / L];
+        kv->written.swap(each);
+        kv->written_layers = L;
+    }
+    if (!mark_anew(kv, layer0, n_lay)) {
+        for (uint32_t l = 0; l < n_lay; l++)
+            if (int rc = block_append(kv, layer0 + l, 1, rows, n, k + l * layer_stride, v + l * layer_stride, row_stride,
+                                      layer_stride, s))
+                return rc;
+        return NI_OK;
+    }
     const auto& entries = kv->block_entries;
     const auto& list = kv->block_list;
     // (a launch holds less than 2^32 threads, a wave to each of K and V of a head)
@@ -2023,7 +2076,9 @@ static int block_append(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const ni_row
         e = launch_block_append(a, ref.inl, ref.inl_bytes, s, ps.t);
     }
     const int rc = release_plan(kv, ref, s);
-    return e != hipSuccess ? kv->hip_fail(e, "block append kernel") : rc;
+    if (e != hipSuccess) return kv->hip_fail(e, "block append kernel");
+    mark_written(kv, layer0, n_lay);
+    return rc;
 } catch (const std::bad_alloc&) {
     return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
 }
@@ -2114,6 +2169,7 @@ int ni_kv_fork(ni_kv* kv, const uint32_t* parents, uint32_t n, uint32_t* seqs, n
         auto& table = tables[c.dst];
         c.dst = kv->free_pages.back();
         kv->free_pages.pop_back();
+        keep_written(kv, c.dst, c.src, c.rows);
         table.push_back(c.dst);
     }
     for (uint32_t i = 0; i < n; i++) {
@@ -2214,11 +2270,16 @@ int ni_kv_reorder(ni_kv* kv, const uint32_t* seqs, const uint32_t* parents, uint
                 kv->free_pages.pop_back();
                 kv->refs[dst] = 1;
             }
+            keep_written(kv, dst, copies[c.copy].src, copies[c.copy].rows);
             c.table.push_back(dst);  // (room was made)
         }
         kv->pages[c.seq].swap(c.table);
     }
-    for (const Change& c : changes) kv->seq_len[c.seq] = c.len;
+    for (const Change& c : changes) {
+        kv->seq_len[c.seq] = c.len;
+        const auto& pg = kv->pages[c.seq];
+        if (c.len % kPage && kv->refs[pg.back()] == 1) keep_written(kv, pg.back(), pg.back(), c.len % kPage);
+    }
     return copy_pages(kv, copies, blob, (hipStream_t)stream);
 } catch (const std::bad_alloc&) {
     return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
@@ -2244,6 +2305,7 @@ int ni_kv_own(ni_kv* kv, uint32_t seq, uint32_t begin, uint32_t end, ni_stream s
         kv->free_pages.pop_back();
         kv->refs[c.src]--;
         kv->refs[c.dst] = 1;
+        keep_written(kv, c.dst, c.src, kPage);
         pg[i] = c.dst;
     }
     return copy_pages(kv, copies, blob, (hipStream_t)stream);
@@ -2268,7 +2330,10 @@ int ni_kv_compact(ni_kv* kv, uint32_t* moved, ni_stream stream) try {
         now[order[from]] = order[to++];
     }
     std::vector<uint8_t> blob(copies_bytes(copies.size()));
-    for (const PageCopy& c : copies) std::swap(kv->refs[c.src], kv->refs[c.dst]);
+    for (const PageCopy& c : copies) {
+        std::swap(kv->refs[c.src], kv->refs[c.dst]);
+        keep_written(kv, c.dst, c.src, kPage);
+    }
     for (auto& pg : kv->pages)
         for (uint32_t& p : pg) p = now[p];
     for (uint32_t i = used; i < n; i++) kv->free_pages[n - 1 - i] = order[i];

@@ -141,11 +141,12 @@ struct PageCopyLaunch {
 
 // Rows that one call appends to one page of a block-scaled pool: the slots set
 // in the low 16 bits of `slots`, taken in order from input rows src, src + 1,
-// ..., or (kListed) from those at list[src], list[src + 1], ....
+// ..., or (kListed) from those at list[src], list[src + 1], ....  kAnew: the page
+// holds no other rows, its scales begin with these.
 struct BlockAppend {
     uint32_t page, src, slots;
 };
-constexpr uint32_t kListed = 1u << 16;
+constexpr uint32_t kListed = 1u << 16, kAnew = 1u << 17;
 
 struct BlockAppendLaunch {
     PoolGeom pool;
