@@ -362,14 +362,15 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
 
     const uint32_t first_pos = min(it.pos0 + it.slot0 / a.group, kWholePos);  // of the item's first slot
     const uint32_t plain_end = min(it.kv_end, first_pos + 1);                 // every slot sees the keys before it
-    uint32_t qpos[NT];
+    const uint32_t plain_pages = first_pos / kPage + 1;                       // and keys of each page before this
+    uint32_t qend[NT];  // the slot sees the keys before it
     half8_t qh[kShared ? 1 : NB][2], ql[kShared ? 1 : NB][2];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         const bool has = t * (int)kSlotTile + col < (int)it.ns;
         const uint32_t slot = it.slot0 + (has ? t * kSlotTile + col : 0u);
         const uint32_t row = slot / a.group, g = slot - row * a.group;
-        qpos[t] = min(it.pos0 + row, kWholePos);
+        qend[t] = min(it.kv_end, min(it.pos0 + row, kWholePos) + 1);
         // step (i, j) of QK: dims 64 i + 16 rg + 8 j .. + 7, as the lane's bytes of K
         const float* qb = a.q + (int64_t)lay * a.q_layer_stride + (int64_t)(it.row0 + row) * a.q_row_stride +
                           (head * a.group + g) * D + 16 * rg;
@@ -414,6 +415,9 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
     }
 
     int unit = kMinExp - 1;  // log2 of the largest value scale so far
+    int seen[NT];            // and of those that a slot sees
+#pragma unroll
+    for (int t = 0; t < NT; t++) seen[t] = unit;
     for (; pg < pg_end; pg += W * PB) {
         // One tile: the next pages' registers beside these.  Two leave no room for that: keys
         // follow the products that read the last ones, values likewise.
@@ -463,38 +467,40 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
         pages(pg + 2 * W * PB, next_id);
         // Outputs are kept in units of the largest value scale so far, 2^unit: exact, as far as
         // f32 reaches.  The weights of pages whose scale is no more than 2^kNear smaller
-        // are taken in those units too, and both pages enter one product.
-        const int e0 = exp_of(vs[0]), e1 = exp_of(vs[1]);
-        if (max(e0, e1) > unit) {
-            if (unit >= kMinExp) {  // (else nothing is summed yet)
-                const float down = pow2(max(unit - max(e0, e1), -126));
+        // are taken in those units too, and both pages enter one product.  What a slot does not
+        // see leaves it as it is: the scale of a second page that not all slots see has no part in
+        // how the first is taken, and a slot's outputs are raised to the scales that it sees (a
+        // slot that does not see a page sees none behind it).
+        const int e[PB] = {exp_of(vs[0]), exp_of(vs[1])};
+        const bool mixed = pg + 1 >= plain_pages && pg + 1 < pg_end;
+        const int u0 = max(unit, mixed ? e[0] : max(e[0], e[1]));
+        const int units[PB] = {u0, max(u0, e[1])};
+        int near_by[PB], far_by[PB];  // log2 of what weights shrink by, or outputs grow by meanwhile
 #pragma unroll
-                for (int t = 0; t < NT; t++)
-#pragma unroll
-                    for (int c = 0; c < NC; c++) o[t][c] *= down;
-            }
-            unit = max(e0, e1);
+        for (int b = 0; b < PB; b++) {
+            const int below = units[b] - e[b];
+            near_by[b] = below <= kNear ? below : 0;
+            far_by[b] = below <= kNear ? 0 : min(below, kFar + 1);
         }
-        const int below[PB] = {unit - e0, unit - e1};
-        const bool near = max(below[0], below[1]) <= kNear;
+        const bool both = units[0] == units[1] && (far_by[0] | far_by[1]) == 0;
         half8_t wh[NT], wl[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             float s[PB][4];
 #pragma unroll
             for (int b = 0; b < PB; b++) {
-                const float ref = mref[t] + (near ? (float)below[b] : 0.f);
+                const float ref = mref[t] + (float)near_by[b];
 #pragma unroll
                 for (int j = 0; j < 4; j++) s[b][j] = fmaf(st[t][b][j], ks[b], -ref);
             }
             if ((pg + PB) * kPage > plain_end) {
 #pragma unroll
-                for (int b = 0; b < PB; b++)
+                for (int b = 0; b < PB; b++) {
+                    const int seen_keys = (int)(qend[t] - (pg + b) * kPage) - 4 * rg;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const uint32_t key = (pg + b) * kPage + 4 * rg + j;
-                        if (key >= it.kv_end || key > qpos[t]) s[b][j] = -INFINITY;
-                    }
+                    for (int j = 0; j < 4; j++)
+                        if (j >= seen_keys) s[b][j] = -INFINITY;
+                }
             }
             float lm = s[0][0];
 #pragma unroll
@@ -503,9 +509,9 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
                 for (int j = 0; j < 4; j++) lm = fmaxf(lm, s[b][j]);
             if (__any(lm > kRefLog2 + kRefSlack || !set[t])) {
                 const float mx = rows4_max(lm) - kRefLog2;
-                // The first finite maximum sets the reference, later ones only raise it.
+                // The first finite maximum sets the reference, later ones only raise it (a slot's own, whatever the others have).
                 const bool none = mx == -INFINITY;
-                const float d = set[t] ? fmaxf(mx, 0.f) : none ? 0.f : mx;
+                const float d = set[t] ? mx > kRefSlack ? mx : 0.f : none ? 0.f : mx;
                 const float alpha = set[t] ? fast_exp2(-d) : 1.f;  // (nothing is summed yet)
                 set[t] = set[t] || !none;
                 if (__any(alpha != 1.f)) {
@@ -525,7 +531,7 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
                 float p[4];
 #pragma unroll
                 for (int j = 0; j < 4; j++) p[j] = fast_exp2(s[b][j]);
-                lsum[t] += ((p[0] + p[1]) + (p[2] + p[3])) * (near ? pow2(below[b]) : 1.f);
+                lsum[t] += ((p[0] + p[1]) + (p[2] + p[3])) * pow2(near_by[b]);
                 split4(p, ph[b], pl[b]);
             }
             wh[t] = __builtin_shufflevector(ph[0], ph[1], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -536,9 +542,23 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
         // the compiler kept the outputs twice, 220 registers and two waves to a SIMD in place of 154
         // and three: the prompt below 102 us.)
 #pragma unroll 1
-        for (int b = 0; b < (near ? 1 : PB); b++) {
-            const int by = near ? 0 : min(b ? below[1] : below[0], kFar + 1);
-            const uint32_t with0 = near || (b == 0 && by <= kFar) ? ~0u : 0u, with1 = near || (b == 1 && by <= kFar) ? ~0u : 0u;
+        for (int b = 0; b < (both ? 1 : PB); b++) {
+            const int up = b ? units[1] : units[0], by = b ? far_by[1] : far_by[0];
+            const uint32_t with0 = both || (b == 0 && by <= kFar) ? ~0u : 0u, with1 = both || (b == 1 && by <= kFar) ? ~0u : 0u;
+            if (up > unit) {
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    if ((pg + b) * kPage >= qend[t]) continue;
+                    if (unit >= kMinExp) {  // (else nothing is summed yet)
+                        // (scales lie up to 2^237 apart)
+                        const float down = pow2(max(unit - up, -126)), rest = pow2(min(max(unit - up + 126, -126), 0));
+#pragma unroll
+                        for (int c = 0; c < NC; c++) o[t][c] = o[t][c] * down * rest;
+                    }
+                    seen[t] = up;
+                }
+                unit = up;
+            }
             if (by) {
 #pragma unroll
                 for (int t = 0; t < NT; t++)
@@ -591,7 +611,7 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
             if (rg == 0) *reinterpret_cast<float2*>(&red[wave][col][0]) = float2{set[t] ? mref[t] + kRefLog2 : kMinScore, l * kRefUnscale};
 #pragma unroll
             for (int c = 0; c < NC; c++)
-                *reinterpret_cast<float4_t*>(&red[wave][col][4 + c * 16 + 4 * rg]) = o[t][c] * (kRefUnscale * pow2(max(unit, kMinExp)));
+                *reinterpret_cast<float4_t*>(&red[wave][col][4 + c * 16 + 4 * rg]) = o[t][c] * (kRefUnscale * pow2(max(seen[t], kMinExp)));
         }
         __syncthreads();
         const uint32_t slots = it.ns > first ? min(it.ns - first, kSlotTile) : 0u;
