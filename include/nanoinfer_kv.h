@@ -83,7 +83,8 @@ enum ni_status {
  * device handles, not with NI_KV_Q8): 8-bit floats (e4m3: 3 bits of mantissa, up to 448) and
  * one scale for the 16 positions of a page, each head, K and V by themselves:
  * 64.25 bytes per 64 values.  A scale is the smallest power of two in
- * 2^-117..2^120 that brings the block's values to at most 448, so that scaling
+ * 2^-117..2^120 that brings the block's values to at most 448 (with 2^120 they
+ * are stored as 240 at most, which is within f32), so that scaling
  * is exact and a value is rounded once, to nearest even (half a step: 2^-4 of
  * itself, or 2^-10 of the scale where that is more).  It grows when an appended row needs it,
  * the block's other values being rounded again (which loses nothing above 2^-6 of the new scale),

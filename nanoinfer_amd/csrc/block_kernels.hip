@@ -48,9 +48,13 @@ __device__ __forceinline__ float wave_max(float x) {
     return rows4_max(x);
 }
 
-// Four values times `inv` as e4m3, to nearest even.
-__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float inv) {
-    const auto in = [&](float x) { return fminf(fmaxf(x * inv, -kTop), kTop); };
+// The largest value that is stored with scale 2^e: of the largest scale's, 256 (which f32's
+// largest would become) does not fit f32; 240 is half a step from it.
+__device__ __forceinline__ float largest(int e) { return e == kMaxExp ? 240.f : kTop; }
+
+// Four values times `inv` as e4m3, to nearest even, at most `most`.
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d, float inv, float most = kTop) {
+    const auto in = [&](float x) { return fminf(fmaxf(x * inv, -most), most); };
     const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(in(a), in(b), 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(in(c), in(d), lo, true);
 }
@@ -149,7 +153,7 @@ __global__ __launch_bounds__(256) void block_append_kernel(const BlockAppendLaun
     top = wave_max(top);
     const bool anew = e.slots & kAnew;  // the block begins with this call, whatever its scale was
     const int old = exp_of(before), need = scale_exp(top), now = anew ? need : max(old, need);
-    const float inv = pow2(-now);
+    const float inv = pow2(-now), most = largest(now);
     // Old values that stay: by how much they shrink (nothing is there yet below kMinExp).
     const bool grown = !anew && now > old;
     const float by = old < kMinExp ? 0.f : pow2(max(old - now, -126));
@@ -162,7 +166,7 @@ __global__ __launch_bounds__(256) void block_append_kernel(const BlockAppendLaun
             if (!all && !beside) y = *at;
 #pragma unroll
             for (int w = 0; w < 4; w++) {
-                const uint32_t fresh = e4m3x4(x[i][4 * w], x[i][4 * w + 1], x[i][4 * w + 2], x[i][4 * w + 3], inv);
+                const uint32_t fresh = e4m3x4(x[i][4 * w], x[i][4 * w + 1], x[i][4 * w + 2], x[i][4 * w + 3], inv, most);
                 const uint32_t kept = grown ? rescale4(y[w], by) : y[w];
                 const uint32_t take = (mine[0] ? 0xffu : 0u) | (mine[1] ? 0xff00u : 0u) | (mine[2] ? 0xff0000u : 0u) |
                                       (mine[3] ? 0xff000000u : 0u);
@@ -223,13 +227,13 @@ __global__ __launch_bounds__(256) void block_append_row_kernel(const BlockAppend
     top = fmaxf(top, dpp_move<0x140>(top));
     const bool anew = e.slots & kAnew;  // the block begins with this row, whatever its scale was
     const int old = exp_of(before), need = scale_exp(top), now = anew ? need : max(old, need);
-    const float inv = pow2(-now);
+    const float inv = pow2(-now), most = largest(now);
     const bool grown = !anew && now > old;
     const float by = old < kMinExp ? 0.f : pow2(max(old - now, -126));
 #pragma unroll
     for (int i = 0; i < NB; i++) {
         u32x4* const words = reinterpret_cast<u32x4*>(block + 1024 * i);
-        const uint32_t fresh = e4m3x4(x[i][0], x[i][1], x[i][2], x[i][3], inv);
+        const uint32_t fresh = e4m3x4(x[i][0], x[i][1], x[i][2], x[i][3], inv, most);
         if (grown)
             for (uint32_t hi = 0; hi < 4; hi++) {
                 if (is_v ? hi == slot / 4 : x16 == slot) continue;  // (K: the row itself)
