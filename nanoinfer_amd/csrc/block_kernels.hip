@@ -610,12 +610,16 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
     for (int t = 0; t < NT; t++) {
         if (kShared || t) __syncthreads();  // (the queries, or the last tile's states, are read)
         const uint32_t first = t * kSlotTile;
+        // (sums of values near f32's largest would pass it before they are divided by the weights':
+        // both are kept 2^32 smaller, the reference 32 higher)
+        const float lift = seen[t] > 64 ? 32.f : 0.f, unscale = seen[t] > 64 ? kRefUnscale * 0x1p-32f : kRefUnscale;
         const float l = rows4_sum(lsum[t]);
         if (first + col < it.ns) {
-            if (rg == 0) *reinterpret_cast<float2*>(&red[wave][col][0]) = float2{set[t] ? mref[t] + kRefLog2 : kMinScore, l * kRefUnscale};
+            if (rg == 0)
+                *reinterpret_cast<float2*>(&red[wave][col][0]) = float2{set[t] ? mref[t] + (kRefLog2 + lift) : kMinScore, l * unscale};
 #pragma unroll
             for (int c = 0; c < NC; c++)
-                *reinterpret_cast<float4_t*>(&red[wave][col][4 + c * 16 + 4 * rg]) = o[t][c] * (kRefUnscale * pow2(max(seen[t], kMinExp)));
+                *reinterpret_cast<float4_t*>(&red[wave][col][4 + c * 16 + 4 * rg]) = o[t][c] * (unscale * pow2(max(seen[t], kMinExp)));
         }
         __syncthreads();
         const uint32_t slots = it.ns > first ? min(it.ns - first, kSlotTile) : 0u;
