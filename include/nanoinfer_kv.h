@@ -322,9 +322,9 @@ int ni_kv_decode_steps(ni_kv* kv, const uint32_t* seqs, uint32_t n, uint32_t ste
 int ni_kv_fork(ni_kv* kv, const uint32_t* parents, uint32_t n, uint32_t* seqs, ni_stream stream);
 /* Sequence seqs[i] (each once) becomes a continuation of what parents[i] (live,
  * listed or not) held before the call, as beams of a search do: its whole pages
- * are shared, the page with the end goes to the first that continues a sequence
- * which is itself replaced, and is copied for all others.  parents[i] ==
- * seqs[i]: it stays as it is. */
+ * are shared, the page with the end goes to the first continuation where no sequence
+ * would hold it any more, and is copied for all others, so that each may grow.
+ * parents[i] == seqs[i]: it stays as it is. */
 int ni_kv_reorder(ni_kv* kv, const uint32_t* seqs, const uint32_t* parents, uint32_t n, ni_stream stream);
 /* Pages of its own for positions begin .. end-1 of `seq` (reserved): copies of
  * those it shares. */

@@ -2190,21 +2190,18 @@ int ni_kv_reorder(ni_kv* kv, const uint32_t* seqs, const uint32_t* parents, uint
     if (!parents || !seqs) return kv->fail(NI_ERR_BAD_ARG, "%s is NULL", parents ? "seqs" : "parents");
     DeviceScope device(kv->device, kv->host_only);
     if (int rc = begin_tables(kv, (hipStream_t)stream)) return rc;
-    // Sequences that others replace: whose end page one of its continuations may take over.
-    enum : uint8_t { kStays = 0, kReplaced = 1, kTaken = 2 };
-    std::vector<uint8_t> state(kv->o.max_seqs, kStays);
     std::vector<uint8_t> listed(kv->o.max_seqs, 0);
     for (uint32_t i = 0; i < n; i++) {
         if (int rc = check_live(kv, seqs[i])) return rc;
         if (int rc = check_live(kv, parents[i])) return rc;
         if (listed[seqs[i]]) return kv->fail(NI_ERR_BAD_ARG, "sequence %u appears twice in one call", seqs[i]);
         listed[seqs[i]] = 1;
-        if (parents[i] != seqs[i]) state[seqs[i]] = kReplaced;
     }
     constexpr uint32_t kNone = 0xffffffffu;
     struct Change {
         uint32_t seq, len;
-        uint32_t copy;  // index into copies of its last page, or kNone
+        uint32_t end;   // its parent's last page, where that is no whole one, or kNone
+        uint32_t copy;  // index into copies of that page, or kNone
         std::vector<uint32_t> table;
     };
     std::vector<Change> changes;
@@ -2213,29 +2210,34 @@ int ni_kv_reorder(ni_kv* kv, const uint32_t* seqs, const uint32_t* parents, uint
         if (parents[i] == seqs[i]) continue;
         const uint32_t len = kv->seq_len[parents[i]];
         const auto& pg = kv->pages[parents[i]];
-        Change c{seqs[i], len, kNone, {}};
+        Change c{seqs[i], len, len % kPage ? pg[len / kPage] : kNone, kNone, {}};
         c.table.reserve(len / kPage + 1);
         c.table.assign(pg.begin(), pg.begin() + len / kPage);
-        if (len % kPage) {
-            if (state[parents[i]] == kReplaced) {
-                state[parents[i]] = kTaken;
-                c.table.push_back(pg[len / kPage]);
-            } else {
-                c.copy = (uint32_t)copies.size();
-                copies.push_back({pg[len / kPage], kNone, len % kPage});
-            }
-        }
         changes.push_back(std::move(c));
     }
     if (changes.empty()) return NI_OK;
-    std::vector<uint8_t> blob(copies_bytes(copies.size()));
+    copies.reserve(changes.size());
+    std::vector<uint8_t> blob(copies_bytes(changes.size()));
     // Nothing below throws.  The new holds before the old ones go, so that what
-    // reaches 0 is free: no page that is copied from does.
+    // reaches 0 is free: no page that is copied from does.  A page that a continuation ends in
+    // it takes over if nothing else holds that any more, the first to come; the others copy it.
     size_t released = 0;
     for (const Change& c : changes)
         for (uint32_t p : c.table) kv->refs[p]++;
     for (const Change& c : changes)
         for (uint32_t p : kv->pages[c.seq]) released += --kv->refs[p] == 0;
+    for (Change& c : changes) {
+        if (c.end == kNone) continue;
+        if (kv->refs[c.end] == 0) {
+            released--;
+            kv->refs[c.end] = 1;
+            c.table.push_back(c.end);  // (room was made)
+        } else {
+            c.copy = (uint32_t)copies.size();
+            copies.push_back({c.end, kNone, c.len % kPage});
+        }
+    }
+    blob.resize(copies_bytes(copies.size()));
     if (copies.size() > kv->free_pages.size() + released) {
         for (const Change& c : changes)
             for (uint32_t p : kv->pages[c.seq]) kv->refs[p]++;
