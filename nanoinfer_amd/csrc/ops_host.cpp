@@ -286,10 +286,16 @@ int ni_beam_select(uint32_t dtype, const void* logits, int64_t search_stride, in
     // (a launch holds less than 2^32 threads)
     if (rows * runs >= (1ull << 24) || n_search >= (1u << 22))
         return call_error(NI_ERR_BAD_ARG, "%u searches of %u beams: too many for one call", n_search, n_beam);
+    typedef unsigned __int128 u128;
+    // (extents are compared in 64 bits)
+    const auto extent = [](uint64_t n, int64_t stride, uint64_t width) { return (u128)(n - 1) * (uint64_t)stride + width; };
+    if (hist && n_history && extent(rows, history_stride, n_history) >= (u128)1 << 60)
+        return call_error(NI_ERR_BAD_ARG, "history's strides are too large");
+    if (hist && extent(outs, out_history_stride, (uint64_t)n_history + 1) >= (u128)1 << 60)
+        return call_error(NI_ERR_BAD_ARG, "out_history's strides are too large");
     const auto span = [](const void* p, uint64_t n, int64_t stride, uint64_t width) {
         return Span{static_cast<const char*>(p), p ? 4 * ((n - 1) * (uint64_t)stride + width) : 0};
     };
-    typedef unsigned __int128 u128;
     const u128 read = (u128)(n_search - 1) * (uint64_t)search_stride + (u128)(n_beam - 1) * (uint64_t)beam_stride + vocab;
     if (read >= (u128)1 << 60) return call_error(NI_ERR_BAD_ARG, "logits' strides are too large");
     const Span in[] = {span(scores, 1, 0, rows), span(finished, 1, 0, rows),
