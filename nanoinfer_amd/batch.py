@@ -195,6 +195,14 @@ def _pointer(arr, empty, item):
     return empty.from_buffer(arr) if arr.size and arr.flags.writeable else arr.ctypes.data_as(C.POINTER(item))
 
 
+def _u32(x, name) -> int:
+    """An integer of 32 bits (ctypes would take it modulo 2^32)."""
+    x = index(x)
+    if not 0 <= x <= 0xffffffff:
+        raise ValueError(f"{name} must be in 0..2^32-1")
+    return x
+
+
 def _u32_array(x, name) -> np.ndarray:
     """Host integers of any shape as a flat uint32 array."""
     if type(x) is list:
@@ -456,8 +464,10 @@ class PagedKv:
     def own(self, seq: int, begin: int = 0, end: Optional[int] = None, stream=None):
         """Pages of its own for positions ``begin .. end-1`` (default: the
         committed ones) of ``seq``: copies of those that it shares."""
+        seq, begin = _u32(seq, "seq"), _u32(begin, "begin")
+        end = self.seq_len(seq) if end is None else _u32(end, "end")
         s = self._stream(stream)
-        self._check(self._L.ni_kv_own(self._h, seq, begin, self.seq_len(seq) if end is None else end, s))
+        self._check(self._L.ni_kv_own(self._h, seq, begin, end, s))
 
     def compact(self, stream=None) -> int:
         """Move the pages in use to the front of the order in which pages are
@@ -470,7 +480,7 @@ class PagedKv:
     def page_refs(self, page: int) -> int:
         """Sequences that hold ``page``."""
         n = C.c_uint32()
-        if self._L.ni_kv_page_refs(self._h, page, C.byref(n)) != 0:
+        if self._L.ni_kv_page_refs(self._h, _u32(page, "page"), C.byref(n)) != 0:
             raise ValueError(f"page {page} of {self.opts.kv_blocks}")
         return int(n.value)
 

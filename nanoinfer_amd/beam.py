@@ -32,9 +32,11 @@ def beam_select(logits, scores, k=None, finished=None, pad_token=0, history=None
     if not isinstance(logits, torch.Tensor) or logits.dim() != 3 or dtype_code(logits.dtype) is None:
         raise TypeError("logits must be a float32, float16 or bfloat16 tensor [searches, beams, vocabulary]")
     b, w, v = logits.shape
-    k = w if k is None else int(k)
-    if k < 0 or v == 0 or w == 0:
-        raise ValueError(f"logits are {list(logits.shape)}, k {k}: needs [searches, beams, vocabulary] and k >= 0")
+    given, k = k, w if k is None else int(k)
+    if given is not None and k != given:
+        raise ValueError(f"k {given} is no whole number")
+    if not 0 <= k <= 0xffffffff or v == 0 or w == 0:
+        raise ValueError(f"logits are {list(logits.shape)}, k {k}: needs [searches, beams, vocabulary] and k in 0..2^32-1")
     if not 0 <= pad_token <= 0xffffffff:
         raise ValueError("pad_token must be in 0..2^32-1")
     device, f32, i32 = logits.get_device(), torch.float32, torch.int32
