@@ -2742,6 +2742,33 @@ int ni_kv_append_rotary(ni_kv* kv, int32_t layer, const ni_row* rows, uint32_t n
     return kv->fail(NI_ERR_BAD_ARG, "out of host memory");
 }
 
+// Where the parts of a serialised PrefixPlan begin, and the bytes of its partials.
+struct PrefixSizes {
+    size_t off_pitems, off_merges, off_table, blob, o_bytes, partials;
+};
+static PrefixSizes prefix_sizes(const ni_kv* kv, const PrefixPlan& P, uint32_t n_lay) {
+    PrefixSizes z;
+    z.off_pitems = align_up(P.items.size() * sizeof(PrefixItem), kAlign);
+    z.off_merges = align_up(z.off_pitems + P.pitems.size() * sizeof(PrefixItem), kAlign);
+    z.off_table = align_up(z.off_merges + P.merges.size() * sizeof(PrefixMerge), kAlign);
+    z.blob = align_up(z.off_table + P.table.size() * sizeof(uint32_t), kAlign);
+    const size_t parts = (size_t)P.n_parts * n_lay * kv->o.n_head;
+    z.o_bytes = align_up(parts * kv->o.head_dim * sizeof(float), kAlign);
+    z.partials = parts ? z.o_bytes + parts * 2 * sizeof(float) : 0;
+    return z;
+}
+
+// What a capture has no room for.
+static int check_prefix_capture(ni_kv* kv, const PrefixSizes& z) {
+    if (int rc = check_capture(kv, z.blob)) return rc;
+    const size_t held = std::max(kv->partials_bytes, kv->graph_partials_bytes);
+    if (kv->capturing && z.partials > held)
+        return kv->fail(NI_ERR_BAD_ARG,
+                        "the call needs %zu bytes of partials, the handle holds %zu: make it once outside the capture",
+                        z.partials, held);
+    return NI_OK;
+}
+
 // Plan and enqueue a call of ni_kv_prefix_attention (checked), or any attention
 // over a block-scaled pool.
 static int run_prefix(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const float* q, int64_t q_row_stride,
@@ -2751,31 +2778,20 @@ static int run_prefix(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const float* q
     PrefixPlan& P = kv->prefix_plan;
     if (int rc = plan_prefix(kv, rows, at, prefixes, n_prefix, n_q_head / kv->o.n_head, n_lay, split_tokens, P)) return rc;
     std::vector<uint8_t>& blob = kv->blob;
-    const size_t off_pitems = align_up(P.items.size() * sizeof(PrefixItem), kAlign);
-    const size_t off_merges = align_up(off_pitems + P.pitems.size() * sizeof(PrefixItem), kAlign);
-    const size_t off_table = align_up(off_merges + P.merges.size() * sizeof(PrefixMerge), kAlign);
-    blob.resize(align_up(off_table + P.table.size() * sizeof(uint32_t), kAlign));
+    const PrefixSizes z = prefix_sizes(kv, P, n_lay);
+    blob.resize(z.blob);
     memcpy(blob.data(), P.items.data(), P.items.size() * sizeof(PrefixItem));
-    if (!P.pitems.empty()) memcpy(blob.data() + off_pitems, P.pitems.data(), P.pitems.size() * sizeof(PrefixItem));
-    if (!P.merges.empty()) memcpy(blob.data() + off_merges, P.merges.data(), P.merges.size() * sizeof(PrefixMerge));
-    memcpy(blob.data() + off_table, P.table.data(), P.table.size() * sizeof(uint32_t));
+    if (!P.pitems.empty()) memcpy(blob.data() + z.off_pitems, P.pitems.data(), P.pitems.size() * sizeof(PrefixItem));
+    if (!P.merges.empty()) memcpy(blob.data() + z.off_merges, P.merges.data(), P.merges.size() * sizeof(PrefixMerge));
+    memcpy(blob.data() + z.off_table, P.table.data(), P.table.size() * sizeof(uint32_t));
 
     const uint32_t D = kv->o.head_dim, H = kv->o.n_head;
     DeviceScope device(kv->device);
     if (int rc = begin_call(kv, s)) return rc;
-    if (int rc = check_capture(kv, blob.size())) return rc;
-    const size_t parts = (size_t)P.n_parts * n_lay * H;
-    const size_t o_bytes = align_up(parts * D * sizeof(float), kAlign), bytes = o_bytes + parts * 2 * sizeof(float);
+    if (int rc = check_prefix_capture(kv, z)) return rc;
     float* partials = nullptr;
-    if (parts) {
-        const size_t held = std::max(kv->partials_bytes, kv->graph_partials_bytes);
-        if (kv->capturing && bytes > held)
-            return kv->fail(NI_ERR_BAD_ARG,
-                            "the call needs %zu bytes of partials, the handle holds %zu: make it once outside the "
-                            "capture",
-                            bytes, held);
-        if (int rc = ensure_partials(kv, bytes, s, &partials)) return rc;
-    }
+    if (z.partials)
+        if (int rc = ensure_partials(kv, z.partials, s, &partials)) return rc;
     PlanRef ref;
     if (int rc = place_blob(kv, blob, s, &ref)) return rc;
     PrefixLaunch a{};
@@ -2787,10 +2803,10 @@ static int run_prefix(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const float* q
     a.out_row_stride = out_row_stride;
     a.out_layer_stride = out_layer_stride;
     a.plan = ref.dev;
-    a.off_merges = (uint32_t)off_merges;
-    a.off_table = (uint32_t)off_table;
+    a.off_merges = (uint32_t)z.off_merges;
+    a.off_table = (uint32_t)z.off_table;
     a.part_o = partials;
-    a.part_ml = partials ? partials + o_bytes / sizeof(float) : nullptr;
+    a.part_ml = partials ? partials + z.o_bytes / sizeof(float) : nullptr;
     a.n_merges = (uint32_t)P.merges.size();
     a.layer0 = layer0;
     a.n_lay = n_lay;
@@ -2798,7 +2814,7 @@ static int run_prefix(ni_kv* kv, uint32_t layer0, uint32_t n_lay, const float* q
     a.qscale = (float)(1.4426950408889634 / std::sqrt((double)D));
     hipError_t e = hipSuccess;
     if (!P.pitems.empty()) {
-        a.off_items = (uint32_t)off_pitems;
+        a.off_items = (uint32_t)z.off_pitems;
         a.n_items = (uint32_t)P.pitems.size();
         a.wide = P.wide;
         a.waves = P.waves;
@@ -3158,15 +3174,24 @@ static int block_step(ni_kv* kv, const ni_work* work, uint32_t n_work, const flo
     rows.clear();
     for (uint32_t w = 0; w < n_work; w++)
         for (uint32_t i = 0; i < work[w].n_new; i++) rows.push_back({work[w].seq, kv->seq_len[work[w].seq] + i});
-    if (int rc = block_append(kv, 0, n_lay, rows.data(), (uint32_t)rows.size(), k, v, row_stride, layer_stride, stream))
-        return rc;
     at.clear();
     for (uint32_t w = 0, row = 0; w < n_work; row += work[w++].n_new)
-        for (uint32_t i = work[w].n_new - work[w].n_query; i < work[w].n_new; i++) {
-            rows[at.size()] = rows[row + i];
-            at.push_back(row + i);
-        }
+        for (uint32_t i = work[w].n_new - work[w].n_query; i < work[w].n_new; i++) at.push_back(row + i);
+    {
+        DeviceScope device(kv->device);
+        if (int rc = begin_call(kv, stream)) return rc;
+    }
+    if (kv->capturing && !at.empty()) {  // what the attention below has no room for refuses the append too
+        std::vector<ni_row> asked;
+        for (uint32_t i : at) asked.push_back(rows[i]);
+        const ni_prefix none{0, 0, (uint32_t)at.size()};
+        if (int rc = plan_prefix(kv, asked.data(), at.data(), &none, 1, 1, n_lay, split_tokens, kv->prefix_plan)) return rc;
+        if (int rc = check_prefix_capture(kv, prefix_sizes(kv, kv->prefix_plan, n_lay))) return rc;
+    }
+    if (int rc = block_append(kv, 0, n_lay, rows.data(), (uint32_t)rows.size(), k, v, row_stride, layer_stride, stream))
+        return rc;
     if (at.empty()) return NI_OK;
+    for (size_t i = 0; i < at.size(); i++) rows[i] = rows[at[i]];
     return block_attention(kv, 0, n_lay, q, row_stride, layer_stride, rows.data(), at.data(), (uint32_t)at.size(), out,
                            out_row_stride, out_layer_stride, split_tokens, stream);
 } catch (const std::bad_alloc&) {
