@@ -3181,7 +3181,11 @@ static int block_step(ni_kv* kv, const ni_work* work, uint32_t n_work, const flo
         DeviceScope device(kv->device);
         if (int rc = begin_call(kv, stream)) return rc;
     }
-    if (kv->capturing && !at.empty()) {  // what the attention below has no room for refuses the append too
+    // What the attention below has no room for refuses the append too: looked at first where that may be (else its
+    // plan is made while the append runs).  Its items, at most, of partitions of 256 keys or split_tokens:
+    uint64_t items = 0;
+    for (uint32_t i : at) items += rows[i].pos / (split_tokens ? split_tokens : 256) + 1;
+    if (!at.empty() && (kv->capturing || items * n_lay * kv->o.n_head >= (1ull << 23))) {
         std::vector<ni_row> asked;
         for (uint32_t i : at) asked.push_back(rows[i]);
         const ni_prefix none{0, 0, (uint32_t)at.size()};

@@ -1,5 +1,4 @@
-"""Captured calls on the block-scaled cache that cannot be made: nothing of them
-is in the graph."""
+"""Steps on the block-scaled cache that cannot be made: nothing of them is."""
 import pytest
 import torch
 
@@ -41,3 +40,24 @@ def test_a_step_that_cannot_be_captured_appends_nothing(gpu, why):
     assert [kv.seq_len(s) for s, _, _ in work] == [n] * seqs
     kv.step(work, q, k, v, out=out)  # outside it can be made
     assert kv.seq_len(0) == n + 1 and bool(torch.isfinite(out).all()) and bool((out != 0).any())
+
+
+def test_a_step_too_large_appends_nothing(gpu):
+    """More (partition, layer, head) items than a call takes."""
+    g = torch.Generator("cuda").manual_seed(2)
+    n, n_layer, n_head = 2048 * PAGE, 64, 64
+    kv = _kv(n_layer, n_head, 64, pages=n // PAGE + 1, seqs=1, ctx=n + PAGE, max_rows=1)
+    s = kv.add_seq()
+    kv.reserve(s, n + 1)
+    kv.commit(s, n)
+    held = [torch.randn((n_layer, 1, n_head * 64), generator=g, device="cuda") for _ in range(2)]
+    kv.append([(s, n)], *held)
+    want = [x.clone() for x in kv.gather_values([(s, n)])]
+    q, k, v = (torch.randn((n_layer, 1, n_head * 64), generator=g, device="cuda") * 3 for _ in range(3))
+    with pytest.raises(na.KvError) as e:
+        kv.step([(s, 1, 1)], q, k, v, split_tokens=16)
+    assert "too large" in str(e.value) and kv.seq_len(s) == n
+    assert all(torch.equal(x, y) for x, y in zip(kv.gather_values([(s, n)]), want))
+    kv.step([(s, 1, 1)], q, k, v)
+    assert kv.seq_len(s) == n + 1
+    assert not torch.equal(kv.gather_values([(s, n)])[0], want[0])
