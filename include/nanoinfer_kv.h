@@ -430,8 +430,8 @@ typedef struct ni_prefix {
  * be its prefix.
  * Range: rows that share tiles hold q / sqrt(head_dim) * log2(e) as two f16
  * parts, so |q| is at most 3.6e5 (head_dim 64; 5.1e5 at 128); a larger value
- * may make its row NaN (on the block-scaled cache every row's are so held, in
- * ni_paged_decode_attention and steps too).  On the Q8 cache keys and values that a row sees are
+ * may make its row NaN.  (On the block-scaled cache every call holds q so, relative to
+ * the largest value of its row and head: q of any size, and keys of any.)  On the Q8 cache keys and values that a row sees are
  * finite; what later rows, or no row, may see does not matter.
  * split_tokens: keys per partition, a multiple of 16; 0 = automatic.
  * Under stream capture the call allocates nothing: make the same call once

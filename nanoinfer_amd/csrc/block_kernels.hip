@@ -308,6 +308,7 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
         __device__ Lds() {}
     } lds;
     auto& red = lds.red;
+    __shared__ float tops[kShared ? NT : 1][2 * NB][kSlotTile];  // the queries' largest values, by step
     const int lane = threadIdx.x & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t H = a.pool.n_head, lh = a.n_lay * H;
@@ -368,42 +369,71 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
     const uint32_t plain_end = min(it.kv_end, first_pos + 1);                 // every slot sees the keys before it
     const uint32_t plain_pages = first_pos / kPage + 1;                       // and keys of each page before this
     uint32_t qend[NT];  // the slot sees the keys before it
+    // A slot's query enters products with its largest value in 2^14 .. 2^15, the power of two that
+    // takes on the keys' scales: keys may be of any size, and queries small or large to match.
+    float qs[NT];
     half8_t qh[kShared ? 1 : NB][2], ql[kShared ? 1 : NB][2];
+    // Shared: a wave brings step (wave / 2, wave % 2) of every tile, of one with 64 dims a step of one
+    // (of a single tile two waves bring none).
+    constexpr int STEPS = kShared ? 1 : 2 * NB;
+    static_assert(!kShared || W == 4, "a step of every tile to a wave, or two");
+    const int step0 = NB == 2 ? (int)wave : (int)wave % 2;
+    auto brings = [&](int t) { return !kShared || NB == 2 || (int)wave / 2 == t; };
+    float x[NT][STEPS][8], most[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         const bool has = t * (int)kSlotTile + col < (int)it.ns;
         const uint32_t slot = it.slot0 + (has ? t * kSlotTile + col : 0u);
         const uint32_t row = slot / a.group, g = slot - row * a.group;
         qend[t] = min(it.kv_end, min(it.pos0 + row, kWholePos) + 1);
-        // step (i, j) of QK: dims 64 i + 16 rg + 8 j .. + 7, as the lane's bytes of K
+        most[t] = 0.f;
+        if (!brings(t)) continue;
+        // step (i, j) of QK, number 2 i + j: dims 64 i + 16 rg + 8 j .. + 7, as the lane's bytes of K
         const float* qb = a.q + (int64_t)lay * a.q_layer_stride + (int64_t)(it.row0 + row) * a.q_row_stride +
                           (head * a.group + g) * D + 16 * rg;
-        auto operand = [&](int i, int j, half8_t& hi, half8_t& lo) {
-            const float4 x0 = reinterpret_cast<const float4*>(qb + 64 * i + 8 * j)[0];
-            const float4 x1 = reinterpret_cast<const float4*>(qb + 64 * i + 8 * j)[1];
-            const float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
+            const int step = kShared ? step0 : i;
+            const float4* p = reinterpret_cast<const float4*>(qb + 64 * (step / 2) + 8 * (step % 2));
+            const float4 x0 = p[0], x1 = p[1];
+            const float y[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                x[t][i][e] = has ? y[e] : 0.f;
+                most[t] = fmaxf(most[t], fabsf(x[t][i][e]));
+            }
+        }
+        most[t] = rows4_max(most[t]);
+        if (kShared && rg == 0) tops[t][step0][col] = most[t];
+    }
+    if constexpr (kShared) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        if constexpr (kShared) {
+#pragma unroll
+            for (int i = 0; i < 2 * NB; i++) most[t] = fmaxf(most[t], tops[t][i][col]);
+        }
+        const int up = min(141 - (int)(__float_as_uint(most[t] * a.qscale) >> 23), 126);
+        const float grow = pow2(up);
+        qs[t] = pow2(-up);
+        if (!brings(t)) continue;
+#pragma unroll
+        for (int i = 0; i < STEPS; i++) {
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                y[e] = has ? x[e] * a.qscale : 0.f;
+                y[e] = x[t][i][e] * a.qscale * grow;
                 asm("" : "+v"(y[e]));  // the f32 products, as the split's residual sees them
             }
+            half8_t hi, lo;
             split8(y, hi, lo);
-        };
-        if constexpr (kShared) {
-            static_assert(!kShared || W == 4, "a step of every tile to a wave, or two");
-            if (NB == 2 || wave / 2 == t) {  // (one tile of 64 dims: two waves have none)
-                const int i = NB == 2 ? wave / 2 : 0, j = wave % 2;
-                half8_t hi, lo;
-                operand(i, j, hi, lo);
-                lds.q[t][i][j][0][lane] = hi;
-                lds.q[t][i][j][1][lane] = lo;
+            if constexpr (kShared) {
+                lds.q[t][step0 / 2][step0 % 2][0][lane] = hi;
+                lds.q[t][step0 / 2][step0 % 2][1][lane] = lo;
+            } else {
+                qh[i / 2][i % 2] = hi;
+                ql[i / 2][i % 2] = lo;
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < NB; i++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) operand(i, j, qh[i][j], ql[i][j]);
         }
     }
     if constexpr (kShared) __syncthreads();
@@ -495,7 +525,7 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
             for (int b = 0; b < PB; b++) {
                 const float ref = mref[t] + (float)near_by[b];
 #pragma unroll
-                for (int j = 0; j < 4; j++) s[b][j] = fmaf(st[t][b][j], ks[b], -ref);
+                for (int j = 0; j < 4; j++) s[b][j] = fmaf(st[t][b][j], ks[b] * qs[t], -ref);
             }
             if ((pg + PB) * kPage > plain_end) {
 #pragma unroll
