@@ -284,3 +284,44 @@ def test_layers_written_one_after_another(gpu, head_dim):
         for m, y in zip(models, x):
             m.append([(f, PAGE + 6)], y[layer:layer + 1])
     check()
+
+
+@pytest.mark.parametrize("head_dim,n_head", [(64, 3), (128, 1), (128, 8)])
+@pytest.mark.parametrize("rows", [1, 4, 6, 13, 15])
+def test_copies_leave_what_lies_behind_the_end(gpu, head_dim, n_head, rows):
+    """Of a page that a sequence ends in the rows before the end go over (of V with the rest of the word of four that
+    holds the last), and its scales; nothing else of the pool changes."""
+    kv = _kv(2, n_head, head_dim, pages=6)
+    at, _, size = kv.pools()
+
+    class Pool:
+        __cuda_array_interface__ = dict(shape=(size,), typestr="|u1", data=(at, False), version=2)
+
+    pool = torch.as_tensor(Pool(), device="cuda")
+    pool.copy_(torch.randint(0, 256, pool.shape, device="cuda", dtype=torch.uint8))
+    s = kv.add_seq()
+    kv.reserve(s, 2 * PAGE)
+    kv.commit(s, PAGE + rows)
+    before = pool.clone().view(2, 6, -1)
+    (f,) = kv.fork([s])
+    after = pool.view(2, 6, -1)
+    src, dst = kv.block_table(s)[1], kv.block_table(f)[1]
+    block = PAGE * head_dim
+    copied = torch.zeros((before.shape[2],), dtype=torch.bool)
+    maybe = copied.clone()
+    for head in range(n_head):
+        for d in range(head_dim):
+            for p in range(PAGE):
+                k = head * 2 * block + d // 64 * 1024 + d % 64 // 16 * 256 + p * 16 + d % 16
+                v = (head * 2 + 1) * block + d // 64 * 1024 + p // 4 * 256 + d % 16 * 16 + d % 64 // 16 * 4 + p % 4
+                copied[k] = copied[v] = p < rows
+                maybe[v] = p < (rows + 3) // 4 * 4
+    scales = 2 * n_head * block
+    copied[scales:scales + 8 * n_head] = True
+    maybe[scales:scales + (8 * n_head + 15) // 16 * 16] = True  # (and what fills the unit of the last)
+    copied, maybe = copied.cuda(), maybe.cuda()
+    assert torch.equal(after[:, dst][:, copied], before[:, src][:, copied])
+    left = ~(copied | maybe)
+    assert torch.equal(after[:, dst][:, left], before[:, dst][:, left])
+    others = [p for p in range(6) if p != dst]
+    assert torch.equal(after[:, others], before[:, others])
