@@ -90,13 +90,14 @@ enum ni_status {
  * the block's other values being rounded again (which loses nothing above 2^-6 of the new scale),
  * begins anew with a call that writes every row its page holds (in that layer), and never shrinks else.
  * A page holds the rows written since it was handed out (with it, those of a copied page),
- * by calls made or captured, without those that ni_kv_truncate took back: rows may come in any order and
- * again, but a rejected draft's large values leave the rows kept beside them, and later ones, at the scale that they needed.
+ * by calls made or captured, without those that ni_kv_truncate took back, and for rows behind the sequence's
+ * end those before it.  So rows may come in any order and again; but a rejected draft's
+ * large values leave the rows kept beside them, and later ones, at the scale that they needed.
  * A captured call finds in its pages what they hold when it is captured, and counts as made.
  * Inputs must be finite: a NaN is stored as 0, an infinity as the block's largest value.
  * In attention, values of a block whose scale lies more than 2^83 below the
  * largest that the row has met so far add nothing.
- * The append, steps (not ni_kv_step_noalloc, not one layer at a time), decode
+ * A call takes a position once.  The append, steps (not ni_kv_step_noalloc, not one layer at a time), decode
  * steps, both attention calls and ni_kv_gather_values take such handles, the
  * others refuse them. */
 #define NI_KV_B8 4u

@@ -1950,6 +1950,14 @@ static int block_unsupported(ni_kv* kv, const char* what) {
     return kv->fail(NI_ERR_BAD_ARG, "%s does not take a block-scaled cache", what);
 }
 
+// Above an entry's flags: rows that its page holds by the sequence's length, where the call grows
+// that (they may have come otherwise than by calls, into ni_kv_pools' memory).
+constexpr int kCommittedShift = 18;
+static uint32_t committed_rows(const ni_kv* kv, const ni_row& r) {
+    const uint32_t len = kv->seq_len[r.seq], begin = r.pos - r.pos % kPage;
+    return r.pos >= len && len > begin ? (len - begin) << kCommittedShift : 0;
+}
+
 // Sort a call's rows into the pages they go to (block_entries, block_list).
 static int plan_block_append(ni_kv* kv, const ni_row* rows, uint32_t n) {
     auto& entries = kv->block_entries;
@@ -1968,11 +1976,11 @@ static int plan_block_append(ni_kv* kv, const ni_row* rows, uint32_t n) {
         if (int rc = check_write(kv, rows[i])) return rc;
         const uint32_t page = kv->pages[rows[i].seq][rows[i].pos / kPage], slot = rows[i].pos % kPage;
         if (!entries.empty() && entries.back().page == page && slot > last_slot) {
-            entries.back().slots |= 1u << slot;
+            entries.back().slots |= 1u << slot | committed_rows(kv, rows[i]);
         } else {
             sorted &= kv->page_stamps[page] != kv->page_stamp;
             kv->page_stamps[page] = kv->page_stamp;
-            entries.push_back({page, i, 1u << slot});
+            entries.push_back({page, i, 1u << slot | committed_rows(kv, rows[i])});
         }
         last_slot = slot;
     }
@@ -1996,7 +2004,7 @@ static int plan_block_append(ni_kv* kv, const ni_row* rows, uint32_t n) {
         if (i == 0 || order[i - 1].first != page) entries.push_back({page, i, kListed});
         if (entries.back().slots & slot)
             return kv->fail(NI_ERR_BAD_ARG, "sequence %u: position %u appears twice", r.seq, r.pos);
-        entries.back().slots |= slot;
+        entries.back().slots |= slot | committed_rows(kv, r);
         list.push_back(order[i].second);
     }
     return NI_OK;
@@ -2008,9 +2016,11 @@ static bool mark_anew(ni_kv* kv, uint32_t layer0, uint32_t n_lay) {
     const uint32_t L = kv->written_layers;
     for (BlockAppend& e : kv->block_entries) {
         const uint16_t* w = &kv->written[(size_t)e.page * L + (L > 1 ? layer0 : 0)];
-        const bool anew = (w[0] & ~e.slots) == 0;
+        const uint32_t committed = (1u << (e.slots >> kCommittedShift)) - 1u;
+        auto begins = [&](uint32_t l) { return ((w[l] | committed) & ~e.slots) == 0; };
+        const bool anew = begins(0);
         for (uint32_t l = 1; l < (L > 1 ? n_lay : 1); l++)
-            if (((w[l] & ~e.slots) == 0) != anew) return false;
+            if (begins(l) != anew) return false;
         e.slots = anew ? e.slots | kAnew : e.slots & ~kAnew;
     }
     return true;

@@ -325,3 +325,36 @@ def test_copies_leave_what_lies_behind_the_end(gpu, head_dim, n_head, rows):
     assert torch.equal(after[:, dst][:, left], before[:, dst][:, left])
     others = [p for p in range(6) if p != dst]
     assert torch.equal(after[:, others], before[:, others])
+
+
+@pytest.mark.parametrize("length", [5, 16, 21, 47])
+def test_rows_brought_into_the_pool_by_other_means(gpu, length):
+    """A pool's bytes from another cache of the same tables: appends go on behind the committed rows."""
+    a, b = Caches(), Caches()
+    sa, sb = a.kv.add_seq(), b.kv.add_seq()
+    a.kv.reserve(sa, 4 * PAGE)
+    a.put([(sa, p) for p in range(length)], 2.0)
+    a.kv.commit(sa, length)
+    b.kv.reserve(sb, 4 * PAGE)
+    b.kv.commit(sb, length)
+    assert a.kv.block_table(sa) == b.kv.block_table(sb)
+
+    def pool(kv):
+        at, _, n = kv.pools()
+
+        class Pool:
+            __cuda_array_interface__ = dict(shape=(n,), typestr="|u1", data=(at, False), version=2)
+
+        return torch.as_tensor(Pool(), device="cuda")
+
+    pool(b.kv).copy_(pool(a.kv))
+    b.models = a.models
+    for i, size in enumerate((1e-4, 1.0, 300.0)):
+        b.put([(sb, length + i)], size)
+        b.kv.commit(sb, 1)
+        b.check()
+    (f,) = b.kv.fork([sb])
+    for m in b.models:
+        m.become(f, sb, length + 3)
+    b.put([(f, length + 3), (f, length + 4)], 1e-4)
+    b.check()
