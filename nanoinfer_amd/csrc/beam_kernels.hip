@@ -30,7 +30,7 @@ constexpr uint32_t kGroupLanes = kBeamGroup / kBE;
 static_assert(kBE == 8 && kGroupLanes == 16, "a group is a row of lanes");
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// Whether anything of beam w of search b is read: it is alive, and goes on.
+// Whether a row's beam is finished: its logits are not read, it goes on with the pad token alone.
 __device__ __forceinline__ bool is_finished(const BeamLaunch& a, uint32_t row) { return a.finished && a.finished[row] != 0; }
 
 // Sum over groups of `lanes` lanes, a power of two up to 16.
@@ -267,7 +267,7 @@ __device__ __forceinline__ void pick_equal(Pick& sh, const double (&t)[kPU], con
 
 // Bring the threads' candidates (-infinity: none) into the k best of sh.best, of which
 // `have` are there; gives how many are then.  What lies below the k-th best of the
-// bests of 256 sets of candidates is out; the few others are ranked with the best so
+// bests of 64 sets of candidates is out; the few others are ranked with the best so
 // far.  Every thread of the workgroup calls it.
 __device__ __forceinline__ uint32_t pick_more(Pick& sh, const double (&t)[kPU], const uint32_t (&index)[kPU], uint32_t k,
                                               uint32_t have) {

@@ -291,12 +291,12 @@ constexpr int kFar = 83;
 // ones' loads issued before the products of these; their states are joined through
 // LDS.
 //   Bound by memory for one tile: 16 sequences of 32 k keys, 4 query heads to each of 8 cache
-// heads x 128, 1.03 GB, 159 us, 6.5 TB/s; 64 rows of 1..767 keys, 12 layers x 12 heads x 64, 0.41 GB,
+// heads x 128, 1.03 GB, 158 us, 6.5 TB/s; 64 rows of 1..767 keys, 12 layers x 12 heads x 64, 0.41 GB,
 // 77 us, 5.3 TB/s (short items: a start and a join to each 2 to 24 turns).  Two tiles are bound by
 // what their waves issue: a prompt of 2041 rows x 32 query heads on 8 x 128, 34 GFLOP (69 with hi
-// + lo), 84 us, of which the matrix cores are busy 28 and vector instructions (some 150 of a wave
-// for two tiles of a page, 32 of them conversions) issue for 31; 512 rows x 16 x 12 heads x 64, 12
-// layers, 380 us.
+// + lo), 88 us, of which the matrix cores are busy 28 and vector
+// instructions (some 155 of a wave for two tiles of a page, 32 of them conversions) issue for 34; 512 rows
+// x 16 x 12 heads x 64, 12 layers, 400 us.
 template <int D, int NT, int W, bool MANY, int INL>
 __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a, const PlanArg<INL> pa) {
     constexpr int NB = D / 64, PB = 2, NC = 4 * NB;  // runs of 64 dims; pages of an iteration; 16-dim chunks
@@ -573,8 +573,8 @@ __global__ __launch_bounds__(64 * W) void block_attn_kernel(const PrefixLaunch a
         }
         // Both pages at once, or one at a time, the outputs in its units meanwhile.  (One body for
         // both, which drops the other page's values: with one of its own for pages by themselves
-        // the compiler kept the outputs twice, 220 registers and two waves to a SIMD in place of 154
-        // and three: the prompt below 102 us.)
+        // the compiler kept the outputs twice, 220 registers and two waves to a SIMD in place of 158
+        // and three: the prompt above 102 us.)
 #pragma unroll 1
         for (int b = 0; b < (both ? 1 : PB); b++) {
             const int up = b ? units[1] : units[0], by = b ? far_by[1] : far_by[0];

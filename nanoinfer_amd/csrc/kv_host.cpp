@@ -253,7 +253,7 @@ struct ni_kv {
     std::vector<uint32_t> block_list;
     std::vector<uint32_t> page_stamps;
     uint32_t page_stamp = 0;
-    std::vector<std::pair<uint32_t, uint32_t>> block_rows;  // (page * 16 + slot, row), where they are sorted
+    std::vector<std::pair<uint32_t, uint32_t>> block_rows;  // (page, row), where they are sorted
     std::vector<ni_row> step_rows;     // ni_kv_step on such a pool
     std::vector<uint32_t> step_at;
     std::vector<uint8_t> blob;  // the serialised plan

@@ -280,14 +280,13 @@ int ni_beam_select(uint32_t dtype, const void* logits, int64_t search_stride, in
     const size_t need = ni_beam_workspace(n_search, n_beam, vocab);
     if (!workspace || !aligned(workspace, 16) || workspace_bytes < need)
         return call_error(NI_ERR_BAD_ARG, "workspace must be %zu bytes, 16-byte aligned", need);
-    // (the workgroup of one search reads its beams while another's writes its answers)
     const uint64_t per = std::min<uint64_t>(std::max<uint64_t>(rows * chunks / (8ull * device_cus()), 1), 16);
     const uint64_t runs = (chunks + per - 1) / per;
     // (a launch holds less than 2^32 threads)
     if (rows * runs >= (1ull << 24) || n_search >= (1u << 22))
         return call_error(NI_ERR_BAD_ARG, "%u searches of %u beams: too many for one call", n_search, n_beam);
     typedef unsigned __int128 u128;
-    // (extents are compared in 64 bits)
+    // (the workgroup of one search reads its beams while another's writes its answers; extents are compared in 64 bits)
     const auto extent = [](uint64_t n, int64_t stride, uint64_t width) { return (u128)(n - 1) * (uint64_t)stride + width; };
     if (hist && n_history && extent(rows, history_stride, n_history) >= (u128)1 << 60)
         return call_error(NI_ERR_BAD_ARG, "history's strides are too large");

@@ -124,7 +124,8 @@ struct PrefixLaunch {
 };
 hipError_t launch_prefix_attention(const PrefixLaunch& a, const void* inline_plan, uint32_t inline_bytes,
                                    hipStream_t s, const LaunchTiming& t = {});
-// Items over a block-scaled pool, none of which join partials.  wide: of runs of
+// Items over a block-scaled pool; none joins the partials of an earlier launch, ni_kv_prefix_attention's merge
+// joins theirs.  wide: of runs of
 // many slots, this many tiles of 16 an item; 0: of one tile, 2, 4 or 8 waves to an item.
 hipError_t launch_block_attention(const PrefixLaunch& a, const void* inline_plan, uint32_t inline_bytes, hipStream_t s,
                                   const LaunchTiming& t = {});
